@@ -206,6 +206,27 @@ int mtb_batch_norm2d_backward_f32(int n, int c, int h, int w, const float* dy, c
                                   const float* gamma, const float* beta, double eps, int relu, float* dx, float* dgamma, float* dbeta,
                                   void* workspace, long long workspace_bytes, void* stream);
 
+/* ---- GroupNorm with an activation behind it (no counterpart in the reference) ----
+ * x, y, dy, dx: channels-last [n][hw][c]; mean, rstd: [n][groups], of the c / groups channels of a group at all positions of an image, the variance the
+ * biased one; y = f(gamma (x - mean) rstd + beta).  activation f: 0 none, 1 ReLU (its gradient passes zero, as mtb_relu_backward_f32 does),
+ * 2 SiLU z / (1 + exp(-z)).  gamma, beta may be NULL (1, 0).  Backward: dx, dgamma and dbeta may be NULL each. */
+long long mtb_group_norm_workspace_bytes(int n, int c, int hw, int groups);
+int mtb_group_norm_forward_f32(int n, int c, int hw, int groups, const float* x, const float* gamma, const float* beta, double eps, int activation, float* y,
+                               float* mean, float* rstd, void* stream);
+int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const float* dy, const float* mean, const float* rstd, const float* x, const float* gamma,
+                                const float* beta, int activation, float* dx, float* dgamma, float* dbeta, void* workspace, long long workspace_bytes,
+                                void* stream);
+
+/* ---- embedding (no counterpart in the reference) ----
+ * out[i] = scale * table[tokens[i]] over `count` tokens and a table [rows][width]; kind of the tokens: 0 int32, 1 int64.  A token outside the table
+ * reads nothing: its row of out is NaN, and the gradient leaves it out.
+ * dtable[v] = scale * sum of dy[i] over the tokens i that are v, added in a fixed order; every row is written, with zeros where no token is v and in the
+ * row `padding` (none: a negative number). */
+int mtb_embedding_forward_f32(int kind, const void* tokens, long long count, int rows, int width, const float* table, double scale, float* out, void* stream);
+long long mtb_embedding_backward_workspace_bytes(long long count, int rows, int width);
+int mtb_embedding_backward_f32(int kind, const void* tokens, long long count, int rows, int width, const float* dy, double scale, long long padding,
+                               float* dtable, void* workspace, long long workspace_bytes, void* stream);
+
 /* ---- MaxPool2d (replaces max_pool2d_reference / max_pool2d_backward_reference,
  *      mytorch/native/cuda/pool_ops.cu/1.template:5-52 and 2.template:5-50) ----
  * tiemask: uint16 per output element, bit kh*KW+kw set where the window element equals the
@@ -292,6 +313,17 @@ int mtb_sgd_f32(float* param, const float* grad, float* momentum_buffer, long lo
 int mtb_sgd_multi_f32(int count, float* const* params, const float* const* grads, float* const* momentum_buffers, const long long* sizes,
                       const int* is_first, double lr, double weight_decay, double momentum, double dampening, int nesterov, int maximize,
                       double grad_scale, void* stream);
+/* The norm of all gradients together, and clipping by it (no counterpart in the reference).  mtb_grad_norm_f32 leaves mtb_grad_norm_sums(count) sums of
+ * squares in device memory; the entry points below make of them the norm, that of grad_scale times the gradients where they have a grad_scale, which they leave in
+ * *norm (device memory), and the factor min(1, max_norm / (norm + 1e-6)).  grads / sizes are HOST arrays of length count.
+ * mtb_clip_grads_f32 multiplies the gradients by the factor in place, each tensor that is listed once (max_norm < 0: the norm only);
+ * mtb_sgd_multi_clipped_f32 is mtb_sgd_multi_f32 on gradients so multiplied, without writing them; its tensors may be some of those of the norm. */
+int mtb_grad_norm_sums(int count);
+int mtb_grad_norm_f32(int count, const float* const* grads, const long long* sizes, double* sums, void* stream);
+int mtb_clip_grads_f32(int count, float* const* grads, const long long* sizes, const double* sums, int nsums, double max_norm, float* norm, void* stream);
+int mtb_sgd_multi_clipped_f32(int count, float* const* params, const float* const* grads, float* const* momentum_buffers, const long long* sizes,
+                              const int* is_first, double lr, double weight_decay, double momentum, double dampening, int nesterov, int maximize,
+                              double grad_scale, const double* sums, int nsums, double max_norm, float* norm, void* stream);
 /* gather gradient tensors into one flat all-reduce buffer (no counterpart: the reference has no
  * distributed code); srcs/offsets/sizes are HOST arrays */
 int mtb_pack_scale_f32(int count, const float* const* srcs, const long long* offsets, const long long* sizes, float* dst, double scale,

@@ -615,6 +615,77 @@ def cuda_batch_norm2d_backward(output_grad, mean, var, x, weight, bias, eps, rel
     return [dx, dg, db]
 
 
+# ---------------------------------------------------------------------------- group norm
+
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2}
+
+
+def _image_extents(x):
+    """(n, c, positions) of a channels-last activation, [N, C] counting as one position."""
+    shape = x.shape
+    return shape[0], shape[1], shape[2] * shape[3] if len(shape) == 4 else 1
+
+
+@_reg("cuda", "group_norm")
+def cuda_group_norm(x, num_groups, weight, bias, eps, activation):
+    """(y, mean, rstd): the statistics are [N, groups]."""
+    _f32(x, weight, bias)
+    env = _env(x)
+    n, c, hw = _image_extents(x)
+    y, mean, rstd = _new(x.shape, x), _new((n, num_groups), x), _new((n, num_groups), x)
+    env.lib.group_norm_forward_f32(n, c, hw, num_groups, x, weight, bias, float(eps), _ACTIVATIONS[activation], y, mean, rstd, env.stream())
+    return y, mean, rstd
+
+
+@_reg("cuda", "group_norm_backward")
+def cuda_group_norm_backward(output_grad, mean, rstd, x, weight, bias, num_groups, activation, needed=(True, True, True)):
+    """[dx, dgamma, dbeta]; ``needed``: which of them the caller will use, the others are None."""
+    _f32(output_grad, mean, rstd, x, weight, bias)
+    env = _env(x)
+    n, c, hw = _image_extents(x)
+    dx = _new(x.shape, x) if needed[0] else None
+    dg = _grad_buffer(weight) if weight is not None and needed[1] else None
+    db = _grad_buffer(bias) if bias is not None and needed[2] else None
+    ws, ws_bytes = env.workspace(env.lib.group_norm_workspace_bytes(n, c, hw, num_groups))
+    env.lib.group_norm_backward_f32(n, c, hw, num_groups, output_grad, mean, rstd, x, weight, bias, _ACTIVATIONS[activation], dx, dg, db, ws, ws_bytes,
+                                    env.stream())
+    return [dx, dg, db]
+
+
+# ---------------------------------------------------------------------------- embedding
+
+_TOKEN_KINDS = {int32: 0, int64: 1}
+
+
+@_reg("cuda", "embedding")
+def cuda_embedding(tokens, weight, scale=1.0, channels_first=False):
+    """tokens.shape + (width,); ``channels_first``: [N, H, W] tokens to an image [N, width, H, W], whose memory is the rows as they are."""
+    _f32(weight)
+    env = _env(weight)
+    shape, (rows, width) = tokens.shape, weight.shape
+    image = len(shape) == 3
+    out = _new((shape[0], width, shape[1], shape[2]) if image and channels_first else (_numel(shape), width) if image else shape + (width,), weight)
+    env.lib.embedding_forward_f32(_TOKEN_KINDS[tokens.dtype], tokens, _numel(shape), rows, width, weight, scale, out, env.stream())
+    # four dimensions are stored channels-last, which here is not the order of the rows
+    return cuda_reshape(out, shape + (width,)) if image and not channels_first else out
+
+
+@_reg("cuda", "embedding_backward")
+def cuda_embedding_backward(output_grad, tokens, weight, scale=1.0, padding_idx=None, channels_first=False):
+    """[dweight]"""
+    _f32(output_grad, weight)
+    env = _env(weight)
+    rows, width = weight.shape
+    count = _numel(tokens.shape)
+    if len(output_grad.shape) == 4 and not channels_first:
+        output_grad = cuda_reshape(output_grad, (count, width))
+    dw = _grad_buffer(weight)
+    ws, ws_bytes = env.workspace(env.lib.embedding_backward_workspace_bytes(count, rows, width))
+    env.lib.embedding_backward_f32(_TOKEN_KINDS[tokens.dtype], tokens, count, rows, width, output_grad, scale, -1 if padding_idx is None else padding_idx,
+                                   dw, ws, ws_bytes, env.stream())
+    return [dw]
+
+
 # ---------------------------------------------------------------------------- pooling
 
 def _pool_args(x, kernel_size, stride, padding):
@@ -1127,3 +1198,32 @@ def cuda_sgd_multi(entries, lr, weight_decay, momentum, dampening, nesterov, max
     env = _env(entries[0][0])
     _refuse_first_step_in_capture(env, any([f for _, _, f in entries]))
     _binding.sgd_step(list(entries), lr, weight_decay, momentum, dampening, bool(nesterov), bool(maximize), grad_scale, env.stream())
+
+
+@_reg("cuda", "sgd_multi_clipped")
+def cuda_sgd_multi_clipped(groups, max_norm, grad_scale=1.0):
+    """groups: [(entries, lr, weight_decay, momentum, dampening, nesterov, maximize)], the entries those of ``sgd_multi``.  The gradients, times
+    ``grad_scale``, are clipped to the norm ``max_norm`` of all of them together on their way into the update; returns that norm."""
+    like = groups[0][0][0][0]
+    env = _env(like)
+    norm, sums = _norm_and_sums(env, like, sum([len(g[0]) for g in groups]))
+    for group in groups:
+        _refuse_first_step_in_capture(env, any([f for _, _, f in group[0]]))
+    _binding.sgd_step_clipped(groups, grad_scale, sums, max_norm, norm, env.stream())
+    return norm
+
+
+@_reg("cuda", "clip_gradients")
+def cuda_clip_gradients(grads, again, max_norm):
+    """The norm of the tensors of both lists together (one element, on the device).  With ``max_norm`` those of the first are multiplied by
+    min(1, max_norm / (norm + 1e-6)) in place; ``again`` holds tensors that are in the first list already, for gradients that share memory."""
+    _f32(*grads)
+    env = _env(grads[0])
+    norm, sums = _norm_and_sums(env, grads[0], len(grads) + len(again))
+    _binding.clip_gradients(grads, again, sums, -1.0 if max_norm is None else max_norm, norm, env.stream())
+    return norm
+
+
+def _norm_and_sums(env, like, count):
+    # the sums are read by launches of a later call, so they are not in the scratch that all operators share
+    return _new((1,), like, float32), CudaMemory(like.device.index, 8 * env.lib.grad_norm_sums(count))

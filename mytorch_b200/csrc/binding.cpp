@@ -246,6 +246,9 @@ constexpr unsigned HOST(I... i) { return (0u | ... | (1u << i)); }
   X(max_pool2d_forward_f32, LAUNCH, 0) X(max_pool2d_backward_f32, LAUNCH, 0) X(max_pool2d_argmax_u8, LAUNCH, 0) \
   X(cross_entropy_workspace_bytes, VALUE, 0) X(cross_entropy_forward_f32, LAUNCH, 0) X(cross_entropy_backward_f32, LAUNCH, 0) \
   X(sgd_f32, LAUNCH, 0) X(sgd_multi_f32, LAUNCH, HOST(1, 2, 3, 4, 5)) X(pack_scale_f32, LAUNCH, HOST(1, 2, 3)) \
+  X(grad_norm_sums, VALUE, 0) X(grad_norm_f32, LAUNCH, HOST(1, 2)) X(clip_grads_f32, LAUNCH, HOST(1, 2)) X(sgd_multi_clipped_f32, LAUNCH, HOST(1, 2, 3, 4, 5)) \
+  X(group_norm_workspace_bytes, VALUE, 0) X(group_norm_forward_f32, LAUNCH, 0) X(group_norm_backward_f32, LAUNCH, 0) X(embedding_forward_f32, LAUNCH, 0) \
+  X(embedding_backward_workspace_bytes, VALUE, 0) X(embedding_backward_f32, LAUNCH, 0) \
   X(conv2d_workspace_bytes, VALUE, 0) X(conv2d_plan_f32, STATUS, HOST(11)) X(conv2d_pair_plan_f32, STATUS, HOST(11)) X(conv2d_pair_choice_f32, STATUS, HOST(11)) X(conv2d_pair_smem_bytes, VALUE, 0) X(conv2d_forward_f32, LAUNCH, 0) \
   X(conv2d_stats_max_rows, VALUE, 0) X(conv2d_forward_stats_f32, LAUNCH, HOST(17)) X(conv2d_bn_forward_f32, LAUNCH, 0) X(conv2d_bn_pool_takes, VALUE, 0) X(conv2d_bn_pool_scratch_bytes, VALUE, 0) X(conv2d_bn_pool_forward_f32, LAUNCH, 0) \
   X(batch_norm2d_forward_prestats_f32, LAUNCH, 0) X(conv2d_dgrad_f32, LAUNCH, 0) X(conv2d_dgrad_add_f32, LAUNCH, 0) \
@@ -451,47 +454,136 @@ PyObject* workspace(PyObject*, PyObject* nbytes) {
   return s.pair;
 }
 
-// sgd_step(entries, lr, weight_decay, momentum, dampening, nesterov, maximize, grad_scale, stream): one update of every
-// (parameter, momentum buffer, first time) of the list; the tables that the entry point reads are gathered here.
-PyObject* sgd_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 9 || !PyList_CheckExact(args[0])) { PyErr_SetString(PyExc_TypeError, "sgd_step takes a list and 8 values"); return nullptr; }
+// The number of elements of a shape.
+bool count_elements(PyObject* shape, long long& total) {
+  if (!PyTuple_Check(shape)) { PyErr_SetString(PyExc_TypeError, "a shape expected"); return false; }
+  total = 1;
+  for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(shape); ++k) {
+    long long extent;
+    if (!from_py(PyTuple_GET_ITEM(shape, k), extent)) return false;
+    total *= extent;
+  }
+  return true;
+}
+
+// clip_gradients(grads, again, sums, max_norm, norm, stream): the norm of the tensors of both lists, to the one-element tensor `norm`; with max_norm >= 0
+// those of the first are then multiplied by the factor that clips them.  `again`: tensors that are in the first list already, and count once more.
+PyObject* clip_gradients(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6 || !PyList_CheckExact(args[0]) || !PyList_CheckExact(args[1])) { PyErr_SetString(PyExc_TypeError, "clip_gradients takes two lists and 4 values"); return nullptr; }
   if (!ready()) return nullptr;
-  const Py_ssize_t count = PyList_GET_SIZE(args[0]);
-  std::vector<float*> params(count), bufs(count);
-  std::vector<const float*> grads(count);
+  const Py_ssize_t scaled = PyList_GET_SIZE(args[0]), count = scaled + PyList_GET_SIZE(args[1]);
+  std::vector<float*> grads(count);
   std::vector<long long> sizes(count);
-  std::vector<int> first(count);
-  double h[4], scale;
-  int nesterov, maximize;
+  double* sums;
+  double max_norm;
+  float* norm;
   void* st;
-  for (int i = 0; i < 4; ++i)
-    if (!from_py(args[1 + i], h[i])) return nullptr;
-  if (!from_py(args[5], nesterov) || !from_py(args[6], maximize) || !from_py(args[7], scale) || !pointer<false>(args[8], st)) return nullptr;
+  if (!pointer<false>(args[2], sums) || !from_py(args[3], max_norm) || !pointer<false>(args[4], norm) || !pointer<false>(args[5], st)) return nullptr;
   for (Py_ssize_t i = 0; i < count; ++i) {
-    PyObject* e = PyList_GET_ITEM(args[0], i);
-    if (!PyTuple_CheckExact(e) || PyTuple_GET_SIZE(e) != 3) { PyErr_SetString(PyExc_TypeError, "(parameter, buffer, first) expected"); return nullptr; }
-    PyObject* param = PyTuple_GET_ITEM(e, 0);
-    Ref grad(PyObject_GetAttr(param, N_grad)), shape(PyObject_GetAttr(param, N_shape));
-    if (!grad || !shape || !pointer<false>(param, params[i]) || !pointer<false>((PyObject*)grad, grads[i]) ||
-        !pointer<false>(PyTuple_GET_ITEM(e, 1), bufs[i]))
-      return nullptr;
-    const int is_first = PyObject_IsTrue(PyTuple_GET_ITEM(e, 2));
-    if (is_first < 0 || !params[i] || !grads[i] || !bufs[i] || !PyTuple_Check(shape)) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "sgd_step: a parameter without device memory, gradient or buffer"); return nullptr; }
-    first[i] = is_first;
-    sizes[i] = 1;
-    for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(shape.p); ++k) {
-      long long extent;
-      if (!from_py(PyTuple_GET_ITEM(shape.p, k), extent)) return nullptr;
-      sizes[i] *= extent;
-    }
+    PyObject* t = i < scaled ? PyList_GET_ITEM(args[0], i) : PyList_GET_ITEM(args[1], i - scaled);
+    Ref shape(PyObject_GetAttr(t, N_shape));
+    if (!shape || !count_elements(shape, sizes[i]) || !pointer<false>(t, grads[i])) return nullptr;
   }
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = E_sgd_multi_f32::fn((int)count, params.data(), grads.data(), bufs.data(), sizes.data(), first.data(), h[0], h[1], h[2], h[3], nesterov, maximize,
-                           scale, st);
+  rc = E_grad_norm_f32::fn((int)count, grads.data(), sizes.data(), sums, st);
+  if (!rc) rc = E_clip_grads_f32::fn((int)scaled, grads.data(), sizes.data(), sums, E_grad_norm_sums::fn((int)count), max_norm, norm, st);
+  Py_END_ALLOW_THREADS
+  if (rc) return raise_native("mtb_clip_grads_f32", rc);
+  g_launches += 2;
+  Py_RETURN_NONE;
+}
+
+// The tables that an SGD entry point reads, gathered from a list of (parameter, momentum buffer, first time).
+struct SgdTables {
+  std::vector<float*> params, bufs;
+  std::vector<const float*> grads;
+  std::vector<long long> sizes;
+  std::vector<int> first;
+  double h[4];
+  int nesterov, maximize;
+
+  // hyper: lr, weight_decay, momentum, dampening, nesterov, maximize
+  bool gather(PyObject* entries, PyObject* const* hyper) {
+    if (!PyList_CheckExact(entries)) { PyErr_SetString(PyExc_TypeError, "a list of (parameter, buffer, first) expected"); return false; }
+    for (int i = 0; i < 4; ++i)
+      if (!from_py(hyper[i], h[i])) return false;
+    if (!from_py(hyper[4], nesterov) || !from_py(hyper[5], maximize)) return false;
+    const Py_ssize_t base = (Py_ssize_t)params.size(), count = base + PyList_GET_SIZE(entries);
+    params.resize(count); bufs.resize(count); grads.resize(count); sizes.resize(count); first.resize(count);
+    for (Py_ssize_t i = base; i < count; ++i) {
+      PyObject* e = PyList_GET_ITEM(entries, i - base);
+      if (!PyTuple_CheckExact(e) || PyTuple_GET_SIZE(e) != 3) { PyErr_SetString(PyExc_TypeError, "(parameter, buffer, first) expected"); return false; }
+      PyObject* param = PyTuple_GET_ITEM(e, 0);
+      Ref grad(PyObject_GetAttr(param, N_grad)), shape(PyObject_GetAttr(param, N_shape));
+      if (!grad || !shape || !pointer<false>(param, params[i]) || !pointer<false>((PyObject*)grad, grads[i]) ||
+          !pointer<false>(PyTuple_GET_ITEM(e, 1), bufs[i]))
+        return false;
+      const int is_first = PyObject_IsTrue(PyTuple_GET_ITEM(e, 2));
+      if (is_first < 0 || !params[i] || !grads[i] || !bufs[i] || !PyTuple_Check(shape)) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "sgd_step: a parameter without device memory, gradient or buffer"); return false; }
+      first[i] = is_first;
+      if (!count_elements(shape, sizes[i])) return false;
+    }
+    return true;
+  }
+};
+
+// sgd_step(entries, lr, weight_decay, momentum, dampening, nesterov, maximize, grad_scale, stream): one update of every
+// (parameter, momentum buffer, first time) of the list.
+PyObject* sgd_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9 || !PyList_CheckExact(args[0])) { PyErr_SetString(PyExc_TypeError, "sgd_step takes a list and 8 values"); return nullptr; }
+  if (!ready()) return nullptr;
+  SgdTables t;
+  double scale;
+  void* st;
+  if (!t.gather(args[0], args + 1) || !from_py(args[7], scale) || !pointer<false>(args[8], st)) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = E_sgd_multi_f32::fn((int)t.params.size(), t.params.data(), t.grads.data(), t.bufs.data(), t.sizes.data(), t.first.data(), t.h[0], t.h[1], t.h[2], t.h[3],
+                           t.nesterov, t.maximize, scale, st);
   Py_END_ALLOW_THREADS
   if (rc) return raise_native("mtb_sgd_multi_f32", rc);
   ++g_launches;
+  Py_RETURN_NONE;
+}
+
+// sgd_step_clipped(groups, grad_scale, sums, max_norm, norm, stream): the same for a list of groups, each a tuple (entries, lr, weight_decay, momentum,
+// dampening, nesterov, maximize), by gradients clipped to max_norm: the norm is that of all groups together and goes to the one-element tensor `norm`.
+PyObject* sgd_step_clipped(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6 || !PyList_CheckExact(args[0])) { PyErr_SetString(PyExc_TypeError, "sgd_step_clipped takes a list and 5 values"); return nullptr; }
+  if (!ready()) return nullptr;
+  const Py_ssize_t groups = PyList_GET_SIZE(args[0]);
+  std::vector<SgdTables> tables(groups);
+  std::vector<const float*> grads;
+  std::vector<long long> sizes;
+  double scale, max_norm;
+  double* sums;
+  float* norm;
+  void* st;
+  if (!from_py(args[1], scale) || !pointer<false>(args[2], sums) || !from_py(args[3], max_norm) || !pointer<false>(args[4], norm) || !pointer<false>(args[5], st))
+    return nullptr;
+  for (Py_ssize_t g = 0; g < groups; ++g) {
+    PyObject* group = PyList_GET_ITEM(args[0], g);
+    if (!PyTuple_CheckExact(group) || PyTuple_GET_SIZE(group) != 7) { PyErr_SetString(PyExc_TypeError, "a group of 7 expected"); return nullptr; }
+    PyObject* hyper[6];
+    for (int i = 0; i < 6; ++i) hyper[i] = PyTuple_GET_ITEM(group, 1 + i);
+    if (!tables[g].gather(PyTuple_GET_ITEM(group, 0), hyper)) return nullptr;
+    grads.insert(grads.end(), tables[g].grads.begin(), tables[g].grads.end());
+    sizes.insert(sizes.end(), tables[g].sizes.begin(), tables[g].sizes.end());
+  }
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  const int nsums = E_grad_norm_sums::fn((int)grads.size());
+  rc = E_grad_norm_f32::fn((int)grads.size(), grads.data(), sizes.data(), sums, st);
+  for (auto& t : tables) {
+    if (rc || t.params.empty()) continue;
+    rc = E_sgd_multi_clipped_f32::fn((int)t.params.size(), t.params.data(), t.grads.data(), t.bufs.data(), t.sizes.data(), t.first.data(), t.h[0], t.h[1], t.h[2],
+                                     t.h[3], t.nesterov, t.maximize, scale, sums, nsums, max_norm, norm, st);
+    norm = nullptr;  // left by the first of them
+  }
+  Py_END_ALLOW_THREADS
+  if (rc) return raise_native("mtb_sgd_multi_clipped_f32", rc);
+  g_launches += 1 + groups;
   Py_RETURN_NONE;
 }
 
@@ -562,6 +654,8 @@ PyMethodDef methods[] = {
     {"enter", enter, METH_O, "Make the tensor's device current; the CUDA state."},
     {"stream", stream, METH_NOARGS, "The compute stream of the current device."},
     {"sgd_step", (PyCFunction)(void (*)())sgd_step, METH_FASTCALL, "One SGD update of a list of (parameter, buffer, first)."},
+    {"sgd_step_clipped", (PyCFunction)(void (*)())sgd_step_clipped, METH_FASTCALL, "One SGD update of several groups, by gradients clipped to a norm."},
+    {"clip_gradients", (PyCFunction)(void (*)())clip_gradients, METH_FASTCALL, "The norm of a list of tensors, and clipping in place."},
     {"workspace", workspace<0>, METH_O, "(address, bytes) of scratch for compute-stream kernels."},
     {"side_workspace", workspace<1>, METH_O, "(address, bytes) of scratch for side-stream kernels."},
 #define X(n, k, h) {#n, (PyCFunction)(void (*)())E_##n::call, METH_FASTCALL, nullptr},

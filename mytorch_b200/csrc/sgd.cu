@@ -1,7 +1,7 @@
 // SGD with momentum / dampening / Nesterov / weight decay / maximize, per tensor and as a
 // multi-tensor launch (pointer table passed by value in kernel parameters, so a whole model
 // updates in a few launches and the launch can be captured in a CUDA graph).
-#include "common.cuh"
+#include "clip.cuh"
 
 namespace {
 
@@ -57,9 +57,12 @@ struct SgdTable {
 
 // One CTA per chunk of kSgdChunk elements of one tensor (a model has a few large tensors and dozens of
 // tiny ones: a grid of tensors x the largest tensor's chunks would be mostly empty CTAs).
-__global__ void __launch_bounds__(256) sgd_multi_kernel(const __grid_constant__ SgdTable t, SgdHyper h) {
+// CLIP: the gradients are multiplied by the factor that clips them, which nothing writes back.
+template <bool CLIP>
+__global__ void __launch_bounds__(256) sgd_multi_kernel(const __grid_constant__ SgdTable t, SgdHyper h, MtbClip clip) {
   mtb_launch_dependents();
   mtb_wait_prior();
+  if (CLIP) h.grad_scale *= mtb_clip_factor<256>(clip);
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {  // last k with chunk_start[k] <= blockIdx.x
     const int mid = (lo + hi + 1) >> 1;
@@ -105,10 +108,9 @@ MTB_API int mtb_sgd_f32(float* param, const float* grad, float* momentum_buffer,
   return MTB_OK;
 }
 
-// `count` parameter tensors with shared hyper-parameters. Host arrays of device pointers.
-MTB_API int mtb_sgd_multi_f32(int count, float* const* params, const float* const* grads, float* const* momentum_buffers, const long long* sizes,
-                              const int* is_first, double lr, double weight_decay, double momentum, double dampening, int nesterov,
-                              int maximize, double grad_scale, void* stream) {
+static int sgd_multi(int count, float* const* params, const float* const* grads, float* const* momentum_buffers, const long long* sizes, const int* is_first,
+                     double lr, double weight_decay, double momentum, double dampening, int nesterov, int maximize, double grad_scale, MtbClip clip,
+                     void* stream) {
   MTB_REQUIRE(count >= 0 && (count == 0 || (params && grads && momentum_buffers && sizes && is_first)), "sgd_multi: bad arguments");
   SgdHyper h{(float)lr, (float)weight_decay, (float)momentum, (float)(1.0 - dampening), (float)grad_scale, nesterov, maximize, 0};
   for (int base = 0; base < count; base += kMaxTensors) {
@@ -127,12 +129,30 @@ MTB_API int mtb_sgd_multi_f32(int count, float* const* params, const float* cons
       MTB_REQUIRE(chunks < (1LL << 30), "sgd_multi: too many elements in one call");
     }
     t.chunk_start[t.count] = (int)chunks;
+    if (chunks == 0 && clip.norm) chunks = 1;  // nothing to update: one CTA leaves the norm
     if (chunks == 0) continue;
     dim3 grid((unsigned int)chunks);
-    MTB_LAUNCH(sgd_multi_kernel, grid, 256, 0, (cudaStream_t)stream, t, h);
+    MTB_LAUNCH(clip.sums ? sgd_multi_kernel<true> : sgd_multi_kernel<false>, grid, 256, 0, (cudaStream_t)stream, t, h, clip);
     MTB_LAUNCH_CHECK("sgd_multi_kernel");
+    clip.norm = nullptr;  // left by the first launch
   }
   return MTB_OK;
+}
+
+// `count` parameter tensors with shared hyper-parameters. Host arrays of device pointers.
+MTB_API int mtb_sgd_multi_f32(int count, float* const* params, const float* const* grads, float* const* momentum_buffers, const long long* sizes,
+                              const int* is_first, double lr, double weight_decay, double momentum, double dampening, int nesterov,
+                              int maximize, double grad_scale, void* stream) {
+  return sgd_multi(count, params, grads, momentum_buffers, sizes, is_first, lr, weight_decay, momentum, dampening, nesterov, maximize, grad_scale, MtbClip{}, stream);
+}
+
+// The same with the gradients clipped to max_norm on the way, by the sums that mtb_grad_norm_f32 left of all gradients.
+MTB_API int mtb_sgd_multi_clipped_f32(int count, float* const* params, const float* const* grads, float* const* momentum_buffers, const long long* sizes,
+                                      const int* is_first, double lr, double weight_decay, double momentum, double dampening, int nesterov, int maximize,
+                                      double grad_scale, const double* sums, int nsums, double max_norm, float* norm, void* stream) {
+  MTB_REQUIRE(sums && nsums > 0 && max_norm >= 0, "sgd_multi_clipped: bad arguments");
+  return sgd_multi(count, params, grads, momentum_buffers, sizes, is_first, lr, weight_decay, momentum, dampening, nesterov, maximize, grad_scale,
+                   MtbClip{sums, nsums, grad_scale, max_norm, norm}, stream);
 }
 
 // dst[offsets[k] : offsets[k] + sizes[k]] = scale * srcs[k][:] for k < count.
