@@ -77,14 +77,16 @@ int lookup(const void* tokens, long long count, int rows, int width, const float
 // tokens and a row of counters, one for each digit; a token's place is what all smaller digits take, what its digit takes in the stretches before, and
 // its rank in its own.  The order among equal tokens is kept, so the sums below have the same bits every time.
 // The clusters behind the first clear the gradient meanwhile: rows that no token names stay so.
+// What bounds it: latency, and scattered stores, of which an SM takes one line a cycle.  So a token and its place travel as one 8-byte entry, and a CTA puts its
+// share in order in shared memory first and writes stretches of a digit.  SORTED_FIGURES
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kDigitBits = 9, kDigits = 1 << kDigitBits;
-constexpr int kSortAhead = 4;
+constexpr int kSortAhead = 8, kSortCtas = 16, kStaged = 8192;
 
 struct SortPlan {
   int count, rows, passes, bits;  // bits of a digit
   long long padding;
-  int *keys[2], *places[2];  // scratch; the last pass leaves its result in the first of each
-  int* runs;                 // cleared: how many long runs there are
+  int2* entries[2];  // scratch, (token, place); the last pass leaves its result in the first
+  int* runs;         // cleared: how many long runs there are
   float* dtable;
   long long cells;
 };
@@ -109,7 +111,7 @@ __device__ __forceinline__ void clear_cells(float* p, long long n, int block, in
 
 template <class T>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const void* __restrict__ tokens, SortPlan p) {
-  extern __shared__ int counters[];  // [kSortWarps][kDigits], then the digits' totals and first places
+  extern __shared__ int2 staged[];  // [kStaged], then counters [kSortWarps][kDigits], the CTA's totals of the digits, where they go
   mtb_launch_dependents();
   mtb_wait_prior();
   cg::cluster_group cluster = cg::this_cluster();
@@ -119,87 +121,107 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const void
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int *mine = counters + warp * kDigits, *totals = counters + kSortWarps * kDigits, *first = totals + kDigits, *sums = first + kDigits;
+  int *counters = (int*)(staged + kStaged), *mine = counters + warp * kDigits, *totals = counters + kSortWarps * kDigits;
+  int *local = totals + kDigits, *shift_to = local + kDigits, *sums = shift_to + kDigits;
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
   const int each = ((p.count + ctas * kSortWarps - 1) / (ctas * kSortWarps) + 31) / 32 * 32;
-  const long long begin = (long long)(cta * kSortWarps + warp) * each;
-  const int lo = (int)(begin < p.count ? begin : p.count), hi = begin + each < p.count ? (int)(begin + each) : p.count;
+  auto bounded = [&](long long i) { return (int)(i < p.count ? i : p.count); };
+  const int lo = bounded((long long)(cta * kSortWarps + warp) * each), hi = bounded((long long)(cta * kSortWarps + warp + 1) * each);
+  const int share = bounded((long long)(cta + 1) * kSortWarps * each) - bounded((long long)cta * kSortWarps * each);
   const unsigned below = (1u << lane) - 1;
+  const bool held = each <= 32 * kSortAhead, stage = share <= kStaged;
   for (int pass = 0; pass < p.passes; ++pass) {
-    const int to = (p.passes - 1 - pass) & 1, from = to ^ 1, shift = pass * p.bits, digits = 1 << p.bits;
-    for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) counters[i] = 0;
+    const int to = (p.passes - 1 - pass) & 1, shift = pass * p.bits, digits = 1 << p.bits;
+    for (int i = threadIdx.x; i < kSortWarps * kDigits / 4; i += kSortThreads) ((int4*)counters)[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    // what other CTAs wrote is read past the L1 cache
-    auto key = [&](int i) { return pass ? __ldcg(p.keys[from] + i) : key_of<T>(tokens, i, p); };
-    for (int i0 = lo; i0 < hi; i0 += 32 * kSortAhead) {
-      int d[kSortAhead];
+    int2 entry[kSortAhead];
+    auto load = [&](int i0) {
 #pragma unroll
       for (int u = 0; u < kSortAhead; ++u) {
         const int i = i0 + 32 * u + lane;
-        d[u] = i < hi ? key(i) >> shift & (digits - 1) : digits;
+        // what other CTAs wrote is read past the L1 cache
+        if (i < hi) entry[u] = pass ? __ldcg(p.entries[to ^ 1] + i) : make_int2(key_of<T>(tokens, i, p), i);
       }
+    };
+    for (int i0 = lo; i0 < hi; i0 += 32 * kSortAhead) {
+      load(i0);
 #pragma unroll
-      for (int u = 0; u < kSortAhead; ++u) {
-        const unsigned same = __match_any_sync(0xffffffffu, d[u]);
-        if (d[u] < digits && !(same & below)) mine[d[u]] += __popc(same);
-        __syncwarp();
-      }
+      for (int u = 0; u < kSortAhead; ++u)
+        if (i0 + 32 * u + lane < hi) atomicAdd(mine + (entry[u].x >> shift & (digits - 1)), 1);
     }
     __syncthreads();
+    int total = 0;
     if (threadIdx.x < digits) {
-      int sum = 0;
-      for (int w = 0; w < kSortWarps; ++w) {
-        const int n = counters[w * kDigits + threadIdx.x];
-        counters[w * kDigits + threadIdx.x] = sum;
-        sum += n;
+      for (int w0 = 0; w0 < kSortWarps; w0 += 16) {
+        int n[16];
+#pragma unroll
+        for (int w = 0; w < 16; ++w) n[w] = counters[(w0 + w) * kDigits + threadIdx.x];
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+          counters[(w0 + w) * kDigits + threadIdx.x] = total;
+          total += n[w];
+        }
       }
-      totals[threadIdx.x] = sum;
+      totals[threadIdx.x] = total;
     }
     cluster.sync();
     int before = 0, all = 0;
     if (threadIdx.x < digits) {
-      for (int r = 0; r < ctas; ++r) {
-        const int n = cluster.map_shared_rank(totals, r)[threadIdx.x];
+#pragma unroll
+      for (int r = 0; r < kSortCtas; ++r) {
+        const int n = r < ctas ? cluster.map_shared_rank(totals, r)[threadIdx.x] : 0;
         if (r < cta) before += n;
         all += n;
       }
     }
-    int upto = all;  // inclusive over the digits
+    int upto_all = all, upto_total = total;  // inclusive over the digits
     for (int o = 1; o < 32; o <<= 1) {
-      const int n = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += n;
+      const int a = __shfl_up_sync(0xffffffffu, upto_all, o), b = __shfl_up_sync(0xffffffffu, upto_total, o);
+      if (lane >= o) { upto_all += a; upto_total += b; }
     }
-    if (lane == 31) sums[warp] = upto;
+    if (lane == 31) { sums[warp] = upto_all; sums[kSortWarps + warp] = upto_total; }
     __syncthreads();
-    int offset = 0;
-    for (int w = 0; w < warp; ++w) offset += sums[w];
-    if (threadIdx.x < digits) first[threadIdx.x] = offset + upto - all + before;
+    if (threadIdx.x < digits) {
+      int offset = upto_all - all + before, here = upto_total - total;
+      for (int w = 0; w < warp; ++w) { offset += sums[w]; here += sums[kSortWarps + w]; }
+      local[threadIdx.x] = here;
+      shift_to[threadIdx.x] = offset - here;
+    }
     __syncthreads();
     for (int i0 = lo; i0 < hi; i0 += 32 * kSortAhead) {
-      int k[kSortAhead], at[kSortAhead];
+      if (!held) load(i0);
 #pragma unroll
       for (int u = 0; u < kSortAhead; ++u) {
-        const int i = i0 + 32 * u + lane;
-        k[u] = i < hi ? key(i) : 0;
-        at[u] = i < hi && pass ? __ldcg(p.places[from] + i) : i;
-      }
+        if (i0 + 32 * u >= hi) break;
+        const bool in = i0 + 32 * u + lane < hi;
+        const int d = entry[u].x >> shift & (digits - 1);
+        // the lanes with the same digit, bit by bit (__match_any_sync took some 500 cycles for 32 different ones)
+        unsigned same = __ballot_sync(0xffffffffu, in);
 #pragma unroll
-      for (int u = 0; u < kSortAhead; ++u) {
-        const int d = i0 + 32 * u + lane < hi ? k[u] >> shift & (digits - 1) : digits;
-        const unsigned same = __match_any_sync(0xffffffffu, d);
+        for (int b = 0; b < kDigitBits; ++b) {
+          const unsigned set = __ballot_sync(0xffffffffu, d >> b & 1);
+          same &= d >> b & 1 ? set : ~set;
+        }
         int taken = 0;
-        if (d < digits) taken = mine[d];
+        if (in) taken = mine[d];
         __syncwarp();
-        if (d < digits) {
-          const int place = first[d] + taken + __popc(same & below);
-          p.keys[to][place] = k[u];
-          p.places[to][place] = at[u];
+        if (in) {
+          const int place = local[d] + taken + __popc(same & below);
+          if (stage) staged[place] = entry[u];
+          else p.entries[to][place + shift_to[d]] = entry[u];
           if (!(same & below)) mine[d] = taken + __popc(same);
         }
         __syncwarp();
       }
     }
-    cluster.sync();  // also makes this pass's places visible to the others
+    if (stage) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < share; i += kSortThreads) {
+        const int2 e = staged[i];
+        p.entries[to][i + shift_to[e.x >> shift & (digits - 1)]] = e;
+      }
+    }
+    cluster.sync();  // also makes this pass's entries visible to the others
   }
 }
 
@@ -211,13 +233,15 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const void
 constexpr int kRun = 32, kMaxTile = kRun, kSumAhead = 8;  // a longer tile could hold a whole long run
 
 struct SumPlan {
-  const int *keys, *places;
+  const int2* entries;
   int count, rows, width, tile, lanes, groups;  // threads to a tile, tiles to a CTA
   float scale;
   const float* dy;
   float* dtable;
   float* pieces;  // [tiles][2][width]: of the long run that begins before the tile, of the one that begins in it
-  int *runs, *run_tiles;
+  int* runs;              // how many long runs there are,
+  int2* run_starts;       // of each, the tile that it begins in and its token
+  int* run_ends;          // [rows]: the tile that a long run of this token ends in
 };
 
 template <int V>
@@ -234,96 +258,106 @@ __global__ void __launch_bounds__(128) embedding_sum_kernel(SumPlan p) {
     for (int j = lane; j < p.tile + 2 * kRun + 2; j += p.lanes) {
       const int i = t0 - kRun - 1 + j;
       const bool in = i >= 0 && i < p.count;
-      keys[j] = in ? p.keys[i] : -1;
-      places[j] = in ? p.places[i] : 0;
+      const int2 entry = in ? p.entries[i] : make_int2(-1, 0);
+      keys[j] = entry.x;
+      places[j] = entry.y;
     }
   }
   __syncthreads();
   if (t0 >= p.count) return;
   const int col = (blockIdx.y * p.lanes + lane) * V;
-  const bool in_row = col < p.width;
-  constexpr int kFirst = kRun + 1;  // where the tile begins
-  const int end = kFirst + (p.tile < p.count - t0 ? p.tile : p.count - t0);
-  float* pieces = p.pieces + 2LL * (t0 / p.tile) * p.width + col;
-  int e = kFirst;
-  while (e < end) {
+  if (col >= p.width) return;
+  // the entries [e, to) are this tile's: without the end of a short run that began before it, with the rest of one that begins in it
+  int e = kRun + 1, to = e + (p.tile < p.count - t0 ? p.tile : p.count - t0);
+  while (to > e && keys[to - 1] >= p.rows) --to;  // those that count nothing are last
+  if (e == to) return;
+  bool begun = keys[e - 1] == keys[e], left = false;  // long runs that began before, that go on behind
+  if (begun) {
     const int k = keys[e];
-    if (k >= p.rows) break;  // those that count nothing are last
-    int s = e, stop = e;  // the run's ends, as far as kRun from the tile's
-    if (e == kFirst)
-      while (s > 0 && keys[s - 1] == k) --s;
-    while (stop < end && keys[stop] == k) ++stop;
-    const int inside = stop;
-    if (inside == end)
-      while (stop - s <= kRun && keys[stop] == k) ++stop;
-    const bool whole = stop - s <= kRun;
-    if (whole && s < e) { e = inside; continue; }  // the tile before has it
-    const int last = whole ? stop : inside;
-    VecF<V> sum;
+    int s = e - 1, stop = e + 1;
+    while (s > 0 && keys[s - 1] == k) --s;
+    while (stop - s <= kRun && keys[stop] == k) ++stop;
+    if (stop - s <= kRun) {
+      begun = false;
+      e = stop < to ? stop : to;
+      if (e == to) return;
+    } else if (keys[to] != k && blockIdx.y == 0 && lane == 0) {
+      p.run_ends[k] = t0 / p.tile;
+    }
+  }
+  if (keys[to] == keys[to - 1] && !(begun && keys[e] == keys[to - 1])) {
+    const int k = keys[to];
+    int s = to - 1, stop = to + 1;
+    while (s > e && keys[s - 1] == k) --s;
+    while (stop - s <= kRun && keys[stop] == k) ++stop;
+    left = stop - s > kRun;
+    if (!left) to = stop;
+    else if (blockIdx.y == 0 && lane == 0) p.run_starts[atomicAdd(p.runs, 1)] = make_int2(t0 / p.tile, k);
+  }
+  float* pieces = p.pieces + 2LL * (t0 / p.tile) * p.width + col;
+  const float* dy = p.dy + col;
+  VecF<V> sum;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum.v[i] = 0.f;
+  int k = keys[e];
+  auto flush = [&](bool is_last) {
+    float* to_row = begun ? pieces : is_last && left ? pieces + p.width : p.dtable + (long long)k * p.width + col;
+    if (!begun && !(is_last && left)) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum.v[i] *= p.scale;
+    }
+    vstore<V>(to_row, sum);
+    begun = false;
 #pragma unroll
     for (int i = 0; i < V; ++i) sum.v[i] = 0.f;
-    if (in_row) {
-      for (int j0 = e; j0 < last; j0 += kSumAhead) {
-        VecF<V> v[kSumAhead];
+  };
+  // rows are loaded kSumAhead at a time, whichever runs they belong to
+  for (; e < to; e += kSumAhead) {
+    VecF<V> v[kSumAhead];
 #pragma unroll
-        for (int u = 0; u < kSumAhead; ++u)
-          if (j0 + u < last) v[u] = vload<V>(p.dy + (long long)places[j0 + u] * p.width + col);
+    for (int u = 0; u < kSumAhead; ++u)
+      if (e + u < to) v[u] = vload<V>(dy + (long long)places[e + u] * p.width);
 #pragma unroll
-        for (int u = 0; u < kSumAhead; ++u)
-          if (j0 + u < last)
-#pragma unroll
-            for (int i = 0; i < V; ++i) sum.v[i] += v[u].v[i];
+    for (int u = 0; u < kSumAhead; ++u) {
+      if (e + u >= to) break;
+      if (keys[e + u] != k) {
+        flush(false);
+        k = keys[e + u];
       }
-      if (whole) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum.v[i] *= p.scale;
-        vstore<V>(p.dtable + (long long)k * p.width + col, sum);
-      } else {
-        vstore<V>(pieces + (s < e ? 0 : p.width), sum);
-      }
+      for (int i = 0; i < V; ++i) sum.v[i] += v[u].v[i];
     }
-    if (!whole && s == e && lane == 0 && blockIdx.y == 0) p.run_tiles[atomicAdd(p.runs, 1)] = t0 / p.tile;
-    e = inside;
   }
+  flush(true);
 }
 
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 256, kJoinAhead = 4;
 
 // One CTA a long run and 32 lanes' columns: its warps add up a part of the pieces each, and those sums are added in their order.
 template <int V>
-__global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(SumPlan p) {
+__global__ void __launch_bounds__(kJoinThreads, 5) embedding_join_kernel(SumPlan p) {
   mtb_launch_dependents();
   mtb_wait_prior();
   __shared__ float sums[kJoinThreads / 32][32 * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kJoinThreads / 32;
-  const int columns = (p.width + 32 * V - 1) / (32 * V), tiles = (p.count + p.tile - 1) / p.tile;
+  const int columns = (p.width + 32 * V - 1) / (32 * V);
   const int items = *p.runs * columns;
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int t = p.run_tiles[item / columns], col = (item % columns * 32 + lane) * V;
-    const int last = t + 1 < tiles ? (t + 1) * p.tile - 1 : p.count - 1, k = p.keys[last];  // the run that begins in the tile and ends behind it
-    int a = t, b = tiles;  // tile a begins within the run (or is t), tile b does not: 32 probes at a time
-    while (b - a > 1) {
-      const int step = (b - a + 31) / 32, probe = a + 1 + lane * step;
-      const unsigned yes = __ballot_sync(0xffffffffu, probe < b && p.keys[(long long)probe * p.tile] == k);
-      const int n = __popc(yes);
-      if (n == 0) { b = a + 1; break; }
-      const int na = a + 1 + (n - 1) * step, nb = na + step;
-      a = na;
-      b = nb < b ? nb : b;
-    }
-    const int count = a - t + 1;  // pieces
+    const int2 start = p.run_starts[item / columns];
+    const int t = start.x, k = start.y, col = (item % columns * 32 + lane) * V;
+    const int count = p.run_ends[k] - t + 1;  // pieces
     const int lo = (int)((long long)count * warp / warps), hi = (int)((long long)count * (warp + 1) / warps);
     VecF<V> sum;
 #pragma unroll
     for (int i = 0; i < V; ++i) sum.v[i] = 0.f;
     if (col < p.width) {
-      for (int j0 = lo; j0 < hi; j0 += kSumAhead) {
-        VecF<V> v[kSumAhead];
+      for (int j0 = lo; j0 < hi; j0 += kJoinAhead) {
+        VecF<V> v[kJoinAhead];
 #pragma unroll
-        for (int u = 0; u < kSumAhead; ++u)
+        for (int u = 0; u < kJoinAhead; ++u)
           if (j0 + u < hi) v[u] = vload<V>(p.pieces + (2LL * (t + j0 + u) + (j0 + u == 0 ? 1 : 0)) * p.width + col);
 #pragma unroll
-        for (int u = 0; u < kSumAhead; ++u)
+        for (int u = 0; u < kJoinAhead; ++u)
           if (j0 + u < hi)
 #pragma unroll
             for (int i = 0; i < V; ++i) sum.v[i] += v[u].v[i];
@@ -349,7 +383,7 @@ struct GradPlan {
   long long bytes;
 };
 
-// Scratch: two sets of keys and places, the list of long runs, the pieces.
+// Scratch: two sets of entries, the long runs' starts and ends, the pieces.
 GradPlan plan_gradient(long long count, int rows, int width, bool four) {
   GradPlan g{};
   int bits = 1;
@@ -357,7 +391,7 @@ GradPlan plan_gradient(long long count, int rows, int width, bool four) {
   g.passes = (bits + kDigitBits - 1) / kDigitBits;
   g.bits = (bits + g.passes - 1) / g.passes;
   g.ctas = 1;
-  while (g.ctas < 16 && count > (long long)g.ctas * kSortThreads * 4) g.ctas *= 2;
+  while (g.ctas < kSortCtas && count > (long long)g.ctas * kSortThreads) g.ctas *= 2;
   const int vectors = four ? width / 4 : width;
   g.lanes = 4;
   while (g.lanes < vectors && g.lanes < 32) g.lanes *= 2;
@@ -368,14 +402,14 @@ GradPlan plan_gradient(long long count, int rows, int width, bool four) {
   g.tile = 8;
   while (g.tile < kMaxTile && count / (2LL * g.tile * g.groups) * g.columns >= mtb_sm_count() * 16LL) g.tile *= 2;
   g.tiles = (int)((count + g.tile - 1) / g.tile);
-  g.bytes = 16 * count + 4LL * g.tiles + 512 + 8LL * g.tiles * width;
+  g.bytes = 16 * count + 4LL * rows + 8LL * g.tiles + 512 + 8LL * g.tiles * width;
   return g;
 }
 
 template <class T>
 int sort_tokens(const void* tokens, const SortPlan& p, int ctas, cudaStream_t st) {
   static unsigned long long opted;
-  constexpr int smem = (kSortWarps * kDigits + 2 * kDigits + kSortWarps) * 4;
+  constexpr int smem = kStaged * 8 + (kSortWarps * kDigits + 3 * kDigits + 2 * kSortWarps) * 4;
   if (int rc = mtb_opt_in_smem((const void*)embedding_sort_kernel<T>, smem, &opted)) return rc;
   static unsigned long long wide;
   int device = 0;
@@ -408,7 +442,7 @@ template <int V>
 int add_up(const SumPlan& p, const GradPlan& g, cudaStream_t st) {
   const int smem = g.groups * 2 * (kMaxTile + 2 * kRun + 2) * 4;
   MTB_LAUNCH(embedding_sum_kernel<V>, dim3(mtb_div_up(g.tiles, g.groups), g.columns), g.lanes * g.groups, smem, st, p);
-  if (p.count > kRun) MTB_LAUNCH(embedding_join_kernel<V>, mtb_sm_count() * 2, kJoinThreads, 0, st, p);
+  if (p.count > kRun) MTB_LAUNCH(embedding_join_kernel<V>, mtb_sm_count() * 5, kJoinThreads, 0, st, p);
   return MTB_OK;
 }
 
@@ -445,12 +479,11 @@ MTB_API int mtb_embedding_backward_f32(int kind, const void* tokens, long long c
   const GradPlan g = plan_gradient(count, rows, width, four);
   MTB_REQUIRE(g.columns < 65536, "embedding_backward: rows of %d values", width);
   float* pieces = (float*)workspace;  // first: read and written four at a time
-  int* ints = (int*)(pieces + 2LL * g.tiles * width);
-  int* keys[2] = {ints, ints + count};
-  int* places[2] = {ints + 2 * count, ints + 3 * count};
-  int *run_tiles = ints + 4 * count, *runs = run_tiles + g.tiles;
-  SortPlan s{(int)count, rows, g.passes, g.bits, padding, {keys[0], keys[1]}, {places[0], places[1]}, runs, dtable, (long long)rows * width};
+  int2* entries = (int2*)(pieces + 2LL * g.tiles * width);
+  int2* run_starts = entries + 2 * count;
+  int *run_ends = (int*)(run_starts + g.tiles), *runs = run_ends + rows;
+  SortPlan s{(int)count, rows, g.passes, g.bits, padding, {entries, entries + count}, runs, dtable, (long long)rows * width};
   if (int rc = kind == 0 ? sort_tokens<int>(tokens, s, g.ctas, st) : sort_tokens<long long>(tokens, s, g.ctas, st)) return rc;
-  const SumPlan p{keys[0], places[0], (int)count, rows, width, g.tile, g.lanes, g.groups, (float)scale, dy, dtable, pieces, runs, run_tiles};
+  const SumPlan p{entries, (int)count, rows, width, g.tile, g.lanes, g.groups, (float)scale, dy, dtable, pieces, runs, run_starts, run_ends};
   return four ? add_up<4>(p, g, st) : add_up<1>(p, g, st);
 }
