@@ -1,11 +1,8 @@
 // Embedding: out[i] = scale * table[token[i]], and the table's gradient: dtable[v] = scale * the sum of dy[i] over the tokens
 // that are v.  A token outside the table reads nothing: its row of the result is NaN, and the gradient leaves it out.
 #include "colreduce.cuh"
-#include <cooperative_groups.h>
 
 namespace {
-
-namespace cg = cooperative_groups;
 
 template <class T>
 __device__ __forceinline__ long long token_at(const void* tokens, long long i) { return (long long)static_cast<const T*>(tokens)[i]; }
@@ -73,22 +70,23 @@ int lookup(const void* tokens, long long count, int rows, int width, const float
 
 // ---------------------------------------------------------------- gradient: order the tokens
 
-// Least digits first, by one cluster of CTAs, so that a pass costs two barriers of the cluster and no launch.  A warp owns a stretch of
-// tokens and a row of counters, one for each digit; a token's place is what all smaller digits take, what its digit takes in the stretches before, and
-// its rank in its own.  The order among equal tokens is kept, so the sums below have the same bits every time.
-// The clusters behind the first clear the gradient meanwhile: rows that no token names stay so.
-// What bounds it: latency, and scattered stores, of which an SM takes one line a cycle.  So a token and its place travel as one 8-byte entry, and a CTA puts its
-// share in order in shared memory first and writes stretches of a digit.  SORTED_FIGURES
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kDigitBits = 9, kDigits = 1 << kDigitBits;
-constexpr int kSortAhead = 8, kSortCtas = 16, kStaged = 8192;
+// Least digits first.  A CTA has a share of the tokens, a warp of it a stretch and a row of counters, one for each digit; a token's place is what all
+// smaller digits take, what its digit takes in the shares and stretches before, and its rank in its own.  The order among equal tokens is
+// kept, so the sums below have the same bits every time.  Up to kOneCta tokens are ordered by one CTA in one launch; more by a launch that counts
+// the first digits and one for each pass, which counts the next pass's digits where it puts the tokens.
+// What bounds it: latency, the ranking's instructions (on the 16 SMs of one cluster, with barriers instead of
+// launches, 131072 tokens took 35 us) and scattered stores, of which an SM takes one line a cycle.  So all SMs take part, a token and its place
+// travel as one 8-byte entry, and a CTA puts its share in order in shared memory first and writes stretches of a digit.
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigitBits = 8, kDigits = 1 << kDigitBits;
+constexpr int kSortAhead = 4, kOneCta = kSortThreads * kSortAhead, kStaged = 8192;
 
 struct SortPlan {
   int count, rows, passes, bits;  // bits of a digit
+  int share_bits, ctas;           // tokens to a CTA: 1 << share_bits
   long long padding;
-  int2* entries[2];  // scratch, (token, place); the last pass leaves its result in the first
-  int* runs;         // cleared: how many long runs there are
-  float* dtable;
-  long long cells;
+  int2 *from, *to;  // scratch, (token, place)
+  int* table;       // scratch, [passes][ctas][digits]: how many of each digit a CTA's share has in each pass
+  int* runs;        // cleared: how many long runs there are
 };
 
 // The table's row of token i, or `rows` for those that count nothing.
@@ -98,135 +96,238 @@ __device__ __forceinline__ int key_of(const void* tokens, int i, const SortPlan&
   return t >= 0 && t < p.rows && t != p.padding ? (int)t : p.rows;
 }
 
-__device__ __forceinline__ void clear_cells(float* p, long long n, int block, int blocks) {
-  long long head = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) / 4 % 4;
-  if (head > n) head = n;
-  const long long tid = (long long)block * kSortThreads + threadIdx.x, step = (long long)blocks * kSortThreads;
-  if (tid < head) p[tid] = 0.f;
-  p += head;
-  n -= head;
-  for (long long v = tid; v < n / 4; v += step) st4(p + 4 * v, make_float4(0.f, 0.f, 0.f, 0.f));
-  if (tid < n % 4) p[n / 4 * 4 + tid] = 0.f;
+struct SortShared {
+  int counters[kSortWarps][kDigits];
+  unsigned lanes[kSortWarps][kDigits];  // 0 between two uses
+  int local[kDigits];     // where a digit begins in the CTA's own order
+  int shift_to[kDigits];  // from there to its place among all
+  int sums[2][kSortWarps];
+};
+
+// Exclusive sums over the digits of `a` and `b`, one digit a thread.  All threads call it; `sums` is free again after the next barrier.
+__device__ __forceinline__ void scan_digits(int& a, int& b, SortShared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int ua = a, ub = b;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int na = __shfl_up_sync(0xffffffffu, ua, o), nb = __shfl_up_sync(0xffffffffu, ub, o);
+    if (lane >= o) { ua += na; ub += nb; }
+  }
+  if (lane == 31) { sh.sums[0][warp] = ua; sh.sums[1][warp] = ub; }
+  __syncthreads();
+  ua -= a;
+  ub -= b;
+  for (int w = 0; w < warp; ++w) { ua += sh.sums[0][w]; ub += sh.sums[1][w]; }
+  a = ua;
+  b = ub;
+}
+
+// Turns the warps' counts of a digit into what the warps before have of it; the whole CTA's count.
+__device__ __forceinline__ int sum_warps(SortShared& sh, int digits) {
+  int total = 0;
+  if (threadIdx.x < digits) {
+    int n[kSortWarps];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) n[w] = sh.counters[w][threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      sh.counters[w][threadIdx.x] = total;
+      total += n[w];
+    }
+  }
+  return total;
+}
+
+// An entry's place in its CTA's order; advances the warp's counters.  All lanes call it; `in`: the lane has an entry.  The lanes with the same digit find one
+// another in a word of shared memory: 20 instructions, against 40 and more bit by bit with ballots, and some 500 cycles of __match_any_sync.
+__device__ __forceinline__ int place_of(bool in, int digit, int* mine, unsigned* lanes, const int* local) {
+  const int lane = threadIdx.x & 31;
+  if (in) atomicOr(lanes + digit, 1u << lane);
+  __syncwarp();
+  unsigned same = 0;
+  int place = 0;
+  if (in) {
+    same = lanes[digit];
+    place = mine[digit];
+  }
+  __syncwarp();
+  const int rank = __popc(same & ((1u << lane) - 1));
+  if (in && rank == 0) {
+    mine[digit] = place + __popc(same);
+    lanes[digit] = 0;
+  }
+  __syncwarp();
+  return in ? local[digit] + place + rank : 0;
 }
 
 template <class T>
-__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const void* __restrict__ tokens, SortPlan p) {
-  extern __shared__ int2 staged[];  // [kStaged], then counters [kSortWarps][kDigits], the CTA's totals of the digits, where they go
+__global__ void __launch_bounds__(kSortThreads) embedding_order_kernel(const void* __restrict__ tokens, SortPlan p) {
+  __shared__ SortShared sh;
+  extern __shared__ int2 staged[];  // [kOneCta]
   mtb_launch_dependents();
   mtb_wait_prior();
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = (int)cluster.num_blocks(), cta = (int)cluster.block_rank();
-  if (blockIdx.x >= ctas) {
-    clear_cells(p.dtable, p.cells, (int)blockIdx.x - ctas, (int)gridDim.x - ctas);
-    return;
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int *counters = (int*)(staged + kStaged), *mine = counters + warp * kDigits, *totals = counters + kSortWarps * kDigits;
-  int *local = totals + kDigits, *shift_to = local + kDigits, *sums = shift_to + kDigits;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
-  const int each = ((p.count + ctas * kSortWarps - 1) / (ctas * kSortWarps) + 31) / 32 * 32;
-  auto bounded = [&](long long i) { return (int)(i < p.count ? i : p.count); };
-  const int lo = bounded((long long)(cta * kSortWarps + warp) * each), hi = bounded((long long)(cta * kSortWarps + warp + 1) * each);
-  const int share = bounded((long long)(cta + 1) * kSortWarps * each) - bounded((long long)cta * kSortWarps * each);
-  const unsigned below = (1u << lane) - 1;
-  const bool held = each <= 32 * kSortAhead, stage = share <= kStaged;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, lo = warp * 32 * kSortAhead + lane;
+  if (threadIdx.x == 0) *p.runs = 0;
+  for (int i = threadIdx.x; i < kSortWarps * kDigits / 4; i += kSortThreads) ((int4*)sh.lanes)[i] = make_int4(0, 0, 0, 0);
+  int2 entry[kSortAhead];
+#pragma unroll
+  for (int u = 0; u < kSortAhead; ++u)
+    if (lo + 32 * u < p.count) entry[u] = make_int2(key_of<T>(tokens, lo + 32 * u, p), lo + 32 * u);
   for (int pass = 0; pass < p.passes; ++pass) {
-    const int to = (p.passes - 1 - pass) & 1, shift = pass * p.bits, digits = 1 << p.bits;
-    for (int i = threadIdx.x; i < kSortWarps * kDigits / 4; i += kSortThreads) ((int4*)counters)[i] = make_int4(0, 0, 0, 0);
+    const int shift = pass * p.bits;
+    for (int i = threadIdx.x; i < kSortWarps * kDigits / 4; i += kSortThreads) ((int4*)sh.counters)[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    int2 entry[kSortAhead];
-    auto load = [&](int i0) {
 #pragma unroll
-      for (int u = 0; u < kSortAhead; ++u) {
-        const int i = i0 + 32 * u + lane;
-        // what other CTAs wrote is read past the L1 cache
-        if (i < hi) entry[u] = pass ? __ldcg(p.entries[to ^ 1] + i) : make_int2(key_of<T>(tokens, i, p), i);
-      }
-    };
-    for (int i0 = lo; i0 < hi; i0 += 32 * kSortAhead) {
-      load(i0);
-#pragma unroll
-      for (int u = 0; u < kSortAhead; ++u)
-        if (i0 + 32 * u + lane < hi) atomicAdd(mine + (entry[u].x >> shift & (digits - 1)), 1);
-    }
+    for (int u = 0; u < kSortAhead; ++u)
+      if (lo + 32 * u < p.count) atomicAdd(&sh.counters[warp][entry[u].x >> shift & (digits - 1)], 1);
     __syncthreads();
-    int total = 0;
-    if (threadIdx.x < digits) {
-      for (int w0 = 0; w0 < kSortWarps; w0 += 16) {
-        int n[16];
-#pragma unroll
-        for (int w = 0; w < 16; ++w) n[w] = counters[(w0 + w) * kDigits + threadIdx.x];
-#pragma unroll
-        for (int w = 0; w < 16; ++w) {
-          counters[(w0 + w) * kDigits + threadIdx.x] = total;
-          total += n[w];
-        }
-      }
-      totals[threadIdx.x] = total;
-    }
-    cluster.sync();
-    int before = 0, all = 0;
-    if (threadIdx.x < digits) {
-#pragma unroll
-      for (int r = 0; r < kSortCtas; ++r) {
-        const int n = r < ctas ? cluster.map_shared_rank(totals, r)[threadIdx.x] : 0;
-        if (r < cta) before += n;
-        all += n;
-      }
-    }
-    int upto_all = all, upto_total = total;  // inclusive over the digits
-    for (int o = 1; o < 32; o <<= 1) {
-      const int a = __shfl_up_sync(0xffffffffu, upto_all, o), b = __shfl_up_sync(0xffffffffu, upto_total, o);
-      if (lane >= o) { upto_all += a; upto_total += b; }
-    }
-    if (lane == 31) { sums[warp] = upto_all; sums[kSortWarps + warp] = upto_total; }
+    int total = sum_warps(sh, digits), unused = 0;
+    scan_digits(total, unused, sh);
+    if (threadIdx.x < digits) sh.local[threadIdx.x] = total;
     __syncthreads();
-    if (threadIdx.x < digits) {
-      int offset = upto_all - all + before, here = upto_total - total;
-      for (int w = 0; w < warp; ++w) { offset += sums[w]; here += sums[kSortWarps + w]; }
-      local[threadIdx.x] = here;
-      shift_to[threadIdx.x] = offset - here;
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      if (lo - lane + 32 * u < p.count) {
+        const bool in = lo + 32 * u < p.count;
+        const int place = place_of(in, entry[u].x >> shift & (digits - 1), sh.counters[warp], sh.lanes[warp], sh.local);
+        if (in) staged[place] = entry[u];
+      }
     }
     __syncthreads();
-    for (int i0 = lo; i0 < hi; i0 += 32 * kSortAhead) {
-      if (!held) load(i0);
 #pragma unroll
-      for (int u = 0; u < kSortAhead; ++u) {
-        if (i0 + 32 * u >= hi) break;
-        const bool in = i0 + 32 * u + lane < hi;
-        const int d = entry[u].x >> shift & (digits - 1);
-        // the lanes with the same digit, bit by bit (__match_any_sync took some 500 cycles for 32 different ones)
-        unsigned same = __ballot_sync(0xffffffffu, in);
-#pragma unroll
-        for (int b = 0; b < kDigitBits; ++b) {
-          const unsigned set = __ballot_sync(0xffffffffu, d >> b & 1);
-          same &= d >> b & 1 ? set : ~set;
-        }
-        int taken = 0;
-        if (in) taken = mine[d];
-        __syncwarp();
-        if (in) {
-          const int place = local[d] + taken + __popc(same & below);
-          if (stage) staged[place] = entry[u];
-          else p.entries[to][place + shift_to[d]] = entry[u];
-          if (!(same & below)) mine[d] = taken + __popc(same);
-        }
-        __syncwarp();
-      }
-    }
-    if (stage) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < share; i += kSortThreads) {
-        const int2 e = staged[i];
-        p.entries[to][i + shift_to[e.x >> shift & (digits - 1)]] = e;
-      }
-    }
-    cluster.sync();  // also makes this pass's entries visible to the others
+    for (int u = 0; u < kSortAhead; ++u)
+      if (lo + 32 * u < p.count) entry[u] = staged[lo + 32 * u];
   }
+#pragma unroll
+  for (int u = 0; u < kSortAhead; ++u)
+    if (lo + 32 * u < p.count) p.to[lo + 32 * u] = entry[u];
+}
+
+template <class T>
+__global__ void __launch_bounds__(kSortThreads) embedding_count_kernel(const void* __restrict__ tokens, SortPlan p) {
+  __shared__ int counts[kDigits];
+  mtb_launch_dependents();
+  mtb_wait_prior();
+  const int digits = 1 << p.bits, lo = blockIdx.x << p.share_bits, stop = lo + (1 << p.share_bits), hi = stop < p.count ? stop : p.count;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.runs = 0;
+  if (threadIdx.x < digits) counts[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i0 = lo + threadIdx.x; i0 < hi; i0 += kSortThreads * kSortAhead) {
+    int k[kSortAhead];
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u)
+      if (i0 + u * kSortThreads < hi) k[u] = key_of<T>(tokens, i0 + u * kSortThreads, p);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u)
+      if (i0 + u * kSortThreads < hi) atomicAdd(counts + (k[u] & (digits - 1)), 1);
+  }
+  __syncthreads();
+  if (threadIdx.x < digits) {
+    int* row = p.table + blockIdx.x * digits + threadIdx.x;
+    *row = counts[threadIdx.x];
+    for (int pass = 1; pass < p.passes; ++pass) row[pass * p.ctas * digits] = 0;
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kSortThreads) embedding_place_kernel(const void* __restrict__ tokens, SortPlan p, int pass) {
+  __shared__ SortShared sh;
+  extern __shared__ int2 staged[];
+  mtb_launch_dependents();
+  mtb_wait_prior();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << p.bits, shift = pass * p.bits;
+  const int first = blockIdx.x << p.share_bits, each = 1 << p.share_bits >> 4;  // a warp's stretch
+  static_assert(kSortWarps == 16, "a stretch is a sixteenth of a share");
+  auto bounded = [&](int i) { return i < p.count ? i : p.count; };
+  const int lo = bounded(first + warp * each), hi = bounded(first + (warp + 1) * each), share = bounded(first + (1 << p.share_bits)) - first;
+  const bool held = each <= 32 * kSortAhead, stage = share <= kStaged;
+  for (int i = threadIdx.x; i < kSortWarps * kDigits / 4; i += kSortThreads) ((int4*)sh.counters)[i] = make_int4(0, 0, 0, 0);
+  __syncthreads();
+  int2 entry[kSortAhead];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const int i = i0 + 32 * u + lane;
+      if (i < hi) entry[u] = pass ? p.from[i] : make_int2(key_of<T>(tokens, i, p), i);
+    }
+  };
+  for (int i0 = lo; i0 < hi; i0 += 32 * kSortAhead) {
+    load(i0);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u)
+      if (i0 + 32 * u + lane < hi) atomicAdd(&sh.counters[warp][entry[u].x >> shift & (digits - 1)], 1);
+  }
+  // The shares before, and all of them: four digits a thread, an eighth of the shares each.  A CTA begins at its own, since all of them at
+  // the same lines wait for one another.
+  constexpr int kParts = kSortThreads * 4 / kDigits;
+  static_assert(2 * kParts == kSortWarps, "the parts' sums take the place of the lanes' words");
+  int(*of_part)[kDigits] = (int(*)[kDigits])sh.lanes;
+  const int quad = threadIdx.x % (kDigits / 4), part = threadIdx.x / (kDigits / 4);
+  const int* table = p.table + pass * p.ctas * digits;
+  if (quad * 4 < digits) {
+    int4 before = make_int4(0, 0, 0, 0), all = before;
+    for (int i0 = part; i0 < p.ctas; i0 += kParts * 8) {
+      int4 n[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        int c = i0 + kParts * u + blockIdx.x;
+        if (c >= p.ctas) c -= p.ctas;
+        n[u] = i0 + kParts * u < p.ctas ? *(const int4*)(table + c * digits + 4 * quad) : make_int4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        all.x += n[u].x; all.y += n[u].y; all.z += n[u].z; all.w += n[u].w;
+        if (i0 + kParts * u + blockIdx.x >= p.ctas) { before.x += n[u].x; before.y += n[u].y; before.z += n[u].z; before.w += n[u].w; }
+      }
+    }
+    *(int4*)(of_part[part] + 4 * quad) = before;
+    *(int4*)(of_part[kParts + part] + 4 * quad) = all;
+  }
+  __syncthreads();
+  int total = sum_warps(sh, digits), begin = total, before = 0, all = 0;
+  if (threadIdx.x < digits) {
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) {
+      before += of_part[u][threadIdx.x];
+      all += of_part[kParts + u][threadIdx.x];
+    }
+  }
+  scan_digits(all, begin, sh);  // the parts' sums are read
+  for (int i = threadIdx.x; i < kSortWarps * kDigits / 4; i += kSortThreads) ((int4*)sh.lanes)[i] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x < digits) {
+    sh.local[threadIdx.x] = begin;
+    sh.shift_to[threadIdx.x] = all + before - begin;
+  }
+  __syncthreads();
+  int* next = p.table + (pass + 1) * p.ctas * digits;
+  auto put = [&](int2 e, int place) {
+    const int at = place + sh.shift_to[e.x >> shift & (digits - 1)];
+    p.to[at] = e;
+    if (pass + 1 < p.passes) atomicAdd(next + (at >> p.share_bits) * digits + (e.x >> (shift + p.bits) & (digits - 1)), 1);
+  };
+  for (int i0 = lo; i0 < hi; i0 += 32 * kSortAhead) {
+    if (!held) load(i0);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      if (i0 + 32 * u < hi) {
+        const bool in = i0 + 32 * u + lane < hi;
+        const int place = place_of(in, entry[u].x >> shift & (digits - 1), sh.counters[warp], sh.lanes[warp], sh.local);
+        if (in) {
+          if (stage) staged[place] = entry[u];
+          else put(entry[u], place);
+        }
+      }
+    }
+  }
+  if (!stage) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < share; i += kSortThreads) put(staged[i], i);
 }
 
 // ---------------------------------------------------------------- gradient: add up
 
+// Rows of the table that no token names are cleared by CTAs of their own, 32 rows a warp.  (Clearing the whole table while the tokens are put in order costs more:
+// 102 MB of it take longer than that, and half of them are written again: 131072 tokens, 50000 x 512: 115 us, 104 this way.)
+//
 // The ordered tokens are cut into tiles of `tile`.  A run of equal tokens of up to kRun is added up by the tile it begins in, past the tile's end if need be,
 // and goes to the table; a longer one is added up piece by piece, each tile its own, and the pieces are added by the kernel behind, in
 // their order.  Frequent tokens thus keep no tile waiting, and the rest has no second step.
@@ -235,6 +336,7 @@ constexpr int kRun = 32, kMaxTile = kRun, kSumAhead = 8;  // a longer tile could
 struct SumPlan {
   const int2* entries;
   int count, rows, width, tile, lanes, groups;  // threads to a tile, tiles to a CTA
+  int clearing;                                 // CTAs that clear rows, in front of the others
   float scale;
   const float* dy;
   float* dtable;
@@ -244,6 +346,29 @@ struct SumPlan {
   int* run_ends;          // [rows]: the tile that a long run of this token ends in
 };
 
+// Whether an ordered entry names `row`.
+__device__ __forceinline__ bool is_named(const SumPlan& p, int row) {
+  int lo = 0, hi = p.count;  // the first entry not below `row` is in [lo, hi]
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (p.entries[mid].x < row) lo = mid + 1; else hi = mid;
+  }
+  return lo < p.count && p.entries[lo].x == row;
+}
+
+template <int V>
+__device__ __forceinline__ void clear_rows(const SumPlan& p, int block) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x / 32, row = (block * warps + threadIdx.x / 32) * 32 + lane;
+  VecF<V> zero;
+#pragma unroll
+  for (int i = 0; i < V; ++i) zero.v[i] = 0.f;
+  unsigned bare = __ballot_sync(0xffffffffu, row < p.rows && !is_named(p, row));
+  for (; bare; bare &= bare - 1) {
+    float* to = p.dtable + (long long)(row - lane + __ffs(bare) - 1) * p.width;
+    for (int col = lane * V; col < p.width; col += 32 * V) vstore<V>(to + col, zero);
+  }
+}
+
 template <int V>
 __global__ void __launch_bounds__(128) embedding_sum_kernel(SumPlan p) {
   // keys from kRun before a tile to kRun behind it; one more on either side tells where a run ends
@@ -251,8 +376,12 @@ __global__ void __launch_bounds__(128) embedding_sum_kernel(SumPlan p) {
   extern __shared__ int shared[];
   mtb_launch_dependents();
   mtb_wait_prior();
+  if (blockIdx.x < p.clearing) {
+    if (blockIdx.y == 0) clear_rows<V>(p, blockIdx.x);
+    return;
+  }
   const int group = threadIdx.x / p.lanes, lane = threadIdx.x - group * p.lanes;
-  const int t0 = (blockIdx.x * p.groups + group) * p.tile;
+  const int t0 = ((blockIdx.x - p.clearing) * p.groups + group) * p.tile;
   int *keys = shared + group * 2 * kSpan, *places = keys + kSpan;
   if (t0 < p.count) {
     for (int j = lane; j < p.tile + 2 * kRun + 2; j += p.lanes) {
@@ -379,19 +508,22 @@ __global__ void __launch_bounds__(kJoinThreads, 5) embedding_join_kernel(SumPlan
 }
 
 struct GradPlan {
-  int passes, bits, ctas, tile, tiles, lanes, groups, columns;
+  int passes, bits, ctas, share_bits, tile, tiles, lanes, groups, columns;
   long long bytes;
 };
 
-// Scratch: two sets of entries, the long runs' starts and ends, the pieces.
+// Scratch: two sets of entries, the digits' counts, the long runs' starts and ends, the pieces.
 GradPlan plan_gradient(long long count, int rows, int width, bool four) {
   GradPlan g{};
-  int bits = 1;
+  int bits = 2;  // digits are read four at a time
   while ((1LL << bits) <= rows) ++bits;  // the largest key is `rows`
   g.passes = (bits + kDigitBits - 1) / kDigitBits;
   g.bits = (bits + g.passes - 1) / g.passes;
-  g.ctas = 1;
-  while (g.ctas < kSortCtas && count > (long long)g.ctas * kSortThreads) g.ctas *= 2;
+  g.ctas = g.share_bits = 0;
+  if (count > kOneCta) {
+    for (g.share_bits = 9; (count >> g.share_bits) >= mtb_sm_count();) ++g.share_bits;
+    g.ctas = (int)((count + (1LL << g.share_bits) - 1) >> g.share_bits);
+  }
   const int vectors = four ? width / 4 : width;
   g.lanes = 4;
   while (g.lanes < vectors && g.lanes < 32) g.lanes *= 2;
@@ -402,46 +534,36 @@ GradPlan plan_gradient(long long count, int rows, int width, bool four) {
   g.tile = 8;
   while (g.tile < kMaxTile && count / (2LL * g.tile * g.groups) * g.columns >= mtb_sm_count() * 16LL) g.tile *= 2;
   g.tiles = (int)((count + g.tile - 1) / g.tile);
-  g.bytes = 16 * count + 4LL * rows + 8LL * g.tiles + 512 + 8LL * g.tiles * width;
+  g.bytes = 16 * count + 4LL * g.passes * g.ctas * kDigits + 4LL * rows + 8LL * g.tiles + 512 + 8LL * g.tiles * width;
   return g;
 }
 
 template <class T>
-int sort_tokens(const void* tokens, const SortPlan& p, int ctas, cudaStream_t st) {
-  static unsigned long long opted;
-  constexpr int smem = kStaged * 8 + (kSortWarps * kDigits + 3 * kDigits + 2 * kSortWarps) * 4;
-  if (int rc = mtb_opt_in_smem((const void*)embedding_sort_kernel<T>, smem, &opted)) return rc;
-  static unsigned long long wide;
-  int device = 0;
-  MTB_CUDA(cudaGetDevice(&device));
-  if (device >= 64 || !((__atomic_load_n(&wide, __ATOMIC_ACQUIRE) >> device) & 1ull)) {
-    MTB_CUDA(cudaFuncSetAttribute((const void*)embedding_sort_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    if (device < 64) __atomic_fetch_or(&wide, 1ull << device, __ATOMIC_RELEASE);
+int sort_tokens(const void* tokens, SortPlan p, int2* entries, cudaStream_t st) {
+  if (p.ctas == 0) {
+    static unsigned long long opted;
+    if (int rc = mtb_opt_in_smem((const void*)embedding_order_kernel<T>, kOneCta * 8, &opted)) return rc;
+    p.to = entries;
+    MTB_LAUNCH(embedding_order_kernel<T>, 1, kSortThreads, kOneCta * 8, st, tokens, p);
+    return MTB_OK;
   }
-  cudaLaunchConfig_t cfg = {};
-  const long long clear = (p.cells + 4LL * kSortThreads * 4 - 1) / (4LL * kSortThreads * 4);  // four vectors a thread
-  long long blocks = mtb_sm_count() / ctas * ctas - ctas;
-  if (clear < blocks) blocks = (clear + ctas - 1) / ctas * ctas;
-  cfg.gridDim = dim3((unsigned)(ctas + (blocks < ctas ? ctas : blocks)));
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ctas;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  MTB_CUDA(cudaLaunchKernelEx(&cfg, embedding_sort_kernel<T>, tokens, p));
+  static unsigned long long opted;
+  if (int rc = mtb_opt_in_smem((const void*)embedding_place_kernel<T>, kStaged * 8, &opted)) return rc;
+  MTB_LAUNCH(embedding_count_kernel<T>, p.ctas, kSortThreads, 0, st, tokens, p);
+  const int smem = (1 << p.share_bits) <= kStaged ? 8 << p.share_bits : 0;
+  for (int pass = 0; pass < p.passes; ++pass) {  // the last one's result is the first set
+    const bool second = (p.passes - 1 - pass) & 1;
+    p.to = entries + (second ? p.count : 0);
+    p.from = entries + (second ? 0 : p.count);
+    MTB_LAUNCH(embedding_place_kernel<T>, p.ctas, kSortThreads, smem, st, tokens, p, pass);
+  }
   return MTB_OK;
 }
 
 template <int V>
 int add_up(const SumPlan& p, const GradPlan& g, cudaStream_t st) {
   const int smem = g.groups * 2 * (kMaxTile + 2 * kRun + 2) * 4;
-  MTB_LAUNCH(embedding_sum_kernel<V>, dim3(mtb_div_up(g.tiles, g.groups), g.columns), g.lanes * g.groups, smem, st, p);
+  MTB_LAUNCH(embedding_sum_kernel<V>, dim3(p.clearing + mtb_div_up(g.tiles, g.groups), g.columns), g.lanes * g.groups, smem, st, p);
   if (p.count > kRun) MTB_LAUNCH(embedding_join_kernel<V>, mtb_sm_count() * 5, kJoinThreads, 0, st, p);
   return MTB_OK;
 }
@@ -478,12 +600,13 @@ MTB_API int mtb_embedding_backward_f32(int kind, const void* tokens, long long c
   const bool four = width % 4 == 0 && mtb_aligned16(dy) && mtb_aligned16(dtable) && mtb_aligned16(workspace);
   const GradPlan g = plan_gradient(count, rows, width, four);
   MTB_REQUIRE(g.columns < 65536, "embedding_backward: rows of %d values", width);
-  float* pieces = (float*)workspace;  // first: read and written four at a time
+  int* table = (int*)workspace;  // read four at a time, like the pieces
+  float* pieces = (float*)(table + g.passes * g.ctas * (1 << g.bits));
   int2* entries = (int2*)(pieces + 2LL * g.tiles * width);
   int2* run_starts = entries + 2 * count;
   int *run_ends = (int*)(run_starts + g.tiles), *runs = run_ends + rows;
-  SortPlan s{(int)count, rows, g.passes, g.bits, padding, {entries, entries + count}, runs, dtable, (long long)rows * width};
-  if (int rc = kind == 0 ? sort_tokens<int>(tokens, s, g.ctas, st) : sort_tokens<long long>(tokens, s, g.ctas, st)) return rc;
-  const SumPlan p{entries, (int)count, rows, width, g.tile, g.lanes, g.groups, (float)scale, dy, dtable, pieces, runs, run_starts, run_ends};
+  const SortPlan s{(int)count, rows, g.passes, g.bits, g.share_bits, g.ctas, padding, nullptr, nullptr, table, runs};
+  if (int rc = kind == 0 ? sort_tokens<int>(tokens, s, entries, st) : sort_tokens<long long>(tokens, s, entries, st)) return rc;
+  const SumPlan p{entries, (int)count, rows, width, g.tile, g.lanes, g.groups, mtb_div_up(rows, g.lanes * g.groups), (float)scale, dy, dtable, pieces, runs, run_starts, run_ends};
   return four ? add_up<4>(p, g, st) : add_up<1>(p, g, st);
 }
