@@ -209,10 +209,11 @@ int mtb_batch_norm2d_backward_f32(int n, int c, int h, int w, const float* dy, c
 /* ---- GroupNorm with an activation behind it (no counterpart in the reference) ----
  * x, y, dy, dx: channels-last [n][hw][c]; mean, rstd: [n][groups], of the c / groups channels of a group at all positions of an image, the variance the
  * biased one; y = f(gamma (x - mean) rstd + beta).  activation f: 0 none, 1 ReLU (its gradient passes zero, as mtb_relu_backward_f32 does),
- * 2 SiLU z / (1 + exp(-z)).  gamma, beta may be NULL (1, 0).  Backward: dx, dgamma and dbeta may be NULL each. */
+ * 2 SiLU z / (1 + exp(-z)).  gamma, beta may be NULL (1, 0).  Backward: dx, dgamma and dbeta may be NULL each.
+ * The forward's workspace is read only for images that do not fit on the chip; it may be NULL where they do. */
 long long mtb_group_norm_workspace_bytes(int n, int c, int hw, int groups);
 int mtb_group_norm_forward_f32(int n, int c, int hw, int groups, const float* x, const float* gamma, const float* beta, double eps, int activation, float* y,
-                               float* mean, float* rstd, void* stream);
+                               float* mean, float* rstd, void* workspace, long long workspace_bytes, void* stream);
 int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const float* dy, const float* mean, const float* rstd, const float* x, const float* gamma,
                                 const float* beta, int activation, float* dx, float* dgamma, float* dbeta, void* workspace, long long workspace_bytes,
                                 void* stream);

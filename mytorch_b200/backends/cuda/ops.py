@@ -633,7 +633,8 @@ def cuda_group_norm(x, num_groups, weight, bias, eps, activation):
     env = _env(x)
     n, c, hw = _image_extents(x)
     y, mean, rstd = _new(x.shape, x), _new((n, num_groups), x), _new((n, num_groups), x)
-    env.lib.group_norm_forward_f32(n, c, hw, num_groups, x, weight, bias, float(eps), _ACTIVATIONS[activation], y, mean, rstd, env.stream())
+    ws, ws_bytes = env.workspace(env.lib.group_norm_workspace_bytes(n, c, hw, num_groups))
+    env.lib.group_norm_forward_f32(n, c, hw, num_groups, x, weight, bias, float(eps), _ACTIVATIONS[activation], y, mean, rstd, ws, ws_bytes, env.stream())
     return y, mean, rstd
 
 

@@ -80,11 +80,11 @@ def test_entry_points_refuse_bad_arguments():
     lib, a = _binding, ADDRESS
     big = 1 << 40
     refused = [
-        lambda: lib.group_norm_forward_f32(2, 8, 9, 3, a, a, a, 1e-5, 0, a, a, a, None),
-        lambda: lib.group_norm_forward_f32(2, 8, 9, 0, a, a, a, 1e-5, 0, a, a, a, None),
-        lambda: lib.group_norm_forward_f32(-1, 8, 9, 2, a, a, a, 1e-5, 0, a, a, a, None),
-        lambda: lib.group_norm_forward_f32(2, 8, 9, 2, a, a, a, 1e-5, 3, a, a, a, None),
-        lambda: lib.group_norm_forward_f32(2, 8, 9, 2, None, a, a, 1e-5, 0, a, a, a, None),
+        lambda: lib.group_norm_forward_f32(2, 8, 9, 3, a, a, a, 1e-5, 0, a, a, a, a, big, None),
+        lambda: lib.group_norm_forward_f32(2, 8, 9, 0, a, a, a, 1e-5, 0, a, a, a, a, big, None),
+        lambda: lib.group_norm_forward_f32(-1, 8, 9, 2, a, a, a, 1e-5, 0, a, a, a, a, big, None),
+        lambda: lib.group_norm_forward_f32(2, 8, 9, 2, a, a, a, 1e-5, 3, a, a, a, a, big, None),
+        lambda: lib.group_norm_forward_f32(2, 8, 9, 2, None, a, a, 1e-5, 0, a, a, a, a, big, None),
         lambda: lib.group_norm_backward_f32(2, 8, 9, 3, a, a, a, a, a, a, 0, a, a, a, a, big, None),
         lambda: lib.group_norm_backward_f32(2, 8, 9, 2, a, a, a, a, a, a, -1, a, a, a, a, big, None),
         lambda: lib.group_norm_backward_f32(2, 8, 9, 2, None, a, a, a, a, a, 0, a, a, a, a, big, None),
@@ -105,5 +105,5 @@ def test_entry_points_refuse_bad_arguments():
         with pytest.raises(NativeError):
             call()
     # over no elements: nothing to do, and no GPU needed
-    assert lib.group_norm_forward_f32(0, 8, 9, 2, None, None, None, 1e-5, 0, None, None, None, None) == 0
+    assert lib.group_norm_forward_f32(0, 8, 9, 2, None, None, None, 1e-5, 0, None, None, None, None, 0, None) == 0
     assert lib.embedding_forward_f32(1, None, 0, 10, 4, None, 1.0, None, None) == 0
