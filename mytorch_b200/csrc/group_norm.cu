@@ -6,9 +6,11 @@
 // A = sum gamma dz, B = sum gamma dz xh over the group.
 //
 // HBM-bound: 8 bytes a value forward, 12 backward, if the values stay on the chip between the sums and what is made of them.  So a cluster of CTAs holds
-// a slab, some whole groups of one image (32 channels or more: a line of memory), in its shared memory, each CTA a stretch of positions.  A thread copies (cp.async) and later
-// reads its own vectors only, so the copies need no barrier; the CTAs exchange their sums through distributed shared memory.  A slab that no
-// cluster can hold goes through memory twice instead, see the kernels at the end.
+// a slab, some whole groups of one image, in its shared memory, each CTA a stretch of the positions; four CTAs or so on an SM, one of which loads
+// while another one adds up or stores.  A thread copies (cp.async) and later reads its own vectors only, so the copies need no barrier; the CTAs exchange their sums
+// through distributed shared memory.
+// SLAB_FIGURES
+// A slab that no cluster can hold goes through memory twice instead, see the kernels at the end.
 #include "colreduce.cuh"
 #include <cooperative_groups.h>
 
@@ -50,6 +52,65 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 
 template <int V> struct alignas(4 * V) Vec { float v[V]; };
 template <int V> __device__ __forceinline__ Vec<V>& vec(float* p) { return *reinterpret_cast<Vec<V>*>(p); }
+template <int V> __device__ __forceinline__ Vec<V> all(float x) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = x;
+  return r;
+}
+// Two values an instruction: arithmetic would otherwise take as long as memory does.
+#define MTB_PAIRS(name, op, scalar)                                                                                                     \
+  template <int V> __device__ __forceinline__ Vec<V> name(Vec<V> a, Vec<V> b) {                                                         \
+    Vec<V> r;                                                                                                                           \
+    if constexpr (V == 1) r.v[0] = scalar(a.v[0], b.v[0]);                                                                              \
+    else                                                                                                                                \
+      for (int i = 0; i < V; i += 2)                                                                                                    \
+        asm("{.reg .b64 a, b, r; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; " op ".rn.f32x2 r, a, b; mov.b64 {%0, %1}, r;}"              \
+            : "=f"(r.v[i]), "=f"(r.v[i + 1]) : "f"(a.v[i]), "f"(a.v[i + 1]), "f"(b.v[i]), "f"(b.v[i + 1]));                             \
+    return r;                                                                                                                           \
+  }
+MTB_PAIRS(add, "add", __fadd_rn)
+MTB_PAIRS(mul, "mul", __fmul_rn)
+#undef MTB_PAIRS
+template <int V> __device__ __forceinline__ Vec<V> fma(Vec<V> a, Vec<V> b, Vec<V> c) {
+  Vec<V> r;
+  if constexpr (V == 1) r.v[0] = fmaf(a.v[0], b.v[0], c.v[0]);
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      asm("{.reg .b64 a, b, c, r; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 r, a, b, c; mov.b64 {%0, %1}, r;}"
+          : "=f"(r.v[i]), "=f"(r.v[i + 1])
+          : "f"(a.v[i]), "f"(a.v[i + 1]), "f"(b.v[i]), "f"(b.v[i + 1]), "f"(c.v[i]), "f"(c.v[i + 1]));
+  return r;
+}
+// 1 / (1 + e^-z) as 1 / (1 + 2^(-z log2 e)), by the approximate power and reciprocal of the hardware: off by about 2^-21 of itself, next to the error of a
+// normalisation in z
+template <int V> __device__ __forceinline__ Vec<V> sigmoid(Vec<V> z) {
+  Vec<V> e = mul(z, all<V>(-1.4426950408889634f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.v[i]));
+  e = add(e, all<V>(1.f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.v[i]));
+  return e;
+}
+template <int V, int ACT> __device__ __forceinline__ Vec<V> activated(Vec<V> z) {
+  if (ACT == ACT_SILU) return mul(z, sigmoid(z));
+  if (ACT == ACT_RELU)
+#pragma unroll
+    for (int i = 0; i < V; ++i) z.v[i] = z.v[i] < 0.f ? 0.f : z.v[i];
+  return z;
+}
+template <int V, int ACT> __device__ __forceinline__ Vec<V> activated_grad(Vec<V> dy, Vec<V> z) {
+  if (ACT == ACT_SILU) {
+    const Vec<V> s = sigmoid(z);
+    return mul(dy, fma(mul(s, z), fma(s, all<V>(-1.f), all<V>(1.f)), s));
+  }
+  if (ACT == ACT_RELU)
+#pragma unroll
+    for (int i = 0; i < V; ++i) dy.v[i] = z.v[i] < 0.f ? 0.f : dy.v[i];
+  return dy;
+}
 
 // ---------------------------------------------------------------- a slab on the chip
 
@@ -57,262 +118,331 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 
 struct Slabs {
   int hw, c, groups, each;  // channels of a group
-  int wide, slabs;          // channels of a slab (the last one may have fewer), slabs of an image
+  int wide, slabs, units;   // channels of a slab (the last of an image may have fewer), slabs of an image, of all images
+  int of_slab;              // groups of a slab
   int ctas, stretch;        // CTAs of a cluster, positions of a CTA
+  int lanes, rows;          // threads to a position (its vectors, up to a power of two), positions that the CTA's threads take at a time
+  int lane_bits, row_bits;  // of the two
   int steps;                // positions of a thread at most
-  int sums;                 // floats of shared memory between the values and what the other CTAs read
-  PoolDiv by_each;
+  // A slot is what a warp makes of its rows, or a row of more than a warp.  Where a thread's channels are of several groups it has several entries in it; `merged`
+  // lanes' entries are made one, and a group has `entries` of them.
+  int of_vector, entries, merged, slots, slot_rows;
+  bool vectors;                    // gamma and beta can be read as the values are
+  float inv_positions, inv_group;  // 1 / hw, 1 / M
+  PoolDiv by_slabs, by_each, by_groups;
 };
 
-// What a CTA and a thread of it have to do.
+// What a thread has to do.
+template <int V>
 struct Share {
-  int n, c0, width, vectors, rows;  // image, first channel, channels; vectors of a position, positions a step
-  int row, col, positions, steps;   // a thread's position within a step and its channels' offset; positions of the CTA, steps of the thread
-  long long first;                  // of the thread's values
-  template <int V>
-  __device__ __forceinline__ void of(const Slabs& p, int unit, int rank) {
-    n = unit / p.slabs;
-    c0 = (unit - n * p.slabs) * p.wide;
+  int rank, row, col, full, more;  // CTA of the cluster; position within a step, first channel; steps of all rows, rows with one more
+  int positions, steps;            // of the CTA, of the thread
+  int group[V];                    // of each channel, within the slab
+  __device__ __forceinline__ Share(const Slabs& p, int rank_) : rank(rank_) {
+    row = threadIdx.x >> p.lane_bits;
+    col = (threadIdx.x & (p.lanes - 1)) * V;
+    const int left = p.hw - rank * p.stretch;
+    positions = p.stretch < left ? p.stretch : left;
+    full = positions >> p.row_bits;
+    more = positions & (p.rows - 1);
+    steps = full + (row < more ? 1 : 0);
+    unsigned in;
+    group[0] = (int)p.by_each.divmod((unsigned)col, in);
+#pragma unroll
+    for (int i = 1; i < V; ++i) {
+      const bool next = ++in == (unsigned)p.each;
+      group[i] = group[i - 1] + (next ? 1 : 0);
+      if (next) in = 0;
+    }
+  }
+  __device__ __forceinline__ int slot(const Slabs& p) const { return p.lanes < 32 ? threadIdx.x >> 5 : row; }
+  __device__ __forceinline__ int of_slot(const Slabs& p, int slot) const {  // positions
+    const int extra = more - slot * p.slot_rows;
+    return full * p.slot_rows + (extra < 0 ? 0 : extra < p.slot_rows ? extra : p.slot_rows);
+  }
+};
+struct Unit {
+  int n, c0, width, groups;  // image, first channel, channels, their groups
+  __device__ __forceinline__ Unit(const Slabs& p, int unit) {
+    unsigned slab;
+    n = (int)p.by_slabs.divmod((unsigned)unit, slab);
+    c0 = (int)slab * p.wide;
     width = p.wide < p.c - c0 ? p.wide : p.c - c0;
-    vectors = width / V;
-    rows = kThreads / vectors;
-    row = threadIdx.x / vectors;
-    col = (threadIdx.x - row * vectors) * V;
-    const int p0 = rank * p.stretch;
-    positions = p.stretch < p.hw - p0 ? p.stretch : p.hw - p0;
-    steps = row < rows && row < positions ? (positions - row - 1) / rows + 1 : 0;
-    first = ((long long)n * p.hw + p0 + row) * p.c + c0 + col;
+    groups = p.of_slab < p.groups - (int)slab * p.of_slab ? p.of_slab : p.groups - (int)slab * p.of_slab;
+  }
+  // of the thread's first value
+  template <int V>
+  __device__ __forceinline__ long long first(const Slabs& p, const Share<V>& s) const {
+    return ((long long)n * p.hw + s.rank * p.stretch + s.row) * p.c + c0 + s.col;
   }
 };
 
-// The sum of `part` [rows][width] over a group's channels, by a warp.
-__device__ __forceinline__ float sum_group(const float* part, const Share& s, const Slabs& p, int g) {
-  float sum = 0.f;
-  for (unsigned q = threadIdx.x & 31; q < (unsigned)(s.rows * p.each); q += 32) {
-    unsigned ch;
-    const unsigned row = p.by_each.divmod(q, ch);
-    sum += part[row * s.width + g * p.each + ch];
+// f(j) for the thread's steps, four at a time; `full` is the same for all threads that have any.
+template <class F>
+__device__ __forceinline__ void each_step(int full, int steps, F f) {
+  int j = 0;
+  for (; j + 4 <= full; j += 4) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f(j + u);
   }
-  return warp_sum(sum);
+  for (; j < full; ++j) f(j);
+  if (j < steps) f(j);
+}
+
+// V values of gamma or beta, or as many of `otherwise`.
+template <int V>
+__device__ __forceinline__ Vec<V> parameter(const float* from, bool there, bool vectors, float otherwise) {
+  Vec<V> r = all<V>(otherwise);
+  if (from && there) {
+    if (vectors) r = *reinterpret_cast<const Vec<V>*>(from);
+    else
+#pragma unroll
+      for (int i = 0; i < V; ++i) r.v[i] = from[i];
+  }
+  return r;
+}
+
+// Adds up over the lanes of a warp that hold the same channels.
+__device__ __forceinline__ float sum_rows(float t, const Slabs& p) {
+  for (int o = p.lanes; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
+}
+
+// A warp's mean and M2 of each of its entries, to slots [slots][lanes * E / merged]; E: entries of a thread.
+template <int V, int E>
+__device__ __forceinline__ void slot_statistics(float* mine, int full, int steps, const Slabs& p, const Share<V>& s, float2* slots) {
+  constexpr int N = V / E;  // channels of an entry
+  Vec<V> sum = all<V>(0.f), m2 = sum, off = sum;
+  each_step(full, steps, [&](int j) { sum = add(sum, vec<V>(mine + j * kThreads * V)); });
+  const int count = s.of_slot(p, s.slot(p)) * p.merged * N;
+  const float inv = count ? __frcp_rn((float)count) : 0.f;
+  float mean[E];
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t += sum.v[k * N + i];
+    for (int o = 1; o < p.merged; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    mean[k] = sum_rows(t, p) * inv;
+#pragma unroll
+    for (int i = 0; i < N; ++i) off.v[k * N + i] = -mean[k];
+  }
+  each_step(full, steps, [&](int j) {
+    const Vec<V> d = add(vec<V>(mine + j * kThreads * V), off);
+    m2 = fma(d, d, m2);
+  });
+  const int in_row = threadIdx.x & (p.lanes - 1);
+  float2* to = slots + s.slot(p) * (p.lanes * E / p.merged) + in_row / p.merged * E;
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t += m2.v[k * N + i];
+    for (int o = 1; o < p.merged; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    t = sum_rows(t, p);
+    if ((threadIdx.x & 31) < p.lanes && (in_row & (p.merged - 1)) == 0) to[k] = make_float2(mean[k], t);
+  }
 }
 
 template <int V, int ACT>
-__global__ void __launch_bounds__(kThreads) gn_forward_kernel(const __grid_constant__ Slabs p, const float* __restrict__ x, const float* __restrict__ gamma,
-                                                               const float* __restrict__ beta, float eps, float* __restrict__ y,
-                                                               float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  extern __shared__ __align__(16) float held[];  // [steps][kThreads][V], then the threads' sums and the groups' statistics
+__global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_constant__ Slabs p, const float* __restrict__ x, const float* __restrict__ gamma,
+                                                                  const float* __restrict__ beta, float eps, float* __restrict__ y,
+                                                                  float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  extern __shared__ __align__(16) float held[];  // [steps][kThreads][V]; the warps' (mean, M2); the CTAs' [ctas][groups of a slab]
   mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = p.ctas > 1 ? (int)cluster.block_rank() : 0;
-  Share s;
-  s.of<V>(p, blockIdx.x / p.ctas, rank);
-  float *mine = held + threadIdx.x * V, *part = held + p.steps * kThreads * V, *mean_of = part + p.sums, *m2_of = mean_of + p.wide;
-  const int groups = s.width / p.each, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool active = s.row < s.rows;
+  const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
+  const Unit u(p, blockIdx.x / p.ctas);
+  const int per_slot = p.lanes * p.of_vector / p.merged;
+  float* mine = held + threadIdx.x * V;
+  float2 *slots = (float2*)(held + p.steps * kThreads * V), *of_cta = slots + p.slots * per_slot;
+  const bool active = s.col < u.width;
+  const int full = active ? s.full : 0, steps = active ? s.steps : 0;
+  const unsigned step = p.rows * p.c;  // of an image's values
   mtb_wait_prior();
-  const float* from = x + s.first;
-  const long long step = (long long)s.rows * p.c;
-  for (int j = 0; j < s.steps; ++j) copy_async<V>(mine + j * kThreads * V, from + j * step);
-  int of[V];  // group
-  float scale[V], shift[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    of[i] = (s.col + i) / p.each;
-    scale[i] = active && gamma ? gamma[s.c0 + s.col + i] : 1.f;
-    shift[i] = active && beta ? beta[s.c0 + s.col + i] : 0.f;
-  }
+  const float* from = x + u.first(p, s);
+  each_step(full, steps, [&](int j) { copy_async<V>(mine + j * kThreads * V, from + j * step); });
+  Vec<V> scale = parameter<V>(gamma + u.c0 + s.col, gamma && active, p.vectors, 1.f);
+  const Vec<V> shift = parameter<V>(beta + u.c0 + s.col, beta && active, p.vectors, 0.f);
   copies_done();
-
-  // the CTA's mean, then the squares of what differs from it
-  float sum[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) sum[i] = 0.f;
-  for (int j = 0; j < s.steps; ++j) {
-    const Vec<V> v = vec<V>(mine + j * kThreads * V);
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] += v.v[i];
-  }
-  if (active)
-#pragma unroll
-    for (int i = 0; i < V; ++i) part[threadIdx.x * V + i] = sum[i];
+  if (V >= 4 && p.of_vector == 4) slot_statistics<V, V >= 4 ? 4 : 1>(mine, full, steps, p, s, slots);
+  else if (V >= 2 && p.of_vector == 2) slot_statistics<V, V >= 2 ? 2 : 1>(mine, full, steps, p, s, slots);
+  else slot_statistics<V, 1>(mine, full, steps, p, s, slots);
   __syncthreads();
-  const float inv = 1.f / ((float)p.each * s.positions);
-  for (int g = warp; g < groups; g += kWarps) {
-    const float t = sum_group(part, s, p, g);
-    if (lane == 0) mean_of[g] = t * inv;
+  // Chan's update for several: the mean of the means, and M2_k + n_k (mean_k - mean)^2 added up.  The CTA's of a group, given to each CTA of the cluster ...
+  const float share = (float)(V / p.of_vector * p.merged), inv = __frcp_rn((float)(s.positions * p.each));
+  for (unsigned k = threadIdx.x; k < (unsigned)(p.of_slab * p.ctas); k += kThreads) {
+    unsigned g;
+    const unsigned r = p.by_groups.divmod(k, g);
+    if (g >= (unsigned)u.groups) continue;
+    const float2* entry = slots + g * p.entries;
+    float mean = 0.f, m2 = 0.f;
+    for (int q = 0; q < p.entries; ++q)
+#pragma unroll 8
+      for (int w = 0; w < p.slots; ++w) mean += entry[w * per_slot + q].x * ((float)s.of_slot(p, w) * share);
+    mean *= inv;
+    for (int q = 0; q < p.entries; ++q)
+#pragma unroll 8
+      for (int w = 0; w < p.slots; ++w) {
+        const float2 e = entry[w * per_slot + q];
+        const float d = e.x - mean;
+        m2 += e.y + (float)s.of_slot(p, w) * share * (d * d);
+      }
+    float2* to = of_cta + s.rank * p.of_slab + g;
+    if (p.ctas > 1) to = cluster.map_shared_rank(to, r);
+    *to = make_float2(mean, m2);
   }
-  __syncthreads();
-  float mu[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    mu[i] = active ? mean_of[of[i]] : 0.f;
-    sum[i] = 0.f;
-  }
-  for (int j = 0; j < s.steps; ++j) {
-    const Vec<V> v = vec<V>(mine + j * kThreads * V);
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] += (v.v[i] - mu[i]) * (v.v[i] - mu[i]);
-  }
-  if (active)
-#pragma unroll
-    for (int i = 0; i < V; ++i) part[threadIdx.x * V + i] = sum[i];
-  __syncthreads();
-  for (int g = warp; g < groups; g += kWarps) {
-    const float t = sum_group(part, s, p, g);
-    if (lane == 0) m2_of[g] = t;
-  }
-
-  // the group's, from the CTAs' (Chan): sum of n_k mean_k / N, then M2_k + n_k (mean_k - mean)^2
   if (p.ctas > 1) cluster.sync(); else __syncthreads();
-  float *group_mean = part, *group_rstd = part + p.wide;
-  const float whole = (float)p.hw;
-  for (int g = threadIdx.x; g < groups; g += kThreads) {
-    float mean = mean_of[g], m2 = m2_of[g];
-    if (p.ctas > 1) {
-      mean = 0.f;
-      for (int r = 0; r < p.ctas; ++r) {
-        const int count = r + 1 < p.ctas ? p.stretch : p.hw - r * p.stretch;
-        mean += (float)count / whole * cluster.map_shared_rank(mean_of, r)[g];
-      }
-      m2 = 0.f;
-      for (int r = 0; r < p.ctas; ++r) {
-        const int count = r + 1 < p.ctas ? p.stretch : p.hw - r * p.stretch;
-        const float d = cluster.map_shared_rank(mean_of, r)[g] - mean;
-        m2 += cluster.map_shared_rank(m2_of, r)[g] + (float)count * p.each * (d * d);
-      }
-    }
-    const float rstd = 1.f / sqrtf(m2 / ((float)p.each * whole) + eps);
-    group_mean[g] = mean;
-    group_rstd[g] = rstd;
-    if (rank == 0) {
-      const long long k = (long long)s.n * p.groups + s.c0 / p.each + g;
-      mean_out[k] = mean;
-      rstd_out[k] = rstd;
-    }
-  }
-  if (p.ctas > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");  // this CTA has read the others'
-  __syncthreads();
+  // ... and the group's
+  Vec<V> minus = all<V>(0.f);
+  float mean = 0.f, rstd = 0.f;
+  const float one = p.ctas > 1 ? (float)p.stretch * p.inv_positions : 1.f, end = 1.f - one * (float)(p.ctas - 1), n_one = (float)(p.stretch * p.each),
+              n_end = (float)((p.hw - (p.ctas - 1) * p.stretch) * p.each);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    if (active) {
-      mu[i] = group_mean[of[i]];
-      scale[i] *= group_rstd[of[i]];
+    if (active && (i == 0 || s.group[i] != s.group[i - 1 < 0 ? 0 : i - 1])) {
+      const float2* theirs = of_cta + s.group[i];
+      mean = 0.f;
+      float m2 = 0.f;
+#pragma unroll 8
+      for (int r = 0; r < p.ctas; ++r) mean += theirs[r * p.of_slab].x * (r + 1 < p.ctas ? one : end);
+#pragma unroll 8
+      for (int r = 0; r < p.ctas; ++r) {
+        const float2 e = theirs[r * p.of_slab];
+        const float d = e.x - mean;
+        m2 += e.y + (r + 1 < p.ctas ? n_one : n_end) * (d * d);
+      }
+      rstd = rsqrtf(m2 * p.inv_group + eps);
+      if (s.rank == 0 && s.row == 0 && s.group[i] * p.each == s.col + i) {
+        const long long k = (long long)u.n * p.groups + u.c0 / p.each + s.group[i];
+        mean_out[k] = mean;
+        rstd_out[k] = rstd;
+      }
     }
+    minus.v[i] = -mean;
+    scale.v[i] *= rstd;
   }
-  float* to = y + s.first;
-  for (int j = 0; j < s.steps; ++j) {
-    Vec<V> v = vec<V>(mine + j * kThreads * V);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v.v[i] = activate((v.v[i] - mu[i]) * scale[i] + shift[i], ACT);
-    *reinterpret_cast<Vec<V>*>(to + j * step) = v;
-  }
-  if (p.ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // the others have read this CTA's
+  float* to = y + u.first(p, s);
+  each_step(full, steps, [&](int j) {
+    *reinterpret_cast<Vec<V>*>(to + j * step) = activated<V, ACT>(fma(add(vec<V>(mine + j * kThreads * V), minus), scale, shift));
+  });
 }
 
 // sums (may be NULL): per image and channel the sums of dz and of dz xh, [n][2][c].  dx may be NULL.
 template <int V, int ACT>
-__global__ void __launch_bounds__(kThreads) gn_backward_kernel(const __grid_constant__ Slabs p, const float* __restrict__ dy, const float* __restrict__ x,
-                                                                const float* __restrict__ gamma, const float* __restrict__ beta,
-                                                                const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ dx,
-                                                                float* __restrict__ sums) {
-  extern __shared__ __align__(16) float held[];  // [2][steps][kThreads][V], then the threads' sums, the CTA's and the groups'
+__global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_constant__ Slabs p, const float* __restrict__ dy, const float* __restrict__ x,
+                                                                   const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                                   const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ dx,
+                                                                   float* __restrict__ sums) {
+  extern __shared__ __align__(16) float held[];  // [2][steps][kThreads][V]; the warps' sums; the CTA's, weighted; the CTAs' of channels and of groups
   mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = p.ctas > 1 ? (int)cluster.block_rank() : 0;
-  Share s;
-  s.of<V>(p, blockIdx.x / p.ctas, rank);
-  const int plane = p.steps * kThreads * V;
-  float *mine = held + threadIdx.x * V, *part = held + 2 * plane, *part2 = part + kThreads * V, *sum_of = part + p.sums, *sum2_of = sum_of + p.wide;
-  const int groups = s.width / p.each, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool active = s.row < s.rows;
+  const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
+  const Unit u(p, blockIdx.x / p.ctas);
+  const int plane = p.steps * kThreads * V, both = 2 * p.lanes * V;  // two sums of each channel
+  float *mine = held + threadIdx.x * V, *of_warp = held + 2 * plane, *weighted = of_warp + p.slots * both, *of_channel = weighted + both;
+  float2* of_cta = (float2*)(of_channel + p.ctas * both);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool active = s.col < u.width;
+  const int full = active ? s.full : 0, steps = active ? s.steps : 0;
+  const unsigned step = p.rows * p.c;
   mtb_wait_prior();
-  const long long step = (long long)s.rows * p.c;
-  for (int j = 0; j < s.steps; ++j) {
-    copy_async<V>(mine + j * kThreads * V, x + s.first + j * step);
-    copy_async<V>(mine + plane + j * kThreads * V, dy + s.first + j * step);
+  {
+    const float *from = x + u.first(p, s), *from2 = dy + u.first(p, s);
+    each_step(full, steps, [&](int j) {
+      copy_async<V>(mine + j * kThreads * V, from + j * step);
+      copy_async<V>(mine + plane + j * kThreads * V, from2 + j * step);
+    });
   }
-  int of[V];
-  float mu[V], r[V], ga[V], be[V], a[V], b[V];
+  Vec<V> ga = parameter<V>(gamma + u.c0 + s.col, gamma && active, p.vectors, 1.f);
+  const Vec<V> be = parameter<V>(beta + u.c0 + s.col, beta && active, p.vectors, 0.f);
+  Vec<V> minus = all<V>(0.f), r = minus, a = minus, b = minus;
+  if (active) {
+    const long long k = (long long)u.n * p.groups + u.c0 / p.each;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    of[i] = (s.col + i) / p.each;
-    const long long k = (long long)s.n * p.groups + s.c0 / p.each + of[i];
-    mu[i] = active ? mean[k] : 0.f;
-    r[i] = active ? rstd[k] : 0.f;
-    ga[i] = active && gamma ? gamma[s.c0 + s.col + i] : 1.f;
-    be[i] = active && beta ? beta[s.c0 + s.col + i] : 0.f;
-    a[i] = b[i] = 0.f;
+    for (int i = 0; i < V; ++i) {
+      minus.v[i] = -mean[k + s.group[i]];
+      r.v[i] = rstd[k + s.group[i]];
+    }
   }
   copies_done();
-  for (int j = 0; j < s.steps; ++j) {  // xh and dz take the places of x and dy
-    Vec<V> v = vec<V>(mine + j * kThreads * V), d = vec<V>(mine + plane + j * kThreads * V);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      v.v[i] = (v.v[i] - mu[i]) * r[i];
-      d.v[i] = activate_grad(d.v[i], v.v[i] * ga[i] + be[i], ACT);
-      a[i] += d.v[i];
-      b[i] += d.v[i] * v.v[i];
-    }
+  each_step(full, steps, [&](int j) {  // xh and dz take the places of x and dy
+    const Vec<V> v = mul(add(vec<V>(mine + j * kThreads * V), minus), r);
+    const Vec<V> d = activated_grad<V, ACT>(vec<V>(mine + plane + j * kThreads * V), fma(v, ga, be));
+    a = add(a, d);
+    b = fma(d, v, b);
     vec<V>(mine + j * kThreads * V) = v;
     if (ACT != ACT_NONE) vec<V>(mine + plane + j * kThreads * V) = d;
-  }
-  if (active) {
+  });
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      part[threadIdx.x * V + i] = a[i];
-      part2[threadIdx.x * V + i] = b[i];
-    }
+  for (int i = 0; i < V; ++i) {
+    a.v[i] = sum_rows(a.v[i], p);
+    b.v[i] = sum_rows(b.v[i], p);
+  }
+  if (lane < p.lanes) {
+    vec<V>(of_warp + s.slot(p) * both + s.col) = a;
+    vec<V>(of_warp + s.slot(p) * both + p.lanes * V + s.col) = b;
   }
   __syncthreads();
-  for (int k = warp; k < 2 * s.width; k += kWarps) {  // a channel's sums over the CTA's rows
-    const float* from = k < s.width ? part + k : part2 + k - s.width;
+  for (int k = threadIdx.x; k < both; k += kThreads) {  // the CTA's
+    const int second = k >= p.lanes * V, ch = k - (second ? p.lanes * V : 0);
+    if (ch >= u.width) continue;
+    const float weight = gamma ? gamma[u.c0 + ch] : 1.f;
     float t = 0.f;
-    for (int row = lane; row < s.rows; row += 32) t += from[row * s.width];
-    t = warp_sum(t);
-    if (lane == 0) (k < s.width ? sum_of[k] : sum2_of[k - s.width]) = t;
+#pragma unroll 8
+    for (int w = 0; w < p.slots; ++w) t += of_warp[w * both + k];
+    weighted[k] = t * weight;
+    if (!sums) continue;
+    if (p.ctas > 1) cluster.map_shared_rank(of_channel, 0)[s.rank * both + k] = t;
+    else sums[((long long)u.n * 2 + second) * p.c + u.c0 + ch] = t;
+  }
+  __syncthreads();
+  if (dx) {
+    for (int g = warp; g < u.groups; g += kWarps) {  // the group's in the CTA, given to each CTA of the cluster
+      float t = 0.f, t2 = 0.f;
+      for (int ch = g * p.each + lane; ch < (g + 1) * p.each; ch += 32) {
+        t += weighted[ch];
+        t2 += weighted[p.lanes * V + ch];
+      }
+      const float2 both_sums = make_float2(warp_sum(t) * p.inv_group, warp_sum(t2) * p.inv_group);
+      float2* to = of_cta + s.rank * p.of_slab + g;
+      if (lane < p.ctas) *(p.ctas > 1 ? cluster.map_shared_rank(to, lane) : to) = both_sums;
+    }
   }
   if (p.ctas > 1) cluster.sync(); else __syncthreads();
-  // over the cluster
-  for (int k = threadIdx.x; k < 2 * s.width; k += kThreads) {
-    float* from = k < s.width ? sum_of + k : sum2_of + k - s.width;
-    float t = 0.f;
-    if (p.ctas > 1) {
-      for (int q = 0; q < p.ctas; ++q) t += *cluster.map_shared_rank(from, q);
-    } else {
-      t = *from;
-    }
-    part[k] = t;
-    if (rank == 0 && sums) sums[((long long)s.n * 2 + (k < s.width ? 0 : 1)) * p.c + s.c0 + (k < s.width ? k : k - s.width)] = t;
-  }
-  if (p.ctas > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-  if (dx) {
-    __syncthreads();
-    float* of_group = part + 2 * p.wide;  // A / M, B / M
-    const float inv = 1.f / ((float)p.each * p.hw);
-    for (int k = warp; k < 2 * groups; k += kWarps) {
-      const int g = k >> 1, base = g * p.each;
+  if (p.ctas > 1 && sums && s.rank == 0) {
+    for (int k = threadIdx.x; k < both; k += kThreads) {
+      const int second = k >= p.lanes * V, ch = k - (second ? p.lanes * V : 0);
+      if (ch >= u.width) continue;
       float t = 0.f;
-      for (int ch = lane; ch < p.each; ch += 32) t += (gamma ? gamma[s.c0 + base + ch] : 1.f) * part[(k & 1) * s.width + base + ch];
-      t = warp_sum(t);
-      if (lane == 0) of_group[k] = t * inv;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      a[i] = active ? of_group[2 * of[i]] * r[i] : 0.f;
-      b[i] = active ? of_group[2 * of[i] + 1] * r[i] : 0.f;
-      ga[i] *= r[i];
-    }
-    float* to = dx + s.first;
-    for (int j = 0; j < s.steps; ++j) {
-      Vec<V> v = vec<V>(mine + j * kThreads * V);
-      const Vec<V> d = vec<V>(mine + plane + j * kThreads * V);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v.v[i] = ga[i] * d.v[i] - (a[i] + v.v[i] * b[i]);
-      *reinterpret_cast<Vec<V>*>(to + j * step) = v;
+#pragma unroll 8
+      for (int q = 0; q < p.ctas; ++q) t += of_channel[q * both + k];
+      sums[((long long)u.n * 2 + second) * p.c + u.c0 + ch] = t;
     }
   }
-  if (p.ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (!dx) return;
+  float group_a = 0.f, group_b = 0.f;  // -A / M, -B / M
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (active && (i == 0 || s.group[i] != s.group[i - 1 < 0 ? 0 : i - 1])) {
+      group_a = group_b = 0.f;
+#pragma unroll 8
+      for (int q = 0; q < p.ctas; ++q) {
+        const float2 e = of_cta[q * p.of_slab + s.group[i]];
+        group_a -= e.x;
+        group_b -= e.y;
+      }
+    }
+    a.v[i] = group_a;
+    b.v[i] = group_b;
+  }
+  a = mul(a, r);
+  b = mul(b, r);
+  ga = mul(ga, r);
+  float* to = dx + u.first(p, s);
+  each_step(full, steps, [&](int j) {
+    *reinterpret_cast<Vec<V>*>(to + j * step) = fma(vec<V>(mine + j * kThreads * V), b, fma(ga, vec<V>(mine + plane + j * kThreads * V), a));
+  });
 }
 
 // dgamma and dbeta: the sums over the images, 32 columns of [n][2 c] a CTA, in a fixed order.
@@ -498,69 +628,72 @@ __global__ void __launch_bounds__(256) gn_bwd_dx_kernel(const float* __restrict_
 
 struct Plan {
   bool on_chip;
-  int v, units, smem;
+  int v, smem;
   Slabs s;
 };
 
+constexpr int kMostShared = 225 * 1024, kShared = 227 * 1024;  // of a CTA, of an SM for CTAs that take 1 KB more than they ask for
+
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
-// planes: tensors that the cluster holds (1 forward, 2 backward).
+// planes: tensors that the cluster holds (1 forward, 2 backward).  Of slabs of several widths and clusters of several sizes the pair is taken that is done
+// first by PLAN_COST
 Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
   Plan t{};
   const int each = c / groups;
   t.v = c % 4 == 0 && alignment % 16 == 0 ? 4 : c % 2 == 0 && alignment % 8 == 0 ? 2 : 1;
   const int unit = t.v / gcd(each, t.v);  // groups whose channels are whole vectors
-  // a line of memory a position; with few positions enough channels that every thread has a vector
-  int want = kThreads * t.v / hw;
-  want = want < 32 ? 32 : want > kThreads * t.v ? kThreads * t.v : want;
-  for (int attempt = 0; attempt < 2; ++attempt) {
-    int of_slab = attempt ? unit : ((want + each - 1) / each + unit - 1) / unit * unit;
-    if (of_slab * each > kThreads * t.v && of_slab > unit) of_slab = kThreads * t.v / each / unit * unit;
-    if (of_slab < unit) of_slab = unit;
+  const int sms = mtb_sm_count();
+  double best = 0;
+  for (int want = 8; want <= kThreads * t.v; want *= 2) {
+    int of_slab = ((want + each - 1) / each + unit - 1) / unit * unit;
     if (of_slab > groups) of_slab = groups;
-    const int wide = of_slab * each;
-    if (wide > kThreads * t.v) return t;
-    const int rows = kThreads / (wide / t.v), slabs = (groups + of_slab - 1) / of_slab;
-    auto steps_of = [&](int ctas) { const int stretch = (hw + ctas - 1) / ctas; return (stretch + rows - 1) / rows; };
-    auto bytes_of = [&](int ctas) { return 4LL * planes * kThreads * t.v * steps_of(ctas); };
-    // The fewest CTAs that leave an SM room for four of them, or two, or one.
-    int ctas = 0;
-    for (int most : {48, 100, 200}) {
-      for (int k = 1; k <= 8 && !ctas; ++k)
-        if (bytes_of(k) <= most * 1024LL) ctas = k;
-      if (!ctas && most > 48 && bytes_of(16) <= most * 1024LL) ctas = 16;
-      if (ctas) break;
+    const int wide = of_slab * each, vectors = wide / t.v;
+    if (vectors > kThreads) break;
+    int lanes = 1;
+    while (lanes < vectors) lanes *= 2;
+    const int rows = kThreads / lanes, slabs = (groups + of_slab - 1) / of_slab, of_vector = t.v / gcd(each, t.v);
+    const long long units = (long long)n * slabs;
+    // a group's lanes become one where they are a power of two of whole vectors
+    int merged = 1;
+    if (of_vector == 1 && ((each / t.v) & (each / t.v - 1)) == 0) merged = each / t.v < 32 ? each / t.v : 32;
+    const int entries = each * of_vector / t.v / merged, slots = lanes < 32 ? kWarps : rows;
+    for (int ctas = 1; ctas <= 16; ctas = ctas == 8 ? 16 : ctas + 1) {
+      const int stretch = (hw + ctas - 1) / ctas, steps = (stretch + rows - 1) / rows;
+      if ((ctas > 1 && (hw + stretch - 1) / stretch != ctas) || units * ctas >= 1LL << 31) continue;
+      const long long sums = planes == 1 ? 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab) : 2 * lanes * t.v * (slots + 1 + ctas) + 2 * ctas * of_slab;
+      const long long smem = 4 * ((long long)planes * steps * kThreads * t.v + sums);
+      if (smem > kMostShared) continue;
+      int at_once = (int)(kShared / (smem + 1024));
+      if (at_once > 4) at_once = 4;
+      const long long together = (long long)sms * at_once / ctas, rounds = together ? (units + together - 1) / together : units;
+      const double cost = rounds * (at_once * steps * t.v * planes * (wide < 16 ? 1.3 : 1.0) + (ctas > 1 ? 100 + 10 * ctas : 60));
+      if (t.on_chip && cost >= best) continue;
+      best = cost;
+      t.on_chip = true;
+      t.smem = (int)smem;
+      t.s = Slabs{hw, c, groups, each, wide, slabs, (int)units, of_slab, ctas, stretch, lanes, rows, __builtin_ctz(lanes), __builtin_ctz(rows), steps,
+                  of_vector, entries, merged, slots, lanes < 32 ? 32 / lanes : 1, false, 1.f / (float)hw, (float)(1.0 / ((double)each * hw)),
+                  PoolDiv((unsigned)slabs), PoolDiv((unsigned)each), PoolDiv((unsigned)of_slab)};
     }
-    if (!ctas) continue;
-    // few slabs: more CTAs each, as long as a thread has several positions
-    while (ctas < 8 && (long long)n * slabs * ctas < mtb_sm_count() && steps_of(ctas) > 2) ++ctas;
-    const int stretch = (hw + ctas - 1) / ctas;
-    ctas = (hw + stretch - 1) / stretch;
-    // the threads' sums, and then a slab's and its groups'
-    const int sums = planes * kThreads * t.v > 4 * wide ? planes * kThreads * t.v : 4 * wide;
-    t.s = Slabs{hw, c, groups, each, wide, slabs, ctas, stretch, steps_of(ctas), sums, PoolDiv((unsigned)each)};
-    t.smem = (int)bytes_of(ctas) + 4 * (sums + 2 * wide);
-    if ((long long)n * slabs * ctas >= 1LL << 31) return t;
-    t.units = n * slabs;
-    t.on_chip = true;
-    return t;
+    if (of_slab == groups) break;
   }
   return t;
 }
 
 template <class... P, class... A>
-int launch_slabs(unsigned long long* opted, unsigned long long* wide, const Plan& t, cudaStream_t st, void (*kernel)(P...), A... args) {
-  if (int rc = mtb_opt_in_smem((const void*)kernel, 227 * 1024, opted)) return rc;
+int launch_slabs(unsigned long long* opted, unsigned long long* large, const Plan& t, cudaStream_t st, void (*kernel)(P...), A... args) {
+  if (int rc = mtb_opt_in_smem((const void*)kernel, kMostShared, opted)) return rc;
   if (t.s.ctas > 8) {
     int device = 0;
     MTB_CUDA(cudaGetDevice(&device));
-    if (device >= 64 || !((__atomic_load_n(wide, __ATOMIC_ACQUIRE) >> device) & 1ull)) {
+    if (device >= 64 || !((__atomic_load_n(large, __ATOMIC_ACQUIRE) >> device) & 1ull)) {
       MTB_CUDA(cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-      if (device < 64) __atomic_fetch_or(wide, 1ull << device, __ATOMIC_RELEASE);
+      if (device < 64) __atomic_fetch_or(large, 1ull << device, __ATOMIC_RELEASE);
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(t.units * t.s.ctas));
+  cfg.gridDim = dim3((unsigned)(t.s.units * t.s.ctas));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = t.smem;
   cfg.stream = st;
@@ -578,13 +711,13 @@ int launch_slabs(unsigned long long* opted, unsigned long long* wide, const Plan
 
 template <int V, int ACT, class... A>
 int forward_on_chip(const Plan& t, cudaStream_t st, A... args) {
-  static unsigned long long opted, wide;
-  return launch_slabs(&opted, &wide, t, st, gn_forward_kernel<V, ACT>, t.s, args...);
+  static unsigned long long opted, large;
+  return launch_slabs(&opted, &large, t, st, gn_forward_kernel<V, ACT>, t.s, args...);
 }
 template <int V, int ACT, class... A>
 int backward_on_chip(const Plan& t, cudaStream_t st, A... args) {
-  static unsigned long long opted, wide;
-  return launch_slabs(&opted, &wide, t, st, gn_backward_kernel<V, ACT>, t.s, args...);
+  static unsigned long long opted, large;
+  return launch_slabs(&opted, &large, t, st, gn_backward_kernel<V, ACT>, t.s, args...);
 }
 
 #define MTB_GN_PICK(f, t, act, ...)                                                                                                               \
@@ -623,7 +756,8 @@ MTB_API int mtb_group_norm_forward_f32(int n, int c, int hw, int groups, const f
   MTB_REQUIRE(x && y && mean && rstd, "group_norm_forward: null tensor");
   MTB_REQUIRE((long long)n * groups < 1LL << 31 && (long long)hw * c < 1LL << 31, "group_norm_forward: too many values");
   cudaStream_t st = (cudaStream_t)stream;
-  const Plan t = plan_slabs(n, c, hw, groups, 1, alignment_of(x, y, nullptr));
+  Plan t = plan_slabs(n, c, hw, groups, 1, alignment_of(x, y, nullptr));
+  t.s.vectors = alignment_of(gamma, beta, nullptr) % (4 * t.v) == 0;
   if (t.on_chip) return MTB_GN_PICK(forward_on_chip, t, activation, st, x, gamma, beta, (float)eps, y, mean, rstd);
   MTB_REQUIRE(workspace && workspace_bytes >= mtb_group_norm_workspace_bytes(n, c, hw, groups), "group_norm_forward: workspace too small");
   MTB_REQUIRE((long long)n * groups < 65536 && n < 65536, "group_norm_forward: %d images of %d groups", n, groups);
@@ -653,7 +787,8 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
   MTB_REQUIRE(workspace_bytes >= mtb_group_norm_workspace_bytes(n, c, hw, groups), "group_norm_backward: workspace too small");
   float* sums = (float*)workspace;
   const bool params = dgamma || dbeta;
-  const Plan t = plan_slabs(n, c, hw, groups, 2, alignment_of(dy, x, dx));
+  Plan t = plan_slabs(n, c, hw, groups, 2, alignment_of(dy, x, dx));
+  t.s.vectors = alignment_of(gamma, beta, nullptr) % (4 * t.v) == 0;
   if (t.on_chip) {
     if (int rc = MTB_GN_PICK(backward_on_chip, t, activation, st, dy, x, gamma, beta, mean, rstd, dx, params ? sums : nullptr)) return rc;
   } else {
