@@ -13,6 +13,7 @@
 // A slab that no cluster can hold goes through memory twice instead, see the kernels at the end.
 #include "colreduce.cuh"
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace {
 
@@ -189,6 +190,14 @@ __device__ __forceinline__ void each_step(int full, int steps, F f) {
   if (j < steps) f(j);
 }
 
+// The same in batches: f(first step, number of steps as a type), so that f can load all of a batch before it stores any.
+template <class F>
+__device__ __forceinline__ void each_batch(int full, int steps, F f) {
+  int j = 0;
+  for (; j + 4 <= full; j += 4) f(j, std::integral_constant<int, 4>());
+  for (; j < steps; ++j) f(j, std::integral_constant<int, 1>());
+}
+
 // V values of gamma or beta, or as many of `otherwise`.
 template <int V>
 __device__ __forceinline__ Vec<V> parameter(const float* from, bool there, bool vectors, float otherwise) {
@@ -202,10 +211,21 @@ __device__ __forceinline__ Vec<V> parameter(const float* from, bool there, bool 
   return r;
 }
 
-// Adds up over the lanes of a warp that hold the same channels.
-__device__ __forceinline__ float sum_rows(float t, const Slabs& p) {
-  for (int o = p.lanes; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+// Adds up over the lanes of a warp that hold the same entry: those of other rows, and `merged` neighbours.
+__device__ __forceinline__ float sum_entry(float t, const Slabs& p) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+    if (o < p.merged || o >= p.lanes) t += __shfl_xor_sync(0xffffffffu, t, o);
   return t;
+}
+
+// f(r) for the CTAs of a cluster.
+template <class F>
+__device__ __forceinline__ void each_cta(const Slabs& p, F f) {
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    if (r < p.ctas) f(r);
+  for (int r = 8; r < p.ctas; ++r) f(r);
 }
 
 // A warp's mean and M2 of each of its entries, to slots [slots][lanes * E / merged]; E: entries of a thread.
@@ -222,8 +242,7 @@ __device__ __forceinline__ void slot_statistics(float* mine, int full, int steps
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) t += sum.v[k * N + i];
-    for (int o = 1; o < p.merged; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    mean[k] = sum_rows(t, p) * inv;
+    mean[k] = sum_entry(t, p) * inv;
 #pragma unroll
     for (int i = 0; i < N; ++i) off.v[k * N + i] = -mean[k];
   }
@@ -238,8 +257,7 @@ __device__ __forceinline__ void slot_statistics(float* mine, int full, int steps
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) t += m2.v[k * N + i];
-    for (int o = 1; o < p.merged; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    t = sum_rows(t, p);
+    t = sum_entry(t, p);
     if ((threadIdx.x & 31) < p.lanes && (in_row & (p.merged - 1)) == 0) to[k] = make_float2(mean[k], t);
   }
 }
@@ -248,14 +266,14 @@ template <int V, int ACT>
 __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_constant__ Slabs p, const float* __restrict__ x, const float* __restrict__ gamma,
                                                                   const float* __restrict__ beta, float eps, float* __restrict__ y,
                                                                   float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  extern __shared__ __align__(16) float held[];  // [steps][kThreads][V]; the warps' (mean, M2); the CTAs' [ctas][groups of a slab]
+  extern __shared__ __align__(16) float held[];  // [positions][lanes][V]; the warps' (mean, M2); the CTAs' [ctas][groups of a slab]
   mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
   const Unit u(p, blockIdx.x / p.ctas);
   const int per_slot = p.lanes * p.of_vector / p.merged;
   float* mine = held + threadIdx.x * V;
-  float2 *slots = (float2*)(held + p.steps * kThreads * V), *of_cta = slots + p.slots * per_slot;
+  float2 *slots = (float2*)(held + (p.stretch * p.lanes * V + 1) / 2 * 2), *of_cta = slots + p.slots * per_slot;
   const bool active = s.col < u.width;
   const int full = active ? s.full : 0, steps = active ? s.steps : 0;
   const unsigned step = p.rows * p.c;  // of an image's values
@@ -269,28 +287,34 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
   else if (V >= 2 && p.of_vector == 2) slot_statistics<V, V >= 2 ? 2 : 1>(mine, full, steps, p, s, slots);
   else slot_statistics<V, 1>(mine, full, steps, p, s, slots);
   __syncthreads();
-  // Chan's update for several: the mean of the means, and M2_k + n_k (mean_k - mean)^2 added up.  The CTA's of a group, given to each CTA of the cluster ...
+  // Chan's update for several: the mean of the means, and M2_k + n_k (mean_k - mean)^2 added up.  The CTA's of a group by eight lanes, a slot each, who give it to
+  // each CTA of the cluster ...
   const float share = (float)(V / p.of_vector * p.merged), inv = __frcp_rn((float)(s.positions * p.each));
-  for (unsigned k = threadIdx.x; k < (unsigned)(p.of_slab * p.ctas); k += kThreads) {
-    unsigned g;
-    const unsigned r = p.by_groups.divmod(k, g);
-    if (g >= (unsigned)u.groups) continue;
-    const float2* entry = slots + g * p.entries;
+  const int w = threadIdx.x & 7;
+  for (int g = threadIdx.x >> 3; g < (p.of_slab + 3) / 4 * 4; g += kThreads / 8) {  // whole warps
+    const float2* entry = slots + w * per_slot + g * p.entries;
+    const bool in = w < p.slots && g < u.groups;
+    const float count = in ? (float)s.of_slot(p, w) * share : 0.f;
     float mean = 0.f, m2 = 0.f;
-    for (int q = 0; q < p.entries; ++q)
-#pragma unroll 8
-      for (int w = 0; w < p.slots; ++w) mean += entry[w * per_slot + q].x * ((float)s.of_slot(p, w) * share);
+    if (in)
+      for (int q = 0; q < p.entries; ++q) mean += entry[q].x;
+    mean *= count;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
     mean *= inv;
-    for (int q = 0; q < p.entries; ++q)
-#pragma unroll 8
-      for (int w = 0; w < p.slots; ++w) {
-        const float2 e = entry[w * per_slot + q];
-        const float d = e.x - mean;
-        m2 += e.y + (float)s.of_slot(p, w) * share * (d * d);
+    if (in)
+      for (int q = 0; q < p.entries; ++q) {
+        const float d = entry[q].x - mean;
+        m2 += entry[q].y + count * (d * d);
       }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m2 += __shfl_xor_sync(0xffffffffu, m2, o);
     float2* to = of_cta + s.rank * p.of_slab + g;
-    if (p.ctas > 1) to = cluster.map_shared_rank(to, r);
-    *to = make_float2(mean, m2);
+    if (g < u.groups) {
+      if (p.ctas == 1) *to = make_float2(mean, m2);  // by eight lanes alike
+      else
+        for (int r = w; r < p.ctas; r += 8) *cluster.map_shared_rank(to, r) = make_float2(mean, m2);
+    }
   }
   if (p.ctas > 1) cluster.sync(); else __syncthreads();
   // ... and the group's
@@ -304,14 +328,12 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
       const float2* theirs = of_cta + s.group[i];
       mean = 0.f;
       float m2 = 0.f;
-#pragma unroll 8
-      for (int r = 0; r < p.ctas; ++r) mean += theirs[r * p.of_slab].x * (r + 1 < p.ctas ? one : end);
-#pragma unroll 8
-      for (int r = 0; r < p.ctas; ++r) {
+      each_cta(p, [&](int r) { mean += theirs[r * p.of_slab].x * (r + 1 < p.ctas ? one : end); });
+      each_cta(p, [&](int r) {
         const float2 e = theirs[r * p.of_slab];
         const float d = e.x - mean;
         m2 += e.y + (r + 1 < p.ctas ? n_one : n_end) * (d * d);
-      }
+      });
       rstd = rsqrtf(m2 * p.inv_group + eps);
       if (s.rank == 0 && s.row == 0 && s.group[i] * p.each == s.col + i) {
         const long long k = (long long)u.n * p.groups + u.c0 / p.each + s.group[i];
@@ -328,21 +350,42 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
   });
 }
 
-// sums (may be NULL): per image and channel the sums of dz and of dz xh, [n][2][c].  dx may be NULL.
+// A warp's sums of `a` and `b` over each of its entries, to slots [slots][lanes * E / merged].
+template <int V, int E>
+__device__ __forceinline__ void slot_sums(Vec<V> a, Vec<V> b, bool active, const Slabs& p, const Share<V>& s, float2* slots) {
+  constexpr int N = V / E;
+  const int in_row = threadIdx.x & (p.lanes - 1);
+  float2* to = slots + s.slot(p) * (p.lanes * E / p.merged) + in_row / p.merged * E;
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      t.x += a.v[k * N + i];
+      t.y += b.v[k * N + i];
+    }
+    if (!active) t = make_float2(0.f, 0.f);
+    t.x = sum_entry(t.x, p);
+    t.y = sum_entry(t.y, p);
+    if ((threadIdx.x & 31) < p.lanes && (in_row & (p.merged - 1)) == 0) to[k] = t;
+  }
+}
+
+// sums (may be NULL): per image, CTA and channel the sums of dz and of dz xh, [n][ctas][2][c].  dx may be NULL.
 template <int V, int ACT>
 __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_constant__ Slabs p, const float* __restrict__ dy, const float* __restrict__ x,
                                                                    const float* __restrict__ gamma, const float* __restrict__ beta,
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ dx,
                                                                    float* __restrict__ sums) {
-  extern __shared__ __align__(16) float held[];  // [2][steps][kThreads][V]; the warps' sums; the CTA's, weighted; the CTAs' of channels and of groups
+  extern __shared__ __align__(16) float held[];  // [2][positions][lanes][V]; the rows' sums of channels; the warps' of groups; the CTAs'
   mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
   const Unit u(p, blockIdx.x / p.ctas);
-  const int plane = p.steps * kThreads * V, both = 2 * p.lanes * V;  // two sums of each channel
-  float *mine = held + threadIdx.x * V, *of_warp = held + 2 * plane, *weighted = of_warp + p.slots * both, *of_channel = weighted + both;
-  float2* of_cta = (float2*)(of_channel + p.ctas * both);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int plane = p.stretch * p.lanes * V, both = 2 * p.lanes * V, pitch = both + 4;  // two sums of each channel; of a row of them
+  const int per_slot = p.lanes * p.of_vector / p.merged;
+  float *mine = held + threadIdx.x * V, *of_row = held + 2 * plane;
+  float2 *slots = (float2*)(of_row + p.rows * pitch), *of_cta = slots + p.slots * per_slot;
   const bool active = s.col < u.width;
   const int full = active ? s.full : 0, steps = active ? s.steps : 0;
   const unsigned step = p.rows * p.c;
@@ -359,79 +402,104 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
   Vec<V> minus = all<V>(0.f), r = minus, a = minus, b = minus;
   if (active) {
     const long long k = (long long)u.n * p.groups + u.c0 / p.each;
+    if (p.of_vector == 1) {
+      minus = all<V>(-mean[k + s.group[0]]);
+      r = all<V>(rstd[k + s.group[0]]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      minus.v[i] = -mean[k + s.group[i]];
-      r.v[i] = rstd[k + s.group[i]];
+      for (int i = 0; i < V; ++i) {
+        minus.v[i] = -mean[k + s.group[i]];
+        r.v[i] = rstd[k + s.group[i]];
+      }
     }
   }
   copies_done();
-  each_step(full, steps, [&](int j) {  // xh and dz take the places of x and dy
-    const Vec<V> v = mul(add(vec<V>(mine + j * kThreads * V), minus), r);
-    const Vec<V> d = activated_grad<V, ACT>(vec<V>(mine + plane + j * kThreads * V), fma(v, ga, be));
-    a = add(a, d);
-    b = fma(d, v, b);
-    vec<V>(mine + j * kThreads * V) = v;
-    if (ACT != ACT_NONE) vec<V>(mine + plane + j * kThreads * V) = d;
-  });
+  each_batch(full, steps, [&](int j, auto count) {  // xh and dz take the places of x and dy
+    constexpr int N = decltype(count)::value;
+    Vec<V> v[N], d[N];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    a.v[i] = sum_rows(a.v[i], p);
-    b.v[i] = sum_rows(b.v[i], p);
+    for (int i = 0; i < N; ++i) {
+      v[i] = vec<V>(mine + (j + i) * kThreads * V);
+      d[i] = vec<V>(mine + plane + (j + i) * kThreads * V);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = mul(add(v[i], minus), r);
+      d[i] = activated_grad<V, ACT>(d[i], fma(v[i], ga, be));
+      a = add(a, d[i]);
+      b = fma(d[i], v[i], b);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      vec<V>(mine + (j + i) * kThreads * V) = v[i];
+      if (ACT != ACT_NONE) vec<V>(mine + plane + (j + i) * kThreads * V) = d[i];
+    }
+  });
+  // The sums of groups are on the way of all that follows: a warp's, the CTA's by eight lanes a group, then to the others.  Those of channels are added up
+  // while they travel.
+  if (sums) {
+    vec<V>(of_row + s.row * pitch + s.col) = a;
+    vec<V>(of_row + s.row * pitch + p.lanes * V + s.col) = b;
   }
-  if (lane < p.lanes) {
-    vec<V>(of_warp + s.slot(p) * both + s.col) = a;
-    vec<V>(of_warp + s.slot(p) * both + p.lanes * V + s.col) = b;
-  }
-  __syncthreads();
-  for (int k = threadIdx.x; k < both; k += kThreads) {  // the CTA's
-    const int second = k >= p.lanes * V, ch = k - (second ? p.lanes * V : 0);
-    if (ch >= u.width) continue;
-    const float weight = gamma ? gamma[u.c0 + ch] : 1.f;
-    float t = 0.f;
-#pragma unroll 8
-    for (int w = 0; w < p.slots; ++w) t += of_warp[w * both + k];
-    weighted[k] = t * weight;
-    if (!sums) continue;
-    if (p.ctas > 1) cluster.map_shared_rank(of_channel, 0)[s.rank * both + k] = t;
-    else sums[((long long)u.n * 2 + second) * p.c + u.c0 + ch] = t;
+  if (dx) {
+    if (V >= 4 && p.of_vector == 4) slot_sums<V, V >= 4 ? 4 : 1>(mul(a, ga), mul(b, ga), active, p, s, slots);
+    else if (V >= 2 && p.of_vector == 2) slot_sums<V, V >= 2 ? 2 : 1>(mul(a, ga), mul(b, ga), active, p, s, slots);
+    else slot_sums<V, 1>(mul(a, ga), mul(b, ga), active, p, s, slots);
   }
   __syncthreads();
   if (dx) {
-    for (int g = warp; g < u.groups; g += kWarps) {  // the group's in the CTA, given to each CTA of the cluster
-      float t = 0.f, t2 = 0.f;
-      for (int ch = g * p.each + lane; ch < (g + 1) * p.each; ch += 32) {
-        t += weighted[ch];
-        t2 += weighted[p.lanes * V + ch];
+    const int w = threadIdx.x & 7;
+    for (int g = threadIdx.x >> 3; g < (p.of_slab + 3) / 4 * 4; g += kThreads / 8) {  // whole warps
+      float2 t = make_float2(0.f, 0.f);
+      if (w < p.slots && g < u.groups)
+        for (int q = 0; q < p.entries; ++q) {
+          const float2 e = slots[w * per_slot + g * p.entries + q];
+          t.x += e.x;
+          t.y += e.y;
+        }
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
+        t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
       }
-      const float2 both_sums = make_float2(warp_sum(t) * p.inv_group, warp_sum(t2) * p.inv_group);
+      t.x *= -p.inv_group;
+      t.y *= -p.inv_group;
       float2* to = of_cta + s.rank * p.of_slab + g;
-      if (lane < p.ctas) *(p.ctas > 1 ? cluster.map_shared_rank(to, lane) : to) = both_sums;
+      if (g < u.groups) {
+        if (p.ctas == 1) *to = t;  // by eight lanes alike
+        else
+          for (int r = w; r < p.ctas; r += 8) *cluster.map_shared_rank(to, r) = t;
+      }
     }
   }
-  if (p.ctas > 1) cluster.sync(); else __syncthreads();
-  if (p.ctas > 1 && sums && s.rank == 0) {
-    for (int k = threadIdx.x; k < both; k += kThreads) {
-      const int second = k >= p.lanes * V, ch = k - (second ? p.lanes * V : 0);
-      if (ch >= u.width) continue;
+  __syncwarp();
+  if (p.ctas > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+  if (sums) {
+    // a column by as many neighbouring lanes as there are threads for, or by one thread
+    const int share = both < kThreads ? kThreads / both : 1, parts = share < 32 ? share : 32;
+    float* to = sums + ((long long)u.n * p.ctas + s.rank) * 2 * p.c + u.c0;
+    for (int k = threadIdx.x; k < parts * both; k += kThreads) {
+      const int col = k / parts, part = k & (parts - 1), ch = col & (p.lanes * V - 1);
       float t = 0.f;
 #pragma unroll 8
-      for (int q = 0; q < p.ctas; ++q) t += of_channel[q * both + k];
-      sums[((long long)u.n * 2 + second) * p.c + u.c0 + ch] = t;
+      for (int row = part; row < p.rows; row += parts) t += of_row[row * pitch + col];
+      for (int o = 1; o < parts; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      if (part == 0 && ch < u.width) to[(col == ch ? 0 : p.c) + ch] = t;
     }
   }
+  __syncwarp();
+  if (p.ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); else __syncthreads();
   if (!dx) return;
   float group_a = 0.f, group_b = 0.f;  // -A / M, -B / M
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (active && (i == 0 || s.group[i] != s.group[i - 1 < 0 ? 0 : i - 1])) {
       group_a = group_b = 0.f;
-#pragma unroll 8
-      for (int q = 0; q < p.ctas; ++q) {
+      each_cta(p, [&](int q) {
         const float2 e = of_cta[q * p.of_slab + s.group[i]];
-        group_a -= e.x;
-        group_b -= e.y;
-      }
+        group_a += e.x;
+        group_b += e.y;
+      });
     }
     a.v[i] = group_a;
     b.v[i] = group_b;
@@ -445,22 +513,23 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
   });
 }
 
-// dgamma and dbeta: the sums over the images, 32 columns of [n][2 c] a CTA, in a fixed order.
-__global__ void __launch_bounds__(256) gn_params_kernel(const float* __restrict__ sums, int n, int c, float* __restrict__ dgamma, float* __restrict__ dbeta) {
+// dgamma and dbeta: the sums of [rows][2 c] over the rows, 32 columns a CTA, in a fixed order.
+__global__ void __launch_bounds__(1024) gn_params_kernel(const float* __restrict__ sums, int rows, int c, float* __restrict__ dgamma, float* __restrict__ dbeta) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  __shared__ float part[8][33];
+  __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   float t = 0.f;
   if (col < 2 * c)
 #pragma unroll 8
-    for (int i = row; i < n; i += 8) t += sums[(long long)i * 2 * c + col];
+    for (int i = row; i < rows; i += 32) t += sums[(long long)i * 2 * c + col];
   part[row][lane] = t;
   __syncthreads();
-  if (row != 0 || col >= 2 * c) return;
-  for (int k = 1; k < 8; ++k) t += part[k][lane];
-  if (col < c) { if (dbeta) dbeta[col] = t; }
-  else if (dgamma) dgamma[col - c] = t;
+  t = warp_sum(part[lane][row]);
+  const int of = blockIdx.x * 32 + row;
+  if (lane != 0 || of >= 2 * c) return;
+  if (of < c) { if (dbeta) dbeta[of] = t; }
+  else if (dgamma) dgamma[of - c] = t;
 }
 
 // ---------------------------------------------------------------- a slab through memory
@@ -636,6 +705,9 @@ constexpr int kMostShared = 225 * 1024, kShared = 227 * 1024;  // of a CTA, of a
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
+// CTAs of a cluster at most: their sums of channels are in the caller's scratch.
+int most_ctas(int hw) { return hw < 16 ? 1 : hw / 16 > 16 ? 16 : hw / 16; }
+
 // planes: tensors that the cluster holds (1 forward, 2 backward).  Of slabs of several widths and clusters of several sizes the pair is taken that is done
 // first by PLAN_COST
 Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
@@ -660,9 +732,9 @@ Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
     const int entries = each * of_vector / t.v / merged, slots = lanes < 32 ? kWarps : rows;
     for (int ctas = 1; ctas <= 16; ctas = ctas == 8 ? 16 : ctas + 1) {
       const int stretch = (hw + ctas - 1) / ctas, steps = (stretch + rows - 1) / rows;
-      if ((ctas > 1 && (hw + stretch - 1) / stretch != ctas) || units * ctas >= 1LL << 31) continue;
-      const long long sums = planes == 1 ? 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab) : 2 * lanes * t.v * (slots + 1 + ctas) + 2 * ctas * of_slab;
-      const long long smem = 4 * ((long long)planes * steps * kThreads * t.v + sums);
+      if ((ctas > 1 && ((hw + stretch - 1) / stretch != ctas || ctas > most_ctas(hw))) || units * ctas >= 1LL << 31) continue;
+      const long long sums = planes == 1 ? 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab) : rows * (2 * lanes * t.v + 4) + 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab);
+      const long long smem = 4 * ((long long)planes * stretch * lanes * t.v + sums);
       if (smem > kMostShared) continue;
       int at_once = (int)(kShared / (smem + 1024));
       if (at_once > 4) at_once = 4;
@@ -743,7 +815,8 @@ int alignment_of(const void* a, const void* b, const void* c) {
 // Scratch of both directions: what slabs that go through memory leave of their stretches, and the backward's sums.
 MTB_API long long mtb_group_norm_workspace_bytes(int n, int c, int hw, int groups) {
   if (n <= 0 || c <= 0 || hw <= 0 || groups <= 0) return 256;
-  const long long forward = 12LL * n * groups * splits_of(n, hw, groups), backward = 8LL * n * c * splits_of(n, hw, mtb_div_up(c, 32)) + 8LL * n * groups;
+  const long long forward = 12LL * n * groups * splits_of(n, hw, groups), splits = splits_of(n, hw, mtb_div_up(c, 32)),
+                  backward = 8LL * n * c * (splits > most_ctas(hw) ? splits : most_ctas(hw)) + 8LL * n * groups;
   return (forward > backward ? forward : backward) + 256;
 }
 
@@ -787,6 +860,7 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
   MTB_REQUIRE(workspace_bytes >= mtb_group_norm_workspace_bytes(n, c, hw, groups), "group_norm_backward: workspace too small");
   float* sums = (float*)workspace;
   const bool params = dgamma || dbeta;
+  if (!params && !dx) return MTB_OK;
   Plan t = plan_slabs(n, c, hw, groups, 2, alignment_of(dy, x, dx));
   t.s.vectors = alignment_of(gamma, beta, nullptr) % (4 * t.v) == 0;
   if (t.on_chip) {
@@ -802,6 +876,6 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
     if (dx) MTB_LAUNCH(gn_bwd_dx_kernel, dim3(mtb_stream_grid(image, 256), n), 256, 0, st, dy, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta,
                        activation, mean, rstd, of_group, dx);
   }
-  if (params) MTB_LAUNCH(gn_params_kernel, mtb_div_up(2LL * c, 32), 256, 0, st, sums, n, c, dgamma, dbeta);
+  if (params) MTB_LAUNCH(gn_params_kernel, mtb_div_up(2LL * c, 32), 1024, 0, st, sums, t.on_chip ? n * t.s.ctas : n, c, dgamma, dbeta);
   return MTB_OK;
 }
