@@ -9,11 +9,13 @@
 // a slab, some whole groups of one image, in its shared memory, each CTA a stretch of the positions; four CTAs or so on an SM, one of which loads
 // while another one adds up or stores.  A thread copies (cp.async) and later reads its own vectors only, so the copies need no barrier; the CTAs exchange their sums
 // through distributed shared memory.
-// SLAB_FIGURES
+// 256 x 128 x 56 x 56 with SiLU: forward 145 us (5.7 TB/s, 87 % of a copy), backward 295 (4.2 TB/s).  What bounds it now: the CTAs of a cluster wait for the
+// slowest of them, and an SM has two to four beside one another (backward without the exchange 190 us, with the exchange but alone in a cluster
+// 230).  Tried: clusters that stay and fetch the next slab meanwhile (forward 155 us, backward 337), sums sent with st.async (152, 319), two readings from the L2 cache
+// by tickets or by launches (backward 377).
 // A slab that no cluster can hold goes through memory twice instead, see the kernels at the end.
 #include "colreduce.cuh"
 #include <cooperative_groups.h>
-#include <type_traits>
 
 namespace {
 
@@ -190,14 +192,6 @@ __device__ __forceinline__ void each_step(int full, int steps, F f) {
   if (j < steps) f(j);
 }
 
-// The same in batches: f(first step, number of steps as a type), so that f can load all of a batch before it stores any.
-template <class F>
-__device__ __forceinline__ void each_batch(int full, int steps, F f) {
-  int j = 0;
-  for (; j + 4 <= full; j += 4) f(j, std::integral_constant<int, 4>());
-  for (; j < steps; ++j) f(j, std::integral_constant<int, 1>());
-}
-
 // V values of gamma or beta, or as many of `otherwise`.
 template <int V>
 __device__ __forceinline__ Vec<V> parameter(const float* from, bool there, bool vectors, float otherwise) {
@@ -211,21 +205,10 @@ __device__ __forceinline__ Vec<V> parameter(const float* from, bool there, bool 
   return r;
 }
 
-// Adds up over the lanes of a warp that hold the same entry: those of other rows, and `merged` neighbours.
-__device__ __forceinline__ float sum_entry(float t, const Slabs& p) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1)
-    if (o < p.merged || o >= p.lanes) t += __shfl_xor_sync(0xffffffffu, t, o);
+// Adds up over the lanes of a warp that hold the same channels.
+__device__ __forceinline__ float sum_rows(float t, const Slabs& p) {
+  for (int o = p.lanes; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
   return t;
-}
-
-// f(r) for the CTAs of a cluster.
-template <class F>
-__device__ __forceinline__ void each_cta(const Slabs& p, F f) {
-#pragma unroll
-  for (int r = 0; r < 8; ++r)
-    if (r < p.ctas) f(r);
-  for (int r = 8; r < p.ctas; ++r) f(r);
 }
 
 // A warp's mean and M2 of each of its entries, to slots [slots][lanes * E / merged]; E: entries of a thread.
@@ -242,7 +225,8 @@ __device__ __forceinline__ void slot_statistics(float* mine, int full, int steps
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) t += sum.v[k * N + i];
-    mean[k] = sum_entry(t, p) * inv;
+    for (int o = 1; o < p.merged; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    mean[k] = sum_rows(t, p) * inv;
 #pragma unroll
     for (int i = 0; i < N; ++i) off.v[k * N + i] = -mean[k];
   }
@@ -257,7 +241,8 @@ __device__ __forceinline__ void slot_statistics(float* mine, int full, int steps
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) t += m2.v[k * N + i];
-    t = sum_entry(t, p);
+    for (int o = 1; o < p.merged; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    t = sum_rows(t, p);
     if ((threadIdx.x & 31) < p.lanes && (in_row & (p.merged - 1)) == 0) to[k] = make_float2(mean[k], t);
   }
 }
@@ -328,12 +313,14 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
       const float2* theirs = of_cta + s.group[i];
       mean = 0.f;
       float m2 = 0.f;
-      each_cta(p, [&](int r) { mean += theirs[r * p.of_slab].x * (r + 1 < p.ctas ? one : end); });
-      each_cta(p, [&](int r) {
+#pragma unroll 8
+      for (int r = 0; r < p.ctas; ++r) mean += theirs[r * p.of_slab].x * (r + 1 < p.ctas ? one : end);
+#pragma unroll 8
+      for (int r = 0; r < p.ctas; ++r) {
         const float2 e = theirs[r * p.of_slab];
         const float d = e.x - mean;
         m2 += e.y + (r + 1 < p.ctas ? n_one : n_end) * (d * d);
-      });
+      }
       rstd = rsqrtf(m2 * p.inv_group + eps);
       if (s.rank == 0 && s.row == 0 && s.group[i] * p.each == s.col + i) {
         const long long k = (long long)u.n * p.groups + u.c0 / p.each + s.group[i];
@@ -350,42 +337,21 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
   });
 }
 
-// A warp's sums of `a` and `b` over each of its entries, to slots [slots][lanes * E / merged].
-template <int V, int E>
-__device__ __forceinline__ void slot_sums(Vec<V> a, Vec<V> b, bool active, const Slabs& p, const Share<V>& s, float2* slots) {
-  constexpr int N = V / E;
-  const int in_row = threadIdx.x & (p.lanes - 1);
-  float2* to = slots + s.slot(p) * (p.lanes * E / p.merged) + in_row / p.merged * E;
-#pragma unroll
-  for (int k = 0; k < E; ++k) {
-    float2 t = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      t.x += a.v[k * N + i];
-      t.y += b.v[k * N + i];
-    }
-    if (!active) t = make_float2(0.f, 0.f);
-    t.x = sum_entry(t.x, p);
-    t.y = sum_entry(t.y, p);
-    if ((threadIdx.x & 31) < p.lanes && (in_row & (p.merged - 1)) == 0) to[k] = t;
-  }
-}
-
-// sums (may be NULL): per image, CTA and channel the sums of dz and of dz xh, [n][ctas][2][c].  dx may be NULL.
+// sums (may be NULL): per image and channel the sums of dz and of dz xh, [n][2][c].  dx may be NULL.
 template <int V, int ACT>
 __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_constant__ Slabs p, const float* __restrict__ dy, const float* __restrict__ x,
                                                                    const float* __restrict__ gamma, const float* __restrict__ beta,
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ dx,
                                                                    float* __restrict__ sums) {
-  extern __shared__ __align__(16) float held[];  // [2][positions][lanes][V]; the rows' sums of channels; the warps' of groups; the CTAs'
+  extern __shared__ __align__(16) float held[];  // [2][positions][lanes][V]; the warps' sums; the CTA's, weighted; the CTAs' of channels and of groups
   mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
   const Unit u(p, blockIdx.x / p.ctas);
-  const int plane = p.stretch * p.lanes * V, both = 2 * p.lanes * V, pitch = both + 4;  // two sums of each channel; of a row of them
-  const int per_slot = p.lanes * p.of_vector / p.merged;
-  float *mine = held + threadIdx.x * V, *of_row = held + 2 * plane;
-  float2 *slots = (float2*)(of_row + p.rows * pitch), *of_cta = slots + p.slots * per_slot;
+  const int plane = p.stretch * p.lanes * V, both = 2 * p.lanes * V;  // two sums of each channel
+  float *mine = held + threadIdx.x * V, *of_warp = held + 2 * plane, *weighted = of_warp + p.slots * both, *of_channel = weighted + both;
+  float2* of_cta = (float2*)(of_channel + p.ctas * both);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool active = s.col < u.width;
   const int full = active ? s.full : 0, steps = active ? s.steps : 0;
   const unsigned step = p.rows * p.c;
@@ -414,92 +380,72 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
     }
   }
   copies_done();
-  each_batch(full, steps, [&](int j, auto count) {  // xh and dz take the places of x and dy
-    constexpr int N = decltype(count)::value;
-    Vec<V> v[N], d[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = vec<V>(mine + (j + i) * kThreads * V);
-      d[i] = vec<V>(mine + plane + (j + i) * kThreads * V);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = mul(add(v[i], minus), r);
-      d[i] = activated_grad<V, ACT>(d[i], fma(v[i], ga, be));
-      a = add(a, d[i]);
-      b = fma(d[i], v[i], b);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      vec<V>(mine + (j + i) * kThreads * V) = v[i];
-      if (ACT != ACT_NONE) vec<V>(mine + plane + (j + i) * kThreads * V) = d[i];
-    }
+  each_step(full, steps, [&](int j) {  // xh and dz take the places of x and dy
+    const Vec<V> v = mul(add(vec<V>(mine + j * kThreads * V), minus), r);
+    const Vec<V> d = activated_grad<V, ACT>(vec<V>(mine + plane + j * kThreads * V), fma(v, ga, be));
+    a = add(a, d);
+    b = fma(d, v, b);
+    vec<V>(mine + j * kThreads * V) = v;
+    if (ACT != ACT_NONE) vec<V>(mine + plane + j * kThreads * V) = d;
   });
-  // The sums of groups are on the way of all that follows: a warp's, the CTA's by eight lanes a group, then to the others.  Those of channels are added up
-  // while they travel.
-  if (sums) {
-    vec<V>(of_row + s.row * pitch + s.col) = a;
-    vec<V>(of_row + s.row * pitch + p.lanes * V + s.col) = b;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    a.v[i] = sum_rows(a.v[i], p);
+    b.v[i] = sum_rows(b.v[i], p);
   }
-  if (dx) {
-    if (V >= 4 && p.of_vector == 4) slot_sums<V, V >= 4 ? 4 : 1>(mul(a, ga), mul(b, ga), active, p, s, slots);
-    else if (V >= 2 && p.of_vector == 2) slot_sums<V, V >= 2 ? 2 : 1>(mul(a, ga), mul(b, ga), active, p, s, slots);
-    else slot_sums<V, 1>(mul(a, ga), mul(b, ga), active, p, s, slots);
+  if (lane < p.lanes) {
+    vec<V>(of_warp + s.slot(p) * both + s.col) = a;
+    vec<V>(of_warp + s.slot(p) * both + p.lanes * V + s.col) = b;
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < both; k += kThreads) {  // the CTA's
+    const int second = k >= p.lanes * V, ch = k - (second ? p.lanes * V : 0);
+    if (ch >= u.width) continue;
+    const float weight = gamma ? gamma[u.c0 + ch] : 1.f;
+    float t = 0.f;
+#pragma unroll 8
+    for (int w = 0; w < p.slots; ++w) t += of_warp[w * both + k];
+    weighted[k] = t * weight;
+    if (!sums) continue;
+    if (p.ctas > 1) cluster.map_shared_rank(of_channel, 0)[s.rank * both + k] = t;
+    else sums[((long long)u.n * 2 + second) * p.c + u.c0 + ch] = t;
   }
   __syncthreads();
   if (dx) {
-    const int w = threadIdx.x & 7;
-    for (int g = threadIdx.x >> 3; g < (p.of_slab + 3) / 4 * 4; g += kThreads / 8) {  // whole warps
-      float2 t = make_float2(0.f, 0.f);
-      if (w < p.slots && g < u.groups)
-        for (int q = 0; q < p.entries; ++q) {
-          const float2 e = slots[w * per_slot + g * p.entries + q];
-          t.x += e.x;
-          t.y += e.y;
-        }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
-        t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
+    for (int g = warp; g < u.groups; g += kWarps) {  // the group's in the CTA, given to each CTA of the cluster
+      float t = 0.f, t2 = 0.f;
+      for (int ch = g * p.each + lane; ch < (g + 1) * p.each; ch += 32) {
+        t += weighted[ch];
+        t2 += weighted[p.lanes * V + ch];
       }
-      t.x *= -p.inv_group;
-      t.y *= -p.inv_group;
+      const float2 both_sums = make_float2(warp_sum(t) * p.inv_group, warp_sum(t2) * p.inv_group);
       float2* to = of_cta + s.rank * p.of_slab + g;
-      if (g < u.groups) {
-        if (p.ctas == 1) *to = t;  // by eight lanes alike
-        else
-          for (int r = w; r < p.ctas; r += 8) *cluster.map_shared_rank(to, r) = t;
-      }
+      if (lane < p.ctas) *(p.ctas > 1 ? cluster.map_shared_rank(to, lane) : to) = both_sums;
     }
   }
-  __syncwarp();
-  if (p.ctas > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-  if (sums) {
-    // a column by as many neighbouring lanes as there are threads for, or by one thread
-    const int share = both < kThreads ? kThreads / both : 1, parts = share < 32 ? share : 32;
-    float* to = sums + ((long long)u.n * p.ctas + s.rank) * 2 * p.c + u.c0;
-    for (int k = threadIdx.x; k < parts * both; k += kThreads) {
-      const int col = k / parts, part = k & (parts - 1), ch = col & (p.lanes * V - 1);
+  if (p.ctas > 1) cluster.sync(); else __syncthreads();
+  if (p.ctas > 1 && sums && s.rank == 0) {
+    for (int k = threadIdx.x; k < both; k += kThreads) {
+      const int second = k >= p.lanes * V, ch = k - (second ? p.lanes * V : 0);
+      if (ch >= u.width) continue;
       float t = 0.f;
 #pragma unroll 8
-      for (int row = part; row < p.rows; row += parts) t += of_row[row * pitch + col];
-      for (int o = 1; o < parts; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (part == 0 && ch < u.width) to[(col == ch ? 0 : p.c) + ch] = t;
+      for (int q = 0; q < p.ctas; ++q) t += of_channel[q * both + k];
+      sums[((long long)u.n * 2 + second) * p.c + u.c0 + ch] = t;
     }
   }
-  __syncwarp();
-  if (p.ctas > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); else __syncthreads();
   if (!dx) return;
   float group_a = 0.f, group_b = 0.f;  // -A / M, -B / M
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     if (active && (i == 0 || s.group[i] != s.group[i - 1 < 0 ? 0 : i - 1])) {
       group_a = group_b = 0.f;
-      each_cta(p, [&](int q) {
+#pragma unroll 8
+      for (int q = 0; q < p.ctas; ++q) {
         const float2 e = of_cta[q * p.of_slab + s.group[i]];
-        group_a += e.x;
-        group_b += e.y;
-      });
+        group_a -= e.x;
+        group_b -= e.y;
+      }
     }
     a.v[i] = group_a;
     b.v[i] = group_b;
@@ -513,23 +459,22 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
   });
 }
 
-// dgamma and dbeta: the sums of [rows][2 c] over the rows, 32 columns a CTA, in a fixed order.
-__global__ void __launch_bounds__(1024) gn_params_kernel(const float* __restrict__ sums, int rows, int c, float* __restrict__ dgamma, float* __restrict__ dbeta) {
+// dgamma and dbeta: the sums over the images, 32 columns of [n][2 c] a CTA, in a fixed order.
+__global__ void __launch_bounds__(256) gn_params_kernel(const float* __restrict__ sums, int n, int c, float* __restrict__ dgamma, float* __restrict__ dbeta) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  __shared__ float part[32][33];
+  __shared__ float part[8][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   float t = 0.f;
   if (col < 2 * c)
 #pragma unroll 8
-    for (int i = row; i < rows; i += 32) t += sums[(long long)i * 2 * c + col];
+    for (int i = row; i < n; i += 8) t += sums[(long long)i * 2 * c + col];
   part[row][lane] = t;
   __syncthreads();
-  t = warp_sum(part[lane][row]);
-  const int of = blockIdx.x * 32 + row;
-  if (lane != 0 || of >= 2 * c) return;
-  if (of < c) { if (dbeta) dbeta[of] = t; }
-  else if (dgamma) dgamma[of - c] = t;
+  if (row != 0 || col >= 2 * c) return;
+  for (int k = 1; k < 8; ++k) t += part[k][lane];
+  if (col < c) { if (dbeta) dbeta[col] = t; }
+  else if (dgamma) dgamma[col - c] = t;
 }
 
 // ---------------------------------------------------------------- a slab through memory
@@ -705,26 +650,25 @@ constexpr int kMostShared = 225 * 1024, kShared = 227 * 1024;  // of a CTA, of a
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
-// CTAs of a cluster at most: their sums of channels are in the caller's scratch.
-int most_ctas(int hw) { return hw < 16 ? 1 : hw / 16 > 16 ? 16 : hw / 16; }
-
-// planes: tensors that the cluster holds (1 forward, 2 backward).  Of slabs of several widths and clusters of several sizes the pair is taken that is done
-// first by PLAN_COST
+// planes: tensors that the cluster holds (1 forward, 2 backward).  Of slabs of several widths (the widest for so many lanes) and clusters of several sizes the pair is
+// taken that is done first.  A turn of all SMs takes 6.5 us, 0.015 us for each value of each thread of an SM's CTAs and 0.01 for one thread's: hardly
+// more if four CTAs share an SM than if two do (256 x 128 x 56 x 56 forward: 13.8 turns of two CTAs of 100 KB or four of 51, 147 and 145 us; backward: 27.7
+// turns of two of 105 KB or three of 69, 300 and 292), so the number of turns decides, and what fills the shared memory wins.  Measured beside that: a single CTA
+// on an SM, with nobody beside it while it loads, 2.4 us; pieces of 32 bytes 3.7 (of 64 bytes 0.15); 16 CTAs wait 2 us longer for one another, one CTA for
+// nobody.  (30 x 150 x 37 x 41, groups of ten: 5 CTAs for 30 channels 28 us, 3 for 10 53 us.)
 Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
   Plan t{};
   const int each = c / groups;
   t.v = c % 4 == 0 && alignment % 16 == 0 ? 4 : c % 2 == 0 && alignment % 8 == 0 ? 2 : 1;
   const int unit = t.v / gcd(each, t.v);  // groups whose channels are whole vectors
-  const int sms = mtb_sm_count();
+  const int sms = mtb_sm_count(), of_vector = t.v / gcd(each, t.v);
   double best = 0;
-  for (int want = 8; want <= kThreads * t.v; want *= 2) {
-    int of_slab = ((want + each - 1) / each + unit - 1) / unit * unit;
+  for (int lanes = 1, before = 0; lanes <= kThreads; lanes *= 2) {
+    int of_slab = lanes * t.v / each / unit * unit;
     if (of_slab > groups) of_slab = groups;
-    const int wide = of_slab * each, vectors = wide / t.v;
-    if (vectors > kThreads) break;
-    int lanes = 1;
-    while (lanes < vectors) lanes *= 2;
-    const int rows = kThreads / lanes, slabs = (groups + of_slab - 1) / of_slab, of_vector = t.v / gcd(each, t.v);
+    if (of_slab == before) continue;
+    before = of_slab;
+    const int wide = of_slab * each, rows = kThreads / lanes, slabs = (groups + of_slab - 1) / of_slab;
     const long long units = (long long)n * slabs;
     // a group's lanes become one where they are a power of two of whole vectors
     int merged = 1;
@@ -732,14 +676,19 @@ Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
     const int entries = each * of_vector / t.v / merged, slots = lanes < 32 ? kWarps : rows;
     for (int ctas = 1; ctas <= 16; ctas = ctas == 8 ? 16 : ctas + 1) {
       const int stretch = (hw + ctas - 1) / ctas, steps = (stretch + rows - 1) / rows;
-      if ((ctas > 1 && ((hw + stretch - 1) / stretch != ctas || ctas > most_ctas(hw))) || units * ctas >= 1LL << 31) continue;
-      const long long sums = planes == 1 ? 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab) : rows * (2 * lanes * t.v + 4) + 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab);
+      if ((ctas > 1 && (hw + stretch - 1) / stretch != ctas) || units * ctas >= 1LL << 31) continue;
+      const long long sums = planes == 1 ? 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab) + 1 : 2 * lanes * t.v * (slots + 1 + ctas) + 2 * ctas * of_slab;
       const long long smem = 4 * ((long long)planes * stretch * lanes * t.v + sums);
       if (smem > kMostShared) continue;
-      int at_once = (int)(kShared / (smem + 1024));
+      int at_once = (int)(kShared / (smem + 1024));  // CTAs on an SM
       if (at_once > 4) at_once = 4;
-      const long long together = (long long)sms * at_once / ctas, rounds = together ? (units + together - 1) / together : units;
-      const double cost = rounds * (at_once * steps * t.v * planes * (wide < 16 ? 1.3 : 1.0) + (ctas > 1 ? 100 + 10 * ctas : 60));
+      double turns = (double)units * ctas / ((double)sms * at_once);
+      turns = turns > 1 ? turns + 0.25 : 1;
+      const long long there = (units * ctas + sms - 1) / sms;
+      if (there < at_once) at_once = (int)there;
+      const double values = (double)steps * t.v * planes;
+      const double cost = turns * (6.5 + 0.015 * at_once * values + 0.01 * values + (at_once == 1 && turns > 1 ? 2.4 : 0.0) +
+                                   (wide < 16 ? 3.7 : wide < 32 ? 0.15 : 0.0) + (ctas == 16 ? 2.0 : ctas == 1 ? -1.5 : 0.0));
       if (t.on_chip && cost >= best) continue;
       best = cost;
       t.on_chip = true;
@@ -815,8 +764,7 @@ int alignment_of(const void* a, const void* b, const void* c) {
 // Scratch of both directions: what slabs that go through memory leave of their stretches, and the backward's sums.
 MTB_API long long mtb_group_norm_workspace_bytes(int n, int c, int hw, int groups) {
   if (n <= 0 || c <= 0 || hw <= 0 || groups <= 0) return 256;
-  const long long forward = 12LL * n * groups * splits_of(n, hw, groups), splits = splits_of(n, hw, mtb_div_up(c, 32)),
-                  backward = 8LL * n * c * (splits > most_ctas(hw) ? splits : most_ctas(hw)) + 8LL * n * groups;
+  const long long forward = 12LL * n * groups * splits_of(n, hw, groups), backward = 8LL * n * c * splits_of(n, hw, mtb_div_up(c, 32)) + 8LL * n * groups;
   return (forward > backward ? forward : backward) + 256;
 }
 
@@ -876,6 +824,6 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
     if (dx) MTB_LAUNCH(gn_bwd_dx_kernel, dim3(mtb_stream_grid(image, 256), n), 256, 0, st, dy, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta,
                        activation, mean, rstd, of_group, dx);
   }
-  if (params) MTB_LAUNCH(gn_params_kernel, mtb_div_up(2LL * c, 32), 1024, 0, st, sums, t.on_chip ? n * t.s.ctas : n, c, dgamma, dbeta);
+  if (params) MTB_LAUNCH(gn_params_kernel, mtb_div_up(2LL * c, 32), 256, 0, st, sums, n, c, dgamma, dbeta);
   return MTB_OK;
 }
