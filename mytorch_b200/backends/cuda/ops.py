@@ -1202,29 +1202,19 @@ def cuda_sgd_multi(entries, lr, weight_decay, momentum, dampening, nesterov, max
 
 
 @_reg("cuda", "sgd_multi_clipped")
-def cuda_sgd_multi_clipped(groups, max_norm, grad_scale=1.0):
-    """groups: [(entries, lr, weight_decay, momentum, dampening, nesterov, maximize)], the entries those of ``sgd_multi``.  The gradients, times
-    ``grad_scale``, are clipped to the norm ``max_norm`` of all of them together on their way into the update; returns that norm."""
-    like = groups[0][0][0][0]
-    env = _env(like)
-    norm, sums = _norm_and_sums(env, like, sum([len(g[0]) for g in groups]))
+def cuda_sgd_multi_clipped(groups, states, max_norm, grad_scale=1.0):
+    """groups: [(params, lr, weight_decay, momentum, dampening, nesterov, maximize, set of those whose first update it is)], states: {param: {"momentum_buffer":
+    tensor}}.  The gradients, times ``grad_scale``, are clipped to the norm ``max_norm`` of all of them together on their way into the update; returns that
+    norm, a tensor of one element, or None where a tensor is missing, or is not float32 on the device of the first."""
     for group in groups:
-        _refuse_first_step_in_capture(env, any([f for _, _, f in group[0]]))
-    _binding.sgd_step_clipped(groups, grad_scale, sums, max_norm, norm, env.stream())
-    return norm
+        if group[7]:
+            _refuse_first_step_in_capture(CudaEnv.instance(), True)
+    return _binding.sgd_step_clipped(groups, states, grad_scale, max_norm)
 
 
 @_reg("cuda", "clip_gradients")
-def cuda_clip_gradients(grads, again, max_norm):
-    """The norm of the tensors of both lists together (one element, on the device).  With ``max_norm`` those of the first are multiplied by
-    min(1, max_norm / (norm + 1e-6)) in place; ``again`` holds tensors that are in the first list already, for gradients that share memory."""
-    _f32(*grads)
-    env = _env(grads[0])
-    norm, sums = _norm_and_sums(env, grads[0], len(grads) + len(again))
-    _binding.clip_gradients(grads, again, sums, -1.0 if max_norm is None else max_norm, norm, env.stream())
-    return norm
-
-
-def _norm_and_sums(env, like, count):
-    # the sums are read by launches of a later call, so they are not in the scratch that all operators share
-    return _new((1,), like, float32), CudaMemory(like.device.index, 8 * env.lib.grad_norm_sums(count))
+def cuda_clip_gradients(params, max_norm):
+    """The norm of the gradients of a list of parameters together, a tensor of one element.  With ``max_norm`` they are multiplied by
+    min(1, max_norm / (norm + 1e-6)) in place, memory that several of them share once.  None where there is none, or one is not float32 on the device of
+    the first."""
+    return _binding.clip_gradients(params, -1.0 if max_norm is None else max_norm)

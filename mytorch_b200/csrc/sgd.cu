@@ -37,6 +37,50 @@ __device__ __forceinline__ void sgd_span(float* p, const float* g, float* buf, l
   }
 }
 
+// sgd_span over at most VECTORS * 4 * 256 elements, the gradients times the factor that clips them (CTAs of 256 threads): everything is on its way
+// while the CTA adds up the norm.  The gradients were read just now, and some are still in L2: what is used once is marked to leave it first.
+// Bound by memory.  Norm and update of 161 tensors, 25.5 M elements, one step after the other: 97.7 us, 5.2 TB/s of the 20 bytes an element that an update
+// must move; the update without a norm 81 us.  Without the marks 100.9 us; chunks of 4096 elements 99.0 us, of 1024 103.9 us; the factor before the loads and
+// the chunks forwards 104 us.
+template <int VECTORS>
+__device__ __forceinline__ void sgd_span_clipped(float* p, const float* g, float* buf, int n, SgdHyper h, const MtbClip& clip) {
+  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(buf)) & 15u) != 0) {
+    h.grad_scale *= mtb_clip_factor<256>(clip);
+    sgd_span(p, g, buf, n, h, threadIdx.x, 256);
+    return;
+  }
+  float4 pp[VECTORS], gg[VECTORS], bb[VECTORS];
+#pragma unroll
+  for (int u = 0; u < VECTORS; ++u) {
+    const int v = threadIdx.x + u * 256;
+    bb[u] = make_float4(0, 0, 0, 0);
+    if (v < n / 4) {
+      gg[u] = __ldcs((const float4*)g + v);
+      pp[u] = __ldcs((const float4*)p + v);
+      if (!h.first) bb[u] = __ldcs((const float4*)buf + v);
+    }
+  }
+  h.grad_scale *= mtb_clip_factor<256>(clip);
+#pragma unroll
+  for (int u = 0; u < VECTORS; ++u) {
+    const int v = threadIdx.x + u * 256;
+    if (v < n / 4) {
+      sgd_update(pp[u].x, gg[u].x, bb[u].x, h);
+      sgd_update(pp[u].y, gg[u].y, bb[u].y, h);
+      sgd_update(pp[u].z, gg[u].z, bb[u].z, h);
+      sgd_update(pp[u].w, gg[u].w, bb[u].w, h);
+      __stcs((float4*)p + v, pp[u]);
+      __stcs((float4*)buf + v, bb[u]);
+    }
+  }
+  for (int t = n / 4 * 4 + threadIdx.x; t < n; t += 256) {
+    float q = p[t], b = h.first ? 0.f : buf[t];
+    sgd_update(q, g[t], b, h);
+    p[t] = q;
+    buf[t] = b;
+  }
+}
+
 __global__ void __launch_bounds__(256) sgd_kernel(float* p, const float* g, float* buf, long long n, SgdHyper h) {
   mtb_launch_dependents();
   mtb_wait_prior();
@@ -45,6 +89,7 @@ __global__ void __launch_bounds__(256) sgd_kernel(float* p, const float* g, floa
 
 constexpr int kMaxTensors = 96;
 constexpr int kSgdChunk = 4096;  // elements per CTA: four float4 per thread and array in flight
+constexpr int kClipChunk = 2048;  // of the clipped update: two float4 per thread and array
 struct SgdTable {
   float* p[kMaxTensors];
   const float* g[kMaxTensors];
@@ -57,22 +102,27 @@ struct SgdTable {
 
 // One CTA per chunk of kSgdChunk elements of one tensor (a model has a few large tensors and dozens of
 // tiny ones: a grid of tensors x the largest tensor's chunks would be mostly empty CTAs).
-// CLIP: the gradients are multiplied by the factor that clips them, which nothing writes back.
+// CLIP: the gradients are multiplied by the factor that clips them, which nothing writes back; the chunks are taken backwards.
 template <bool CLIP>
 __global__ void __launch_bounds__(256) sgd_multi_kernel(const __grid_constant__ SgdTable t, SgdHyper h, MtbClip clip) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  if (CLIP) h.grad_scale *= mtb_clip_factor<256>(clip);
+  const int chunk = CLIP ? t.chunk_start[t.count] - 1 - (int)blockIdx.x : (int)blockIdx.x;
+  if (CLIP && chunk < 0) {  // nothing to update: one CTA leaves the norm
+    mtb_clip_factor<256>(clip);
+    return;
+  }
   int lo = 0, hi = t.count - 1;
-  while (lo < hi) {  // last k with chunk_start[k] <= blockIdx.x
+  while (lo < hi) {  // last k with chunk_start[k] <= chunk
     const int mid = (lo + hi + 1) >> 1;
-    if (t.chunk_start[mid] <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
+    if (t.chunk_start[mid] <= chunk) lo = mid; else hi = mid - 1;
   }
   const int k = lo;
-  const long long e0 = (long long)((int)blockIdx.x - t.chunk_start[k]) * kSgdChunk;
+  const long long e0 = (long long)(chunk - t.chunk_start[k]) * (CLIP ? kClipChunk : kSgdChunk);
   const long long left = t.n[k] - e0;
   h.first = t.first[k];
-  sgd_span(t.p[k] + e0, t.g[k] + e0, t.buf[k] + e0, left < kSgdChunk ? left : kSgdChunk, h, threadIdx.x, blockDim.x);
+  if (CLIP) sgd_span_clipped<kClipChunk / 1024>(t.p[k] + e0, t.g[k] + e0, t.buf[k] + e0, left < kClipChunk ? (int)left : kClipChunk, h, clip);
+  else sgd_span(t.p[k] + e0, t.g[k] + e0, t.buf[k] + e0, left < kSgdChunk ? left : kSgdChunk, h, threadIdx.x, blockDim.x);
 }
 
 // Gather `count` gradient tensors into one flat buffer, scaling on the way.
@@ -113,7 +163,9 @@ static int sgd_multi(int count, float* const* params, const float* const* grads,
                      void* stream) {
   MTB_REQUIRE(count >= 0 && (count == 0 || (params && grads && momentum_buffers && sizes && is_first)), "sgd_multi: bad arguments");
   SgdHyper h{(float)lr, (float)weight_decay, (float)momentum, (float)(1.0 - dampening), (float)grad_scale, nesterov, maximize, 0};
-  for (int base = 0; base < count; base += kMaxTensors) {
+  const int chunk = clip.sums ? kClipChunk : kSgdChunk, last = count > 0 ? (count - 1) / kMaxTensors * kMaxTensors : -1;
+  for (int turn = 0; turn <= last; turn += kMaxTensors) {
+    const int base = clip.sums ? last - turn : turn;
     SgdTable t;
     t.count = count - base < kMaxTensors ? count - base : kMaxTensors;
     long long chunks = 0;
@@ -125,11 +177,11 @@ static int sgd_multi(int count, float* const* params, const float* const* grads,
       t.n[k] = sizes[base + k];
       t.first[k] = is_first[base + k];
       t.chunk_start[k] = (int)chunks;
-      chunks += (t.n[k] + kSgdChunk - 1) / kSgdChunk;
+      chunks += (t.n[k] + chunk - 1) / chunk;
       MTB_REQUIRE(chunks < (1LL << 30), "sgd_multi: too many elements in one call");
     }
     t.chunk_start[t.count] = (int)chunks;
-    if (chunks == 0 && clip.norm) chunks = 1;  // nothing to update: one CTA leaves the norm
+    if (chunks == 0 && clip.norm) chunks = 1;  // for the norm
     if (chunks == 0) continue;
     dim3 grid((unsigned int)chunks);
     MTB_LAUNCH(clip.sums ? sgd_multi_kernel<true> : sgd_multi_kernel<false>, grid, 256, 0, (cudaStream_t)stream, t, h, clip);

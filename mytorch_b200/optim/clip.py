@@ -1,6 +1,7 @@
 """The norm of all gradients together, and clipping by it (no counterpart in the reference)."""
+from mytorch_b200.dtype import float32
 from mytorch_b200.ops._common import dispatch
-from mytorch_b200.tensor import MismatchDevicesError, Tensor
+from mytorch_b200.tensor import InvalidDataTypeError, MismatchDevicesError, Tensor
 
 
 def grad_norm(params):
@@ -20,23 +21,17 @@ def clip_grad_norm_(params, max_norm):
 
 
 def _clip(params, max_norm):
-    grads, again, known = [], [], set()
-    device = None
-    for p in [params] if isinstance(params, Tensor) else params:
-        grad = p.grad
-        if grad is None:
-            continue
-        if device is None:
-            device = grad.device
-        elif grad.device is not device:
-            raise MismatchDevicesError([device, grad.device])
-        memory = grad._native_array
-        at = id(grad) if memory is None else memory.ptr
-        if at in known and 0 not in grad.shape:
-            again.append(grad)
-        else:
-            known.add(at)
-            grads.append(grad)
-    if device is None:
+    params = [params] if isinstance(params, Tensor) else list(params)
+    for p in params:
+        if p.grad is not None:
+            norm = dispatch(p.grad.device, "clip_gradients")(params, max_norm)
+            if norm is not None:
+                return norm
+            break
+    else:
         raise RuntimeError("there is no gradient to take the norm of")
-    return dispatch(device, "clip_gradients")(grads, again, max_norm)
+    grads = [p.grad for p in params if p.grad is not None]  # what is wrong with one of them
+    for g in grads:
+        if g.device is not grads[0].device:
+            raise MismatchDevicesError([grads[0].device, g.device])
+    raise InvalidDataTypeError([g.dtype for g in grads if g.dtype is not float32])
