@@ -9,46 +9,52 @@ __device__ __forceinline__ long long token_at(const void* tokens, long long i) {
 
 // ---------------------------------------------------------------- lookup
 
+// Bound by memory: 131072 rows of 512 values out of 50000, 318 MB read and written at least: 50.3 us, 6.3 TB/s.  Two steps ahead 53.7 us, eight (fewer threads) 58.7;
+// a result that is not marked 53.2; steps a grid apart instead of side by side 55.2; as many CTAs as fit the SMs, with a loop, 57.4.  Eight
+// tokens: a launch.
 constexpr int kLookupAhead = 4;
+constexpr long long kStreamed = 64 << 20;  // bytes: half of L2
 
-// One value or four a thread and step, kLookupAhead steps at a time: tokens, then rows, then results.
-template <class T, int V, class I>
+// One value or four a thread and step, kLookupAhead steps at once: tokens, then rows, then results.  STREAM: the result is more than L2 holds, and is
+// marked to leave it first, so that rows which are read again stay.
+template <class T, int V, class I, bool STREAM>
 __global__ void __launch_bounds__(256) embedding_rows_kernel(const void* __restrict__ tokens, I total, int rows, int width, PoolDiv by_row, const float* __restrict__ table,
                                                               float scale, float* __restrict__ out) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const I per = (I)gridDim.x * 256, vectors = width / V;
-  for (I k0 = (I)blockIdx.x * 256 + threadIdx.x; k0 < total; k0 += per * kLookupAhead) {
-    long long t[kLookupAhead];
-    unsigned col[kLookupAhead];
-    VecF<V> v[kLookupAhead];
+  const I k0 = (I)blockIdx.x * 256 * kLookupAhead + threadIdx.x, per = 256, vectors = width / V;
+  long long t[kLookupAhead];
+  unsigned col[kLookupAhead];
+  VecF<V> v[kLookupAhead];
 #pragma unroll
-    for (int u = 0; u < kLookupAhead; ++u) {
-      const I k = k0 + per * u;
-      t[u] = -1;
-      col[u] = 0;
-      if (k < total) {
-        I row;
-        if (sizeof(I) == 4) row = by_row.divmod((unsigned)k, col[u]);
-        else { row = k / vectors; col[u] = (unsigned)(k - row * vectors); }
-        t[u] = token_at<T>(tokens, row);
-      }
+  for (int u = 0; u < kLookupAhead; ++u) {
+    const I k = k0 + per * u;
+    t[u] = -1;
+    col[u] = 0;
+    if (k < total) {
+      I row;
+      if (sizeof(I) == 4) row = by_row.divmod((unsigned)k, col[u]);
+      else { row = k / vectors; col[u] = (unsigned)(k - row * vectors); }
+      t[u] = token_at<T>(tokens, row);
     }
+  }
 #pragma unroll
-    for (int u = 0; u < kLookupAhead; ++u) {
-      if (t[u] >= 0 && t[u] < rows) v[u] = vload<V>(table + t[u] * width + (long long)col[u] * V);
-      else
+  for (int u = 0; u < kLookupAhead; ++u) {
+    if (t[u] >= 0 && t[u] < rows) v[u] = vload<V>(table + t[u] * width + (long long)col[u] * V);
+    else
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[u].v[i] = __int_as_float(0x7fc00000);
-    }
+      for (int i = 0; i < V; ++i) v[u].v[i] = __int_as_float(0x7fc00000);
+  }
 #pragma unroll
-    for (int u = 0; u < kLookupAhead; ++u) {
-      const I k = k0 + per * u;
-      if (k >= total) break;
+  for (int u = 0; u < kLookupAhead; ++u) {
+    const I k = k0 + per * u;
+    if (k >= total) break;
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[u].v[i] *= scale;
-      vstore<V>(out + (long long)k * V, v[u]);
-    }
+    for (int i = 0; i < V; ++i) v[u].v[i] *= scale;
+    float* to = out + (long long)k * V;
+    if (!STREAM) vstore<V>(to, v[u]);
+    else if (V == 4) __stcs((float4*)to, make_float4(v[u].v[0], v[u].v[1 % V], v[u].v[2 % V], v[u].v[3 % V]));
+    else __stcs(to, v[u].v[0]);
   }
 }
 
@@ -56,10 +62,15 @@ template <class T>
 int lookup(const void* tokens, long long count, int rows, int width, const float* table, float scale, float* out, cudaStream_t st) {
   const bool four = width % 4 == 0 && mtb_aligned16(table) && mtb_aligned16(out);
   const long long total = count * (four ? width / 4 : width);
-  const int grid = mtb_stream_grid((total + kLookupAhead - 1) / kLookupAhead, 256);
+  const long long grid = (total + 256 * kLookupAhead - 1) / (256 * kLookupAhead);
+  MTB_REQUIRE(grid < 1LL << 31, "embedding_forward: too many values");
   const PoolDiv by_row((unsigned)(four ? width / 4 : width));
-  const bool wide = total + (long long)grid * 256 * kLookupAhead >= 1LL << 31;
-#define MTB_LOOKUP(V, I) MTB_LAUNCH((embedding_rows_kernel<T, V, I>), grid, 256, 0, st, tokens, (I)total, rows, width, by_row, table, scale, out)
+  const bool wide = total + 256 * kLookupAhead >= 1LL << 31, stream = 4 * count * width > kStreamed;
+#define MTB_LOOKUP(V, I)                                                                                                              \
+  do {                                                                                                                                \
+    if (stream) MTB_LAUNCH((embedding_rows_kernel<T, V, I, true>), (int)grid, 256, 0, st, tokens, (I)total, rows, width, by_row, table, scale, out); \
+    else MTB_LAUNCH((embedding_rows_kernel<T, V, I, false>), (int)grid, 256, 0, st, tokens, (I)total, rows, width, by_row, table, scale, out);       \
+  } while (0)
   if (four && wide) MTB_LOOKUP(4, long long);
   else if (four) MTB_LOOKUP(4, int);
   else if (wide) MTB_LOOKUP(1, long long);
@@ -369,6 +380,19 @@ __device__ __forceinline__ void clear_rows(const SumPlan& p, int block) {
   }
 }
 
+// A load that L2 need not keep.
+template <int V>
+__device__ __forceinline__ VecF<V> vload_once(const float* p) {
+  VecF<V> r;
+  if (V == 4) {
+    const float4 t = __ldcs((const float4*)p);
+    r.v[0] = t.x; r.v[1 % V] = t.y; r.v[2 % V] = t.z; r.v[3 % V] = t.w;
+  } else {
+    r.v[0] = __ldcs(p);
+  }
+  return r;
+}
+
 template <int V>
 __global__ void __launch_bounds__(128) embedding_sum_kernel(SumPlan p) {
   // keys from kRun before a tile to kRun behind it; one more on either side tells where a run ends
@@ -445,7 +469,7 @@ __global__ void __launch_bounds__(128) embedding_sum_kernel(SumPlan p) {
     VecF<V> v[kSumAhead];
 #pragma unroll
     for (int u = 0; u < kSumAhead; ++u)
-      if (e + u < to) v[u] = vload<V>(dy + (long long)places[e + u] * p.width);
+      if (e + u < to) v[u] = vload_once<V>(dy + (long long)places[e + u] * p.width);
 #pragma unroll
     for (int u = 0; u < kSumAhead; ++u) {
       if (e + u >= to) break;
