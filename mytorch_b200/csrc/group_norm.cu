@@ -9,10 +9,12 @@
 // a slab, some whole groups of one image, in its shared memory, each CTA a stretch of the positions; four CTAs or so on an SM, one of which loads
 // while another one adds up or stores.  A thread copies (cp.async) and later reads its own vectors only, so the copies need no barrier; the CTAs exchange their sums
 // through distributed shared memory.
-// 256 x 128 x 56 x 56 with SiLU: forward 145 us (5.7 TB/s, 87 % of a copy), backward 295 (4.2 TB/s).  What bounds it now: the CTAs of a cluster wait for the
-// slowest of them, and an SM has two to four beside one another (backward without the exchange 190 us, with the exchange but alone in a cluster
-// 230).  Tried: clusters that stay and fetch the next slab meanwhile (forward 155 us, backward 337), sums sent with st.async (152, 319), two readings from the L2 cache
-// by tickets or by launches (backward 377).
+// 256 x 128 x 56 x 56 with SiLU: forward 144 us (5.7 TB/s, 87 % of a copy), backward 247 (5.0 TB/s, 76 %).  What bounds the backward now: a CTA's time from its
+// last value to its first store, in which the cluster waits for its slowest, and an SM has four of them to overlap (backward without the exchange 190 us).
+// It went from 292 us by instructions and waits taken out of that time: xh recomputed instead of written back 275, sums over rows all at once 258 and by halves 250,
+// gamma from shared memory 247.  The 64 registers of four CTAs are what it may not pass: 12 bytes spilled cost 20 us.  Tried: clusters that stay and fetch
+// the next slab meanwhile (forward 155 us, backward 337), sums sent with st.async (152, 319), two readings from the L2 cache by tickets or by launches (backward
+// 377), adding up while copies are on their way (+1 % to +11 %), marks for L2 (no change), CTAs that begin one after another (no change).
 // A slab that no cluster can hold goes through memory twice instead, see the kernels at the end.
 #include "colreduce.cuh"
 #include <cooperative_groups.h>
@@ -45,8 +47,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 template <int V>
-__device__ __forceinline__ void copy_async(float* to, const float* from) {
-  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+__device__ __forceinline__ void copy_async(unsigned at, const float* from) {
   if (V == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
   else if (V == 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at), "l"(from) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
@@ -129,7 +130,7 @@ struct Slabs {
   int steps;                // positions of a thread at most
   // A slot is what a warp makes of its rows, or a row of more than a warp.  Where a thread's channels are of several groups it has several entries in it; `merged`
   // lanes' entries are made one, and a group has `entries` of them.
-  int of_vector, entries, merged, slots, slot_rows;
+  int of_vector, entries, merged, slots, slot_rows, slot_stride;
   bool vectors;                    // gamma and beta can be read as the values are
   float inv_positions, inv_group;  // 1 / hw, 1 / M
   PoolDiv by_slabs, by_each, by_groups;
@@ -180,13 +181,13 @@ struct Unit {
   }
 };
 
-// f(j) for the thread's steps, four at a time; `full` is the same for all threads that have any.
-template <class F>
+// f(j) for the thread's steps, U at a time; `full` is the same for all threads that have any.
+template <int U = 4, class F>
 __device__ __forceinline__ void each_step(int full, int steps, F f) {
   int j = 0;
-  for (; j + 4 <= full; j += 4) {
+  for (; j + U <= full; j += U) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) f(j + u);
+    for (int u = 0; u < U; ++u) f(j + u);
   }
   for (; j < full; ++j) f(j);
   if (j < steps) f(j);
@@ -264,7 +265,8 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
   const unsigned step = p.rows * p.c;  // of an image's values
   mtb_wait_prior();
   const float* from = x + u.first(p, s);
-  each_step(full, steps, [&](int j) { copy_async<V>(mine + j * kThreads * V, from + j * step); });
+  const unsigned at = (unsigned)__cvta_generic_to_shared(mine);
+  each_step(full, steps, [&](int j) { copy_async<V>(at + j * kThreads * V * 4, from + j * step); });
   Vec<V> scale = parameter<V>(gamma + u.c0 + s.col, gamma && active, p.vectors, 1.f);
   const Vec<V> shift = parameter<V>(beta + u.c0 + s.col, beta && active, p.vectors, 0.f);
   copies_done();
@@ -337,19 +339,64 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
   });
 }
 
+// Sums of a and b over the lanes of a warp that hold the same channels, to `to` and to [lanes * V] behind.  While a lane has several values, it gives half of them
+// to the lane opposite for half of its own: 7 shuffles for 8 values of 8 rows instead of 24.
+template <int V>
+__device__ __forceinline__ void add_rows(Vec<V> a, Vec<V> b, int lane, int lanes, float* to) {
+  if (lanes >= 32) {
+    vec<V>(to) = a;
+    vec<V>(to + lanes * V) = b;
+    return;
+  }
+  bool upper = lane & 16;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float give = upper ? a.v[i] : b.v[i], keep = upper ? b.v[i] : a.v[i];
+    a.v[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+  }
+  if (upper) to += lanes * V;
+  int o = 8;
+  if (V == 4) {
+    if (lanes > 8) { vec<V>(to) = a; return; }
+    upper = lane & 8;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float give = upper ? a.v[i] : a.v[V / 2 + i], keep = upper ? a.v[V / 2 + i] : a.v[i];
+      a.v[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+    }
+    if (upper) to += 2;
+    o = 4;
+  }
+  if (V >= 2) {
+    if (lanes > o) { vec<2>(to) = Vec<2>{{a.v[0], a.v[1 % V]}}; return; }
+    upper = lane & o;
+    const float give = upper ? a.v[0] : a.v[1 % V], keep = upper ? a.v[1 % V] : a.v[0];
+    a.v[0] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    if (upper) to += 1;
+    o >>= 1;
+  }
+  float t = a.v[0];
+  int first = 0;  // of the lanes that differ in these bits one writes
+  for (; o >= lanes; o >>= 1) {
+    t += __shfl_xor_sync(0xffffffffu, t, o);
+    first |= o;
+  }
+  if ((lane & first) == 0) *to = t;
+}
+
 // sums (may be NULL): per image and channel the sums of dz and of dz xh, [n][2][c].  dx may be NULL.
 template <int V, int ACT>
 __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_constant__ Slabs p, const float* __restrict__ dy, const float* __restrict__ x,
                                                                    const float* __restrict__ gamma, const float* __restrict__ beta,
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ dx,
                                                                    float* __restrict__ sums) {
-  extern __shared__ __align__(16) float held[];  // [2][positions][lanes][V]; the warps' sums; the CTA's, weighted; the CTAs' of channels and of groups
+  extern __shared__ __align__(16) float held[];  // [2][positions][lanes][V]; the warps' sums; the CTAs' of channels and of groups
   mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
   const Unit u(p, blockIdx.x / p.ctas);
   const int plane = p.stretch * p.lanes * V, both = 2 * p.lanes * V;  // two sums of each channel
-  float *mine = held + threadIdx.x * V, *of_warp = held + 2 * plane, *weighted = of_warp + p.slots * both, *of_channel = weighted + both;
+  float *mine = held + threadIdx.x * V, *of_warp = held + 2 * plane, *weights = of_warp + p.slots * p.slot_stride, *of_channel = weights + (p.lanes * V + 3 & ~3);
   float2* of_cta = (float2*)(of_channel + p.ctas * both);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool active = s.col < u.width;
@@ -358,10 +405,14 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
   mtb_wait_prior();
   {
     const float *from = x + u.first(p, s), *from2 = dy + u.first(p, s);
+    const unsigned at = (unsigned)__cvta_generic_to_shared(mine);
     each_step(full, steps, [&](int j) {
-      copy_async<V>(mine + j * kThreads * V, from + j * step);
-      copy_async<V>(mine + plane + j * kThreads * V, from2 + j * step);
+      copy_async<V>(at + j * kThreads * V * 4, from + j * step);
+      copy_async<V>(at + plane * 4 + j * kThreads * V * 4, from2 + j * step);
     });
+  }
+  for (int ch = threadIdx.x; ch < u.width; ch += kThreads) {  // for the groups' sums
+    if (gamma) copy_async<1>((unsigned)__cvta_generic_to_shared(weights + ch), gamma + u.c0 + ch); else weights[ch] = 1.f;
   }
   Vec<V> ga = parameter<V>(gamma + u.c0 + s.col, gamma && active, p.vectors, 1.f);
   const Vec<V> be = parameter<V>(beta + u.c0 + s.col, beta && active, p.vectors, 0.f);
@@ -379,48 +430,43 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
       }
     }
   }
+  ga = mul(ga, r);
   copies_done();
-  each_step(full, steps, [&](int j) {  // xh and dz take the places of x and dy
-    const Vec<V> v = mul(add(vec<V>(mine + j * kThreads * V), minus), r);
+  each_step<6>(full, steps, [&](int j) {  // dz takes the place of dy
+    const Vec<V> v = add(vec<V>(mine + j * kThreads * V), minus);
     const Vec<V> d = activated_grad<V, ACT>(vec<V>(mine + plane + j * kThreads * V), fma(v, ga, be));
     a = add(a, d);
     b = fma(d, v, b);
-    vec<V>(mine + j * kThreads * V) = v;
     if (ACT != ACT_NONE) vec<V>(mine + plane + j * kThreads * V) = d;
   });
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    a.v[i] = sum_rows(a.v[i], p);
-    b.v[i] = sum_rows(b.v[i], p);
-  }
-  if (lane < p.lanes) {
-    vec<V>(of_warp + s.slot(p) * both + s.col) = a;
-    vec<V>(of_warp + s.slot(p) * both + p.lanes * V + s.col) = b;
-  }
-  __syncthreads();
-  for (int k = threadIdx.x; k < both; k += kThreads) {  // the CTA's
-    const int second = k >= p.lanes * V, ch = k - (second ? p.lanes * V : 0);
-    if (ch >= u.width) continue;
-    const float weight = gamma ? gamma[u.c0 + ch] : 1.f;
-    float t = 0.f;
-#pragma unroll 8
-    for (int w = 0; w < p.slots; ++w) t += of_warp[w * both + k];
-    weighted[k] = t * weight;
-    if (!sums) continue;
-    if (p.ctas > 1) cluster.map_shared_rank(of_channel, 0)[s.rank * both + k] = t;
-    else sums[((long long)u.n * 2 + second) * p.c + u.c0 + ch] = t;
-  }
+  b = mul(b, r);
+  add_rows<V>(a, b, lane, p.lanes, of_warp + s.slot(p) * p.slot_stride + s.col);
   __syncthreads();
   if (dx) {
+    const int entries = p.each * p.slots;
     for (int g = warp; g < u.groups; g += kWarps) {  // the group's in the CTA, given to each CTA of the cluster
       float t = 0.f, t2 = 0.f;
-      for (int ch = g * p.each + lane; ch < (g + 1) * p.each; ch += 32) {
-        t += weighted[ch];
-        t2 += weighted[p.lanes * V + ch];
+      for (int e = lane; e < entries; e += 32) {
+        unsigned in;
+        const float* from = of_warp + p.by_each.divmod((unsigned)e, in) * p.slot_stride + g * p.each;
+        const float weight = weights[g * p.each + in];
+        t = fmaf(weight, from[in], t);
+        t2 = fmaf(weight, from[p.lanes * V + in], t2);
       }
       const float2 both_sums = make_float2(warp_sum(t) * p.inv_group, warp_sum(t2) * p.inv_group);
       float2* to = of_cta + s.rank * p.of_slab + g;
       if (lane < p.ctas) *(p.ctas > 1 ? cluster.map_shared_rank(to, lane) : to) = both_sums;
+    }
+  }
+  if (sums) {
+    for (int k = kThreads - 1 - threadIdx.x; k < both; k += kThreads) {  // the CTA's of its channels, by the warps without a group
+      const int second = k >= p.lanes * V, ch = k - (second ? p.lanes * V : 0);
+      if (ch >= u.width) continue;
+      float t = 0.f;
+#pragma unroll 8
+      for (int w = 0; w < p.slots; ++w) t += of_warp[w * p.slot_stride + k];
+      if (p.ctas > 1) cluster.map_shared_rank(of_channel, 0)[s.rank * both + k] = t;
+      else sums[((long long)u.n * 2 + second) * p.c + u.c0 + ch] = t;
     }
   }
   if (p.ctas > 1) cluster.sync(); else __syncthreads();
@@ -436,26 +482,32 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
   }
   if (!dx) return;
   float group_a = 0.f, group_b = 0.f;  // -A / M, -B / M
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (active && (i == 0 || s.group[i] != s.group[i - 1 < 0 ? 0 : i - 1])) {
-      group_a = group_b = 0.f;
+  auto add_up = [&](int group) {
+    group_a = group_b = 0.f;
 #pragma unroll 8
-      for (int q = 0; q < p.ctas; ++q) {
-        const float2 e = of_cta[q * p.of_slab + s.group[i]];
-        group_a -= e.x;
-        group_b -= e.y;
-      }
+    for (int q = 0; q < p.ctas; ++q) {
+      const float2 e = of_cta[q * p.of_slab + group];
+      group_a -= e.x;
+      group_b -= e.y;
     }
-    a.v[i] = group_a;
-    b.v[i] = group_b;
+  };
+  if (p.of_vector == 1) {
+    if (active) add_up(s.group[0]);
+    a = all<V>(group_a);
+    b = all<V>(group_b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (active && (i == 0 || s.group[i] != s.group[i - 1 < 0 ? 0 : i - 1])) add_up(s.group[i]);
+      a.v[i] = group_a;
+      b.v[i] = group_b;
+    }
   }
   a = mul(a, r);
-  b = mul(b, r);
-  ga = mul(ga, r);
+  b = mul(mul(b, r), r);
   float* to = dx + u.first(p, s);
-  each_step(full, steps, [&](int j) {
-    *reinterpret_cast<Vec<V>*>(to + j * step) = fma(vec<V>(mine + j * kThreads * V), b, fma(ga, vec<V>(mine + plane + j * kThreads * V), a));
+  each_step<2>(full, steps, [&](int j) {
+    *reinterpret_cast<Vec<V>*>(to + j * step) = fma(add(vec<V>(mine + j * kThreads * V), minus), b, fma(ga, vec<V>(mine + plane + j * kThreads * V), a));
   });
 }
 
@@ -673,11 +725,11 @@ Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
     // a group's lanes become one where they are a power of two of whole vectors
     int merged = 1;
     if (of_vector == 1 && ((each / t.v) & (each / t.v - 1)) == 0) merged = each / t.v < 32 ? each / t.v : 32;
-    const int entries = each * of_vector / t.v / merged, slots = lanes < 32 ? kWarps : rows;
+    const int entries = each * of_vector / t.v / merged, slots = lanes < 32 ? kWarps : rows, slot_stride = 2 * lanes * t.v + 4;
     for (int ctas = 1; ctas <= 16; ctas = ctas == 8 ? 16 : ctas + 1) {
       const int stretch = (hw + ctas - 1) / ctas, steps = (stretch + rows - 1) / rows;
       if ((ctas > 1 && (hw + stretch - 1) / stretch != ctas) || units * ctas >= 1LL << 31) continue;
-      const long long sums = planes == 1 ? 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab) + 1 : 2 * lanes * t.v * (slots + 1 + ctas) + 2 * ctas * of_slab;
+      const long long sums = planes == 1 ? 2 * (slots * (lanes * of_vector / merged) + ctas * of_slab) + 1 : slots * slot_stride + (lanes * t.v + 3 & ~3) + ctas * (2 * lanes * t.v + 2 * of_slab);
       const long long smem = 4 * ((long long)planes * stretch * lanes * t.v + sums);
       if (smem > kMostShared) continue;
       int at_once = (int)(kShared / (smem + 1024));  // CTAs on an SM
@@ -694,7 +746,7 @@ Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
       t.on_chip = true;
       t.smem = (int)smem;
       t.s = Slabs{hw, c, groups, each, wide, slabs, (int)units, of_slab, ctas, stretch, lanes, rows, __builtin_ctz(lanes), __builtin_ctz(rows), steps,
-                  of_vector, entries, merged, slots, lanes < 32 ? 32 / lanes : 1, false, 1.f / (float)hw, (float)(1.0 / ((double)each * hw)),
+                  of_vector, entries, merged, slots, lanes < 32 ? 32 / lanes : 1, slot_stride, false, 1.f / (float)hw, (float)(1.0 / ((double)each * hw)),
                   PoolDiv((unsigned)slabs), PoolDiv((unsigned)each), PoolDiv((unsigned)of_slab)};
     }
     if (of_slab == groups) break;
