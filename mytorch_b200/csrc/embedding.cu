@@ -344,6 +344,10 @@ __global__ void __launch_bounds__(kSortThreads) embedding_place_kernel(const voi
 // The ordered tokens are cut into tiles of `tile`.  A run of equal tokens of up to kRun is added up by the tile it begins in, past the tile's end if need be,
 // and goes to the table; a longer one is added up piece by piece, each tile its own, and the pieces are added by the kernel behind, in
 // their order.  Frequent tokens thus keep no tile waiting, and the rest has no second step.
+//
+// Bound by memory: 131072 tokens of 512 values to 50000 rows 64 us, 5.8 TB/s of the 371 MB of gradients read and rows written; 90 us with the ordering (19) and the
+// joining (12, the pieces of the most frequent token one after another).  Sixteen rows ahead 94 us in all, runs of 16 96; 4096 tokens are 2 us faster
+// with runs of 16.
 constexpr int kRun = 32, kMaxTile = kRun, kSumAhead = 8;  // a longer tile could hold a whole long run
 
 struct SumPlan {
@@ -486,7 +490,7 @@ __global__ void __launch_bounds__(128) embedding_sum_kernel(SumPlan p) {
   flush(true);
 }
 
-constexpr int kJoinThreads = 256, kJoinAhead = 4;
+constexpr int kJoinThreads = 256, kJoinAhead = 4;  // eight ahead spill: 102 us of the whole gradient above instead of 91; 512 threads 95
 
 // One CTA a long run and 32 lanes' columns: its warps add up a part of the pieces each, and those sums are added in their order.
 template <int V>

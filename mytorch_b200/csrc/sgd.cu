@@ -39,9 +39,9 @@ __device__ __forceinline__ void sgd_span(float* p, const float* g, float* buf, l
 
 // sgd_span over at most VECTORS * 4 * 256 elements, the gradients times the factor that clips them (CTAs of 256 threads): everything is on its way
 // while the CTA adds up the norm.  The gradients were read just now, and some are still in L2: what is used once is marked to leave it first.
-// Bound by memory.  Norm and update of 161 tensors, 25.5 M elements, one step after the other: 97.7 us, 5.2 TB/s of the 20 bytes an element that an update
-// must move; the update without a norm 81 us.  Without the marks 100.9 us; chunks of 4096 elements 99.0 us, of 1024 103.9 us; the factor before the loads and
-// the chunks forwards 104 us.
+// Bound by memory.  Norm and update of 161 tensors, 25.6 M elements, one step after the other: 93.5 us, 5.5 TB/s of the 20 bytes an element that an update
+// must move; the update without a norm 81 us.  Measured when the norm took 4 us longer: 97.7; without the marks 100.9; chunks of 4096 elements 99.0, of 1024
+// 103.9; the factor before the loads and the chunks forwards 104.
 template <int VECTORS>
 __device__ __forceinline__ void sgd_span_clipped(float* p, const float* g, float* buf, int n, SgdHyper h, const MtbClip& clip) {
   if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(buf)) & 15u) != 0) {
