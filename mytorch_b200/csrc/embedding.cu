@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_place_kernel(const voi
   static_assert(kSortWarps == 16, "a stretch is a sixteenth of a share");
   auto bounded = [&](int i) { return i < p.count ? i : p.count; };
   const int lo = bounded(first + warp * each), hi = bounded(first + (warp + 1) * each), share = bounded(first + (1 << p.share_bits)) - first;
-  const bool held = each <= 32 * kSortAhead, stage = share <= kStaged;
+  const bool held = each <= 32 * kSortAhead, stage = 1 << p.share_bits <= kStaged;  // of all CTAs, whose shared memory the launch sized
   for (int i = threadIdx.x; i < kSortWarps * kDigits / 4; i += kSortThreads) ((int4*)sh.counters)[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
   int2 entry[kSortAhead];

@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
     }
   }
   a = mul(a, r);
-  b = mul(mul(b, r), r);
+  b = mul(mul(b, r), r);  // of x - mean; finite for every r below 1.8e19, as any eps of 1e-38 makes it
   float* to = dx + u.first(p, s);
   each_step<2>(full, steps, [&](int j) {
     *reinterpret_cast<Vec<V>*>(to + j * step) = fma(add(vec<V>(mine + j * kThreads * V), minus), b, fma(ga, vec<V>(mine + plane + j * kThreads * V), a));

@@ -240,3 +240,57 @@ def test_example_learns():
 
     losses, accuracy = train_token_cnn(steps=300, log=lambda line: None)
     assert np.isfinite(losses).all() and np.mean(losses[-20:]) < 0.5 * np.mean(losses[:20]) and accuracy > 0.8
+
+
+def test_parameters_that_join_later():
+    """A group that joins after the first step has its first update among others that have had theirs."""
+    import gpu_util as g
+    import mytorch_b200.nn as nn
+    from mytorch_b200.optim import SGD
+
+    rng = np.random.default_rng(12)
+    values = [rng.standard_normal(s).astype(np.float32) for s in (300, 5000, 9)]
+    params = [nn.Parameter(g.dev(v)) for v in values]
+    opt = SGD(params[:1], lr=0.1, momentum=0.9, max_grad_norm=0.5)
+    want, bufs = [v.astype(np.float64) for v in values], [np.zeros(v.shape) for v in values]
+    for step in range(3):
+        if step == 1:
+            opt.param_groups.append(dict(opt.param_groups[0], params=params[1:]))
+        grads = [rng.standard_normal(v.shape).astype(np.float32) for v in values[:3 if step else 1]]
+        for p, a in zip(params, grads):
+            p.grad = g.dev(a)
+        opt.step()
+        factor = min(1.0, 0.5 / (_norm(grads) + 1e-6))
+        for k, a in enumerate(grads):
+            want[k], bufs[k] = _sgd(want[k], a.astype(np.float64), bufs[k], factor, 0.1, 0.0, 0.9, False, False, 1.0, step == (k > 0))
+            assert (np.abs(g.host(params[k]) - want[k]) <= 40 * U * (np.abs(want[k]) + 2 * np.abs(bufs[k]) + np.abs(a) + 1)).all()
+
+
+def test_refusals_of_a_step():
+    import gpu_util as g
+    import mytorch_b200 as mt
+    import mytorch_b200.nn as nn
+    from mytorch_b200.optim import SGD, clip_grad_norm_
+    from mytorch_b200.tensor import InvalidDataTypeError, MismatchDevicesError
+
+    p, q = nn.Parameter(g.dev(np.ones(8, np.float32))), nn.Parameter(g.dev(np.ones((2, 4), np.float32)))
+    opt = SGD([p, q], lr=1.0, momentum=0.9, max_grad_norm=100.0)
+    p.grad = g.dev(np.ones(8, np.float32))
+    for wrong, error in ((np.ones((4, 2), np.float32), RuntimeError), (np.ones((2, 4), np.int64), InvalidDataTypeError)):
+        q.grad = g.dev(wrong)
+        with pytest.raises(error):
+            opt.step()
+        assert not opt.state and (g.host(p) == 1).all()
+    with pytest.raises(InvalidDataTypeError):
+        clip_grad_norm_([p, q], 1.0)
+    q.grad = mt.tensor(np.ones((2, 4), np.float32))
+    for call in (opt.step, lambda: clip_grad_norm_([p, q], 1.0)):
+        with pytest.raises((RuntimeError, MismatchDevicesError)):
+            call()
+    assert (g.host(p.grad) == 1).all()
+    q.grad = g.dev(np.ones((2, 4), np.float32))
+    opt.step()
+    opt.state[q]["momentum_buffer"] = g.dev(np.ones(3, np.float32))
+    with pytest.raises(RuntimeError, match="momentum buffer"):
+        opt.step()
+    assert (g.host(p) == 0).all()

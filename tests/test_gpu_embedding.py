@@ -196,3 +196,62 @@ def test_the_layer_and_a_table_used_twice():
     (layer(g.dev(a)) * g.dev(dy[0]) + layer(g.dev(b)) * g.dev(dy[1])).sum().backward()
     want, bound = _gradient(np.concatenate([a, b]), dy, 20, 1.0, 2)
     assert (np.abs(g.host(layer.weight.grad) - want) <= 2 * bound).all()
+
+
+@pytest.mark.parametrize("count", [511, 512, 513, 2048, 4095, 4096, 4098])
+@pytest.mark.parametrize("skew", ["uniform", "same", "text"])
+def test_as_many_tokens_as_one_block_orders(count, skew):
+    import gpu_util as g
+
+    rng = np.random.default_rng(count)
+    tokens = _tokens(rng, count, 3000, skew)
+    table, dy = np.zeros((3000, 6), np.float32), rng.standard_normal((count, 6), dtype=np.float32)
+    want, bound = _gradient(tokens, dy, 3000, 1.0)
+    got = g.host(g.op("embedding_backward")(g.dev(dy), g.dev(tokens), g.dev(table), 1.0)[0])
+    assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("count", [1300000, 1310000, 1212415])
+def test_shares_larger_than_shared_memory(count):
+    """Where a CTA's share of the tokens is written straight to memory, the last one's rest is too."""
+    import gpu_util as g
+
+    rng = np.random.default_rng(count)
+    tokens, dy = rng.integers(0, 5000, count), rng.standard_normal((count, 4), dtype=np.float32)
+    want, bound = _gradient(tokens, dy, 5000, 1.0)
+    got = g.host(g.op("embedding_backward")(g.dev(dy), g.dev(tokens), g.dev(np.zeros((5000, 4), np.float32)), 1.0)[0])
+    assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("count,width", [(33000, 512), (50000, 337)])
+def test_results_larger_than_half_of_l2(count, width):
+    import gpu_util as g
+    import mytorch_b200.nn.functional as F
+
+    rng = np.random.default_rng(width)
+    tokens, table = rng.integers(-1, 301, count), rng.standard_normal((300, width), dtype=np.float32)
+    out = g.host(F.embedding(g.dev(tokens), g.dev(table), scale=2.0))
+    inside = (tokens >= 0) & (tokens < 300)
+    assert np.array_equal(out[inside], 2 * table[tokens[inside]]) and np.isnan(out[~inside]).all()
+
+
+@pytest.mark.parametrize("count,width", [(2100001, 1023), (8400001, 1024)])
+def test_offsets_beyond_32_bits(count, width):
+    """2^31 values and more, 2^31 vectors of four and more: whole numbers, whose sums are exact."""
+    import gpu_util as g
+    import mytorch_b200 as mt
+    import mytorch_b200.nn.functional as F
+    from mytorch_b200.backends.cuda.env import CudaEnv, CudaMemoryView
+
+    rng = np.random.default_rng(1)
+    tokens, table = rng.integers(0, 700, count).astype(np.int32), rng.integers(-3, 4, (700, width)).astype(np.float32)
+    tt, wt = g.dev(tokens), g.dev(table)
+    out = F.embedding(tt, wt)
+    rows = 5
+    for first in (0, count // 2, count - rows):
+        part = CudaMemoryView(out._native_array, 4 * first * width, 4 * rows * width, 0)
+        assert np.array_equal(g.host(mt.Tensor._on_device((rows, width), mt.float32, out.device, part)), table[tokens[first:first + rows]])
+    got = g.host(g.op("embedding_backward")(out, tt, wt, 1.0)[0])
+    assert np.array_equal(got, np.bincount(tokens, minlength=700)[:, None] * table)
+    del out
+    CudaEnv.instance().lib.pool_trim()
