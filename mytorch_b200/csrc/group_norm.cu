@@ -539,8 +539,8 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const float* __restrict__
   mtb_launch_dependents();
   mtb_wait_prior();
   __shared__ float sm[3][8];
-  const int each = c / groups, g = blockIdx.y % groups, n = blockIdx.y / groups, stretch = (hw + splits - 1) / splits;
-  const int p0 = blockIdx.x * stretch, p1 = p0 + stretch < hw ? p0 + stretch : hw;
+  const int each = c / groups, g = blockIdx.x % groups, n = blockIdx.x / groups, stretch = (hw + splits - 1) / splits;
+  const int p0 = blockIdx.y * stretch, p1 = p0 + stretch < hw ? p0 + stretch : hw;
   const float* base = x + ((long long)n * hw + p0) * c + (long long)g * each;
   const int lanes = each < 256 ? each : 256, rows = 256 / lanes, row = threadIdx.x / lanes, lane = threadIdx.x - row * lanes;
   float count = 0.f, s1 = 0.f, s2 = 0.f, pivot = 0.f;
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const float* __restrict__
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int w = 1; w < 8; ++w) merge(sm[0][w], sm[1][w], sm[2][w]);
-  float* to = partial + ((long long)blockIdx.y * splits + blockIdx.x) * 3;
+  float* to = partial + ((long long)blockIdx.x * splits + blockIdx.y) * 3;
   to[0] = count;
   to[1] = mean;
   to[2] = m2;
@@ -602,11 +602,11 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* __restrict__
                                                         const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ y) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const long long first = blockIdx.y * image;
-  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < image; i += gridDim.x * 256) {
+  const long long first = blockIdx.x * image;
+  for (unsigned i = blockIdx.y * 256 + threadIdx.x; i < image; i += gridDim.y * 256) {
     unsigned ch, unused;
     by_c.divmod(i, ch);
-    const int k = blockIdx.y * groups + by_each.divmod(ch, unused);
+    const int k = blockIdx.x * groups + by_each.divmod(ch, unused);
     const float z = (x[first + i] - mean[k]) * rstd[k] * (gamma ? gamma[ch] : 1.f) + (beta ? beta[ch] : 0.f);
     y[first + i] = activate(z, act);
   }
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const float* __restric
   mtb_launch_dependents();
   mtb_wait_prior();
   __shared__ float sa[8][33], sb[8][33];
-  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, ch = blockIdx.x * 32 + lane, n = blockIdx.y, stretch = (hw + splits - 1) / splits;
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, ch = blockIdx.y * 32 + lane, n = blockIdx.x, stretch = (hw + splits - 1) / splits;
   const int p0 = blockIdx.z * stretch, p1 = p0 + stretch < hw ? p0 + stretch : hw;
   float a = 0.f, b = 0.f;
   if (ch < c) {
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const float* __restric
   __syncthreads();
   if (row == 0 && ch < c) {
     for (int k = 1; k < 8; ++k) { a += sa[k][lane]; b += sb[k][lane]; }
-    float* to = partial + ((long long)blockIdx.z * gridDim.y + n) * 2 * c + ch;
+    float* to = partial + ((long long)blockIdx.z * gridDim.x + n) * 2 * c + ch;
     to[0] = a;
     to[c] = b;
   }
@@ -679,11 +679,11 @@ __global__ void __launch_bounds__(256) gn_bwd_dx_kernel(const float* __restrict_
                                                          const float* __restrict__ of_group, float* __restrict__ dx) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const long long first = blockIdx.y * image;
-  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < image; i += gridDim.x * 256) {
+  const long long first = blockIdx.x * image;
+  for (unsigned i = blockIdx.y * 256 + threadIdx.x; i < image; i += gridDim.y * 256) {
     unsigned ch, unused;
     by_c.divmod(i, ch);
-    const int k = blockIdx.y * groups + by_each.divmod(ch, unused);
+    const int k = blockIdx.x * groups + by_each.divmod(ch, unused);
     const float ga = gamma ? gamma[ch] : 1.f, r = rstd[k], xh = (x[first + i] - mean[k]) * r;
     const float dz = activate_grad(dy[first + i], xh * ga + (beta ? beta[ch] : 0.f), act);
     dx[first + i] = r * (ga * dz - (of_group[2 * k] + xh * of_group[2 * k + 1]));
@@ -833,13 +833,12 @@ MTB_API int mtb_group_norm_forward_f32(int n, int c, int hw, int groups, const f
   t.s.vectors = alignment_of(gamma, beta, nullptr) % (4 * t.v) == 0;
   if (t.on_chip) return MTB_GN_PICK(forward_on_chip, t, activation, st, x, gamma, beta, (float)eps, y, mean, rstd);
   MTB_REQUIRE(workspace && workspace_bytes >= mtb_group_norm_workspace_bytes(n, c, hw, groups), "group_norm_forward: workspace too small");
-  MTB_REQUIRE((long long)n * groups < 65536 && n < 65536, "group_norm_forward: %d images of %d groups", n, groups);
   const int splits = splits_of(n, hw, groups);
   float* partial = (float*)workspace;
   const long long image = (long long)hw * c;
-  MTB_LAUNCH(gn_stats_kernel, dim3(splits, n * groups), 256, 0, st, x, hw, c, groups, splits, partial);
+  MTB_LAUNCH(gn_stats_kernel, dim3(n * groups, splits), 256, 0, st, x, hw, c, groups, splits, partial);
   MTB_LAUNCH(gn_stats_final_kernel, mtb_div_up((long long)n * groups, 128), 128, 0, st, partial, n * groups, splits, (float)eps, mean, rstd);
-  MTB_LAUNCH(gn_apply_kernel, dim3(mtb_stream_grid(image, 256), n), 256, 0, st, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta, activation, mean, rstd, y);
+  MTB_LAUNCH(gn_apply_kernel, dim3(n, mtb_stream_grid(image, 256)), 256, 0, st, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta, activation, mean, rstd, y);
   return MTB_OK;
 }
 
@@ -866,14 +865,14 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
   if (t.on_chip) {
     if (int rc = MTB_GN_PICK(backward_on_chip, t, activation, st, dy, x, gamma, beta, mean, rstd, dx, params ? sums : nullptr)) return rc;
   } else {
-    MTB_REQUIRE((long long)n * groups < 65536 && n < 65536, "group_norm_backward: %d images of %d groups", n, groups);
     const int blocks = mtb_div_up(c, 32), splits = splits_of(n, hw, blocks);
+    MTB_REQUIRE(blocks < 65536, "group_norm_backward: %d channels", c);
     float* of_group = sums + 2LL * n * c * splits;
     const long long image = (long long)hw * c;
-    MTB_LAUNCH(gn_bwd_sums_kernel, dim3(blocks, n, splits), 256, 0, st, dy, x, hw, c, groups, splits, gamma, beta, activation, mean, rstd, sums);
+    MTB_LAUNCH(gn_bwd_sums_kernel, dim3(n, blocks, splits), 256, 0, st, dy, x, hw, c, groups, splits, gamma, beta, activation, mean, rstd, sums);
     MTB_LAUNCH(gn_bwd_groups_kernel, mtb_div_up((long long)n * groups, 4), 128, 0, st, sums, n, c, groups, splits, gamma,
                (float)(1.0 / ((double)(c / groups) * hw)), of_group);
-    if (dx) MTB_LAUNCH(gn_bwd_dx_kernel, dim3(mtb_stream_grid(image, 256), n), 256, 0, st, dy, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta,
+    if (dx) MTB_LAUNCH(gn_bwd_dx_kernel, dim3(n, mtb_stream_grid(image, 256)), 256, 0, st, dy, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta,
                        activation, mean, rstd, of_group, dx);
   }
   if (params) MTB_LAUNCH(gn_params_kernel, mtb_div_up(2LL * c, 32), 256, 0, st, sums, n, c, dgamma, dbeta);

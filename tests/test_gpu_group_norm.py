@@ -132,6 +132,28 @@ def test_rows_without_positions(n, c, groups):
     _check_backward([g.host(xt.grad).reshape(x.shape), g.host(gt.grad), g.host(bt.grad)], o, dy, "silu")
 
 
+@pytest.mark.parametrize("n,c,groups", [(65600, 1028, 1), (70001, 96, 4)])
+def test_as_many_rows_as_tokens(n, c, groups):
+    """More rows than a grid has blocks in y, of groups too wide for a block's lanes and of others."""
+    import gpu_util as g
+    import mytorch_b200.nn.functional as F
+
+    x, dy, gamma, beta = _inputs((n, c, 1, 1), groups, c)
+    xt, gt, bt = g.dev(x.reshape(n, c), True), g.dev(gamma, True), g.dev(beta, True)
+    y = F.group_norm(xt, groups, gt, bt, activation="silu")
+    (y * g.dev(dy.reshape(n, c))).sum().backward()
+    y, dx = g.host(y).reshape(x.shape), g.host(xt.grad).reshape(x.shape)
+    sums = np.zeros((4, c))
+    for i in range(0, n, 8192):
+        o = Oracle(x[i:i + 8192], groups, gamma, beta, 1e-5, "silu")
+        _check_forward(y[i:i + 8192], o)
+        want, units = o.backward(dy[i:i + 8192], "silu")
+        assert (np.abs(dx[i:i + 8192] - want[0]) <= 4 * STEPS * U * units[0]).all()
+        sums += np.stack([*want[1:], *units[1:]])
+    for got, want, unit in zip((gt.grad, bt.grad), sums[:2], sums[2:]):
+        assert (np.abs(g.host(got) - want) <= 4 * STEPS * U * unit).all()
+
+
 @pytest.mark.parametrize("which", ["neither", "weight", "bias"])
 @pytest.mark.parametrize("shape,groups", [((3, 24, 6, 5), 4), ((2, 15, 12, 12), 5)])
 def test_without_weight_or_bias(shape, groups, which):
