@@ -511,67 +511,96 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
   });
 }
 
-// dgamma and dbeta: the sums over the images, 32 columns of [n][2 c] a CTA, in a fixed order.
-__global__ void __launch_bounds__(256) gn_params_kernel(const float* __restrict__ sums, int n, int c, float* __restrict__ dgamma, float* __restrict__ dbeta) {
+// dgamma and dbeta: the sums over the images, 32 columns of [n][2 c] a CTA, in a fixed order; of many images first those of stretches of them, to
+// stretches[gridDim.y][2 c].  Backward of 2000 images of 64 x 8 x 8 28 us, 37 with one stretch; of 70001 rows of 96 channels 431, not 1007.
+constexpr int kStretches = 128;
+int stretches_of(int n) { return n < 1024 ? 1 : n / 256 < kStretches ? n / 256 : kStretches; }
+
+__global__ void __launch_bounds__(256) gn_params_kernel(const float* __restrict__ sums, int n, int c, float* __restrict__ stretches, float* __restrict__ dgamma,
+                                                         float* __restrict__ dbeta) {
   mtb_launch_dependents();
   mtb_wait_prior();
   __shared__ float part[8][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  const int each = (n + gridDim.y - 1) / gridDim.y, first = blockIdx.y * each, end = first + each < n ? first + each : n;
   float t = 0.f;
   if (col < 2 * c)
 #pragma unroll 8
-    for (int i = row; i < n; i += 8) t += sums[(long long)i * 2 * c + col];
+    for (int i = first + row; i < end; i += 8) t += sums[(long long)i * 2 * c + col];
   part[row][lane] = t;
   __syncthreads();
   if (row != 0 || col >= 2 * c) return;
   for (int k = 1; k < 8; ++k) t += part[k][lane];
-  if (col < c) { if (dbeta) dbeta[col] = t; }
+  if (gridDim.y > 1) stretches[(long long)blockIdx.y * 2 * c + col] = t;
+  else if (col < c) { if (dbeta) dbeta[col] = t; }
   else if (dgamma) dgamma[col - c] = t;
 }
 
 // ---------------------------------------------------------------- a slab through memory
 
 // Images that no cluster can hold, and groups of more channels than a CTA has threads' vectors: partial statistics of stretches of positions,
-// statistics, result.
+// statistics, result.  Bound by latency and by reading twice: 2 x 64 x 400 x 400 in 2 groups forward 86 us (3.8 readings' and writings' time; 170 with a value a thread
+// on its way instead of kAhead), backward 126.  Rare among images that are trained on, so simple.
+
+constexpr int kAhead = 8;
+
+// Chan's update of (count, mean, M2) by another such.
+__device__ __forceinline__ void merge(float& count, float& mean, float& m2, float nb, float mb, float qb) {
+  if (nb == 0.f) return;
+  const float total = count + nb, d = mb - mean;
+  mean += d * (nb / total);
+  m2 += qb + d * d * count * (nb / total);
+  count = total;
+}
+// Those of a warp, to its first lane.
+__device__ __forceinline__ void merge_lanes(float& count, float& mean, float& m2) {
+  for (int o = 16; o > 0; o >>= 1) {
+    const float nb = __shfl_down_sync(0xffffffffu, count, o), mb = __shfl_down_sync(0xffffffffu, mean, o), qb = __shfl_down_sync(0xffffffffu, m2, o);
+    merge(count, mean, m2, nb, mb, qb);
+  }
+}
 
 // partial[group][split][3]: count, mean, M2, of shifted sums
-__global__ void __launch_bounds__(256) gn_stats_kernel(const float* __restrict__ x, int hw, int c, int groups, int splits, float* __restrict__ partial) {
+__global__ void __launch_bounds__(256) gn_stats_kernel(const float* __restrict__ x, int hw, int c, int groups, int splits, PoolDiv by_each,
+                                                        float* __restrict__ partial) {
   mtb_launch_dependents();
   mtb_wait_prior();
   __shared__ float sm[3][8];
   const int each = c / groups, g = blockIdx.x % groups, n = blockIdx.x / groups, stretch = (hw + splits - 1) / splits;
   const int p0 = blockIdx.y * stretch, p1 = p0 + stretch < hw ? p0 + stretch : hw;
   const float* base = x + ((long long)n * hw + p0) * c + (long long)g * each;
-  const int lanes = each < 256 ? each : 256, rows = 256 / lanes, row = threadIdx.x / lanes, lane = threadIdx.x - row * lanes;
-  float count = 0.f, s1 = 0.f, s2 = 0.f, pivot = 0.f;
-  if (row < rows && p0 + row < p1) {
-    pivot = base[(long long)row * c + lane];
-    for (int pos = row; pos < p1 - p0; pos += rows) {
-#pragma unroll 4
-      for (int ch = lane; ch < each; ch += lanes) {
-        const float d = base[(long long)pos * c + ch] - pivot;
-        s1 += d;
-        s2 += d * d;
-        count += 1.f;
+  const unsigned total = p1 > p0 ? (unsigned)(p1 - p0) * each : 0;  // the stretch's values of the group, 256 a step, kAhead steps at once
+  float s1 = 0.f, s2 = 0.f, pivot = 0.f;
+  if (threadIdx.x < total) {
+    unsigned ch;
+    const unsigned pos = by_each.divmod(threadIdx.x, ch);
+    pivot = base[(long long)pos * c + ch];
+  }
+  for (unsigned e = threadIdx.x; e < total; e += 256 * kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      v[u] = pivot;
+      if (e + 256 * u < total) {
+        unsigned ch;
+        const unsigned pos = by_each.divmod(e + 256 * u, ch);
+        v[u] = base[(long long)pos * c + ch];
       }
     }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float d = v[u] - pivot;
+      s1 += d;
+      s2 += d * d;
+    }
   }
+  float count = threadIdx.x < total ? (float)((total - threadIdx.x + 255) / 256) : 0.f;
   float mean = count > 0.f ? pivot + s1 / count : 0.f, m2 = count > 0.f ? s2 - s1 * s1 / count : 0.f;
-  auto merge = [&](float nb, float mb, float qb) {
-    if (nb == 0.f) return;
-    const float total = count + nb, d = mb - mean;
-    mean += d * (nb / total);
-    m2 += qb + d * d * count * (nb / total);
-    count = total;
-  };
-  for (int o = 16; o > 0; o >>= 1) {
-    const float nb = __shfl_down_sync(0xffffffffu, count, o), mb = __shfl_down_sync(0xffffffffu, mean, o), qb = __shfl_down_sync(0xffffffffu, m2, o);
-    merge(nb, mb, qb);
-  }
+  merge_lanes(count, mean, m2);
   if ((threadIdx.x & 31) == 0) { sm[0][threadIdx.x >> 5] = count; sm[1][threadIdx.x >> 5] = mean; sm[2][threadIdx.x >> 5] = m2; }
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int w = 1; w < 8; ++w) merge(sm[0][w], sm[1][w], sm[2][w]);
+  for (int w = 1; w < 8; ++w) merge(count, mean, m2, sm[0][w], sm[1][w], sm[2][w]);
   float* to = partial + ((long long)blockIdx.x * splits + blockIdx.y) * 3;
   to[0] = count;
   to[1] = mean;
@@ -582,17 +611,15 @@ __global__ void __launch_bounds__(128) gn_stats_final_kernel(const float* __rest
                                                               float* __restrict__ rstd_out) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const int k = blockIdx.x * 128 + threadIdx.x;
+  const int k = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // a warp a group
   if (k >= count) return;
   float n = 0.f, mean = 0.f, m2 = 0.f;
-  for (int i = 0; i < splits; ++i) {
+  for (int i = lane; i < splits; i += 32) {
     const float* q = partial + ((long long)k * splits + i) * 3;
-    if (q[0] == 0.f) continue;
-    const float total = n + q[0], d = q[1] - mean;
-    mean += d * (q[0] / total);
-    m2 += q[2] + d * d * n * (q[0] / total);
-    n = total;
+    merge(n, mean, m2, q[0], q[1], q[2]);
   }
+  merge_lanes(n, mean, m2);
+  if (lane != 0) return;
   mean_out[k] = mean;
   rstd_out[k] = 1.f / sqrtf(m2 / n + eps);
 }
@@ -603,12 +630,21 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* __restrict__
   mtb_launch_dependents();
   mtb_wait_prior();
   const long long first = blockIdx.x * image;
-  for (unsigned i = blockIdx.y * 256 + threadIdx.x; i < image; i += gridDim.y * 256) {
-    unsigned ch, unused;
-    by_c.divmod(i, ch);
-    const int k = blockIdx.x * groups + by_each.divmod(ch, unused);
-    const float z = (x[first + i] - mean[k]) * rstd[k] * (gamma ? gamma[ch] : 1.f) + (beta ? beta[ch] : 0.f);
-    y[first + i] = activate(z, act);
+  const unsigned values = (unsigned)image;
+  for (unsigned i0 = blockIdx.y * 256 * kAhead + threadIdx.x; i0 < values; i0 += gridDim.y * 256 * kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) v[u] = i0 + 256 * u < values ? x[first + i0 + 256 * u] : 0.f;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const unsigned i = i0 + 256 * u;
+      if (i >= values) break;
+      unsigned ch, unused;
+      by_c.divmod(i, ch);
+      const int k = blockIdx.x * groups + by_each.divmod(ch, unused);
+      const float z = (v[u] - mean[k]) * rstd[k] * (gamma ? gamma[ch] : 1.f) + (beta ? beta[ch] : 0.f);
+      y[first + i] = activate(z, act);
+    }
   }
 }
 
@@ -680,13 +716,26 @@ __global__ void __launch_bounds__(256) gn_bwd_dx_kernel(const float* __restrict_
   mtb_launch_dependents();
   mtb_wait_prior();
   const long long first = blockIdx.x * image;
-  for (unsigned i = blockIdx.y * 256 + threadIdx.x; i < image; i += gridDim.y * 256) {
-    unsigned ch, unused;
-    by_c.divmod(i, ch);
-    const int k = blockIdx.x * groups + by_each.divmod(ch, unused);
-    const float ga = gamma ? gamma[ch] : 1.f, r = rstd[k], xh = (x[first + i] - mean[k]) * r;
-    const float dz = activate_grad(dy[first + i], xh * ga + (beta ? beta[ch] : 0.f), act);
-    dx[first + i] = r * (ga * dz - (of_group[2 * k] + xh * of_group[2 * k + 1]));
+  const unsigned values = (unsigned)image;
+  for (unsigned i0 = blockIdx.y * 256 * kAhead + threadIdx.x; i0 < values; i0 += gridDim.y * 256 * kAhead) {
+    float v[kAhead], d[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const bool in = i0 + 256 * u < values;
+      v[u] = in ? x[first + i0 + 256 * u] : 0.f;
+      d[u] = in ? dy[first + i0 + 256 * u] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const unsigned i = i0 + 256 * u;
+      if (i >= values) break;
+      unsigned ch, unused;
+      by_c.divmod(i, ch);
+      const int k = blockIdx.x * groups + by_each.divmod(ch, unused);
+      const float ga = gamma ? gamma[ch] : 1.f, r = rstd[k], xh = (v[u] - mean[k]) * r;
+      const float dz = activate_grad(d[u], xh * ga + (beta ? beta[ch] : 0.f), act);
+      dx[first + i] = r * (ga * dz - (of_group[2 * k] + xh * of_group[2 * k + 1]));
+    }
   }
 }
 
@@ -799,9 +848,12 @@ int backward_on_chip(const Plan& t, cudaStream_t st, A... args) {
                 : (act == ACT_SILU ? f<1, ACT_SILU>(t, __VA_ARGS__) : act == ACT_RELU ? f<1, ACT_RELU>(t, __VA_ARGS__) : f<1, ACT_NONE>(t, __VA_ARGS__)))
 
 // Stretches that the positions of an image are cut into where slabs go through memory.
-int splits_of(int n, int hw, int parts) {
+// Stretches of the positions, of 64 at least, or of 4096 values of a part whose threads take whatever there is.
+int splits_of(int n, int hw, int parts, int values = 64) {
   long long want = (4LL * mtb_sm_count() + (long long)n * parts - 1) / ((long long)n * parts);
-  if (want > hw / 64) want = hw / 64;
+  const long long most = (long long)hw * values / 4096;
+  if (want > most) want = most;
+  if (want > hw) want = hw;
   return want < 1 ? 1 : want > 256 ? 256 : (int)want;
 }
 
@@ -816,7 +868,7 @@ int alignment_of(const void* a, const void* b, const void* c) {
 // Scratch of both directions: what slabs that go through memory leave of their stretches, and the backward's sums.
 MTB_API long long mtb_group_norm_workspace_bytes(int n, int c, int hw, int groups) {
   if (n <= 0 || c <= 0 || hw <= 0 || groups <= 0) return 256;
-  const long long forward = 12LL * n * groups * splits_of(n, hw, groups), backward = 8LL * n * c * splits_of(n, hw, mtb_div_up(c, 32)) + 8LL * n * groups;
+  const long long forward = 12LL * n * groups * splits_of(n, hw, groups, c / groups), backward = 8LL * n * c * splits_of(n, hw, mtb_div_up(c, 32)) + 8LL * n * groups + 8LL * c * kStretches;
   return (forward > backward ? forward : backward) + 256;
 }
 
@@ -833,12 +885,12 @@ MTB_API int mtb_group_norm_forward_f32(int n, int c, int hw, int groups, const f
   t.s.vectors = alignment_of(gamma, beta, nullptr) % (4 * t.v) == 0;
   if (t.on_chip) return MTB_GN_PICK(forward_on_chip, t, activation, st, x, gamma, beta, (float)eps, y, mean, rstd);
   MTB_REQUIRE(workspace && workspace_bytes >= mtb_group_norm_workspace_bytes(n, c, hw, groups), "group_norm_forward: workspace too small");
-  const int splits = splits_of(n, hw, groups);
+  const int splits = splits_of(n, hw, groups, c / groups);
   float* partial = (float*)workspace;
   const long long image = (long long)hw * c;
-  MTB_LAUNCH(gn_stats_kernel, dim3(n * groups, splits), 256, 0, st, x, hw, c, groups, splits, partial);
-  MTB_LAUNCH(gn_stats_final_kernel, mtb_div_up((long long)n * groups, 128), 128, 0, st, partial, n * groups, splits, (float)eps, mean, rstd);
-  MTB_LAUNCH(gn_apply_kernel, dim3(n, mtb_stream_grid(image, 256)), 256, 0, st, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta, activation, mean, rstd, y);
+  MTB_LAUNCH(gn_stats_kernel, dim3(n * groups, splits), 256, 0, st, x, hw, c, groups, splits, PoolDiv(c / groups), partial);
+  MTB_LAUNCH(gn_stats_final_kernel, mtb_div_up((long long)n * groups, 4), 128, 0, st, partial, n * groups, splits, (float)eps, mean, rstd);
+  MTB_LAUNCH(gn_apply_kernel, dim3(n, mtb_stream_grid((image + kAhead - 1) / kAhead, 256)), 256, 0, st, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta, activation, mean, rstd, y);
   return MTB_OK;
 }
 
@@ -857,7 +909,7 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
   MTB_REQUIRE(dy && mean && rstd && x && workspace, "group_norm_backward: null tensor");
   MTB_REQUIRE((long long)n * groups < 1LL << 31 && (long long)hw * c < 1LL << 31, "group_norm_backward: too many values");
   MTB_REQUIRE(workspace_bytes >= mtb_group_norm_workspace_bytes(n, c, hw, groups), "group_norm_backward: workspace too small");
-  float* sums = (float*)workspace;
+  float *sums = (float*)workspace, *after = sums + 2LL * n * c;  // what is left of the scratch
   const bool params = dgamma || dbeta;
   if (!params && !dx) return MTB_OK;
   Plan t = plan_slabs(n, c, hw, groups, 2, alignment_of(dy, x, dx));
@@ -868,13 +920,22 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
     const int blocks = mtb_div_up(c, 32), splits = splits_of(n, hw, blocks);
     MTB_REQUIRE(blocks < 65536, "group_norm_backward: %d channels", c);
     float* of_group = sums + 2LL * n * c * splits;
+    after = of_group + 2LL * n * groups;
     const long long image = (long long)hw * c;
     MTB_LAUNCH(gn_bwd_sums_kernel, dim3(n, blocks, splits), 256, 0, st, dy, x, hw, c, groups, splits, gamma, beta, activation, mean, rstd, sums);
     MTB_LAUNCH(gn_bwd_groups_kernel, mtb_div_up((long long)n * groups, 4), 128, 0, st, sums, n, c, groups, splits, gamma,
                (float)(1.0 / ((double)(c / groups) * hw)), of_group);
-    if (dx) MTB_LAUNCH(gn_bwd_dx_kernel, dim3(n, mtb_stream_grid(image, 256)), 256, 0, st, dy, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta,
+    if (dx) MTB_LAUNCH(gn_bwd_dx_kernel, dim3(n, mtb_stream_grid((image + kAhead - 1) / kAhead, 256)), 256, 0, st, dy, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta,
                        activation, mean, rstd, of_group, dx);
   }
-  if (params) MTB_LAUNCH(gn_params_kernel, mtb_div_up(2LL * c, 32), 256, 0, st, sums, n, c, dgamma, dbeta);
+  if (params) {
+    const int columns = mtb_div_up(2LL * c, 32), stretches = stretches_of(n);
+    if (stretches > 1) {
+      MTB_LAUNCH(gn_params_kernel, dim3(columns, stretches), 256, 0, st, sums, n, c, after, nullptr, nullptr);
+      MTB_LAUNCH(gn_params_kernel, columns, 256, 0, st, after, stretches, c, nullptr, dgamma, dbeta);
+    } else {
+      MTB_LAUNCH(gn_params_kernel, columns, 256, 0, st, sums, n, c, nullptr, dgamma, dbeta);
+    }
+  }
   return MTB_OK;
 }
