@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(256) gn_params_kernel(const float* __restrict_
 // ---------------------------------------------------------------- a slab through memory
 
 // Images that no cluster can hold, and groups of more channels than a CTA has threads' vectors: partial statistics of stretches of positions,
-// statistics, result.  Bound by latency and by reading twice: 2 x 64 x 400 x 400 in 2 groups forward 86 us (3.8 readings' and writings' time; 170 with a value a thread
+// statistics, result.  Bound by latency and by reading twice: 2 x 64 x 400 x 400 in 2 groups forward 86 us (25 is HBM's time for 8 bytes a value; 170 with a value a thread
 // on its way instead of kAhead), backward 126.  Rare among images that are trained on, so simple.
 
 constexpr int kAhead = 8;
