@@ -57,8 +57,8 @@ __device__ __forceinline__ void sum_squares(const float* p, int n, double& a, do
 
 // The CTAs go through the chunks side by side, so that what was read last is what the next kernel, which goes through them backwards, begins with.
 __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_constant__ Table<const float> t, double* __restrict__ sums) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   double a = 0, b = 0;
   for (int c = blockIdx.x; c < t.chunk_start[t.count]; c += gridDim.x) {
     const int k = tensor_of(t, c);
@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
 
 // Writes nothing where the gradients are under the limit: a factor of one changes no value.
 __global__ void __launch_bounds__(kThreads) scale_grads_kernel(const __grid_constant__ Table<float> t, MtbClip clip) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   const float factor = mtb_clip_factor<kThreads>(clip);
   if (factor == 1.f) return;
   for (int c = t.chunk_start[t.count] - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {

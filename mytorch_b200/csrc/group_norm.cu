@@ -9,7 +9,7 @@
 // a slab, some whole groups of one image, in its shared memory, each CTA a stretch of the positions; four CTAs or so on an SM, one of which loads
 // while another one adds up or stores.  A thread copies (cp.async) and later reads its own vectors only, so the copies need no barrier; the CTAs exchange their sums
 // through distributed shared memory.
-// 256 x 128 x 56 x 56 with SiLU: forward 144 us (5.7 TB/s, 87 % of a copy), backward 247 (5.0 TB/s, 76 %).  What bounds the backward now: a CTA's time from its
+// 256 x 128 x 56 x 56 with SiLU: forward 144 us (5.7 TB/s, 87 % of a copy), backward 246 (5.0 TB/s, 76 %).  What bounds the backward now: a CTA's time from its
 // last value to its first store, in which the cluster waits for its slowest, and an SM has four of them to overlap (backward without the exchange 190 us).
 // It went from 292 us by instructions and waits taken out of that time: xh recomputed instead of written back 275, sums over rows all at once 258 and by halves 250,
 // gamma from shared memory 247.  The 64 registers of four CTAs are what it may not pass: 12 bytes spilled cost 20 us.  Tried: clusters that stay and fetch
@@ -253,7 +253,6 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
                                                                   const float* __restrict__ beta, float eps, float* __restrict__ y,
                                                                   float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   extern __shared__ __align__(16) float held[];  // [positions][lanes][V]; the warps' (mean, M2); the CTAs' [ctas][groups of a slab]
-  mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
   const Unit u(p, blockIdx.x / p.ctas);
@@ -264,6 +263,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
   const int full = active ? s.full : 0, steps = active ? s.steps : 0;
   const unsigned step = p.rows * p.c;  // of an image's values
   mtb_wait_prior();
+  mtb_launch_dependents();  // not before: the next kernel's CTAs would take places from this one's
   const float* from = x + u.first(p, s);
   const unsigned at = (unsigned)__cvta_generic_to_shared(mine);
   each_step(full, steps, [&](int j) { copy_async<V>(at + j * kThreads * V * 4, from + j * step); });
@@ -391,7 +391,6 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
                                                                    const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ dx,
                                                                    float* __restrict__ sums) {
   extern __shared__ __align__(16) float held[];  // [2][positions][lanes][V]; the warps' sums; the CTAs' of channels and of groups
-  mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
   const Unit u(p, blockIdx.x / p.ctas);
@@ -403,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
   const int full = active ? s.full : 0, steps = active ? s.steps : 0;
   const unsigned step = p.rows * p.c;
   mtb_wait_prior();
+  mtb_launch_dependents();  // not before: the next kernel's CTAs would take places from this one's
   {
     const float *from = x + u.first(p, s), *from2 = dy + u.first(p, s);
     const unsigned at = (unsigned)__cvta_generic_to_shared(mine);
@@ -518,8 +518,8 @@ int stretches_of(int n) { return n < 1024 ? 1 : n / 256 < kStretches ? n / 256 :
 
 __global__ void __launch_bounds__(256) gn_params_kernel(const float* __restrict__ sums, int n, int c, float* __restrict__ stretches, float* __restrict__ dgamma,
                                                          float* __restrict__ dbeta) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   __shared__ float part[8][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   const int each = (n + gridDim.y - 1) / gridDim.y, first = blockIdx.y * each, end = first + each < n ? first + each : n;
@@ -563,8 +563,8 @@ __device__ __forceinline__ void merge_lanes(float& count, float& mean, float& m2
 // partial[group][split][3]: count, mean, M2, of shifted sums
 __global__ void __launch_bounds__(256) gn_stats_kernel(const float* __restrict__ x, int hw, int c, int groups, int splits, PoolDiv by_each,
                                                         float* __restrict__ partial) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   __shared__ float sm[3][8];
   const int each = c / groups, g = blockIdx.x % groups, n = blockIdx.x / groups, stretch = (hw + splits - 1) / splits;
   const int p0 = blockIdx.y * stretch, p1 = p0 + stretch < hw ? p0 + stretch : hw;
@@ -609,8 +609,8 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const float* __restrict__
 
 __global__ void __launch_bounds__(128) gn_stats_final_kernel(const float* __restrict__ partial, int count, int splits, float eps, float* __restrict__ mean_out,
                                                               float* __restrict__ rstd_out) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   const int k = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;  // a warp a group
   if (k >= count) return;
   float n = 0.f, mean = 0.f, m2 = 0.f;
@@ -627,8 +627,8 @@ __global__ void __launch_bounds__(128) gn_stats_final_kernel(const float* __rest
 __global__ void __launch_bounds__(256) gn_apply_kernel(const float* __restrict__ x, long long image, PoolDiv by_c, PoolDiv by_each, int groups,
                                                         const float* __restrict__ gamma, const float* __restrict__ beta, int act,
                                                         const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ y) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   const long long first = blockIdx.x * image;
   const unsigned values = (unsigned)image;
   for (unsigned i0 = blockIdx.y * 256 * kAhead + threadIdx.x; i0 < values; i0 += gridDim.y * 256 * kAhead) {
@@ -652,8 +652,8 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* __restrict__
 __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const float* __restrict__ dy, const float* __restrict__ x, int hw, int c, int groups, int splits,
                                                            const float* __restrict__ gamma, const float* __restrict__ beta, int act,
                                                            const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ partial) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   __shared__ float sa[8][33], sb[8][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, ch = blockIdx.y * 32 + lane, n = blockIdx.x, stretch = (hw + splits - 1) / splits;
   const int p0 = blockIdx.z * stretch, p1 = p0 + stretch < hw ? p0 + stretch : hw;
@@ -683,8 +683,8 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const float* __restric
 // sums[n][2][c] over the splits, in place of the first; then A / M and B / M of each group.  A warp a group.
 __global__ void __launch_bounds__(128) gn_bwd_groups_kernel(float* __restrict__ sums, int n, int c, int groups, int splits, const float* __restrict__ gamma,
                                                              float inv_m, float* __restrict__ of_group) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   const int k = blockIdx.x * 4 + (threadIdx.x >> 5), each = c / groups;
   if (k >= n * groups) return;
   float* s = sums + (long long)(k / groups) * 2 * c + (k % groups) * each;
@@ -713,8 +713,8 @@ __global__ void __launch_bounds__(256) gn_bwd_dx_kernel(const float* __restrict_
                                                          int groups, const float* __restrict__ gamma, const float* __restrict__ beta, int act,
                                                          const float* __restrict__ mean, const float* __restrict__ rstd,
                                                          const float* __restrict__ of_group, float* __restrict__ dx) {
-  mtb_launch_dependents();
   mtb_wait_prior();
+  mtb_launch_dependents();
   const long long first = blockIdx.x * image;
   const unsigned values = (unsigned)image;
   for (unsigned i0 = blockIdx.y * 256 * kAhead + threadIdx.x; i0 < values; i0 += gridDim.y * 256 * kAhead) {
