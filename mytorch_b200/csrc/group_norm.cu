@@ -54,6 +54,12 @@ __device__ __forceinline__ void copy_async(unsigned at, const float* from) {
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// A CTA's shared memory is there for the others of its cluster once it has started.  So each arrives first of all and waits for the others just before it
+// writes to them; its own values are on their way meanwhile.  A CTA without a cluster is one of one: the backward asks it too, since a branch here costs it
+// registers that it has not (12 bytes spilled).
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 template <int V> struct alignas(4 * V) Vec { float v[V]; };
 template <int V> __device__ __forceinline__ Vec<V>& vec(float* p) { return *reinterpret_cast<Vec<V>*>(p); }
 template <int V> __device__ __forceinline__ Vec<V> all(float x) {
@@ -254,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
                                                                   float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   extern __shared__ __align__(16) float held[];  // [positions][lanes][V]; the warps' (mean, M2); the CTAs' [ctas][groups of a slab]
   cg::cluster_group cluster = cg::this_cluster();
+  if (p.ctas > 1) cluster_arrive();
   const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
   const Unit u(p, blockIdx.x / p.ctas);
   const int per_slot = p.lanes * p.of_vector / p.merged;
@@ -274,6 +281,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_forward_kernel(const __grid_co
   else if (V >= 2 && p.of_vector == 2) slot_statistics<V, V >= 2 ? 2 : 1>(mine, full, steps, p, s, slots);
   else slot_statistics<V, 1>(mine, full, steps, p, s, slots);
   __syncthreads();
+  if (p.ctas > 1) cluster_wait();
   // Chan's update for several: the mean of the means, and M2_k + n_k (mean_k - mean)^2 added up.  The CTA's of a group by eight lanes, a slot each, who give it to
   // each CTA of the cluster ...
   const float share = (float)(V / p.of_vector * p.merged), inv = __frcp_rn((float)(s.positions * p.each));
@@ -392,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
                                                                    float* __restrict__ sums) {
   extern __shared__ __align__(16) float held[];  // [2][positions][lanes][V]; the warps' sums; the CTAs' of channels and of groups
   cg::cluster_group cluster = cg::this_cluster();
+  cluster_arrive();
   const Share<V> s(p, p.ctas > 1 ? (int)cluster.block_rank() : 0);
   const Unit u(p, blockIdx.x / p.ctas);
   const int plane = p.stretch * p.lanes * V, both = 2 * p.lanes * V;  // two sums of each channel
@@ -442,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
   b = mul(b, r);
   add_rows<V>(a, b, lane, p.lanes, of_warp + s.slot(p) * p.slot_stride + s.col);
   __syncthreads();
+  cluster_wait();
   if (dx) {
     const int entries = p.each * p.slots;
     for (int g = warp; g < u.groups; g += kWarps) {  // the group's in the CTA, given to each CTA of the cluster
