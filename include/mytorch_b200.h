@@ -222,7 +222,7 @@ int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const float* d
  * out[i] = scale * table[tokens[i]] over `count` tokens and a table [rows][width]; kind of the tokens: 0 int32, 1 int64.  A token outside the table
  * reads nothing: its row of out is NaN, and the gradient leaves it out.
  * dtable[v] = scale * sum of dy[i] over the tokens i that are v, added in a fixed order; every row is written, with zeros where no token is v and in the
- * row `padding` (none: a negative number). */
+ * row `padding` (none: a negative number).  The workspace begins at a 16-byte boundary. */
 int mtb_embedding_forward_f32(int kind, const void* tokens, long long count, int rows, int width, const float* table, double scale, float* out, void* stream);
 long long mtb_embedding_backward_workspace_bytes(long long count, int rows, int width);
 int mtb_embedding_backward_f32(int kind, const void* tokens, long long count, int rows, int width, const float* dy, double scale, long long padding,

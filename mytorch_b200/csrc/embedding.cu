@@ -625,12 +625,13 @@ MTB_API int mtb_embedding_backward_f32(int kind, const void* tokens, long long c
   MTB_REQUIRE(count == 0 || (tokens && dy), "embedding_backward: null tensor");
   MTB_REQUIRE(count <= 1LL << 30 && rows <= 1 << 30, "embedding_backward: %lld tokens, %d rows", count, rows);
   MTB_REQUIRE(workspace && workspace_bytes >= mtb_embedding_backward_workspace_bytes(count, rows, width), "embedding_backward: workspace too small");
+  MTB_REQUIRE(mtb_aligned16(workspace), "embedding_backward: the workspace does not begin at a 16-byte boundary");
   cudaStream_t st = (cudaStream_t)stream;
   if (count == 0) {
     MTB_CUDA(cudaMemsetAsync(dtable, 0, 4LL * rows * width, st));
     return MTB_OK;
   }
-  const bool four = width % 4 == 0 && mtb_aligned16(dy) && mtb_aligned16(dtable) && mtb_aligned16(workspace);
+  const bool four = width % 4 == 0 && mtb_aligned16(dy) && mtb_aligned16(dtable);
   const GradPlan g = plan_gradient(count, rows, width, four);
   MTB_REQUIRE(g.columns < 65536, "embedding_backward: rows of %d values", width);
   int* table = (int*)workspace;  // read four at a time, like the pieces
