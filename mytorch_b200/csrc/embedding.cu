@@ -111,13 +111,14 @@ __device__ __forceinline__ int key_of(const void* tokens, int i, const SortPlan&
   return t >= 0 && t < p.rows && t != p.padding ? (int)t : p.rows;
 }
 
-struct SortShared {
+struct alignas(16) SortShared {
   int counters[kSortWarps][kDigits];
   unsigned lanes[kSortWarps][kDigits];  // 0 between two uses
   int local[kDigits];     // where a digit begins in the CTA's own order
   int shift_to[kDigits];  // from there to its place among all
   int sums[2][kSortWarps];
 };
+static_assert(alignof(SortShared) % 16 == 0 && offsetof(SortShared, lanes) % 16 == 0, "counters and lanes are cleared, and take sums, 16 bytes at a time");
 
 // Exclusive sums over the digits of `a` and `b`, one digit a thread.  All threads call it; `sums` is free again after the next barrier.
 __device__ __forceinline__ void scan_digits(int& a, int& b, SortShared& sh) {
