@@ -317,7 +317,7 @@ int mtb_sgd_multi_f32(int count, float* const* params, const float* const* grads
 /* The norm of all gradients together, and clipping by it (no counterpart in the reference).  mtb_grad_norm_f32 leaves mtb_grad_norm_sums(count) sums of
  * squares in device memory; the entry points below make of them the norm, that of grad_scale times the gradients where they have a grad_scale, which they leave in
  * *norm (device memory), and the factor min(1, max_norm / (norm + 1e-6)).  grads / sizes are HOST arrays of length count.
- * mtb_clip_grads_f32 multiplies the gradients by the factor in place, each tensor that is listed once (max_norm < 0: the norm only);
+ * mtb_clip_grads_f32 multiplies the gradients by the factor in place; no two may overlap (max_norm < 0: the norm only);
  * mtb_sgd_multi_clipped_f32 is mtb_sgd_multi_f32 on gradients so multiplied, without writing them; its tensors may be some of those of the norm. */
 int mtb_grad_norm_sums(int count);
 int mtb_grad_norm_f32(int count, const float* const* grads, const long long* sizes, double* sums, void* stream);

@@ -602,16 +602,19 @@ PyObject* clip_gradients(PyObject*, PyObject* const* args, Py_ssize_t n) {
     sizes.push_back(size);
   }
   if (!like) Py_RETURN_NONE;
-  // all count; of those that begin at the same address one, the longest, is multiplied
+  // all count; memory that several of them share, whole or in part, is multiplied once
   std::vector<size_t> order(grads.size());
   for (size_t i = 0; i < order.size(); ++i) order[i] = i;
-  std::sort(order.begin(), order.end(), [&](size_t a, size_t b) { return grads[a] != grads[b] ? grads[a] < grads[b] : sizes[a] > sizes[b]; });
+  std::sort(order.begin(), order.end(), [&](size_t a, size_t b) { return grads[a] < grads[b]; });
   std::vector<float*> once;
   std::vector<long long> once_sizes;
-  for (size_t i = 0; i < order.size(); ++i) {
-    if (i && grads[order[i]] == grads[order[i - 1]]) continue;
-    once.push_back(grads[order[i]]);
-    once_sizes.push_back(sizes[order[i]]);
+  for (const size_t i : order) {
+    if (!once.empty() && grads[i] < once.back() + once_sizes.back()) {
+      once_sizes.back() = std::max(once_sizes.back(), (long long)(grads[i] + sizes[i] - once.back()));
+      continue;
+    }
+    once.push_back(grads[i]);
+    once_sizes.push_back(sizes[i]);
   }
   void* st;
   NormResult result;

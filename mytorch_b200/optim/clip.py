@@ -12,7 +12,7 @@ def grad_norm(params):
 
 def clip_grad_norm_(params, max_norm):
     """Multiplies the gradients of ``params`` by min(1, max_norm / (norm + 1e-6)) in place and returns their norm before that, as ``grad_norm`` does.
-    A tensor that holds the gradient of several parameters (addition hands one to both of its operands) counts for each and is multiplied once.
+    Memory that holds the gradients of several parameters (addition hands one tensor to both of its operands) counts for each and is multiplied once.
     Norms that are infinite or no number show in the gradients: the factor is then 0 or no number."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
