@@ -554,6 +554,10 @@ __global__ void __launch_bounds__(256) gn_params_kernel(const float* __restrict_
 
 constexpr int kAhead = 8;
 
+// z of `v`, a value less the mean, with the roundings of the kernels above: a backward that goes through memory finds each ReLU on the side of zero on
+// which a forward on the chip left it.
+__device__ __forceinline__ float scaled(float v, float gamma, float rstd, float beta) { return fmaf(v, __fmul_rn(gamma, rstd), beta); }
+
 // Chan's update of (count, mean, M2) by another such.
 __device__ __forceinline__ void merge(float& count, float& mean, float& m2, float nb, float mb, float qb) {
   if (nb == 0.f) return;
@@ -652,8 +656,7 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* __restrict__
       unsigned ch, unused;
       by_c.divmod(i, ch);
       const int k = blockIdx.x * groups + by_each.divmod(ch, unused);
-      const float z = (v[u] - mean[k]) * rstd[k] * (gamma ? gamma[ch] : 1.f) + (beta ? beta[ch] : 0.f);
-      y[first + i] = activate(z, act);
+      y[first + i] = activate(scaled(__fadd_rn(v[u], -mean[k]), gamma ? gamma[ch] : 1.f, rstd[k], beta ? beta[ch] : 0.f), act);
     }
   }
 }
@@ -674,7 +677,7 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const float* __restric
 #pragma unroll 4
     for (int s = p0 + row; s < p1; s += 8) {
       const long long i = ((long long)n * hw + s) * c + ch;
-      const float xh = (x[i] - mu) * r, dz = activate_grad(dy[i], xh * ga + be, act);
+      const float v = __fadd_rn(x[i], -mu), xh = v * r, dz = activate_grad(dy[i], scaled(v, ga, r, be), act);
       a += dz;
       b += dz * xh;
     }
@@ -742,8 +745,8 @@ __global__ void __launch_bounds__(256) gn_bwd_dx_kernel(const float* __restrict_
       unsigned ch, unused;
       by_c.divmod(i, ch);
       const int k = blockIdx.x * groups + by_each.divmod(ch, unused);
-      const float ga = gamma ? gamma[ch] : 1.f, r = rstd[k], xh = (v[u] - mean[k]) * r;
-      const float dz = activate_grad(d[u], xh * ga + (beta ? beta[ch] : 0.f), act);
+      const float ga = gamma ? gamma[ch] : 1.f, r = rstd[k], less = __fadd_rn(v[u], -mean[k]), xh = less * r;
+      const float dz = activate_grad(d[u], scaled(less, ga, r, beta ? beta[ch] : 0.f), act);
       dx[first + i] = r * (ga * dz - (of_group[2 * k] + xh * of_group[2 * k + 1]));
     }
   }
