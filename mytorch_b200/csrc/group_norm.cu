@@ -661,15 +661,15 @@ __global__ void __launch_bounds__(256) gn_apply_kernel(const float* __restrict__
   }
 }
 
-// partial[split][n][2][c]: the sums of dz and of dz xh over a stretch of positions
-__global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const float* __restrict__ dy, const float* __restrict__ x, int hw, int c, int groups, int splits,
+// partial[split][n][2][c]: the sums of dz and of dz xh over a stretch of positions.  A CTA has 32 channels, of an image's `blocks`.
+__global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const float* __restrict__ dy, const float* __restrict__ x, int hw, int c, int groups, int splits, int blocks,
                                                            const float* __restrict__ gamma, const float* __restrict__ beta, int act,
                                                            const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ partial) {
   mtb_wait_prior();
   mtb_launch_dependents();
   __shared__ float sa[8][33], sb[8][33];
-  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, ch = blockIdx.y * 32 + lane, n = blockIdx.x, stretch = (hw + splits - 1) / splits;
-  const int p0 = blockIdx.z * stretch, p1 = p0 + stretch < hw ? p0 + stretch : hw;
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, n = blockIdx.x / blocks, ch = (blockIdx.x - n * blocks) * 32 + lane, stretch = (hw + splits - 1) / splits;
+  const int p0 = blockIdx.y * stretch, p1 = p0 + stretch < hw ? p0 + stretch : hw;
   float a = 0.f, b = 0.f;
   if (ch < c) {
     const int k = n * groups + ch / (c / groups);
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(const float* __restric
   __syncthreads();
   if (row == 0 && ch < c) {
     for (int k = 1; k < 8; ++k) { a += sa[k][lane]; b += sb[k][lane]; }
-    float* to = partial + ((long long)blockIdx.z * gridDim.x + n) * 2 * c + ch;
+    float* to = partial + ((long long)blockIdx.y * (gridDim.x / blocks) + n) * 2 * c + ch;
     to[0] = a;
     to[c] = b;
   }
@@ -931,11 +931,11 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
     if (int rc = MTB_GN_PICK(backward_on_chip, t, activation, st, dy, x, gamma, beta, mean, rstd, dx, params ? sums : nullptr)) return rc;
   } else {
     const int blocks = mtb_div_up(c, 32), splits = splits_of(n, hw, blocks);
-    MTB_REQUIRE(blocks < 65536, "group_norm_backward: %d channels", c);
+    MTB_REQUIRE((long long)n * blocks < 1LL << 31, "group_norm_backward: %d images of %d channels", n, c);
     float* of_group = sums + 2LL * n * c * splits;
     after = of_group + 2LL * n * groups;
     const long long image = (long long)hw * c;
-    MTB_LAUNCH(gn_bwd_sums_kernel, dim3(n, blocks, splits), 256, 0, st, dy, x, hw, c, groups, splits, gamma, beta, activation, mean, rstd, sums);
+    MTB_LAUNCH(gn_bwd_sums_kernel, dim3(n * blocks, splits), 256, 0, st, dy, x, hw, c, groups, splits, blocks, gamma, beta, activation, mean, rstd, sums);
     MTB_LAUNCH(gn_bwd_groups_kernel, mtb_div_up((long long)n * groups, 4), 128, 0, st, sums, n, c, groups, splits, gamma,
                (float)(1.0 / ((double)(c / groups) * hw)), of_group);
     if (dx) MTB_LAUNCH(gn_bwd_dx_kernel, dim3(n, mtb_stream_grid((image + kAhead - 1) / kAhead, 256)), 256, 0, st, dy, x, image, PoolDiv(c), PoolDiv(c / groups), groups, gamma, beta,
