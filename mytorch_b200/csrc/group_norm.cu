@@ -935,6 +935,9 @@ int alignment_of(const void* a, const void* b, const void* c) {
 
 }  // namespace
 
+// Values of an image: an int counts them and the positions that the last steps and stretches reach for beyond them.
+constexpr long long kMostValues = (1LL << 31) - (1 << 16);
+
 // Scratch of both directions: what slabs that go through memory leave of their stretches, and the backward's sums.
 MTB_API long long mtb_group_norm_workspace_bytes(int n, int c, int hw, int groups) {
   if (n <= 0 || c <= 0 || hw <= 0 || groups <= 0) return 256;
@@ -949,7 +952,7 @@ MTB_API int mtb_group_norm_forward_f32(int n, int c, int hw, int groups, const f
   MTB_REQUIRE(activation >= ACT_NONE && activation <= ACT_SILU, "group_norm_forward: unknown activation %d", activation);
   if (n == 0 || hw == 0) return MTB_OK;
   MTB_REQUIRE(x && y && mean && rstd, "group_norm_forward: null tensor");
-  MTB_REQUIRE((long long)n * groups < 1LL << 31 && (long long)hw * c < 1LL << 31, "group_norm_forward: too many values");
+  MTB_REQUIRE((long long)n * groups < 1LL << 31 && (long long)hw * c <= kMostValues, "group_norm_forward: too many values");
   cudaStream_t st = (cudaStream_t)stream;
   Plan t = plan_slabs(n, c, hw, groups, 1, alignment_of(x, y, nullptr));
   t.s.vectors = alignment_of(gamma, beta, nullptr) % (4 * t.v) == 0;
@@ -977,7 +980,7 @@ MTB_API int mtb_group_norm_backward_f32(int n, int c, int hw, int groups, const 
     return MTB_OK;
   }
   MTB_REQUIRE(dy && mean && rstd && x && workspace, "group_norm_backward: null tensor");
-  MTB_REQUIRE((long long)n * groups < 1LL << 31 && (long long)hw * c < 1LL << 31, "group_norm_backward: too many values");
+  MTB_REQUIRE((long long)n * groups < 1LL << 31 && (long long)hw * c <= kMostValues, "group_norm_backward: too many values");
   MTB_REQUIRE(workspace_bytes >= mtb_group_norm_workspace_bytes(n, c, hw, groups), "group_norm_backward: workspace too small");
   float *sums = (float*)workspace, *after = sums + 2LL * n * c;  // what is left of the scratch
   const bool params = dgamma || dbeta;
