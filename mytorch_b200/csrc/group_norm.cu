@@ -26,22 +26,6 @@ namespace cg = cooperative_groups;
 
 enum Activation { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2 };
 
-// SiLU by the fast exponential and quotient: a relative error of about 2^-21 of a value whose input carries the error of a normalisation
-__device__ __forceinline__ float activate(float z, int act) {
-  if (act == ACT_RELU) return z < 0.f ? 0.f : z;
-  if (act == ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
-  return z;
-}
-// dy f'(z); a ReLU passes what is at zero, as ReLU's own backward does
-__device__ __forceinline__ float activate_grad(float dy, float z, int act) {
-  if (act == ACT_RELU) return z < 0.f ? 0.f : dy;
-  if (act == ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-z));
-    return dy * (s * (1.f + z * (1.f - s)));
-  }
-  return dy;
-}
-
 __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -94,13 +78,16 @@ template <int V> __device__ __forceinline__ Vec<V> fma(Vec<V> a, Vec<V> b, Vec<V
           : "f"(a.v[i]), "f"(a.v[i + 1]), "f"(b.v[i]), "f"(b.v[i + 1]), "f"(c.v[i]), "f"(c.v[i + 1]));
   return r;
 }
-// 1 / (1 + e^-z) as 1 / (1 + 2^(-z log2 e)), by the approximate power and reciprocal of the hardware: off by about 2^-21 of itself, next to the error of a
-// normalisation in z
+// 1 / (1 + e^-z).  e^-z = 2^h e^-r with h = -z log2 e as 32 bits have it and r = z + h ln 2 what that leaves, so small that e^-r = 1 - r; without r the error would
+// grow with z, to 2^-18 of the result at -80.  By the approximate power and reciprocal of the hardware: under 2^-20 of itself.  Where e^-z overflows or vanishes, r
+// may be anything and counts nothing: it is cut to 1/16, a NaN too.
 template <int V> __device__ __forceinline__ Vec<V> sigmoid(Vec<V> z) {
-  Vec<V> e = mul(z, all<V>(-1.4426950408889634f));
+  Vec<V> e = mul(z, all<V>(-1.4426950408889634f)), r = fma(e, all<V>(0.6931471805599453f), z);
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = __saturatef(fmaf(r.v[i], 8.f, 0.5f));
 #pragma unroll
   for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.v[i]));
-  e = add(e, all<V>(1.f));
+  e = fma(e, fma(r, all<V>(-0.125f), all<V>(1.0625f)), all<V>(1.f));
 #pragma unroll
   for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e.v[i]));
   return e;
@@ -121,6 +108,17 @@ template <int V, int ACT> __device__ __forceinline__ Vec<V> activated_grad(Vec<V
 #pragma unroll
     for (int i = 0; i < V; ++i) dy.v[i] = z.v[i] < 0.f ? 0.f : dy.v[i];
   return dy;
+}
+
+// The same of one value, the activation an argument.
+__device__ __forceinline__ float activate(float z, int act) {
+  const Vec<1> v{{z}};
+  return (act == ACT_SILU ? activated<1, ACT_SILU>(v) : act == ACT_RELU ? activated<1, ACT_RELU>(v) : v).v[0];
+}
+// dy f'(z); a ReLU passes what is at zero, as ReLU's own backward does
+__device__ __forceinline__ float activate_grad(float dy, float z, int act) {
+  const Vec<1> d{{dy}}, v{{z}};
+  return (act == ACT_SILU ? activated_grad<1, ACT_SILU>(d, v) : act == ACT_RELU ? activated_grad<1, ACT_RELU>(d, v) : d).v[0];
 }
 
 // ---------------------------------------------------------------- a slab on the chip
