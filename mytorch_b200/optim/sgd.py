@@ -60,6 +60,8 @@ class SGD(Optimizer):
         first, seen = [], set()
         for group in self.param_groups:
             for p in group["params"]:
+                if p.grad is None:
+                    raise RuntimeError(f"max_grad_norm: there is no gradient of a parameter of shape {p.shape}")
                 if p.shape != p.grad.shape or p.grad.device is not p.device:
                     raise RuntimeError(f"Mismatched shape or device between param and param.grad: {p}, {p.grad}")
                 if p.dtype is not float32 or p.grad.dtype is not float32:
