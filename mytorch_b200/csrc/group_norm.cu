@@ -138,7 +138,7 @@ struct Slabs {
   int of_vector, entries, merged, slots, slot_rows, slot_stride;
   bool vectors;                    // gamma and beta can be read as the values are
   float inv_positions, inv_group;  // 1 / hw, 1 / M
-  PoolDiv by_slabs, by_each, by_groups;
+  PoolDiv by_slabs, by_each;
 };
 
 // What a thread has to do.
@@ -864,7 +864,7 @@ Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
       t.smem = (int)smem;
       t.s = Slabs{hw, c, groups, each, wide, slabs, (int)units, of_slab, ctas, stretch, lanes, rows, __builtin_ctz(lanes), __builtin_ctz(rows), steps,
                   of_vector, entries, merged, slots, lanes < 32 ? 32 / lanes : 1, slot_stride, false, 1.f / (float)hw, (float)(1.0 / ((double)each * hw)),
-                  PoolDiv((unsigned)slabs), PoolDiv((unsigned)each), PoolDiv((unsigned)of_slab)};
+                  PoolDiv((unsigned)slabs), PoolDiv((unsigned)each)};
     }
     if (of_slab == groups) break;
   }
