@@ -22,7 +22,7 @@ class TokenCNN(nn.Module):
     def __init__(self, vocabulary=1000, width=64, classes=CLASSES, groups=8):
         super().__init__()
         self.embed = nn.Embedding(vocabulary, width, padding_idx=0, scale=width ** 0.5, channels_first=True)
-        self.embed.weight.normal_(0, width ** -0.5)
+        self.embed.reset_parameters(width ** -0.5)
         self.conv1 = nn.Conv2d(width, width, (1, 3), padding=(0, 1), bias=False)
         self.norm1 = nn.GroupNorm(groups, width, activation="silu")
         self.conv2 = nn.Conv2d(width, 2 * width, (1, 3), padding=(0, 1), bias=False)

@@ -19,8 +19,9 @@ class Embedding(Module):
         self.register_parameter("weight", Parameter(Tensor(shape=(num_embeddings, embedding_dim), dtype=dtype, device=device)))
         self.reset_parameters()
 
-    def reset_parameters(self):
-        self.weight.normal_(0, 1)
+    def reset_parameters(self, std=1):
+        """Rows N(0, std^2), the padding row zero."""
+        self.weight.normal_(0, std)
         if self.padding_idx is not None:
             rows = self.weight._host_array().copy()
             rows[self.padding_idx] = 0
