@@ -9,10 +9,11 @@
 // a slab, some whole groups of one image, in its shared memory, each CTA a stretch of the positions; four CTAs or so on an SM, one of which loads
 // while another one adds up or stores.  A thread copies (cp.async) and later reads its own vectors only, so the copies need no barrier; the CTAs exchange their sums
 // through distributed shared memory.
-// 256 x 128 x 56 x 56 with SiLU: forward 144 us (5.7 TB/s, 87 % of a copy), backward 246 (5.0 TB/s, 76 %).  What bounds the backward now: a CTA's time from its
-// last value to its first store, in which the cluster waits for its slowest, and an SM has four of them to overlap (backward without the exchange 190 us).
-// It went from 292 us by instructions and waits taken out of that time: xh recomputed instead of written back 275, sums over rows all at once 258 and by halves 250,
-// gamma from shared memory 247.  The 64 registers of four CTAs are what it may not pass: 12 bytes spilled cost 20 us.  Tried: clusters that stay and fetch
+// 256 x 128 x 56 x 56 with SiLU: forward 147 us (5.6 TB/s, 86 % of a copy), backward 252 to 260 (4.8 TB/s, 74 %; with ReLU 246).  What bounds the backward now: a CTA's time
+// from its last value to its first store, in which the cluster waits for its slowest, and an SM has four of them to overlap (backward without the exchange 190 us).
+// Its steps, each measured when it was made, took instructions and waits out of that time: 292 us at first, xh recomputed instead of written back 275, sums over
+// rows all at once 258 and by halves 250, gamma from shared memory 247; what SiLU's exponent leaves (see sigmoid) costs 3.  The 64 registers of four CTAs are
+// what it may not pass: 12 bytes spilled cost 20 us.  Tried: clusters that stay and fetch
 // the next slab meanwhile (forward 155 us, backward 337), sums sent with st.async (152, 319), two readings from the L2 cache by tickets or by launches (backward
 // 377), adding up while copies are on their way (+1 % to +11 %), marks for L2 (no change), CTAs that begin one after another (no change).
 // A slab that no cluster can hold goes through memory twice instead, see the kernels at the end.
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 4) gn_backward_kernel(const __grid_c
 }
 
 // dgamma and dbeta: the sums over the images, 32 columns of [n][2 c] a CTA, in a fixed order; of many images first those of stretches of them, to
-// stretches[gridDim.y][2 c].  Backward of 2000 images of 64 x 8 x 8 28 us, 37 with one stretch; of 70001 rows of 96 channels 431, not 1007.
+// stretches[gridDim.y][2 c].  Backward of 2000 images of 64 x 8 x 8 28 us, 37 with one stretch; of 70001 rows of 96 channels 438, not 1007.
 constexpr int kStretches = 128;
 int stretches_of(int n) { return n < 1024 ? 1 : n / 256 < kStretches ? n / 256 : kStretches; }
 
@@ -555,8 +556,8 @@ __global__ void __launch_bounds__(256) gn_params_kernel(const float* __restrict_
 // ---------------------------------------------------------------- a slab through memory
 
 // Images that no cluster can hold, and groups of more channels than a CTA has threads' vectors: partial statistics of stretches of positions,
-// statistics, result.  Bound by latency and by reading twice: 2 x 64 x 400 x 400 in 2 groups forward 86 us (25 is HBM's time for 8 bytes a value; 170 with a value a thread
-// on its way instead of kAhead), backward 126.  Rare among images that are trained on, so simple.
+// statistics, result.  Bound by latency and by reading twice: 2 x 64 x 400 x 400 in 2 groups forward 82 us (25 is HBM's time for 8 bytes a value; 170 with a value a thread
+// on its way instead of kAhead), backward 114.  Rare among images that are trained on, so simple.
 
 constexpr int kAhead = 8;
 
@@ -820,11 +821,12 @@ constexpr int kMostShared = 225 * 1024, kShared = 227 * 1024;  // of a CTA, of a
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 // planes: tensors that the cluster holds (1 forward, 2 backward).  Of slabs of several widths (the widest for so many lanes) and clusters of several sizes the pair is
-// taken that is done first.  A turn of all SMs takes 6.5 us, 0.015 us for each value of each thread of an SM's CTAs and 0.01 for one thread's: hardly
-// more if four CTAs share an SM than if two do (256 x 128 x 56 x 56 forward: 13.8 turns of two CTAs of 100 KB or four of 51, 147 and 145 us; backward: 27.7
-// turns of two of 105 KB or three of 69, 300 and 292), so the number of turns decides, and what fills the shared memory wins.  Measured beside that: a single CTA
-// on an SM, with nobody beside it while it loads, 2.4 us; pieces of 32 bytes 3.7 (of 64 bytes 0.15); 16 CTAs wait 2 us longer for one another, one CTA for
-// nobody.  (30 x 150 x 37 x 41, groups of ten: 5 CTAs for 30 channels 28 us, 3 for 10 53 us.)
+// taken that is done first.  A turn of all SMs takes 6.5 us, 0.015 us for each value of each thread of an SM's CTAs and 0.01 for one thread's, fitted to the forward:
+// hardly more if four CTAs share an SM than if two do (256 x 128 x 56 x 56 forward: 13.8 turns of two CTAs of 100 KB or four of 51, 147 and 145 us), so the number of
+// turns decides, and what fills the shared memory wins.  The backward is priced the same, by its two tensors: of 256 x 128 x 56 x 56 it takes clusters of eight
+// CTAs of 53 KB.  Measured beside that: a single CTA on an SM, with nobody beside it while it loads, 2.4 us; pieces of 32 bytes 3.7 (of 64 bytes 0.15);
+// 16 CTAs wait 2 us longer for one another, one CTA for nobody.  What the price does not see: 30 x 150 x 37 x 41 backward takes clusters of eight for 30 channels,
+// 1200 CTAs, 30 us; 71 such clusters fit the GPU at once, so the last few have a third turn to themselves.
 Plan plan_slabs(int n, int c, int hw, int groups, int planes, int alignment) {
   Plan t{};
   const int each = c / groups;
@@ -915,8 +917,8 @@ int backward_on_chip(const Plan& t, cudaStream_t st, A... args) {
    : (t).v == 2 ? (act == ACT_SILU ? f<2, ACT_SILU>(t, __VA_ARGS__) : act == ACT_RELU ? f<2, ACT_RELU>(t, __VA_ARGS__) : f<2, ACT_NONE>(t, __VA_ARGS__)) \
                 : (act == ACT_SILU ? f<1, ACT_SILU>(t, __VA_ARGS__) : act == ACT_RELU ? f<1, ACT_RELU>(t, __VA_ARGS__) : f<1, ACT_NONE>(t, __VA_ARGS__)))
 
-// Stretches that the positions of an image are cut into where slabs go through memory.
-// Stretches of the positions, of 64 at least, or of 4096 values of a part whose threads take whatever there is.
+// Stretches that the positions of an image are cut into where slabs go through memory: of 64 positions at least, or of 4096 values of a part whose threads take
+// whatever there is.
 int splits_of(int n, int hw, int parts, int values = 64) {
   long long want = (4LL * mtb_sm_count() + (long long)n * parts - 1) / ((long long)n * parts);
   const long long most = (long long)hw * values / 4096;

@@ -3,7 +3,8 @@
 the whole group is updated by one multi-tensor launch; otherwise (and through the registry's
 ``sgd`` entry) one launch per parameter, as in the reference.  ``max_grad_norm`` (no counterpart there):
 the gradients of all groups together, times ``grad_scale``, are clipped to that norm on their way into the
-update, which leaves ``param.grad`` as it is; ``grad_norm`` is then their norm, a tensor of one element on the device."""
+update, which leaves ``param.grad`` as it is; ``grad_norm`` is then their norm, a tensor of one element on the device.  Every
+parameter needs a gradient, with clipping as without."""
 from mytorch_b200.backends.backend_dispatcher import BackendDispatcher
 from mytorch_b200.dtype import float32
 from mytorch_b200.optim.optimizer import Optimizer
