@@ -306,6 +306,30 @@ int mtb_cross_entropy_forward_f32(int batch, int classes, const float* logits, c
 int mtb_cross_entropy_backward_f32(int batch, int classes, const float* logits, const long long* target, const float* dy, float* dlogits,
                                    void* stream);
 
+/* ---- log probabilities of given tokens, entropy and the most likely alternatives of rows of logits [n][v] (no counterpart in the reference) ----
+ * tokens: one a row, int32 (token_kind 0) or int64 (1); with `ignores` a row whose token is ignore_index has log probability 0 and no gradient from it, another
+ * token outside [0, v) has NaN.  top: how many alternatives, at most 32 and at most v, in descending order of their logits, equal ones by place.  top_log_probs,
+ * top_tokens: [n][top].  stats: [n][3], the largest logit, the sum of exp(z - largest) and the entropy, for the backward; may be NULL.
+ * Backward: dlog_probs, dentropy [n] and dtop [n][top] may be NULL each; the top_tokens of a row are distinct. */
+int mtb_token_log_probs_forward_f32(long long n, int v, const float* logits, int token_kind, const void* tokens, int ignores, long long ignore_index, int top,
+                                    float* log_probs, float* entropy, float* stats, float* top_log_probs, long long* top_tokens, void* stream);
+int mtb_token_log_probs_backward_f32(long long n, int v, const float* logits, int token_kind, const void* tokens, int ignores, long long ignore_index, int top,
+                                     const float* dlog_probs, const float* dentropy, const float* dtop, const float* stats, const long long* top_tokens, float* dlogits,
+                                     void* stream);
+
+/* ---- the norms around a residual block, with its gate (no counterpart in the reference) ----
+ * Rows of c values: out = scale residual + gate inner with inner = block post_weight / sqrt(mean(block^2) + eps), or block where post_weight is NULL;
+ * y = out weight / sqrt(mean(out^2) + eps).  gate: [rows / rows_per_gate][c], a row of it for every rows_per_gate rows; weight and gate may be NULL (1).
+ * block NULL: y is the norm of residual, out is not written.  rstd, block_rstd: [rows], the reciprocal roots, for the backward; may be NULL.
+ * Backward: x is out (block NULL: residual); dnew, dy and each of the results may be NULL. */
+int mtb_add_rms_norm_forward_f32(long long rows, int c, const float* residual, const float* block, const float* weight, const float* post_weight, const float* gate,
+                                 long long rows_per_gate, double scale, double eps, float* out, float* y, float* rstd, float* block_rstd, void* stream);
+long long mtb_add_rms_norm_workspace_bytes(long long rows, int c);
+int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dnew, const float* dy, const float* x, const float* rstd, const float* block,
+                                  const float* block_rstd, const float* weight, const float* post_weight, const float* gate, long long rows_per_gate, double scale,
+                                  float* dresidual, float* dblock, float* dweight, float* dpost_weight, float* dgate, void* workspace, long long workspace_bytes,
+                                  void* stream);
+
 /* ---- SGD (replaces sgd_reference, mytorch/native/cuda/optim.cu/source.cu:3-19, launched per parameter from
  *      mytorch/backends/cuda/ops/sgd.py:8-35) ---- */
 int mtb_sgd_f32(float* param, const float* grad, float* momentum_buffer, long long n, int is_first, double lr, double weight_decay,
@@ -325,6 +349,20 @@ int mtb_clip_grads_f32(int count, float* const* grads, const long long* sizes, c
 int mtb_sgd_multi_clipped_f32(int count, float* const* params, const float* const* grads, float* const* momentum_buffers, const long long* sizes,
                               const int* is_first, double lr, double weight_decay, double momentum, double dampening, int nesterov, int maximize,
                               double grad_scale, const double* sums, int nsums, double max_norm, float* norm, void* stream);
+/* AdamW over `count` tensors (no counterpart in the reference): g = grad_scale grad, clipped to max_norm as above where sums is not NULL;
+ * m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2, p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps).
+ * params: for each tensor five addresses, of parameters, gradients, first moments, second moments and of its t, an int64 that is counted on before the update, once
+ * where tensors share it.  scratch: device memory of mtb_adamw_scratch_bytes(count).
+ * Moments in 8 bits (mtb_adamw8_f32): for every 256 values of a tensor, the last block filled up, instead of the first moments 256 codes of first moments and 256 of
+ * second ones, instead of the second moments two bytes of scales; zeros are zero.  Betas are then rounded to 20 bits.  sizes: for each tensor its size and a seed of the
+ * roundings.  mtb_adamw8_moments_f32 writes what the codes stand for: params are four addresses, of codes, scales, first and second moments.
+ * params and sizes are HOST arrays. */
+long long mtb_adamw_scratch_bytes(int count);
+int mtb_adamw_f32(int count, void* const* params, const long long* sizes, double lr, double beta1, double beta2, double eps, double weight_decay, double grad_scale,
+                  const double* sums, int nsums, double max_norm, float* norm, void* scratch, void* stream);
+int mtb_adamw8_f32(int count, void* const* params, const long long* sizes, double lr, double beta1, double beta2, double eps, double weight_decay, double grad_scale,
+                   const double* sums, int nsums, double max_norm, float* norm, void* scratch, void* stream);
+int mtb_adamw8_moments_f32(int count, void* const* params, const long long* sizes, void* stream);
 /* gather gradient tensors into one flat all-reduce buffer (no counterpart: the reference has no
  * distributed code); srcs/offsets/sizes are HOST arrays */
 int mtb_pack_scale_f32(int count, const float* const* srcs, const long long* offsets, const long long* sizes, float* dst, double scale,

@@ -147,7 +147,7 @@ class CudaEnv:
         self._fork_events, self._join_events = {}, {}
         self.overlap_weight_gradients = not os.environ.get("MTB_SERIAL_WGRAD")
         from mytorch_b200.autograd import DAGTracker
-        from mytorch_b200.dtype import float32
+        from mytorch_b200.dtype import float32, int64, uint8
         from mytorch_b200.tensor import Tensor
 
         # Every operator asks for these, so they are native (csrc/binding.cpp):
@@ -155,7 +155,7 @@ class CudaEnv:
         # (nbytes) -> (address, bytes) of scratch for kernels that need it (split-K partials, per-CTA reduction partials): one
         # buffer per device, shared by all operators, which run in order on one stream; the side stream has its own
         self.workspace, self.side_workspace = _binding.workspace, _binding.side_workspace
-        _binding.set_state(Tensor, float32, CudaMemory, self, self.lib.stream_create, self._grow_scratch)
+        _binding.set_state(Tensor, float32, int64, uint8, CudaMemory, self, self.lib.stream_create, self._grow_scratch)
         DAGTracker.instance().join_hook = self.join_side
 
     # ---- devices, streams

@@ -687,6 +687,53 @@ def cuda_embedding_backward(output_grad, tokens, weight, scale=1.0, padding_idx=
     return [dw]
 
 
+# ---------------------------------------------------------------------------- norms around a residual block
+
+def _channel_rows(x):
+    """(rows, channels) of an activation: the channels of a position are a row; dimension 1 of an image, else the last."""
+    shape = x.shape
+    c = shape[1] if len(shape) == 4 else shape[-1]
+    return _numel(shape) // c if c else 0, c
+
+
+def _rows_per_gate(x, gate):
+    """How many rows share a row of the gate: [C], [first dimension, C], or like ``x``."""
+    if gate is None:
+        return 1
+    rows = _channel_rows(x)[0]
+    return max(1, rows if len(gate.shape) == 1 else 1 if gate.shape == x.shape else rows // max(x.shape[0], 1))
+
+
+@_reg("cuda", "add_rms_norm")
+def cuda_add_rms_norm(residual, block, weight=None, post_weight=None, gate=None, scale=1.0, eps=1e-6, keep=True):
+    """(scale * residual + gate * inner, its norm, rstd, block_rstd): ``block`` None: the norm of ``residual``, and None for the sum.  ``keep`` false: no statistics."""
+    _f32(residual, block, weight, post_weight, gate)
+    env = _env(residual)
+    rows, c = _channel_rows(residual)
+    new = _new(residual.shape, residual) if block is not None else None
+    y = _new(residual.shape, residual)
+    rstd = _new((rows,), residual) if keep else None
+    block_rstd = _new((rows,), residual) if keep and post_weight is not None else None
+    env.lib.add_rms_norm_forward_f32(rows, c, residual, block, weight, post_weight, gate, _rows_per_gate(residual, gate), float(scale), float(eps), new, y, rstd, block_rstd,
+                                     env.stream())
+    return new, y, rstd, block_rstd
+
+
+@_reg("cuda", "add_rms_norm_backward")
+def cuda_add_rms_norm_backward(dnew, dy, new, rstd, block_rstd, residual, block, weight=None, post_weight=None, gate=None, scale=1.0, needed=(True,) * 5):
+    """[dresidual, dblock, dweight, dpost_weight, dgate]; ``new``: the sum that forward returned (``residual`` where there was no block); ``needed``: which of them the
+    caller will use, the others are None.  ``dnew`` or ``dy`` may be None."""
+    _f32(dnew, dy, new, rstd, block_rstd, block, weight, post_weight, gate)
+    env = _env(new)
+    rows, c = _channel_rows(new)
+    out = [_new(new.shape, new) if needed[0] else None, _new(new.shape, new) if needed[1] and block is not None else None]
+    out += [_grad_buffer(t) if n and t is not None else None for n, t in zip(needed[2:], (weight, post_weight, gate))]
+    ws, ws_bytes = env.workspace(env.lib.add_rms_norm_workspace_bytes(rows, c))
+    env.lib.add_rms_norm_backward_f32(rows, c, dnew, dy, new, rstd, block, block_rstd, weight, post_weight, gate, _rows_per_gate(new, gate), float(scale), *out, ws, ws_bytes,
+                                      env.stream())
+    return out
+
+
 # ---------------------------------------------------------------------------- pooling
 
 def _pool_args(x, kernel_size, stride, padding):
@@ -1174,6 +1221,32 @@ def cuda_cross_entropy_backward(output_grad, input, target):
     return [dx]
 
 
+@_reg("cuda", "token_log_probs")
+def cuda_token_log_probs(logits, tokens, top=0, ignore_index=None, keep=True):
+    """(log_probs, entropy, top_log_probs, top_tokens, stats): one value a row of ``logits``, ``top`` alternatives (None without), and what the backward takes (``keep``)."""
+    _f32(logits)
+    env = _env(logits)
+    shape, v = tokens.shape, logits.shape[-1]
+    n = _numel(shape)
+    log_probs, entropy = _new(shape, logits), _new(shape, logits)
+    top_log_probs, top_tokens = (_new(shape + (top,), logits), _new(shape + (top,), logits, int64)) if top else (None, None)
+    stats = _new((n, 3), logits) if keep else None
+    env.lib.token_log_probs_forward_f32(n, v, logits, _TOKEN_KINDS[tokens.dtype], tokens, int(ignore_index is not None), ignore_index or 0, top, log_probs, entropy, stats,
+                                        top_log_probs, top_tokens, env.stream())
+    return log_probs, entropy, top_log_probs, top_tokens, stats
+
+
+@_reg("cuda", "token_log_probs_backward")
+def cuda_token_log_probs_backward(dlog_probs, dentropy, dtop, stats, top_tokens, logits, tokens, ignore_index=None):
+    """[dlogits]; each of the three gradients may be None."""
+    _f32(dlog_probs, dentropy, dtop, stats, logits)
+    env = _env(logits)
+    dlogits = _new(logits.shape, logits)
+    env.lib.token_log_probs_backward_f32(_numel(tokens.shape), logits.shape[-1], logits, _TOKEN_KINDS[tokens.dtype], tokens, int(ignore_index is not None), ignore_index or 0,
+                                         top_tokens.shape[-1] if dtop is not None else 0, dlog_probs, dentropy, dtop, stats, top_tokens, dlogits, env.stream())
+    return [dlogits]
+
+
 # ---------------------------------------------------------------------------- optimiser
 
 def _refuse_first_step_in_capture(env, is_first_time):
@@ -1218,3 +1291,17 @@ def cuda_clip_gradients(params, max_norm):
     min(1, max_norm / (norm + 1e-6)) in place, memory that several of them share once.  None where there is none, or one is not float32 on the device of
     the first."""
     return _binding.clip_gradients(params, -1.0 if max_norm is None else max_norm)
+
+
+@_reg("cuda", "adamw_multi")
+def cuda_adamw_multi(groups, states, bits, grad_scale=1.0, max_norm=None, seed=0):
+    """groups: [(params, lr, beta1, beta2, eps, weight_decay, maximize)], states: {param: {"step", "exp_avg", "exp_avg_sq"}}, with ``bits`` 8 {"step", "moments",
+    "scales"}.  Returns the norm of the gradients, times ``grad_scale``, to which ``max_norm`` clips them on their way into the update (True without), or None where a
+    tensor is missing or is not what it has to be, on the device of the first."""
+    return _binding.adamw_step(groups, states, bits, grad_scale, -1.0 if max_norm is None else max_norm, seed)
+
+
+@_reg("cuda", "adamw8_moments")
+def cuda_adamw8_moments(params, states):
+    """What the moments in 8 bits of a list of parameters stand for: two float32 vectors, the parameters one behind the other in the order of their memory."""
+    return _binding.adamw8_moments(params, states)

@@ -33,8 +33,9 @@ const char* (*g_last_error)() = nullptr;
 
 // Handed over by the Python layer when its CUDA state exists (set_state).
 PyTypeObject *g_tensor_type = nullptr, *g_memory_type = nullptr;
-PyObject *g_float32 = nullptr, *g_env = nullptr, *g_make_stream = nullptr, *g_grow_scratch = nullptr;
-#define MTB_NAMES(X) X(shape) X(dtype) X(device) X(index) X(_nhwc) X(_native_array) X(_itemsize) X(grad) X(momentum_buffer)
+PyObject *g_float32 = nullptr, *g_int64 = nullptr, *g_uint8 = nullptr, *g_env = nullptr, *g_make_stream = nullptr, *g_grow_scratch = nullptr;
+#define MTB_NAMES(X) X(shape) X(dtype) X(device) X(index) X(_nhwc) X(_native_array) X(_itemsize) X(grad) X(momentum_buffer) \
+  X(step) X(exp_avg) X(exp_avg_sq) X(moments) X(scales)
 #define X(n) PyObject* N_##n = nullptr;
 MTB_NAMES(X)
 #undef X
@@ -250,6 +251,9 @@ constexpr unsigned HOST(I... i) { return (0u | ... | (1u << i)); }
   X(grad_norm_sums, VALUE, 0) X(grad_norm_f32, LAUNCH, HOST(1, 2)) X(clip_grads_f32, LAUNCH, HOST(1, 2)) X(sgd_multi_clipped_f32, LAUNCH, HOST(1, 2, 3, 4, 5)) \
   X(group_norm_workspace_bytes, VALUE, 0) X(group_norm_forward_f32, LAUNCH, 0) X(group_norm_backward_f32, LAUNCH, 0) X(embedding_forward_f32, LAUNCH, 0) \
   X(embedding_backward_workspace_bytes, VALUE, 0) X(embedding_backward_f32, LAUNCH, 0) \
+  X(token_log_probs_forward_f32, LAUNCH, 0) X(token_log_probs_backward_f32, LAUNCH, 0) X(add_rms_norm_forward_f32, LAUNCH, 0) \
+  X(add_rms_norm_workspace_bytes, VALUE, 0) X(add_rms_norm_backward_f32, LAUNCH, 0) X(adamw_scratch_bytes, VALUE, 0) X(adamw_f32, LAUNCH, HOST(1, 2)) \
+  X(adamw8_f32, LAUNCH, HOST(1, 2)) X(adamw8_moments_f32, LAUNCH, HOST(1, 2)) \
   X(conv2d_workspace_bytes, VALUE, 0) X(conv2d_plan_f32, STATUS, HOST(11)) X(conv2d_pair_plan_f32, STATUS, HOST(11)) X(conv2d_pair_choice_f32, STATUS, HOST(11)) X(conv2d_pair_smem_bytes, VALUE, 0) X(conv2d_forward_f32, LAUNCH, 0) \
   X(conv2d_stats_max_rows, VALUE, 0) X(conv2d_forward_stats_f32, LAUNCH, HOST(17)) X(conv2d_bn_forward_f32, LAUNCH, 0) X(conv2d_bn_pool_takes, VALUE, 0) X(conv2d_bn_pool_scratch_bytes, VALUE, 0) X(conv2d_bn_pool_forward_f32, LAUNCH, 0) \
   X(batch_norm2d_forward_prestats_f32, LAUNCH, 0) X(conv2d_dgrad_f32, LAUNCH, 0) X(conv2d_dgrad_add_f32, LAUNCH, 0) \
@@ -534,12 +538,13 @@ struct OnDevice {
     if (o) held.push_back(o); else PyErr_Clear();
     return o;
   }
-  bool take(PyObject* t, float*& ptr, PyObject*& shape) {
-    if (!PyObject_TypeCheck(t, g_tensor_type) || look(t, N_dtype) != g_float32 || !(shape = look(t, N_shape))) return false;
+  template <class T>
+  bool take(PyObject* t, T*& ptr, PyObject*& shape, PyObject* dtype = g_float32) {
+    if (!PyObject_TypeCheck(t, g_tensor_type) || look(t, N_dtype) != dtype || !(shape = look(t, N_shape))) return false;
     Block* memory = (Block*)look(t, N__native_array);
     if (!memory || !PyObject_TypeCheck((PyObject*)memory, &BlockType) || !memory->ptr) return false;
     if (index < 0) index = memory->device_index;
-    ptr = (float*)memory->ptr;
+    ptr = (T*)memory->ptr;
     return memory->device_index == index;
   }
   bool take_like(PyObject* t, float*& ptr, PyObject* shape) {
@@ -718,15 +723,195 @@ PyObject* sgd_step_clipped(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return result.norm;
 }
 
-// set_state(Tensor, float32, CudaMemory, env, make_stream, grow_scratch)
+// ---- AdamW: in C++ for the reason above; three tensors of state for each parameter.
+
+// A state's tensor of this type with these extents (0: not looked at).
+template <class T>
+bool take_state(OnDevice& on, PyObject* state, PyObject* name, PyObject* dtype, long long first, long long second, T*& ptr) {
+  PyObject *t = PyDict_GetItemWithError(state, name), *shape;
+  if (!t || !on.take(t, ptr, shape, dtype) || !PyTuple_Check(shape)) return false;
+  const long long want[2] = {first, second};
+  if (PyTuple_GET_SIZE(shape) != (second ? 2 : 1)) return false;
+  for (int i = 0; i < PyTuple_GET_SIZE(shape); ++i)
+    if (PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i)) != want[i]) { PyErr_Clear(); return false; }
+  return true;
+}
+
+constexpr long long kMomentBlock = 256;  // values that share a scale (csrc/adamw.cu)
+
+struct AdamTables {
+  std::vector<void*> params;      // five addresses a tensor
+  std::vector<long long> sizes;   // in 8 bits a size and a seed
+  double h[5];  // lr, beta1, beta2, eps, weight_decay
+  int maximize, count = 0;
+};
+
+// adamw_step(groups, states, bits, grad_scale, max_norm, seed): one update of a list of groups, each a tuple (list of parameters, lr, beta1, beta2, eps,
+// weight_decay, maximize); max_norm < 0: no clipping, the result is then True, else the norm, a tensor of one element.  states: {parameter: {"step": int64
+// tensor of one element, and "exp_avg", "exp_avg_sq" like the parameter, or, of 8 bits, "moments" uint8 [blocks, 512], "scales" uint8 [blocks, 2]}}.  None where
+// something is missing or is not what it has to be, on the device of the first.
+PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  double scale, max_norm;
+  int bits;
+  long long seed;
+  if (n != 6 || !PyList_CheckExact(args[0]) || !PyDict_CheckExact(args[1])) { PyErr_SetString(PyExc_TypeError, "adamw_step(groups, states, bits, grad_scale, max_norm, seed)"); return nullptr; }
+  if (!ready() || !from_py(args[2], bits) || !from_py(args[3], scale) || !from_py(args[4], max_norm) || !from_py(args[5], seed)) return nullptr;
+  const bool clip = max_norm >= 0;
+  const Py_ssize_t groups = PyList_GET_SIZE(args[0]);
+  std::vector<AdamTables> tables(groups);
+  std::vector<const float*> grads;
+  std::vector<long long> sizes;
+  OnDevice on;
+  PyObject* like = nullptr;
+  unsigned ordinal = 0;
+  for (Py_ssize_t g = 0; g < groups; ++g) {
+    PyObject* group = PyList_GET_ITEM(args[0], g);
+    if (!PyTuple_CheckExact(group) || PyTuple_GET_SIZE(group) != 7 || !PyList_CheckExact(PyTuple_GET_ITEM(group, 0))) { PyErr_SetString(PyExc_TypeError, "a group of 7 expected"); return nullptr; }
+    AdamTables& t = tables[g];
+    for (int i = 0; i < 5; ++i)
+      if (!from_py(PyTuple_GET_ITEM(group, 1 + i), t.h[i])) return nullptr;
+    if ((t.maximize = PyObject_IsTrue(PyTuple_GET_ITEM(group, 6))) < 0) return nullptr;
+    PyObject* params = PyTuple_GET_ITEM(group, 0);
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
+      PyObject *param = PyList_GET_ITEM(params, i), *grad = on.look(param, N_grad), *shape;
+      float *p, *d;
+      long long size, *step;
+      if (!grad || grad == Py_None || !on.take(param, p, shape) || !on.take_like(grad, d, shape)) Py_RETURN_NONE;
+      if (!count_elements(shape, size)) return nullptr;
+      PyObject* state = PyDict_GetItemWithError(args[1], param);
+      if (PyErr_Occurred()) return nullptr;
+      if (!state || !PyDict_Check(state)) Py_RETURN_NONE;
+      if (!take_state(on, state, N_step, g_int64, 1, 0, step)) { if (PyErr_Occurred()) return nullptr; Py_RETURN_NONE; }
+      if (bits == 8) {
+        const long long blocks = (size + kMomentBlock - 1) / kMomentBlock;
+        unsigned char *codes, *scales;
+        if (!take_state(on, state, N_moments, g_uint8, blocks, 2 * kMomentBlock, codes) || !take_state(on, state, N_scales, g_uint8, blocks, 2, scales)) {
+          if (PyErr_Occurred()) return nullptr;
+          Py_RETURN_NONE;
+        }
+        t.params.insert(t.params.end(), {p, d, codes, scales, step});
+        t.sizes.insert(t.sizes.end(), {size, (long long)((unsigned)seed + 0x9E3779B1u * ++ordinal)});
+      } else {
+        PyObject *m = PyDict_GetItemWithError(state, N_exp_avg), *v = m ? PyDict_GetItemWithError(state, N_exp_avg_sq) : nullptr;
+        float *mp, *vp;
+        if (PyErr_Occurred()) return nullptr;
+        if (!v || !on.take_like(m, mp, shape) || !on.take_like(v, vp, shape)) Py_RETURN_NONE;
+        t.params.insert(t.params.end(), {p, d, mp, vp, step});
+        t.sizes.push_back(size);
+      }
+      like = param;
+      ++t.count;
+      grads.push_back(d);
+      sizes.push_back(size);
+    }
+  }
+  if (!like) Py_RETURN_NONE;
+  // a counter that two groups share would count twice
+  std::vector<std::pair<void*, Py_ssize_t>> counters;
+  for (Py_ssize_t g = 0; groups > 1 && g < groups; ++g)
+    for (int i = 0; i < tables[g].count; ++i) counters.emplace_back(tables[g].params[5 * i + 4], g);
+  std::sort(counters.begin(), counters.end());
+  for (size_t i = 1; i < counters.size(); ++i)
+    if (counters[i].first == counters[i - 1].first && counters[i].second != counters[i - 1].second) {
+      PyErr_SetString(PyExc_RuntimeError, "AdamW: two groups share a step counter");
+      return nullptr;
+    }
+  void* st;
+  NormResult result;
+  if (!on.enter(st)) return nullptr;
+  if (clip && !result.make(like, (int)grads.size())) return nullptr;
+  Ref device(PyObject_GetAttr(like, N_device));
+  Ref index(device ? PyObject_GetAttr(device, N_index) : nullptr);
+  Ref scratch(index ? g_memory_type->tp_alloc(g_memory_type, 0) : nullptr);
+  if (!scratch || !block_allocate((Block*)scratch.p, index, E_adamw_scratch_bytes::fn((int)grads.size()))) return nullptr;
+  char* corrections = (char*)((Block*)scratch.p)->ptr;
+  float* norm = clip ? result.to() : nullptr;
+  double* sums = clip ? result.partial() : nullptr;
+  const int nsums = clip ? E_grad_norm_sums::fn((int)grads.size()) : 0;
+  int rc = 0;
+  Py_BEGIN_ALLOW_THREADS
+  if (clip) rc = E_grad_norm_f32::fn((int)grads.size(), grads.data(), sizes.data(), sums, st);
+  for (auto& t : tables) {
+    if (rc || !t.count) continue;
+    const auto call = bits == 8 ? E_adamw8_f32::fn : E_adamw_f32::fn;
+    rc = call(t.count, t.params.data(), t.sizes.data(), t.h[0], t.h[1], t.h[2], t.h[3], t.h[4], t.maximize ? -scale : scale, sums, nsums, max_norm, norm, corrections, st);
+    corrections += E_adamw_scratch_bytes::fn(t.count);
+    norm = nullptr;  // left by the first of them
+  }
+  Py_END_ALLOW_THREADS
+  g_launches += groups + (clip ? 1 : 0);
+  if (rc) return raise_native(bits == 8 ? "mtb_adamw8_f32" : "mtb_adamw_f32", rc);
+  if (!clip) Py_RETURN_TRUE;
+  Py_INCREF(result.norm);
+  return result.norm;
+}
+
+// adamw8_moments(params, states): (first, second moments) of a list of parameters, one behind the other in the order of their memory, as float32 vectors;
+// None as above.
+PyObject* adamw8_moments(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2 || !PyList_CheckExact(args[0]) || !PyDict_CheckExact(args[1])) { PyErr_SetString(PyExc_TypeError, "adamw8_moments(params, states)"); return nullptr; }
+  if (!ready()) return nullptr;
+  std::vector<void*> params;  // four addresses a tensor
+  std::vector<long long> sizes;
+  OnDevice on;
+  PyObject* like = nullptr;
+  long long total = 0;
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); ++i) {
+    PyObject *param = PyList_GET_ITEM(args[0], i), *shape;
+    float* p;
+    long long size;
+    if (!on.take(param, p, shape)) Py_RETURN_NONE;
+    if (!count_elements(shape, size)) return nullptr;
+    PyObject* state = PyDict_GetItemWithError(args[1], param);
+    if (PyErr_Occurred()) return nullptr;
+    if (!state || !PyDict_Check(state)) Py_RETURN_NONE;
+    const long long blocks = (size + kMomentBlock - 1) / kMomentBlock;
+    unsigned char *c, *s;
+    if (!take_state(on, state, N_moments, g_uint8, blocks, 2 * kMomentBlock, c) || !take_state(on, state, N_scales, g_uint8, blocks, 2, s)) {
+      if (PyErr_Occurred()) return nullptr;
+      Py_RETURN_NONE;
+    }
+    like = param;
+    params.insert(params.end(), {c, s, nullptr, nullptr});
+    sizes.push_back(size);
+    total += size;
+  }
+  if (!like) Py_RETURN_NONE;
+  void* st;
+  if (!on.enter(st)) return nullptr;
+  Ref shape(Py_BuildValue("(L)", total));
+  PyObject* like_args[2] = {shape, like};
+  if (!shape) return nullptr;
+  Ref m(new_like(nullptr, like_args, 2)), v(m ? new_like(nullptr, like_args, 2) : nullptr);
+  if (!v) return nullptr;
+  Ref m_memory(PyObject_GetAttr(m, N__native_array)), v_memory(PyObject_GetAttr(v, N__native_array));
+  float *mp = (float*)((Block*)m_memory.p)->ptr, *vp = (float*)((Block*)v_memory.p)->ptr;
+  for (size_t i = 0; i < sizes.size(); ++i) {
+    params[4 * i + 2] = mp;
+    params[4 * i + 3] = vp;
+    mp += sizes[i];
+    vp += sizes[i];
+  }
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = E_adamw8_moments_f32::fn((int)sizes.size(), params.data(), sizes.data(), st);
+  Py_END_ALLOW_THREADS
+  if (rc) return raise_native("mtb_adamw8_moments_f32", rc);
+  ++g_launches;
+  return PyTuple_Pack(2, m.p, v.p);
+}
+
+// set_state(Tensor, float32, int64, uint8, CudaMemory, env, make_stream, grow_scratch)
 PyObject* set_state(PyObject*, PyObject* args) {
-  PyObject *tensor, *f32, *memory, *env, *make, *grow;
-  if (!PyArg_ParseTuple(args, "O!OO!OOO", &PyType_Type, &tensor, &f32, &PyType_Type, &memory, &env, &make, &grow)) return nullptr;
+  PyObject *tensor, *f32, *i64, *u8, *memory, *env, *make, *grow;
+  if (!PyArg_ParseTuple(args, "O!OOOO!OOO", &PyType_Type, &tensor, &f32, &i64, &u8, &PyType_Type, &memory, &env, &make, &grow)) return nullptr;
   if (!PyType_IsSubtype((PyTypeObject*)memory, &BlockType)) { PyErr_SetString(PyExc_TypeError, "a Block type expected"); return nullptr; }
 #define MTB_KEEP(slot, type, value) { Py_INCREF(value); type old = slot; slot = (type)value; Py_XDECREF((PyObject*)old); }
   MTB_KEEP(g_tensor_type, PyTypeObject*, tensor)
   MTB_KEEP(g_memory_type, PyTypeObject*, memory)
   MTB_KEEP(g_float32, PyObject*, f32)
+  MTB_KEEP(g_int64, PyObject*, i64)
+  MTB_KEEP(g_uint8, PyObject*, u8)
   MTB_KEEP(g_make_stream, PyObject*, make)
   MTB_KEEP(g_grow_scratch, PyObject*, grow)
   MTB_KEEP(g_env, PyObject*, env)
@@ -787,6 +972,8 @@ PyMethodDef methods[] = {
     {"sgd_step", (PyCFunction)(void (*)())sgd_step, METH_FASTCALL, "One SGD update of a list of (parameter, buffer, first)."},
     {"sgd_step_clipped", (PyCFunction)(void (*)())sgd_step_clipped, METH_FASTCALL, "One SGD update of several groups, by gradients clipped to a norm."},
     {"clip_gradients", (PyCFunction)(void (*)())clip_gradients, METH_FASTCALL, "The norm of the gradients of a list of parameters, and clipping in place."},
+    {"adamw_step", (PyCFunction)(void (*)())adamw_step, METH_FASTCALL, "One AdamW update of several groups."},
+    {"adamw8_moments", (PyCFunction)(void (*)())adamw8_moments, METH_FASTCALL, "What moments in 8 bits stand for, as vectors."},
     {"workspace", workspace<0>, METH_O, "(address, bytes) of scratch for compute-stream kernels."},
     {"side_workspace", workspace<1>, METH_O, "(address, bytes) of scratch for side-stream kernels."},
 #define X(n, k, h) {#n, (PyCFunction)(void (*)())E_##n::call, METH_FASTCALL, nullptr},

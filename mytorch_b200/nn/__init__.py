@@ -7,5 +7,6 @@ from .max_pool import MaxPool2d
 from .module import Module
 from .parameter import Parameter
 from .relu import ReLU
+from .rms_norm import AddRMSNorm, RMSNorm
 from .sequential import Sequential
 from .loss import CrossEntropyLoss
