@@ -4,11 +4,16 @@
 // A logit of -inf has probability 0 and adds nothing to the entropy or its gradient; a row of nothing else, or with a NaN or +inf, is NaN.
 // Alternatives are in the order of their logits, NaN before everything, equal ones by place, which one whole number holds (`key_of`).
 //
-// Bound by memory: forward reads a row once, backward reads and writes it once.  Each thread keeps a running maximum and both sums for its sixteenths of a row, and for
-// the alternatives only in which of its batches the maximum lies.  When the row is through, the top-th largest of the threads' own largest keys is a bound that no
-// alternative is under (so many keys reach it), and only the threads whose largest key reaches it, `top` of them, can hold one: their values are looked at again, out of
-// L2, and what reaches the bound, mostly little more than `top` keys, is put in order by counting.  Nothing of this depends on how the values are distributed but the number of keys that reach the
-// bound; above kCandidates of them, and for rows with a NaN, `top` passes find one each.
+// Bound by memory: forward reads a row once, backward reads and writes it once.  4096 rows of 50000: forward 132 us without alternatives, 6.2 TB/s, 152 with 8, 5.4;
+// backward 246 us, 6.7 TB/s.  Each thread keeps a running maximum and both sums of its share of the row, four loads of 16 bytes on their way at a time (44 registers: 40 warps an
+// SM; a second set on its way ahead of use costs a quarter of the warps: 146 instead of 129 without alternatives).
+//
+// Alternatives.  A thread also keeps the maxima of the four groups that its quads fall into, nothing else.  When the row is through, the r-th largest of the
+// groups' maxima in each of enough warps is a bound that `top` values reach, and only groups whose maximum reaches it can hold an alternative: mostly little more than
+// `top` of the row's 1024 (512, 128) groups, whose values are read again, and what reaches the bound is put in order by counting.  An exact bound by sorting all maxima: 180 us with 8
+// of 50000; one group a thread, which reads four times as much again out of HBM, as the rows under way are more than the L2 holds: 170; candidates picked
+// while the row comes by would cost every batch of values an insertion at first.  Where very many values equal the bound, as where a mask leaves fewer than `top`, those above it are taken
+// and then the first of the row that equal it; rows with a NaN, and more candidates than there is room for, take `top` passes that find one each.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -69,12 +74,20 @@ struct Sums {
     s_low *= f;
     ref = r;
   }
-  __device__ __forceinline__ void join(float most2, float s2, float t2) {
-    const float to = max_nan(most, most2);
-    if (to != most) raise(to);
-    const float d = gap(fmaxf(most2, kLowest), ref), f = exp2_of(d * kLog2e);
-    add(s, s_low, f * s2);
-    add(t, t_low, f * (t2 + s2 * d));
+  // Over the warp, in all its lanes.
+  __device__ __forceinline__ void reduce() {
+    float to = most;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) to = max_nan(to, __shfl_xor_sync(0xFFFFFFFFu, to, o));
+    raise(to);
+    s += s_low;
+    t += t_low;
+    s_low = t_low = 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+      t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+    }
   }
 };
 
@@ -103,156 +116,246 @@ struct Row {
   }
 };
 
-__device__ __forceinline__ Key sorted(Key k, int lane) {  // over the warp, the largest first
+// Over the warp, the largest first.
+template <class T>
+__device__ __forceinline__ T sorted(T k, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
     for (int j = size / 2; j > 0; j /= 2) {
-      const Key o = __shfl_xor_sync(0xFFFFFFFFu, k, j);
+      const T o = __shfl_xor_sync(0xFFFFFFFFu, k, j);
       if (((lane & j) == 0) == ((lane & size) == 0 || size == 32) ? o > k : o < k) k = o;
     }
   return k;
 }
-__device__ __forceinline__ Key merged(Key k, Key other_backwards, int lane) {  // the 32 largest of two sorted lists
-  if (other_backwards > k) k = other_backwards;
+// The 32 largest of two sorted lists, `other` backwards.
+template <class T>
+__device__ __forceinline__ T merged(T k, T other, int lane) {
+  if (other > k) k = other;
 #pragma unroll
   for (int j = 16; j > 0; j /= 2) {
-    const Key o = __shfl_xor_sync(0xFFFFFFFFu, k, j);
+    const T o = __shfl_xor_sync(0xFFFFFFFFu, k, j);
     if ((lane & j) == 0 ? o > k : o < k) k = o;
   }
   return k;
 }
+template <class T>
+__device__ __forceinline__ T merged_across(T k, T other, int lane) { return merged(k, __shfl_xor_sync(0xFFFFFFFFu, other, 31), lane); }
 
 // What W warps that share a row exchange.
 template <int W>
 struct Shared {
-  static constexpr int kCandidates = W == 1 ? 256 : 1024;
-  Key list[W][32], candidate[kCandidates], bound;
-  float part[W][3];
-  int chosen[kMostTop], chosen_count, candidate_count;
+  static constexpr int kCandidates = W == 1 ? 256 : 512, kGroups = W == 1 ? 128 : 256;
+  alignas(16) float part[W][4];
+  Key candidate[kCandidates], list[W];
+  int group[kGroups], groups, candidates;
 };
+constexpr int kSplit = 4;  // a thread's quads fall into groups by their number modulo this
 template <int W>
 __device__ __forceinline__ void meet() {
   if (W == 1) __syncwarp(); else __syncthreads();
 }
 
-// Of the quads [begin, end) of a row: the sums, in all threads, and in `out` (not shared.candidate) the `top` largest keys in their order, 0 where there are fewer.
+// The keys of the groups' values that reach the bound (`above`: that are above it) to the candidates, which are counted beyond what there is room for.
 template <int W>
-__device__ __forceinline__ Sums look(const Row& row, int begin, int end, int top, Shared<W>& shared, Key* out) {
+__device__ __forceinline__ void take(const Row& row, int begin, int end, Shared<W>& shared, int groups, int id, float bound, bool above = false) {
+  constexpr int T = 32 * W, kStride = kSplit * T;
+  const int each = (end - begin + kStride - 1) / kStride;  // quads of a group, rounded up
+  int g = id / each, k = id - g * each;
+  const int step_g = T / each, step_k = T - step_g * each;
+  while (g < groups) {
+    const int q = begin + shared.group[g] + k * kStride;
+    const float4 f = row.quad(q, end);
+    const int i = row.place(q);
+    const float x[4] = {f.x, f.y, f.z, f.w};
+    if (q < end) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((above ? x[j] > bound : x[j] >= bound) && i + j >= 0 && i + j < row.v) {
+          const int at = atomicAdd(&shared.candidates, 1);
+          if (at < Shared<W>::kCandidates) shared.candidate[at] = key_of(x[j], i + j);
+        }
+    }
+    g += step_g;
+    k += step_k;
+    if (k >= each) { k -= each; ++g; }
+  }
+}
+// The r-th largest of the values that the lanes of a warp hold, `more` of them each in descending order, in all lanes.
+template <int MORE>
+__device__ __forceinline__ float largest_but(int r, float (&m)[MORE], int lane) {
+  unsigned o[MORE];
+#pragma unroll
+  for (int i = 0; i < MORE; ++i) o[i] = ordered(m[i]);
+  unsigned most = 0;
+  for (int k = 0; k < r; ++k) {
+    most = __reduce_max_sync(0xFFFFFFFFu, o[0]);
+    if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, o[0] == most)) - 1) {
+#pragma unroll
+      for (int i = 0; i + 1 < MORE; ++i) o[i] = o[i + 1];
+      o[MORE - 1] = 0;
+    }
+  }
+  return value_of((Key)most << 32);
+}
+__device__ __forceinline__ void exchange(float& a, float& b) {
+  const float x = fmaxf(a, b);
+  b = fminf(a, b);
+  a = x;
+}
+
+// By a warp: the first places of a value to the candidates, up to `top` of these; their number.
+template <int W>
+__device__ __forceinline__ int take_equal(const Row& row, int begin, int end, Shared<W>& shared, int lane, float value, int count, int top) {
+  for (int from = begin; from < end && count < top; from += 32) {
+    const int q = from + lane, i = row.place(q);
+    const float4 f = row.quad(q, end);
+    const float x[4] = {f.x, f.y, f.z, f.w};
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mine += q < end && x[j] == value && i + j >= 0 && i + j < row.v;
+    int at = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int other = __shfl_up_sync(0xFFFFFFFFu, at, o);
+      if (lane >= o) at += other;
+    }
+    const int all = __shfl_sync(0xFFFFFFFFu, at, 31);
+    at += count - mine;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (q < end && x[j] == value && i + j >= 0 && i + j < row.v) {
+        if (at < top) shared.candidate[at] = key_of(x[j], i + j);
+        ++at;
+      }
+    count = min(top, count + all);
+    __syncwarp();
+  }
+  return count;
+}
+
+// Of the quads [begin, end) of a row: the sums, in all threads, and in `out` the `top` largest keys in their order, 0 where there are fewer.  given: loads
+// what the caller wants besides, called once while the row comes.
+template <int W, class F>
+__device__ __forceinline__ Sums look(const Row& row, int begin, int end, int top, Shared<W>& shared, Key* out, F given) {
   constexpr int T = 32 * W;
   const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5, id = W == 1 ? lane : threadIdx.x;
   Sums sums;
-  int where = -1;  // the first quad of the batch with the largest value
-  float4 next[4];
+  constexpr int G = kSplit;
+  const int each = (top + W - 1) / W;
+  float most[G];  // of the thread's groups
 #pragma unroll
-  for (int u = 0; u < 4; ++u) next[u] = row.quad(begin + id + u * T, end);
+  for (int u = 0; u < G; ++u) most[u] = -INFINITY;
   for (int q = begin; q < end; q += 4 * T) {
-    float x[16];
+    float4 f[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f[u] = row.quad(q + id + u * T, end);
+    if (q == begin) given();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) most[u % G] = max_nan(most[u % G], max_nan(max_nan(f[u].x, f[u].y), max_nan(f[u].z, f[u].w)));
+    float to = most[0];
+#pragma unroll
+    for (int u = 1; u < G; ++u) to = max_nan(to, most[u]);
+    if (to != sums.most) sums.raise(to);
+    float s[4], t[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      x[4 * u] = next[u].x; x[4 * u + 1] = next[u].y; x[4 * u + 2] = next[u].z; x[4 * u + 3] = next[u].w;
-    }
-    if (q + 4 * T < end) {
+      const float x[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
 #pragma unroll
-      for (int u = 0; u < 4; ++u) next[u] = row.quad(q + 4 * T + id + u * T, end);
-    }
-    float most = x[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) most = max_nan(most, x[i]);
-    most = max_nan(most, sums.most);
-    if (most != sums.most) {
-      where = q;
-      sums.raise(most);
-    }
-    float s[4] = {0, 0, 0, 0}, t[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float d = gap(x[i], sums.ref), e = exp2_of(d * kLog2e);
-      s[i % 4] += e;
-      t[i % 4] = fmaf(e, d, t[i % 4]);
+      for (int j = 0; j < 4; ++j) {
+        const float d = gap(x[j], sums.ref), e = exp2_of(d * kLog2e);
+        s[j] = u ? s[j] + e : e;
+        t[j] = u ? fmaf(e, d, t[j]) : e * d;
+      }
     }
     Sums::add(sums.s, sums.s_low, (s[0] + s[1]) + (s[2] + s[3]));
     Sums::add(sums.t, sums.t_low, (t[0] + t[1]) + (t[2] + t[3]));
   }
-  const float mine = sums.most;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m = __shfl_xor_sync(0xFFFFFFFFu, sums.most, o), s = __shfl_xor_sync(0xFFFFFFFFu, sums.s, o), t = __shfl_xor_sync(0xFFFFFFFFu, sums.t, o);
-    sums.join(m, s, t);
-  }
-  if (W > 1) {
-    if (lane == 0) { shared.part[warp][0] = sums.most; shared.part[warp][1] = sums.s; shared.part[warp][2] = sums.t; }
-  }
-  if (id == 0) shared.chosen_count = shared.candidate_count = 0;
-  // the thread's largest key
-  Key key = 0;
+  sums.reduce();
+  // a bound that `top` values reach: `each` of each warp's groups reach that warp's
+  float bound = INFINITY;
   if (top) {
-    if (where >= 0 && mine == mine) {
+    float m[G];
 #pragma unroll
-      for (int u = 3; u >= 0; --u) {
-        const int q = where + id + u * T, i = row.place(q);
-        const float4 f = row.quad(q, end);
-        if (f.w == mine) key = key_of(mine, i + 3);
-        if (f.z == mine) key = key_of(mine, i + 2);
-        if (f.y == mine) key = key_of(mine, i + 1);
-        if (f.x == mine) key = key_of(mine, i);
-      }
-    } else if (begin + id < end && row.place(begin + id) < row.v) {  // nothing but -inf
-      const int i = row.place(begin + id);
-      key = key_of(-INFINITY, i < 0 ? 0 : i);
-    }
-    Key best = sorted(key, lane);
-    if (W > 1) {
-      shared.list[warp][lane] = best;
-#pragma unroll
-      for (int step = 1; step < W; step *= 2) {
-        __syncthreads();
-        if (warp % (2 * step) == 0) {
-          best = merged(best, shared.list[warp + step][31 - lane], lane);
-          shared.list[warp][lane] = best;
-        }
-      }
-    }
-    if (warp == 0 && lane == top - 1) shared.bound = best;
+    for (int u = 0; u < G; ++u) m[u] = most[u];
+    exchange(m[0], m[1]); exchange(m[2], m[3]); exchange(m[0], m[2]); exchange(m[1], m[3]); exchange(m[1], m[2]);
+    bound = largest_but(each, m, lane);
   }
+  if (W > 1 && lane == 0) { shared.part[warp][0] = sums.most; shared.part[warp][1] = sums.s; shared.part[warp][2] = sums.t; shared.part[warp][3] = bound; }
+  if (id == 0) shared.groups = shared.candidates = 0;
   meet<W>();
   if (W > 1) {
+    const float4 p = *(const float4*)shared.part[lane < W ? lane : 0];
     sums = Sums();
-    for (int w = 0; w < W; ++w) sums.join(shared.part[w][0], shared.part[w][1], shared.part[w][2]);
+    sums.most = p.x;
+    sums.ref = fmaxf(p.x, kLowest);
+    sums.s = lane < W ? p.y : 0.f;
+    sums.t = lane < W ? p.z : 0.f;
+    sums.reduce();
+    if (top) {
+      float m[1] = {lane < W ? p.w : -INFINITY};
+      bound = largest_but((top + each - 1) / each, m, lane);  // so many warps are enough
+    }
   }
   if (!top) return sums;
   bool slow = sums.most != sums.most;
   if (!slow) {
-    const Key bound = shared.bound;
-    if (key != 0 && key >= bound) shared.chosen[atomicAdd(&shared.chosen_count, 1)] = id;  // at most `top` of them, or all that have a key where fewer have
-    meet<W>();
-    const int chosen = shared.chosen_count;
-    for (int c = warp; c < chosen; c += W) {
-      for (int q = begin + shared.chosen[c] + lane * T; q < end; q += 32 * T) {
-        const float4 f = row.quad(q, end);
-        const int i = row.place(q);
-        const float x[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const Key k = key_of(x[j], i + j);
-          if (k >= bound && i + j >= 0 && i + j < row.v) {
-            const int at = atomicAdd(&shared.candidate_count, 1);
-            if (at < Shared<W>::kCandidates) shared.candidate[at] = k;
-          }
+    for (int u = 0; u < G; ++u)
+      if (most[u] >= bound) {  // some more than `top`, many where some are equal
+        const int at = atomicAdd(&shared.groups, 1);
+        if (at < Shared<W>::kGroups) shared.group[at] = id + u * T;
+      }
+    meet<W>();
+    const int groups = shared.groups;
+    const bool equal = groups > Shared<W>::kGroups;
+    take(row, begin, end, shared, equal ? 0 : groups, id, bound);
+    meet<W>();
+    int count = shared.candidates;
+    if (equal || count > Shared<W>::kCandidates) {
+      // many values equal the bound: those above it, and of those that equal it the first of the row
+      meet<W>();
+      if (id == 0) shared.groups = shared.candidates = 0;
+      meet<W>();
+#pragma unroll
+      for (int u = 0; u < G; ++u)
+        if (most[u] > bound) {
+          const int at = atomicAdd(&shared.groups, 1);
+          if (at < Shared<W>::kGroups) shared.group[at] = id + u * T;
+        }
+      meet<W>();
+      count = shared.groups;
+      if (count <= Shared<W>::kGroups) {
+        take(row, begin, end, shared, count, id, bound, true);
+        meet<W>();
+        count = shared.candidates;
+      } else {
+        count = Shared<W>::kCandidates + 1;
+      }
+      if (count < top) {
+        if (warp == 0) count = take_equal(row, begin, end, shared, lane, bound, count, top);
+        if (W > 1) {
+          if (id == 0) shared.candidates = count;
+          __syncthreads();
+          count = shared.candidates;
         }
       }
     }
-    meet<W>();
-    const int count = shared.candidate_count;
     slow = count > Shared<W>::kCandidates;
-    if (!slow) {
-      for (int i = id; i < top; i += T)
-        if (i >= count) out[i] = 0;
-      for (int i = id; i < count; i += T) {
-        const Key k = shared.candidate[i];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += shared.candidate[j] > k;
-        if (rank < top) out[rank] = k;
+    if (!slow && count <= T) {
+      if (id < count || id < top) {
+        const Key best = id < count ? shared.candidate[id] : 0;
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < count; ++j) place += shared.candidate[j] > best;
+        if (id >= count) out[id] = 0;
+        else if (place < top) out[place] = best;
+      }
+    } else if (!slow) {
+      if (warp == 0) {
+        Key best = sorted(shared.candidate[lane], lane);
+        for (int from = 32; from < count; from += 32) best = merged_across(best, sorted(from + lane < count ? shared.candidate[from + lane] : 0, lane), lane);
+        if (lane < top) out[lane] = best;
       }
     }
   }
@@ -276,10 +379,10 @@ __device__ __forceinline__ Sums look(const Row& row, int begin, int end, int top
       }
       if (W > 1) {
         __syncthreads();
-        if (lane == 0) shared.list[warp][0] = best;
+        if (lane == 0) shared.list[warp] = best;
         __syncthreads();
         for (int w = 0; w < W; ++w)
-          if (shared.list[w][0] > best) best = shared.list[w][0];
+          if (shared.list[w] > best) best = shared.list[w];
       }
       if (id == 0) out[k] = best;
       below = best;
@@ -301,13 +404,24 @@ struct Forward {
 
 __device__ __forceinline__ long long token_at(const void* tokens, int wide, long long row) { return wide ? ((const long long*)tokens)[row] : ((const int*)tokens)[row]; }
 
+// The row's token and its logit, which come while the row does; in thread 0 of those that share the row.
+struct Given {
+  const Forward& a;
+  long long row;
+  int id;
+  long long token;
+  float z = 0;
+
+  __device__ __forceinline__ Given(const Forward& a, long long row, int id) : a(a), row(row), id(id), token(id == 0 ? token_at(a.tokens, a.wide, row) : -1) {}
+  __device__ __forceinline__ void operator()() { if (token >= 0 && token < a.v) z = a.logits[row * a.v + token]; }
+};
+
 // By thread `id` of those that share the row.
-__device__ __forceinline__ void leave(const Forward& a, long long row, int id, const Sums& sums, const Key* found) {
+__device__ __forceinline__ void leave(const Forward& a, long long row, int id, const Given& given, const Sums& sums, const Key* found) {
   const bool none = !(sums.most >= kLowest && sums.most < INFINITY);  // a NaN, +inf, or nothing but -inf
   const float s = none ? NAN : sums.s + sums.s_low, log_s = logf(s);
   if (id == 0) {
-    const long long token = token_at(a.tokens, a.wide, row);
-    a.log_probs[row] = a.ignores && token == a.ignore_index ? 0.f : token < 0 || token >= a.v ? NAN : a.logits[row * a.v + token] - sums.most - log_s;
+    a.log_probs[row] = a.ignores && given.token == a.ignore_index ? 0.f : given.token < 0 || given.token >= a.v ? NAN : given.z - sums.most - log_s;
     const float h = log_s - (sums.t + sums.t_low) / s;
     a.entropy[row] = h;
     if (a.stats) {
@@ -324,17 +438,20 @@ __device__ __forceinline__ void leave(const Forward& a, long long row, int id, c
 
 // A row by W warps: 1 (eight rows a CTA) or a whole CTA.
 template <int W>
-__global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_constant__ Forward a) {
-  __shared__ Shared<W> shared[kWarps / W];
-  __shared__ Key found[kWarps / W][kMostTop];
+__global__ void __launch_bounds__(W == 1 ? kThreads : 32 * W) log_probs_kernel(const __grid_constant__ Forward a) {
+  constexpr int kRows = W == 1 ? kWarps : 1;
+  __shared__ Shared<W> shared[kRows];
+  __shared__ Key found[kRows][kMostTop];
   mtb_launch_dependents();
   mtb_wait_prior();
   const int part = W == 1 ? threadIdx.x >> 5 : 0;
   const long long index = W == 1 ? blockIdx.x * (long long)kWarps + part : blockIdx.x;
   if (index >= a.n) return;
   const Row row(a.logits + index * a.v, a.v);
-  const Sums sums = look<W>(row, 0, row.quads, a.top, shared[part], found[part]);
-  leave(a, index, W == 1 ? threadIdx.x & 31 : threadIdx.x, sums, found[part]);
+  const int id = W == 1 ? threadIdx.x & 31 : threadIdx.x;
+  Given given(a, index, id);
+  const Sums sums = look<W>(row, 0, row.quads, a.top, shared[part], found[part], [&] { given(); });
+  leave(a, index, id, given, sums, found[part]);
 }
 
 // A row by a cluster of CTAs, each of which finds the alternatives of its part; the first puts them together.
@@ -350,9 +467,10 @@ __global__ void __launch_bounds__(kThreads) log_probs_cluster_kernel(const __gri
   const long long index = blockIdx.x / ctas;
   const Row row(a.logits + index * a.v, a.v);
   const int each = (row.quads + ctas - 1) / ctas, begin = rank * each < row.quads ? rank * each : row.quads, end = begin + each < row.quads ? begin + each : row.quads;
-  const Sums mine = look<kWarps>(row, begin, end, a.top, shared, found);
+  Given given(a, index, rank == 0 ? threadIdx.x : 1);
+  const Sums mine = look<kWarps>(row, begin, end, a.top, shared, found, [&] { given(); });
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-  if (threadIdx.x < a.top) cluster.map_shared_rank(&all[0][0], 0)[rank * kMostTop + threadIdx.x] = found[threadIdx.x];
+  if (a.top && threadIdx.x < kMostTop) cluster.map_shared_rank(&all[0][0], 0)[rank * kMostTop + threadIdx.x] = threadIdx.x < a.top ? found[threadIdx.x] : 0;
   if (threadIdx.x == 0) {
     float* to = cluster.map_shared_rank(&parts[0][0], 0) + 3 * rank;
     to[0] = mine.most;
@@ -362,18 +480,19 @@ __global__ void __launch_bounds__(kThreads) log_probs_cluster_kernel(const __gri
   cluster.sync();
   if (rank != 0) return;
   Sums sums;
-  for (int r = 0; r < ctas; ++r) sums.join(parts[r][0], parts[r][1], parts[r][2]);
-  if (a.top) {
-    for (int i = threadIdx.x; i < ctas * a.top; i += kThreads) {
-      const Key k = all[i / a.top][i % a.top];
-      int place = i % a.top;  // in its own list
-      for (int r = 0; r < ctas; ++r)
-        for (int j = 0; r != i / a.top && j < a.top && all[r][j] > k; ++j) ++place;
-      if (k != 0 && place < a.top) found[place] = k;
-    }
-    __syncthreads();
+  const int r = (threadIdx.x & 31) < ctas ? threadIdx.x & 31 : 0;
+  sums.most = parts[r][0];
+  sums.ref = fmaxf(sums.most, kLowest);
+  sums.s = (threadIdx.x & 31) < ctas ? parts[r][1] : 0.f;
+  sums.t = (threadIdx.x & 31) < ctas ? parts[r][2] : 0.f;
+  sums.reduce();
+  if (a.top && threadIdx.x < 32) {  // sorted lists
+    Key best = all[0][threadIdx.x];
+    for (int r = 1; r < ctas; ++r) best = merged(best, all[r][31 - threadIdx.x], threadIdx.x);
+    found[threadIdx.x] = best;
+    __syncwarp();
   }
-  leave(a, index, threadIdx.x, sums, found);
+  leave(a, index, threadIdx.x, given, sums, found);
 }
 
 struct Backward {
@@ -399,10 +518,8 @@ struct RowGradient {
   }
 };
 
-constexpr int kPart = 16 * kThreads;  // values of a CTA
-
-// A row by W warps: 1, or `parts` CTAs, four vectors a thread.
-template <int W>
+// A row by W warps: 1, or `parts` CTAs, U vectors a thread.
+template <int W, int U>
 __global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __grid_constant__ Backward a) {
   constexpr int T = 32 * W;
   mtb_launch_dependents();
@@ -413,10 +530,10 @@ __global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __gr
   const Row row(a.logits + index * a.v, a.v);
   float* to = a.dlogits + index * a.v - row.lead;
   const bool together = ((reinterpret_cast<uintptr_t>(to) ^ reinterpret_cast<uintptr_t>(row.z)) & 15u) == 0;
-  const int begin = W == 1 ? 0 : (int)(blockIdx.x % a.parts) * (kPart / 4), end = W == 1 ? row.quads : min(begin + kPart / 4, row.quads);
-  float4 f[4];
+  const int begin = W == 1 ? 0 : (int)(blockIdx.x % a.parts) * (U * kThreads), end = W == 1 ? row.quads : min(begin + U * kThreads, row.quads);
+  float4 f[U];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) f[u] = row.quad(begin + id + u * T, end);
+  for (int u = 0; u < U; ++u) f[u] = row.quad(begin + id + u * T, end);
   // every warp for itself: the row's numbers, an alternative a lane
   const long long token = token_at(a.tokens, a.wide, index);
   RowGradient r;
@@ -433,13 +550,13 @@ __global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __gr
   r.all = extra;
   for (int o = 16; o > 0; o >>= 1) r.all += __shfl_xor_sync(0xFFFFFFFFu, r.all, o);
   r.all += r.g;
-  for (int q = begin; q < end; q += 4 * T) {
+  for (int q = begin; q < end; q += U * T) {
     if (W == 1 && q > begin) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) f[u] = row.quad(q + id + u * T, end);
+      for (int u = 0; u < U; ++u) f[u] = row.quad(q + id + u * T, end);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int at = q + id + u * T, i = row.place(at);
       if (at >= end) continue;
       const float4 d = make_float4(r.at(f[u].x), r.at(f[u].y), r.at(f[u].z), r.at(f[u].w));
@@ -476,9 +593,13 @@ MTB_API int mtb_token_log_probs_forward_f32(long long n, int v, const float* log
   MTB_REQUIRE(logits && tokens && log_probs && entropy && (top == 0 || (top_log_probs && top_tokens)), "token_log_probs_forward: bad arguments");
   cudaStream_t st = (cudaStream_t)stream;
   const Forward a{n, v, token_kind, ignores, top, ignore_index, logits, tokens, log_probs, entropy, stats, top_log_probs, top_tokens};
-  // few rows: CTAs side by side on each, as long as all fit and each has enough of it
+  // Few rows: CTAs side by side on each, as long as all fit (six an SM) and each has enough of it.  One row of 50000 with 8 alternatives 11.8 -> 6.3 us, 300 rows 26 -> 20.6;
+  // 64 rows of 10007 would take 7.6 instead of 5.6.
   int ctas = 1;
-  while (ctas < kMostCtas && n * ctas * 2 <= 2 * mtb_sm_count() && v / (2 * ctas) >= 2048) ctas *= 2;
+  const bool many = n > 8LL * mtb_sm_count();
+  while (ctas < kMostCtas && n * ctas * 2 <= 6 * mtb_sm_count() && v / (2 * ctas) >= 4096) ctas *= 2;
+  // Otherwise a row by so many warps that there are enough of them under way.  With 8 alternatives by 1, 4 and 8 warps: 16384 x 1000 21, 47, 87 us (an earlier bound); 1184 x 4000
+  // 8.7, 9.4, 11.9; 2368 x 8000 32, 20, 25; 4096 x 30000 125, 94, 101; 1600 x 128000 398, 189, 161; of few rows 592 x 4000 8.6, 8.6, 7.7.
   if (ctas > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n * ctas));
@@ -493,8 +614,10 @@ MTB_API int mtb_token_log_probs_forward_f32(long long n, int v, const float* log
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     MTB_CUDA(cudaLaunchKernelEx(&cfg, log_probs_cluster_kernel, a));
-  } else if (v <= 1024) {
+  } else if (v <= 1024 || (v <= 4096 && many)) {
     MTB_LAUNCH(log_probs_kernel<1>, (unsigned)mtb_div_up(n, kWarps), kThreads, 0, st, a);
+  } else if (v <= 32768 && many) {
+    MTB_LAUNCH(log_probs_kernel<4>, (unsigned)n, 128, 0, st, a);
   } else {
     MTB_LAUNCH(log_probs_kernel<kWarps>, (unsigned)n, kThreads, 0, st, a);
   }
@@ -508,14 +631,16 @@ MTB_API int mtb_token_log_probs_backward_f32(long long n, int v, const float* lo
   MTB_REQUIRE(sizes_fine(n, v, token_kind, top), "token_log_probs_backward: bad sizes (at most 2^30 values a row, 32 alternatives)");
   if (n == 0) return MTB_OK;
   MTB_REQUIRE(logits && tokens && stats && dlogits && (top == 0 || !dtop || top_tokens), "token_log_probs_backward: bad arguments");
-  const int parts = mtb_div_up((long long)v + 3, kPart);  // a row may begin three values into its first quad
+  // By one warp 16384 x 1500 takes 34 us, by CTAs of two vectors a thread 46, of four 54; 8192 x 3000 35, 45, 38; eight vectors a thread: 4096 x 10007 58 instead
+  // of 56, 4096 x 50000 246 instead of 262.
+  const bool warps = v <= 1024 || (v <= 4096 && n > 8LL * mtb_sm_count());
+  const int vectors = v <= 2048 ? 2 : v <= 16384 ? 4 : 8, parts = warps ? 1 : mtb_div_up((long long)v + 3, 4 * vectors * kThreads);  // a row may begin three values into its first quad
+  const long long ctas = warps ? mtb_div_up(n, kWarps) : n * parts;
+  MTB_REQUIRE(ctas < 1LL << 31, "token_log_probs_backward: too many values in one call");
   const Backward a{n, v, token_kind, ignores, top, ignore_index, logits, tokens, dlog_probs, dentropy, dtop, stats, top_tokens, dlogits, parts};
-  if (v <= 1024) {
-    MTB_LAUNCH(log_probs_backward_kernel<1>, (unsigned)mtb_div_up(n, kWarps), kThreads, 0, (cudaStream_t)stream, a);
-  } else {
-    MTB_REQUIRE(n * parts < 1LL << 31, "token_log_probs_backward: too many values in one call");
-    MTB_LAUNCH(log_probs_backward_kernel<kWarps>, (unsigned)(n * parts), kThreads, 0, (cudaStream_t)stream, a);
-  }
+  const auto kernel = warps ? log_probs_backward_kernel<1, 4> : vectors == 2 ? log_probs_backward_kernel<kWarps, 2>
+                      : vectors == 4 ? log_probs_backward_kernel<kWarps, 4> : log_probs_backward_kernel<kWarps, 8>;
+  MTB_LAUNCH(kernel, (unsigned)ctas, kThreads, 0, (cudaStream_t)stream, a);
   MTB_LAUNCH_CHECK("log_probs_backward_kernel");
   return MTB_OK;
 }
