@@ -729,8 +729,9 @@ def cuda_add_rms_norm_backward(dnew, dy, new, rstd, block_rstd, residual, block,
     out = [_new(new.shape, new) if needed[0] else None, _new(new.shape, new) if needed[1] and block is not None else None]
     out += [_grad_buffer(t) if n and t is not None else None for n, t in zip(needed[2:], (weight, post_weight, gate))]
     ws, ws_bytes = env.workspace(env.lib.add_rms_norm_workspace_bytes(rows, c))
-    env.lib.add_rms_norm_backward_f32(rows, c, dnew, dy, new, rstd, block, block_rstd, weight, post_weight, gate, _rows_per_gate(new, gate), float(scale), *out, ws, ws_bytes,
-                                      env.stream())
+    dgate = out[4] if rows or gate is None or len(gate.shape) == 1 else None  # a gate of no rows
+    env.lib.add_rms_norm_backward_f32(rows, c, dnew, dy, new, rstd, block, block_rstd, weight, post_weight, gate, _rows_per_gate(new, gate), float(scale), *out[:4], dgate,
+                                      ws, ws_bytes, env.stream())
     return out
 
 
