@@ -19,50 +19,53 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTensors = 192;
-constexpr int kChunk = 2048;   // elements of a CTA with moments in 32 bits
-constexpr int kChunk8 = 4096;  // and in 8: two blocks a warp
 constexpr int kBlock = 256;
+constexpr int kChunk = 2048;  // elements of a CTA: eight a thread, all of whose loads are on their way at once; of 8 bits a block a warp
 constexpr int kSteps = 256;
 
 struct Hyper {
-  float lr, b1, b2, c1, c2, eps, keep, grad_scale;  // c1 = 1 - b1, c2 = 1 - b2 (8 bits: its root), keep = 1 - lr wd
+  float b1, b2, c1, c2, eps, keep;  // c1 = 1 - b1, c2 = 1 - b2 (8 bits: its root), keep = 1 - lr wd
 };
 
-// What a step makes of t, for every counter of a call.
-struct Corrections {
+// What a step makes of t, for every counter of a call, and what multiplies the gradients.
+struct alignas(16) Corrections {
   float step_size, root;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
-  unsigned t, unused;
+  unsigned t;
+  float grad_scale;
 };
 
 struct StepTable {
   long long* step[kSteps];
   int count;
 };
-__global__ void __launch_bounds__(256) adamw_begin_kernel(const __grid_constant__ StepTable t, double lr, double b1, double b2, Corrections* __restrict__ out) {
+// One CTA in front of the update: no CTA of that waits for a sum.
+__global__ void __launch_bounds__(256) adamw_begin_kernel(const __grid_constant__ StepTable t, double lr, double b1, double b2, float grad_scale, MtbClip clip,
+                                                          Corrections* __restrict__ out) {
   mtb_launch_dependents();
   mtb_wait_prior();
+  if (clip.sums) grad_scale *= mtb_clip_factor<256>(clip);
   if ((int)threadIdx.x >= t.count) return;
   const long long step = *t.step[threadIdx.x] + 1;
   *t.step[threadIdx.x] = step;
-  out[threadIdx.x] = Corrections{(float)(lr / (1.0 - pow(b1, (double)step))), (float)(1.0 / sqrt(1.0 - pow(b2, (double)step))), (unsigned)step, 0u};
+  out[threadIdx.x] = Corrections{(float)(lr / (1.0 - pow(b1, (double)step))), (float)(1.0 / sqrt(1.0 - pow(b2, (double)step))), (unsigned)step, grad_scale};
 }
 
-template <class M>
+// N tensors: a table of a few costs its launch less.
+template <class M, int N>
 struct Table {
-  float* p[kTensors];
-  const float* g[kTensors];
-  M* m[kTensors];  // 32 bits: the first moments; 8 bits: [block][first 256 | second 256]
-  M* v[kTensors];  // 32 bits: the second moments; 8 bits: [block][scale of the first, of the second]
-  long long n[kTensors];
-  int chunk_start[kTensors + 1];  // CTA b works on tensor k with chunk_start[k] <= b < chunk_start[k + 1]
-  unsigned short slot[kTensors];  // which corrections
-  unsigned key[kTensors];
+  float* p[N];
+  const float* g[N];
+  M* m[N];  // 32 bits: the first moments; 8 bits: [block][first 256 | second 256]
+  M* v[N];  // 32 bits: the second moments; 8 bits: [block][scale of the first, of the second]
+  long long n[N];
+  int chunk_start[N + 1];  // CTA b works on tensor k with chunk_start[k] <= b < chunk_start[k + 1]
+  unsigned short slot[N];  // which corrections
+  unsigned key[N];
   int count;
 };
 
-template <class M>
-__device__ __forceinline__ int tensor_of(const Table<M>& t, int chunk) {
+template <class T>
+__device__ __forceinline__ int tensor_of(const T& t, int chunk) {
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {  // last k with chunk_start[k] <= chunk
     const int mid = (lo + hi + 1) >> 1;
@@ -71,25 +74,79 @@ __device__ __forceinline__ int tensor_of(const Table<M>& t, int chunk) {
   return lo;
 }
 
+// Root and quotient to 2^-22 of themselves, the step's share of which is far under a parameter's last place.
 __device__ __forceinline__ void update(float& p, float m, float v, const Hyper& h, const Corrections& c) {
-  p = p * h.keep - c.step_size * m / (sqrtf(v) * c.root + h.eps);
+  float root;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
+  p = fmaf(p, h.keep, -__fdividef(c.step_size * m, fmaf(root, c.root, h.eps)));
+}
+__device__ __forceinline__ void moments(float g, float& m, float& v, const Hyper& h) {
+  m = fmaf(h.b1, m, h.c1 * g);
+  v = fmaf(h.b2, v, h.c2 * g * g);
 }
 
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<float> t, Hyper h, const Corrections* __restrict__ corrections, MtbClip clip) {
+// The chunks are taken backwards: what the norm read last is still in L2.  What is used once is marked to leave it first.
+template <int N>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<float, N> t, Hyper h, const Corrections* __restrict__ corrections) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  if (clip.sums) h.grad_scale *= mtb_clip_factor<kThreads>(clip);
-  const int k = tensor_of(t, blockIdx.x);
-  const long long e = (long long)((int)blockIdx.x - t.chunk_start[k]) * kChunk, left = t.n[k] - e;
+  const int chunk = t.chunk_start[t.count] - 1 - (int)blockIdx.x, k = tensor_of(t, chunk);
+  const long long e = (long long)(chunk - t.chunk_start[k]) * kChunk, left = t.n[k] - e;
   const int n = left < kChunk ? (int)left : kChunk;
-  const Corrections c = corrections[t.slot[k]];
   float *p = t.p[k] + e, *m = t.m[k] + e, *v = t.v[k] + e;
   const float* g = t.g[k] + e;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const float gg = g[i] * h.grad_scale;
-    m[i] = h.b1 * m[i] + h.c1 * gg;
-    v[i] = h.b2 * v[i] + h.c2 * gg * gg;
-    update(p[i], m[i], v[i], h, c);
+  const bool vectors = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0;
+  if (vectors && n == kChunk) {
+    float4 pp[2], gg[2], mm[2], vv[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = threadIdx.x + u * kThreads;
+      gg[u] = __ldcs((const float4*)g + i);
+      pp[u] = __ldcs((const float4*)p + i);
+      mm[u] = __ldcs((const float4*)m + i);
+      vv[u] = __ldcs((const float4*)v + i);
+    }
+    const Corrections c = corrections[t.slot[k]];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = threadIdx.x + u * kThreads;
+      float* const ps[4] = {&pp[u].x, &pp[u].y, &pp[u].z, &pp[u].w};
+      float* const ms[4] = {&mm[u].x, &mm[u].y, &mm[u].z, &mm[u].w};
+      float* const vs[4] = {&vv[u].x, &vv[u].y, &vv[u].z, &vv[u].w};
+      const float gs[4] = {gg[u].x, gg[u].y, gg[u].z, gg[u].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        moments(gs[j] * c.grad_scale, *ms[j], *vs[j], h);
+        update(*ps[j], *ms[j], *vs[j], h, c);
+      }
+      __stcs((float4*)p + i, pp[u]);
+      __stcs((float4*)m + i, mm[u]);
+      __stcs((float4*)v + i, vv[u]);
+    }
+    return;
+  }
+  float pp[8], gg[8], mm[8], vv[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int i = threadIdx.x + u * kThreads;
+    if (i < n) {
+      gg[u] = __ldcs(g + i);
+      pp[u] = __ldcs(p + i);
+      mm[u] = __ldcs(m + i);
+      vv[u] = __ldcs(v + i);
+    }
+  }
+  const Corrections c = corrections[t.slot[k]];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int i = threadIdx.x + u * kThreads;
+    if (i < n) {
+      moments(gg[u] * c.grad_scale, mm[u], vv[u], h);
+      update(pp[u], mm[u], vv[u], h, c);
+      __stcs(p + i, pp[u]);
+      __stcs(m + i, mm[u]);
+      __stcs(v + i, vv[u]);
+    }
   }
 }
 
@@ -120,83 +177,151 @@ __device__ __forceinline__ unsigned encode_second(float v, float per, unsigned r
   return v > 0.f && code == 0 ? 1u : code;
 }
 
-// A warp a block, 8 values a lane: 4 at 4 lane, 4 at 128 + 4 lane.
-__global__ void __launch_bounds__(kThreads) adamw8_kernel(const __grid_constant__ Table<unsigned char> t, Hyper h, const Corrections* __restrict__ corrections, MtbClip clip) {
-  mtb_launch_dependents();
-  mtb_wait_prior();
-  if (clip.sums) h.grad_scale *= mtb_clip_factor<kThreads>(clip);
-  const int k = tensor_of(t, blockIdx.x), lane = threadIdx.x & 31;
-  const Corrections c = corrections[t.slot[k]];
-  const unsigned key = mix(t.key[k] + c.t);
-  for (int turn = threadIdx.x >> 5; turn < kChunk8 / kBlock; turn += kThreads / 32) {
-    const long long block = (long long)((int)blockIdx.x - t.chunk_start[k]) * (kChunk8 / kBlock) + turn, e = block * kBlock, left = t.n[k] - e;
-    if (left <= 0) return;
-    const int n = left < kBlock ? (int)left : kBlock;
-    float* p = t.p[k] + e;
-    const float* g = t.g[k] + e;
-    unsigned char *codes = t.m[k] + block * 2 * kBlock, *scales = t.v[k] + block * 2;
-    const float unit_m = unit_of(scales[0]), unit_v = unit_of(scales[1]);
-    float m[8], v[8];
-    unsigned most_m = 0, most_v = 0;
+// A lane's eight values of a block, and their codes, a byte each in four words.  VECTORS: four at 4 lane and four at 128 + 4 lane, where parameters and gradients
+// begin at 16 bytes; else at lane + 32 j, a value or a byte a load, which is as many bytes of memory.
+template <bool VECTORS>
+struct Lane {
+  int lane;
+  __device__ __forceinline__ int at(int j) const { return VECTORS ? 128 * (j / 4) + 4 * lane + j % 4 : lane + 32 * j; }
+  __device__ __forceinline__ void values(const float* from, int n, float (&x)[8]) const {
+    if (VECTORS && n == kBlock) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const unsigned cm = *(const unsigned*)(codes + 128 * u + 4 * lane), cv = *(const unsigned*)(codes + kBlock + 128 * u + 4 * lane);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = 128 * u + 4 * lane + j;
-        float &mm = m[4 * u + j], &vv = v[4 * u + j];
-        mm = vv = 0.f;
-        if (i < n) {
-          const float gg = g[i] * h.grad_scale, root = h.c2 * gg;
-          mm = __fmaf_rn(h.c1, gg, __fmul_rn(h.b1, decode_first(cm >> 8 * j & 0xFFu, unit_m)));
-          vv = __fmaf_rn(root, root, __fmul_rn(h.b2, decode_second(cv >> 8 * j & 0xFFu, unit_v)));
-          update(p[i], mm, vv, h, c);
-        }
-        most_m = max(most_m, __float_as_uint(mm) & 0x7FFFFFFFu);
-        most_v = max(most_v, __float_as_uint(vv) & 0x7FFFFFFFu);
+      for (int u = 0; u < 2; ++u) {
+        const float4 f = __ldcs((const float4*)(from + 128 * u) + lane);
+        x[4 * u] = f.x; x[4 * u + 1] = f.y; x[4 * u + 2] = f.z; x[4 * u + 3] = f.w;
       }
-    }
-    const unsigned scale_m = scale_of(__reduce_max_sync(0xFFFFFFFFu, most_m)), scale_v = scale_of(__reduce_max_sync(0xFFFFFFFFu, most_v));
-    const float per_m = per_unit(scale_m), per_v = per_unit(scale_v);
+    } else {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      unsigned cm = 0, cv = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned r = mix(key + ((unsigned)e + 128 * u + 4 * lane + j) * kGolden);
-        cm |= encode_first(m[4 * u + j], per_m, r >> 16) << 8 * j;
-        cv |= encode_second(v[4 * u + j], per_v, r & 0xFFFFu) << 8 * j;
-      }
-      *(unsigned*)(codes + 128 * u + 4 * lane) = scale_m == 255 ? 0u : cm;
-      *(unsigned*)(codes + kBlock + 128 * u + 4 * lane) = scale_v == 255 ? 0u : cv;
+      for (int j = 0; j < 8; ++j) x[j] = at(j) < n ? __ldcs(from + at(j)) : 0.f;
     }
-    if (lane == 0) *(unsigned short*)scales = (unsigned short)(scale_m | scale_v << 8);
   }
+  __device__ __forceinline__ void put(float* to, int n, const float (&x)[8]) const {
+    if (VECTORS && n == kBlock) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) __stcs((float4*)(to + 128 * u) + lane, make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (at(j) < n) __stcs(to + at(j), x[j]);
+    }
+  }
+  __device__ __forceinline__ void codes(const unsigned char* from, unsigned (&c)[8]) const {
+    if (VECTORS) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const unsigned w = __ldcs((const unsigned*)(from + 128 * u) + lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[4 * u + j] = w >> 8 * j & 0xFFu;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = __ldcs(from + at(j));
+    }
+  }
+  __device__ __forceinline__ void put_codes(unsigned char* to, const unsigned (&c)[8]) const {
+    if (VECTORS) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) __stcs((unsigned*)(to + 128 * u) + lane, c[4 * u] | c[4 * u + 1] << 8 | c[4 * u + 2] << 16 | c[4 * u + 3] << 24);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) __stcs(to + at(j), (unsigned char)c[j]);
+    }
+  }
+};
+
+// A block by a warp.
+template <bool VECTORS>
+__device__ __forceinline__ void update_block(const Lane<VECTORS> l, float* p, const float* g, int n, unsigned char* codes, unsigned char* scales, unsigned first, unsigned key,
+                                             const Hyper& h, const Corrections* corrections) {
+  float pp[8], gg[8];
+  unsigned cm[8], cv[8];
+  l.values(g, n, gg);
+  l.values(p, n, pp);
+  l.codes(codes, cm);
+  l.codes(codes + kBlock, cv);
+  const unsigned scale = *(const unsigned short*)scales;
+  const Corrections c = *corrections;
+  key = mix(key + c.t);
+  const float unit_m = unit_of(scale & 0xFFu), unit_v = unit_of(scale >> 8);
+  float m[8], v[8];
+  unsigned most_m = 0, most_v = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = gg[j] * c.grad_scale, root = h.c2 * x;
+    m[j] = __fmaf_rn(h.c1, x, __fmul_rn(h.b1, decode_first(cm[j], unit_m)));
+    v[j] = __fmaf_rn(root, root, __fmul_rn(h.b2, decode_second(cv[j], unit_v)));
+    if (n < kBlock && l.at(j) >= n) m[j] = v[j] = 0.f;
+    update(pp[j], m[j], v[j], h, c);
+    most_m = max(most_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+    most_v = max(most_v, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+  }
+  l.put(p, n, pp);
+  const unsigned scale_m = scale_of(__reduce_max_sync(0xFFFFFFFFu, most_m)), scale_v = scale_of(__reduce_max_sync(0xFFFFFFFFu, most_v));
+  const float per_m = per_unit(scale_m), per_v = per_unit(scale_v);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned r = mix(key + (first + l.at(j)) * kGolden);
+    cm[j] = scale_m == 255 ? 0u : encode_first(m[j], per_m, r >> 16);
+    cv[j] = scale_v == 255 ? 0u : encode_second(v[j], per_v, r & 0xFFFFu);
+  }
+  l.put_codes(codes, cm);
+  l.put_codes(codes + kBlock, cv);
+  if (l.lane == 0) *(unsigned short*)scales = (unsigned short)(scale_m | scale_v << 8);
 }
 
-struct MomentsTable {
-  const unsigned char *codes[kTensors], *scales[kTensors];
-  float *m[kTensors], *v[kTensors];
-  long long n[kTensors];
-  int chunk_start[kTensors + 1];
-  int count;
-};
-__global__ void __launch_bounds__(kThreads) adamw8_moments_kernel(const __grid_constant__ MomentsTable t) {
+template <int N>
+__global__ void __launch_bounds__(kThreads) adamw8_kernel(const __grid_constant__ Table<unsigned char, N> t, Hyper h, const Corrections* __restrict__ corrections) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.chunk_start[mid] <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
+  const int chunk = t.chunk_start[t.count] - 1 - (int)blockIdx.x, k = tensor_of(t, chunk), lane = threadIdx.x & 31;
+  const long long block = (long long)(chunk - t.chunk_start[k]) * (kChunk / kBlock) + (threadIdx.x >> 5), e = block * kBlock, left = t.n[k] - e;
+  if (left <= 0) return;
+  const int n = left < kBlock ? (int)left : kBlock;
+  float* p = t.p[k] + e;
+  const float* g = t.g[k] + e;
+  unsigned char *codes = t.m[k] + block * 2 * kBlock, *scales = t.v[k] + block * 2;
+  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & 15u) == 0)
+    update_block(Lane<true>{lane}, p, g, n, codes, scales, (unsigned)e, t.key[k], h, corrections + t.slot[k]);
+  else
+    update_block(Lane<false>{lane}, p, g, n, codes, scales, (unsigned)e, t.key[k], h, corrections + t.slot[k]);
+}
+
+template <int N>
+struct MomentsTable {
+  const unsigned char *codes[N], *scales[N];
+  float *m[N], *v[N];
+  long long n[N];
+  int chunk_start[N + 1];
+  int count;
+};
+template <bool VECTORS>
+__device__ __forceinline__ void write_block(const Lane<VECTORS> l, const unsigned char* codes, const unsigned char* scales, float* m, float* v, int n) {
+  unsigned cm[8], cv[8];
+  l.codes(codes, cm);
+  l.codes(codes + kBlock, cv);
+  const unsigned scale = *(const unsigned short*)scales;
+  const float unit_m = unit_of(scale & 0xFFu), unit_v = unit_of(scale >> 8);
+  float x[8], y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] = decode_first(cm[j], unit_m);
+    y[j] = decode_second(cv[j], unit_v);
   }
-  const int k = lo;
-  const long long e = (long long)((int)blockIdx.x - t.chunk_start[k]) * kChunk8;
-  for (long long i = e + threadIdx.x; i < e + kChunk8 && i < t.n[k]; i += kThreads) {
-    const long long block = i / kBlock;
-    const unsigned char *codes = t.codes[k] + block * 2 * kBlock + i % kBlock, *scales = t.scales[k] + 2 * block;
-    t.m[k][i] = decode_first(codes[0], unit_of(scales[0]));
-    t.v[k][i] = decode_second(codes[kBlock], unit_of(scales[1]));
-  }
+  l.put(m, n, x);
+  l.put(v, n, y);
+}
+template <int N>
+__global__ void __launch_bounds__(kThreads) adamw8_moments_kernel(const __grid_constant__ MomentsTable<N> t) {
+  mtb_launch_dependents();
+  mtb_wait_prior();
+  const int k = tensor_of(t, blockIdx.x), lane = threadIdx.x & 31;
+  const long long block = (long long)((int)blockIdx.x - t.chunk_start[k]) * (kChunk / kBlock) + (threadIdx.x >> 5), e = block * kBlock, left = t.n[k] - e;
+  if (left <= 0) return;
+  const int n = left < kBlock ? (int)left : kBlock;
+  float *m = t.m[k] + e, *v = t.v[k] + e;
+  const unsigned char *codes = t.codes[k] + block * 2 * kBlock, *scales = t.scales[k] + block * 2;
+  if (((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0) write_block(Lane<true>{lane}, codes, scales, m, v, n);
+  else write_block(Lane<false>{lane}, codes, scales, m, v, n);
 }
 
 // What `params` says of a tensor.
@@ -212,7 +337,7 @@ Tensor tensor_at(void* const* params, int k) {
 }
 
 // Counts the steps of the call's tensors, each counter once, and leaves which of the corrections a tensor takes.
-int begin(int count, void* const* params, double lr, double b1, double b2, Corrections* out, std::vector<unsigned short>& slots, cudaStream_t st) {
+int begin(int count, void* const* params, double lr, double b1, double b2, double grad_scale, MtbClip clip, Corrections* out, std::vector<unsigned short>& slots, cudaStream_t st) {
   std::vector<long long*> distinct;
   slots.resize(count);
   for (int k = 0; k < count; ++k) {
@@ -228,7 +353,8 @@ int begin(int count, void* const* params, double lr, double b1, double b2, Corre
     StepTable t;
     t.count = (int)(distinct.size() - base < kSteps ? distinct.size() - base : kSteps);
     for (int i = 0; i < t.count; ++i) t.step[i] = distinct[base + i];
-    MTB_LAUNCH(adamw_begin_kernel, 1, 256, 0, st, t, lr, b1, b2, out + base);
+    MTB_LAUNCH(adamw_begin_kernel, 1, 256, 0, st, t, lr, b1, b2, (float)grad_scale, clip, out + base);
+    clip.norm = nullptr;  // left by the first launch
   }
   return MTB_OK;
 }
@@ -239,13 +365,15 @@ bool fine(double lr, double b1, double b2, double eps, double weight_decay) {
   return lr >= 0 && b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1 && eps >= 0 && weight_decay >= 0;
 }
 
+constexpr int kFew = 24, kMany = 192;
+
 // stride: numbers in `sizes` a tensor.
-template <class M, class K>
-int run(const char* name, K kernel, int count, void* const* params, const long long* sizes, int stride, const std::vector<unsigned short>& slots, int chunk, const Hyper& h,
-        const Corrections* corrections, MtbClip clip, cudaStream_t st) {
-  for (int base = (count - 1) / kTensors * kTensors; base >= 0; base -= kTensors) {  // backwards: what the norm read last is still in L2
-    Table<M> t;
-    t.count = count - base < kTensors ? count - base : kTensors;
+template <class M, int N, class K>
+int run(const char* name, K kernel, int count, void* const* params, const long long* sizes, int stride, const std::vector<unsigned short>& slots, const Hyper& h,
+        const Corrections* corrections, cudaStream_t st) {
+  for (int base = (count - 1) / N * N; count > 0 && base >= 0; base -= N) {
+    Table<M, N> t;
+    t.count = count - base < N ? count - base : N;
     long long chunks = 0;
     for (int k = 0; k < t.count; ++k) {
       const Tensor a = tensor_at(params, base + k);
@@ -258,17 +386,21 @@ int run(const char* name, K kernel, int count, void* const* params, const long l
       t.slot[k] = slots[base + k];
       t.key[k] = stride > 1 ? mix((unsigned)size[1]) : 0;
       t.chunk_start[k] = (int)chunks;
-      chunks += (t.n[k] + chunk - 1) / chunk;
-      MTB_REQUIRE(chunks < (1LL << 30), "%s: too many elements in one call", name);
+      chunks += (t.n[k] + kChunk - 1) / kChunk;
     }
     t.chunk_start[t.count] = (int)chunks;
-    if (chunks == 0 && clip.norm) chunks = 1;  // for the norm
     if (chunks == 0) continue;
-    MTB_LAUNCH(kernel, dim3((unsigned)chunks), kThreads, 0, st, t, h, corrections, clip);
+    MTB_LAUNCH(kernel, dim3((unsigned)chunks), kThreads, 0, st, t, h, corrections);
     MTB_LAUNCH_CHECK(name);
-    clip.norm = nullptr;  // left by the first launch
   }
   return MTB_OK;
+}
+
+// Before anything is counted: no launch of the call has too many chunks.
+bool fits(int count, const long long* sizes, int stride) {
+  long long chunks = 0;
+  for (int k = 0; k < count; ++k) chunks += sizes[(long long)stride * k] / kChunk + 1;
+  return chunks < 1LL << 30;
 }
 
 }  // namespace
@@ -285,10 +417,13 @@ MTB_API int mtb_adamw_f32(int count, void* const* params, const long long* sizes
     MTB_REQUIRE(a.step && sizes[k] >= 0 && (sizes[k] == 0 || (a.p && a.g && a.m && a.v)), "adamw: null tensor %d", k);
   }
   std::vector<unsigned short> slots;
-  if (int rc = begin(count, params, lr, beta1, beta2, (Corrections*)scratch, slots, (cudaStream_t)stream)) return rc;
-  const Hyper h{(float)lr, (float)beta1, (float)beta2, (float)(1 - beta1), (float)(1 - beta2), (float)eps, (float)(1 - lr * weight_decay), (float)grad_scale};
-  return run<float>("adamw_kernel", adamw_kernel, count, params, sizes, 1, slots, kChunk, h, (const Corrections*)scratch, MtbClip{sums, nsums, grad_scale, max_norm, norm},
-                    (cudaStream_t)stream);
+  MTB_REQUIRE(fits(count, sizes, 1), "adamw: too many elements in one call");
+  cudaStream_t st = (cudaStream_t)stream;
+  Corrections* corrections = (Corrections*)scratch;
+  if (int rc = begin(count, params, lr, beta1, beta2, grad_scale, MtbClip{sums, nsums, grad_scale, max_norm, norm}, corrections, slots, st)) return rc;
+  const Hyper h{(float)beta1, (float)beta2, (float)(1 - beta1), (float)(1 - beta2), (float)eps, (float)(1 - lr * weight_decay)};
+  return count <= kFew ? run<float, kFew>("adamw_kernel", adamw_kernel<kFew>, count, params, sizes, 1, slots, h, corrections, st)
+                       : run<float, kMany>("adamw_kernel", adamw_kernel<kMany>, count, params, sizes, 1, slots, h, corrections, st);
 }
 
 MTB_API int mtb_adamw8_f32(int count, void* const* params, const long long* sizes, double lr, double beta1, double beta2, double eps, double weight_decay, double grad_scale,
@@ -303,36 +438,46 @@ MTB_API int mtb_adamw8_f32(int count, void* const* params, const long long* size
     MTB_REQUIRE(moments_aligned(a.m, a.v), "adamw8: moments of tensor %d begin off 16 bytes, or scales off 2", k);
   }
   std::vector<unsigned short> slots;
-  if (int rc = begin(count, params, lr, b1, b2, (Corrections*)scratch, slots, (cudaStream_t)stream)) return rc;
-  const Hyper h{(float)lr, (float)b1, (float)b2, (float)(1 - b1), (float)std::sqrt(1 - b2), (float)eps, (float)(1 - lr * weight_decay), (float)grad_scale};
-  return run<unsigned char>("adamw8_kernel", adamw8_kernel, count, params, sizes, 2, slots, kChunk8, h, (const Corrections*)scratch,
-                            MtbClip{sums, nsums, grad_scale, max_norm, norm}, (cudaStream_t)stream);
+  MTB_REQUIRE(fits(count, sizes, 2), "adamw8: too many elements in one call");
+  cudaStream_t st = (cudaStream_t)stream;
+  Corrections* corrections = (Corrections*)scratch;
+  if (int rc = begin(count, params, lr, b1, b2, grad_scale, MtbClip{sums, nsums, grad_scale, max_norm, norm}, corrections, slots, st)) return rc;
+  const Hyper h{(float)b1, (float)b2, (float)(1 - b1), (float)std::sqrt(1 - b2), (float)eps, (float)(1 - lr * weight_decay)};
+  return count <= kFew ? run<unsigned char, kFew>("adamw8_kernel", adamw8_kernel<kFew>, count, params, sizes, 2, slots, h, corrections, st)
+                       : run<unsigned char, kMany>("adamw8_kernel", adamw8_kernel<kMany>, count, params, sizes, 2, slots, h, corrections, st);
 }
 
-MTB_API int mtb_adamw8_moments_f32(int count, void* const* params, const long long* sizes, void* stream) {
-  MTB_REQUIRE(count >= 0 && (count == 0 || (params && sizes)), "adamw8_moments: bad arguments");
-  for (int base = 0; base < count; base += kTensors) {
-    MomentsTable t;
-    t.count = count - base < kTensors ? count - base : kTensors;
+template <int N>
+static int moments_of(int count, void* const* params, const long long* sizes, cudaStream_t st) {
+  for (int base = 0; base < count; base += N) {
+    MomentsTable<N> t;
+    t.count = count - base < N ? count - base : N;
     long long chunks = 0;
     for (int k = 0; k < t.count; ++k) {
       void* const* a = params + 4 * (long long)(base + k);
-      const long long size = sizes[base + k];
-      MTB_REQUIRE(size >= 0 && (size == 0 || (a[0] && a[1] && a[2] && a[3])), "adamw8_moments: null tensor %d", base + k);
-      MTB_REQUIRE(moments_aligned(a[0], a[1]), "adamw8_moments: moments of tensor %d begin off 16 bytes, or scales off 2", base + k);
       t.codes[k] = (const unsigned char*)a[0];
       t.scales[k] = (const unsigned char*)a[1];
       t.m[k] = (float*)a[2];
       t.v[k] = (float*)a[3];
-      t.n[k] = size;
+      t.n[k] = sizes[base + k];
       t.chunk_start[k] = (int)chunks;
-      chunks += (size + kChunk8 - 1) / kChunk8;
-      MTB_REQUIRE(chunks < (1LL << 30), "adamw8_moments: too many elements in one call");
+      chunks += (t.n[k] + kChunk - 1) / kChunk;
     }
     t.chunk_start[t.count] = (int)chunks;
     if (chunks == 0) continue;
-    MTB_LAUNCH(adamw8_moments_kernel, dim3((unsigned)chunks), kThreads, 0, (cudaStream_t)stream, t);
+    MTB_LAUNCH(adamw8_moments_kernel<N>, dim3((unsigned)chunks), kThreads, 0, st, t);
     MTB_LAUNCH_CHECK("adamw8_moments_kernel");
   }
   return MTB_OK;
+}
+
+MTB_API int mtb_adamw8_moments_f32(int count, void* const* params, const long long* sizes, void* stream) {
+  MTB_REQUIRE(count >= 0 && (count == 0 || (params && sizes)), "adamw8_moments: bad arguments");
+  for (int k = 0; k < count; ++k) {
+    void* const* a = params + 4 * (long long)k;
+    MTB_REQUIRE(sizes[k] >= 0 && (sizes[k] == 0 || (a[0] && a[1] && a[2] && a[3])), "adamw8_moments: null tensor %d", k);
+    MTB_REQUIRE(moments_aligned(a[0], a[1]), "adamw8_moments: moments of tensor %d begin off 16 bytes, or scales off 2", k);
+  }
+  MTB_REQUIRE(fits(count, sizes, 1), "adamw8_moments: too many elements in one call");
+  return count <= kFew ? moments_of<kFew>(count, params, sizes, (cudaStream_t)stream) : moments_of<kMany>(count, params, sizes, (cudaStream_t)stream);
 }

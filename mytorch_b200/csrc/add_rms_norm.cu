@@ -6,7 +6,8 @@
 //   dweight = sum of dy x_hat,  dpost_weight = sum of dinner b_hat  over rows; dgate is summed over the rows that share a row of the gate.
 //
 // Bound by memory: 16 bytes a value forward, 24 backward, each once, if a row stays in registers between its sums and what is made of them.  So a group of W warps holds
-// a row, PER vectors a thread and tensor, and goes on to its next one; W is 1 where a row fits a warp, which then waits for no other.
+// a row, PER vectors a thread and tensor, and goes on to its next one; W is 1 where a row fits a warp, which then waits for no other, and narrow rows lie side by side in
+// a warp, LANES lanes each.
 #include <utility>
 
 #include "colreduce.cuh"
@@ -21,16 +22,18 @@ struct Operands {
   float scale, eps;
 };
 
-// Sums over the W warps that share a row, in all their threads.  Two buffers taken in turn: a third sum writes where the first was read before the second.
-template <int W>
+// Sums over the threads that share a row, W warps or LANES lanes of one, in all of them.  Two buffers taken in turn: a third sum writes where the first was read before
+// the second.
+template <int W, int LANES = 32>
 struct GroupSum {
-  static constexpr int kThreads = W == 1 ? 256 : 32 * W, kGroups = W == 1 ? 8 : 1;
+  static constexpr int kThreads = W == 1 ? 256 : 32 * W;
+  static constexpr int kGroups = W == 1 ? 256 / LANES : 1, kShare = W == 1 ? LANES : 32 * W;
   float (*part)[W];
   int turn = 0;
 
   __device__ __forceinline__ float operator()(float x) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     if (W == 1) return x;
     if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = x;
     __syncthreads();
@@ -43,6 +46,29 @@ struct GroupSum {
 };
 
 template <int V>
+__device__ __forceinline__ VecF<V> load(const float* p) {
+  if constexpr (V == 2) {
+    const float2 t = *reinterpret_cast<const float2*>(p);
+    return VecF<V>{{t.x, t.y}};
+  } else {
+    return vload<V>(p);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store(float* p, const VecF<V>& r) {
+  if constexpr (V == 2) *reinterpret_cast<float2*>(p) = make_float2(r.v[0], r.v[1]);
+  else vstore<V>(p, r);
+}
+// A thread's own values come to shared memory while it works on those before them: nobody else reads them there, so nothing waits but the thread for its copies.
+template <int V>
+__device__ __forceinline__ void fetch(float* to, const float* from) {
+  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+  if constexpr (V == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(4 * V) : "memory");
+}
+__device__ __forceinline__ void fetched() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+template <int V>
 __device__ __forceinline__ VecF<V> filled(float x) {
   VecF<V> r;
 #pragma unroll
@@ -50,25 +76,32 @@ __device__ __forceinline__ VecF<V> filled(float x) {
   return r;
 }
 
-template <int V, int PER, int W>
-__global__ void __launch_bounds__(GroupSum<W>::kThreads) add_rms_norm_kernel(const __grid_constant__ Operands a, float* __restrict__ out, float* __restrict__ y, float* __restrict__ rstd,
+template <int V, int PER, int W, int LANES>
+__global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads) add_rms_norm_kernel(const __grid_constant__ Operands a, float* __restrict__ out, float* __restrict__ y, float* __restrict__ rstd,
                                                                              float* __restrict__ block_rstd) {
   __shared__ float part[2][W];
-  GroupSum<W> sum{part};
+  GroupSum<W, LANES> sum{part};
+  constexpr int kShare = GroupSum<W, LANES>::kShare, kGroups = GroupSum<W, LANES>::kGroups;
   mtb_launch_dependents();
   mtb_wait_prior();
-  const int id = W == 1 ? threadIdx.x & 31 : threadIdx.x;
-  const long long groups = (long long)gridDim.x * GroupSum<W>::kGroups;
-  for (long long row = W == 1 ? blockIdx.x * 8LL + (threadIdx.x >> 5) : blockIdx.x; row < a.rows; row += groups) {
+  const int id = threadIdx.x % kShare, beside = W == 1 ? (threadIdx.x & 31) / LANES : 0;
+  const long long groups = (long long)gridDim.x * kGroups;
+  // all lanes of a warp go on as long as one of them has a row
+  for (long long first = blockIdx.x * (long long)kGroups + (W == 1 ? threadIdx.x / 32 * (32 / LANES) : 0); first < a.rows; first += groups) {
+    const long long row = LANES == 32 || first + beside < a.rows ? first + beside : first;
+    const int c = LANES == 32 || first + beside < a.rows ? a.c : 0;
     const long long at = row * a.c;
-    VecF<V> x[PER], b[PER];
+    const float* gate = a.gate ? a.gate + (long long)((unsigned)row / (unsigned)a.rows_per_gate) * a.c : nullptr;
+    VecF<V> x[PER], b[PER], g[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = (id + k * 32 * W) * V;
+      const int i = (id + k * kShare) * V;
       x[k] = b[k] = filled<V>(0);
-      if (i < a.c) {
-        x[k] = vload<V>(a.x + at + i);
-        if (a.block) b[k] = vload<V>(a.block + at + i);
+      g[k] = filled<V>(1);
+      if (i < c) {
+        if (a.block) b[k] = load<V>(a.block + at + i);
+        x[k] = load<V>(a.x + at + i);
+        if (gate) g[k] = load<V>(gate + i);
       }
     }
     if (a.block) {
@@ -80,17 +113,16 @@ __global__ void __launch_bounds__(GroupSum<W>::kThreads) add_rms_norm_kernel(con
 #pragma unroll
           for (int j = 0; j < V; ++j) s = fmaf(b[k].v[j], b[k].v[j], s);
         rb = 1.f / sqrtf(sum(s) / a.c + a.eps);
-        if (block_rstd && id == 0) block_rstd[row] = rb;
+        if (block_rstd && id == 0 && c) block_rstd[row] = rb;
       }
-      const float* gate = a.gate ? a.gate + (long long)((unsigned)row / (unsigned)a.rows_per_gate) * a.c : nullptr;
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * 32 * W) * V;
-        if (i < a.c) {
-          const VecF<V> w = a.post_weight ? vload<V>(a.post_weight + i) : filled<V>(1), g = gate ? vload<V>(gate + i) : filled<V>(1);
+        const int i = (id + k * kShare) * V;
+        if (i < c) {
+          const VecF<V> w = a.post_weight ? load<V>(a.post_weight + i) : filled<V>(1);
 #pragma unroll
-          for (int j = 0; j < V; ++j) x[k].v[j] = fmaf(a.scale, x[k].v[j], b[k].v[j] * rb * w.v[j] * g.v[j]);
-          vstore<V>(out + at + i, x[k]);
+          for (int j = 0; j < V; ++j) x[k].v[j] = fmaf(a.scale, x[k].v[j], b[k].v[j] * rb * w.v[j] * g[k].v[j]);
+          store<V>(out + at + i, x[k]);
         }
       }
     }
@@ -100,16 +132,16 @@ __global__ void __launch_bounds__(GroupSum<W>::kThreads) add_rms_norm_kernel(con
 #pragma unroll
       for (int j = 0; j < V; ++j) s = fmaf(x[k].v[j], x[k].v[j], s);
     const float rho = 1.f / sqrtf(sum(s) / a.c + a.eps);
-    if (rstd && id == 0) rstd[row] = rho;
+    if (rstd && id == 0 && c) rstd[row] = rho;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = (id + k * 32 * W) * V;
-      if (i < a.c) {
-        const VecF<V> w = a.weight ? vload<V>(a.weight + i) : filled<V>(1);
+      const int i = (id + k * kShare) * V;
+      if (i < c) {
+        const VecF<V> w = a.weight ? load<V>(a.weight + i) : filled<V>(1);
         VecF<V> r;
 #pragma unroll
         for (int j = 0; j < V; ++j) r.v[j] = x[k].v[j] * rho * w.v[j];
-        vstore<V>(y + at + i, r);
+        store<V>(y + at + i, r);
       }
     }
   }
@@ -126,45 +158,75 @@ struct Gradients {
   long long stretches, parts, stretch, rows_of_gate;
 };
 
-template <int V, int PER, int W>
-__global__ void __launch_bounds__(GroupSum<W>::kThreads) add_rms_norm_backward_kernel(const __grid_constant__ Operands a, const __grid_constant__ Gradients d) {
-  constexpr int kGroups = GroupSum<W>::kGroups;
-  extern __shared__ float joined[];  // W 1: [3][c]
+// AHEAD: the next row's values come to shared memory meanwhile.  That pays where many warps wait for one another at a row's sums (16384 x 2048 with post norm and gate 153 -> 136 us,
+// 8192 x 4096 167 -> 142), not where rows of other groups are under way on the SM (32768 x 1024 135 -> 146), nor by copies of 4 bytes (32768 x 1023 158 -> 215).
+template <int V, int PER, int W, int LANES, bool AHEAD>
+__global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads) add_rms_norm_backward_kernel(const __grid_constant__ Operands a, const __grid_constant__ Gradients d) {
+  constexpr int kGroups = GroupSum<W, LANES>::kGroups, kShare = GroupSum<W, LANES>::kShare;
+  extern __shared__ __align__(16) float shared[];  // AHEAD: [x, dy, dnew, block][PER][thread][V]; W 1: [3][c]
   __shared__ float part[2][W];
-  GroupSum<W> sum{part};
+  GroupSum<W, LANES> sum{part};
   mtb_launch_dependents();
   mtb_wait_prior();
-  const int id = W == 1 ? threadIdx.x & 31 : threadIdx.x, c = a.c;
+  const int id = threadIdx.x % kShare, beside = W == 1 ? (threadIdx.x & 31) / LANES : 0;
   const long long groups = (long long)gridDim.x * kGroups;
-  const float per_c = 1.f / c;
+  const float per_c = 1.f / a.c;
   VecF<V> dw[PER], dpw[PER], dg[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) dw[k] = dpw[k] = dg[k] = filled<V>(0);
-  for (long long stretch = W == 1 ? blockIdx.x * 8LL + (threadIdx.x >> 5) : blockIdx.x; stretch < d.stretches; stretch += groups) {
-    const long long of_gate = stretch / d.parts, first = of_gate * d.rows_of_gate + (stretch - of_gate * d.parts) * d.stretch;
-    const long long limit = (of_gate + 1) * d.rows_of_gate, last = first + d.stretch < limit ? first + d.stretch : limit;
-    for (long long row = first; row < last; ++row) {
-      const long long at = row * c;
+  // where a row's values of this thread lie
+  const auto slot = [&](int tensor, int j) { return shared + ((tensor * PER + j) * GroupSum<W>::kThreads + (int)threadIdx.x) * V; };
+  const auto fetch_row = [&](long long row) {
+    const long long at = row * a.c;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = (id + j * kShare) * V;
+      if (i < a.c) {
+        fetch<V>(slot(0, j), a.x + at + i);
+        if (d.dy) fetch<V>(slot(1, j), d.dy + at + i);
+        if (d.dnew) fetch<V>(slot(2, j), d.dnew + at + i);
+        if (a.block) fetch<V>(slot(3, j), a.block + at + i);
+      }
+    }
+  };
+  const auto first_of = [&](long long stretch) { const long long g = stretch / d.parts; return g * d.rows_of_gate + (stretch - g * d.parts) * d.stretch; };
+  long long begin = blockIdx.x * (long long)kGroups + (W == 1 ? threadIdx.x / 32 * (32 / LANES) : 0);
+  if (AHEAD && begin < d.stretches) fetch_row(first_of(begin));
+  for (; begin < d.stretches; begin += groups) {
+    const long long stretch = LANES == 32 || begin + beside < d.stretches ? begin + beside : begin;
+    const bool there = LANES == 32 || begin + beside < d.stretches;
+    const long long first = first_of(stretch), limit = (stretch / d.parts + 1) * d.rows_of_gate, last = first + d.stretch < limit ? first + d.stretch : limit;
+    for (long long next = first; next < (LANES == 32 ? last : first + d.stretch); ++next) {
+      // all lanes of a warp go on as long as one of them has a row
+      const bool on = LANES == 32 || (there && next < last);
+      const long long row = on ? next : first, at = row * a.c;
+      const int c = on ? a.c : 0;
       const float rho = d.rstd[row], rb = d.block_rstd ? d.block_rstd[row] : 1.f;
-      const float* gate = a.gate ? a.gate + (long long)((unsigned)row / (unsigned)a.rows_per_gate) * c : nullptr;
-      VecF<V> x[PER], dy[PER], D[PER], b[PER];
+      const float* gate = a.gate ? a.gate + (long long)((unsigned)row / (unsigned)a.rows_per_gate) * a.c : nullptr;
+      VecF<V> x[PER], dy[PER], D[PER], b[PER], g[PER];
+      if (AHEAD) fetched();
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * 32 * W) * V;
+        const int i = (id + k * kShare) * V;
         x[k] = dy[k] = D[k] = b[k] = filled<V>(0);
+        g[k] = filled<V>(1);
         if (i < c) {
-          x[k] = vload<V>(a.x + at + i);
-          if (d.dy) dy[k] = vload<V>(d.dy + at + i);
-          if (d.dnew) D[k] = vload<V>(d.dnew + at + i);
-          if (a.block) b[k] = vload<V>(a.block + at + i);
+          const auto value = [&](int tensor, const float* from) { return AHEAD ? load<V>(slot(tensor, k)) : load<V>(from + at + i); };
+          if (d.dnew) D[k] = value(2, d.dnew);
+          if (a.block) b[k] = value(3, a.block);
+          x[k] = value(0, a.x);
+          if (d.dy) dy[k] = value(1, d.dy);
+          if (gate) g[k] = load<V>(gate + i);
         }
       }
+      const long long then = !AHEAD ? -1 : row + 1 < last ? row + 1 : begin + groups < d.stretches ? first_of(begin + groups) : -1;
+      if (!d.dy && then >= 0) fetch_row(then);
       if (d.dy) {
         float s = 0;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const int i = (id + k * 32 * W) * V;
-          const VecF<V> w = a.weight && i < c ? vload<V>(a.weight + i) : filled<V>(1);
+          const int i = (id + k * kShare) * V;
+          const VecF<V> w = a.weight && i < c ? load<V>(a.weight + i) : filled<V>(1);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             x[k].v[j] *= rho;
@@ -174,6 +236,7 @@ __global__ void __launch_bounds__(GroupSum<W>::kThreads) add_rms_norm_backward_k
           }
         }
         const float mean = sum(s) * per_c;
+        if (then >= 0) fetch_row(then);  // all values have been read
 #pragma unroll
         for (int k = 0; k < PER; ++k)
 #pragma unroll
@@ -182,12 +245,12 @@ __global__ void __launch_bounds__(GroupSum<W>::kThreads) add_rms_norm_backward_k
       if (d.dresidual) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const int i = (id + k * 32 * W) * V;
+          const int i = (id + k * kShare) * V;
           if (i < c) {
             VecF<V> r;
 #pragma unroll
             for (int j = 0; j < V; ++j) r.v[j] = a.scale * D[k].v[j];
-            vstore<V>(d.dresidual + at + i, r);
+            store<V>(d.dresidual + at + i, r);
           }
         }
       }
@@ -195,53 +258,55 @@ __global__ void __launch_bounds__(GroupSum<W>::kThreads) add_rms_norm_backward_k
       float s = 0;
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * 32 * W) * V;
-        const VecF<V> w = a.post_weight && i < c ? vload<V>(a.post_weight + i) : filled<V>(1), g = gate && i < c ? vload<V>(gate + i) : filled<V>(1);
+        const int i = (id + k * kShare) * V;
+        const VecF<V> w = a.post_weight && i < c ? load<V>(a.post_weight + i) : filled<V>(1);
         VecF<V> each;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           b[k].v[j] *= rb;
           each.v[j] = D[k].v[j] * b[k].v[j] * w.v[j];
           dg[k].v[j] += each.v[j];
-          D[k].v[j] *= g.v[j];
+          D[k].v[j] *= g[k].v[j];
           dpw[k].v[j] = fmaf(D[k].v[j], b[k].v[j], dpw[k].v[j]);
           D[k].v[j] *= w.v[j];
           s = fmaf(D[k].v[j], b[k].v[j], s);
         }
-        if (d.gate_each && d.gate_rows && i < c) vstore<V>(d.gate_rows + at + i, each);
+        if (d.gate_each && d.gate_rows && i < c) store<V>(d.gate_rows + at + i, each);
       }
       if (!d.dblock) continue;
       const float mean = a.post_weight ? sum(s) * per_c : 0.f;
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * 32 * W) * V;
+        const int i = (id + k * kShare) * V;
         if (i < c) {
           VecF<V> r;
 #pragma unroll
           for (int j = 0; j < V; ++j) r.v[j] = rb * (D[k].v[j] - b[k].v[j] * mean);
-          vstore<V>(d.dblock + at + i, r);
+          store<V>(d.dblock + at + i, r);
         }
       }
     }
     if (d.gate_rows && !d.gate_each) {
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * 32 * W) * V;
-        if (i < c) vstore<V>(d.gate_rows + stretch * c + i, dg[k]);
+        const int i = (id + k * kShare) * V;
+        if (i < a.c && there) store<V>(d.gate_rows + stretch * a.c + i, dg[k]);
         dg[k] = filled<V>(0);
       }
     }
   }
   if (!d.partial) return;
+  const int c = a.c;
   float* mine = d.partial + (long long)blockIdx.x * 3 * c;
-  if (W == 1) {  // the CTA's eight warps one after the other: the same order every time
+  if (W == 1) {  // the CTA's groups one after the other: the same order every time
+    float* joined = shared;
     for (int w = 0; w < kGroups; ++w) {
-      if ((int)(threadIdx.x >> 5) == w) {
+      if ((int)threadIdx.x / LANES == w) {
 #pragma unroll
         for (int k = 0; k < PER; ++k)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const int i = (id + k * 32) * V + j;
+            const int i = (id + k * kShare) * V + j;
             if (i < c) {
               joined[i] = w ? joined[i] + dw[k].v[j] : dw[k].v[j];
               joined[c + i] = w ? joined[c + i] + dpw[k].v[j] : dpw[k].v[j];
@@ -255,44 +320,56 @@ __global__ void __launch_bounds__(GroupSum<W>::kThreads) add_rms_norm_backward_k
   } else {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = (id + k * 32 * W) * V;
+      const int i = (id + k * kShare) * V;
       if (i < c) {
-        vstore<V>(mine + i, dw[k]);
-        vstore<V>(mine + c + i, dpw[k]);
-        vstore<V>(mine + 2 * c + i, dg[k]);
+        store<V>(mine + i, dw[k]);
+        store<V>(mine + c + i, dpw[k]);
+        store<V>(mine + 2 * c + i, dg[k]);
       }
     }
   }
 }
 
-// Sums over rows of scratch, 32 columns a CTA by eight lanes each: task 0 dweight, 1 dpost_weight, 2 the gate that all rows share, or from 2 on a row of the gate each.
+// Sums over rows of scratch.  The first CTAs add up three rows of c columns, 32 columns a CTA by eight lanes each: dweight, dpost_weight, the gate that all rows share; the others
+// the gate's rows from their stretches', a column a thread.
 struct Columns {
   const float *partial, *gate_rows;
   float *dweight, *dpost_weight, *dgate;
-  int c, ctas, shared_gate, first;  // first: the first task of the launch
-  long long parts;
+  int rows, c, blocks;  // CTAs of one of the three
+  int parts, gates;     // gates 0: one that all rows share
 };
 __global__ void __launch_bounds__(256) add_rms_norm_columns_kernel(const __grid_constant__ Columns t) {
   __shared__ float part[8][33];
   mtb_wait_prior();
-  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, i = blockIdx.x * 32 + lane, task = blockIdx.y + t.first;
-  const bool of_gate = task >= 2 && !t.shared_gate;
-  float* out = task == 0 ? t.dweight : task == 1 ? t.dpost_weight : t.dgate ? t.dgate + (of_gate ? (long long)(task - 2) * t.c : 0) : nullptr;
-  if (!out) return;
-  const float* from = of_gate ? t.gate_rows + (task - 2) * t.parts * t.c : t.partial + (long long)task * t.c;
-  const long long rows = of_gate ? t.parts : t.ctas, stride = of_gate ? t.c : 3LL * t.c;
-  float s[4] = {0, 0, 0, 0};
-  if (i < t.c) {
-    long long r = row;
-    for (; r + 24 < rows; r += 32) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) s[u] += from[(r + 8 * u) * stride + i];
+  const int c = t.c;
+  if ((int)blockIdx.x >= 3 * t.blocks) {
+    const long long count = (long long)t.gates * c, step = (gridDim.x - 3LL * t.blocks) * 256;
+    for (long long n = (blockIdx.x - 3LL * t.blocks) * 256 + threadIdx.x; n < count; n += step) {
+      const float* from = t.gate_rows + n / c * (t.parts - 1) * c + n;
+      float s = 0;
+#pragma unroll 8
+      for (int r = 0; r < t.parts; ++r) s += from[(long long)r * c];
+      t.dgate[n] = s;
     }
-    for (; r < rows; r += 8) s[0] += from[r * stride + i];
+    return;
+  }
+  const int which = blockIdx.x / t.blocks, lane = threadIdx.x & 31, row = threadIdx.x >> 5, i = (blockIdx.x - which * t.blocks) * 32 + lane;
+  float* out = which == 0 ? t.dweight : which == 1 ? t.dpost_weight : t.gates ? nullptr : t.dgate;
+  if (!out) return;
+  const long long stride = 3LL * c;
+  const float* from = t.partial + (long long)which * c + i;
+  float s[4] = {0, 0, 0, 0};
+  if (i < c) {
+    int r = row;
+    for (; r + 24 < t.rows; r += 32) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] += from[(r + 8 * u) * stride];
+    }
+    for (; r < t.rows; r += 8) s[0] += from[r * stride];
   }
   part[row][lane] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
-  if (row == 0 && i < t.c) {
+  if (row == 0 && i < c) {
     float x = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) x += part[k][lane];
@@ -395,29 +472,45 @@ __global__ void __launch_bounds__(kLongThreads) add_rms_norm_backward_long_kerne
 // ------------------------------------------------------------------ which kernel
 
 struct Plan {
-  int v, per, warps;  // warps 0: through memory
+  int v, per, warps, lanes;  // warps 0: through memory
   int groups;         // of a CTA
   int ctas;           // the most that the grid has
+  bool ahead;
 };
 
-Plan forward_plan(long long rows, int c, bool vectors) {
-  const int v = vectors && c % 4 == 0 ? 4 : 1, n = (c + v - 1) / v, sms = mtb_sm_count();
-  const bool many = rows > 8LL * sms;
-  for (const auto [per, warps] : {std::pair{1, 1}, {2, 1}, {4, 1}, {8, 1}, {1, 8}, {2, 8}, {4, 8}, {8, 8}, {v == 4 ? 4 : 8, 32}})
-    if (n <= 32 * warps * per && (warps > 1 || many || per <= 2)) return Plan{v, per, warps, warps == 1 ? 8 : 1, sms * (warps == 32 ? 2 : 8)};
-  return Plan{v, 0, 0, 1, 0};
+// How many CTAs of a kernel an SM holds: the grid is no larger, so that none waits for another to end.
+template <class K>
+int resident(K kernel, int threads, int smem, int* known) {
+  if (!*known && cudaOccupancyMaxActiveBlocksPerMultiprocessor(known, kernel, threads, smem) != cudaSuccess) *known = 0;
+  return *known > 0 ? *known : 1;
 }
 
-Plan backward_plan(long long rows, int c, bool vectors) {
-  const int v = vectors && c % 4 == 0 ? 4 : 1, n = (c + v - 1) / v, sms = mtb_sm_count();
-  if (v == 4) {
-    for (const auto [per, warps] : {std::pair{1, 1}, {2, 1}, {1, 4}, {2, 4}, {2, 8}, {2, 16}, {4, 16}})
-      if (n <= 32 * warps * per) return Plan{v, per, warps, warps == 1 ? 8 : 1, sms * (warps == 16 ? 1 : warps == 4 ? 6 : 3)};
-  } else {
-    for (const auto [per, warps] : {std::pair{1, 1}, {2, 1}, {4, 1}, {8, 1}, {4, 4}, {8, 4}, {8, 8}, {8, 16}})
-      if (n <= 32 * warps * per) return Plan{v, per, warps, warps == 1 ? 8 : 1, sms * (warps == 16 ? 1 : warps == 4 ? 6 : 3)};
-  }
-  return Plan{v, 0, 0, 1, sms};
+// Vectors of four, of two where rows or operands begin at 8 bytes, else single values; as few warps a row as hold it.  Of few rows eight warps a row.
+// Measured with post norm and gate, us: 65536 x 256 by 1 warp 46, by 2 45, by 4 72; 32768 x 1024 by 1 98, by 2 93, by 4 93, by 8 102; 8192 x 4096 by 8 98, by 16 95, by
+// 32 164; in vectors of two 32768 x 750 by 2 warps 74, by 4 70, by 8 92, in single values 78; 32768 x 1023 by 4 107, by 8 111, by 16 198.
+Plan forward_plan(long long rows, int c, int align) {
+  const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, n = c / v;
+  const auto plan = [&](int per, int warps, int lanes = 32) { return Plan{v, per, warps, lanes, warps == 1 ? 256 / lanes : 1, 0, false}; };
+  if (rows <= 8LL * mtb_sm_count() && c > 256)
+    for (const int per : {1, 2, 4})
+      if (n <= 256 * per) return plan(per, 8);
+  if (c <= 128) return plan(4 / v, 1, c <= 32 ? 8 : c <= 64 ? 16 : 32);
+  if (c <= 256) return plan(8 / v, 1);
+  if (v == 4) return n <= 128 ? plan(4, 1) : n <= 256 ? plan(8, 2) : n <= 512 ? plan(2, 8) : n <= 1024 ? plan(2, 16) : n <= 2048 ? plan(4, 16) : n <= 4096 ? plan(4, 32) : plan(0, 0);
+  if (v == 2) return n <= 256 ? plan(4, 2) : n <= 512 ? plan(4, 4) : n <= 1024 ? plan(8, 4) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(8, 32) : plan(0, 0);
+  return n <= 512 ? plan(8, 2) : n <= 1024 ? plan(8, 4) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(8, 32) : plan(0, 0);
+}
+
+// Eight values a thread and tensor.  With post norm and gate, us: 65536 x 300 by 2 warps 101, by 4 107, by 1 (16 values) 121; 32768 x 1024 by 4 135, by 8 136, by 2 138; 32768 x 750 in
+// vectors of two by 4 122, single values 132; 32768 x 1023 by 4 158, by 8 171.
+Plan backward_plan(int c, int align) {
+  const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, n = c / v, sms = mtb_sm_count();
+  const auto plan = [&](int per, int warps, int per_sm, bool ahead = false, int lanes = 32) { return Plan{v, per, warps, lanes, warps == 1 ? 256 / lanes : 1, sms * per_sm, ahead}; };
+  if (c <= 128) return plan(4 / v, 1, 5, false, c <= 32 ? 8 : c <= 64 ? 16 : 32);
+  const int per = 8 / v;
+  for (const auto [warps, most] : {std::pair{1, 3}, {2, 12}, {4, 6}, {8, 3}, {16, 2}, {32, 1}})
+    if (n <= 32 * warps * per) return plan(per, warps, most, v == 4 && warps >= 8);
+  return plan(0, 0, 1);
 }
 
 // How rows come in stretches (see Gradients): as many as there are groups, or more where the gate has more rows.
@@ -425,21 +518,34 @@ struct Stretches {
   long long stretches, parts, stretch, rows_of_gate;
   int ctas;
 };
-Stretches stretches_of(const Plan& p, long long rows, long long rows_of_gate) {
-  const long long gates = rows / rows_of_gate, groups = (long long)p.ctas * p.groups;
-  long long parts = groups / gates;
-  if (parts > (rows_of_gate + 1) / 2) parts = (rows_of_gate + 1) / 2;  // two rows at least
-  if (parts < 1) parts = 1;
-  const long long stretch = (rows_of_gate + parts - 1) / parts;
-  parts = (rows_of_gate + stretch - 1) / stretch;
-  const long long all = gates * parts, needed = (all + p.groups - 1) / p.groups;
-  return {all, parts, stretch, rows_of_gate, (int)(needed < p.ctas ? needed : p.ctas)};
+Stretches stretches_of(const Plan& p, int ctas, long long rows, long long rows_of_gate) {
+  // as many stretches as there are groups, or up to four times as many: what leaves the group with the most rows the fewest
+  const long long gates = rows / rows_of_gate, groups = (long long)ctas * p.groups;
+  Stretches best{};
+  long long least = 0;
+  for (int turns = 1; turns <= 4; ++turns) {
+    long long parts = turns * groups / gates;
+    if (parts > (rows_of_gate + 1) / 2) parts = (rows_of_gate + 1) / 2;  // two rows at least
+    if (parts < 1) parts = 1;
+    const long long stretch = (rows_of_gate + parts - 1) / parts;
+    parts = (rows_of_gate + stretch - 1) / stretch;
+    const long long all = gates * parts, most = (all + groups - 1) / groups * stretch, needed = (all + p.groups - 1) / p.groups;
+    if (turns == 1 || most < least) {
+      best = {all, parts, stretch, rows_of_gate, (int)(needed < ctas ? needed : ctas)};
+      least = most;
+    }
+  }
+  return best;
 }
 
 bool sizes_fine(long long rows, int c, long long rows_per_gate) { return rows >= 0 && rows < 1LL << 31 && c > 0 && c <= 1 << 30 && rows_per_gate > 0 && rows % rows_per_gate == 0; }
 
+// At how many floats all of them begin: 4, 2 or 1.
 template <class... P>
-bool aligned(P... p) { return ((reinterpret_cast<uintptr_t>(p) | ... | 0) & 15u) == 0; }
+int alignment(P... p) {
+  const uintptr_t all = (reinterpret_cast<uintptr_t>(p) | ... | 0);
+  return all % 16 == 0 ? 4 : all % 8 == 0 ? 2 : 1;
+}
 
 }  // namespace
 
@@ -450,17 +556,25 @@ MTB_API int mtb_add_rms_norm_forward_f32(long long rows, int c, const float* res
   MTB_REQUIRE(residual && y && (block ? out != nullptr : !post_weight && !gate), "add_rms_norm_forward: bad arguments");
   cudaStream_t st = (cudaStream_t)stream;
   const Operands a{residual, block, weight, post_weight, gate, rows, c, gate ? rows_per_gate : 1, (float)scale, (float)eps};
-  const Plan p = forward_plan(rows, c, aligned(residual, block, weight, post_weight, gate, out, y));
+  const Plan p = forward_plan(rows, c, alignment(residual, block, weight, post_weight, gate, out, y));
   const long long needed = (rows + p.groups - 1) / p.groups;
-#define MTB_CASE(V, PER, W) \
-  if (p.v == V && p.per == PER && p.warps == W) { \
-    MTB_LAUNCH((add_rms_norm_kernel<V, PER, W>), (unsigned)(needed < p.ctas ? needed : p.ctas), GroupSum<W>::kThreads, 0, st, a, out, y, rstd, block_rstd); \
+#define MTB_CASE(V, PER, W, LANES) \
+  if (p.v == V && p.per == PER && p.warps == W && p.lanes == LANES) { \
+    static int known; \
+    const long long most = (long long)mtb_sm_count() * resident(add_rms_norm_kernel<V, PER, W, LANES>, GroupSum<W>::kThreads, 0, &known); \
+    MTB_LAUNCH((add_rms_norm_kernel<V, PER, W, LANES>), (unsigned)(needed < most ? needed : most), GroupSum<W>::kThreads, 0, st, a, out, y, rstd, block_rstd); \
   } else
-#define MTB_BOTH(PER, W) MTB_CASE(4, PER, W) MTB_CASE(1, PER, W)
-  MTB_BOTH(1, 1) MTB_BOTH(2, 1) MTB_BOTH(4, 1) MTB_BOTH(8, 1) MTB_BOTH(1, 8) MTB_BOTH(2, 8) MTB_BOTH(4, 8) MTB_BOTH(8, 8) MTB_CASE(4, 4, 32) MTB_CASE(1, 8, 32) {
+#define MTB_ALL(PER, W) MTB_CASE(4, PER, W, 32) MTB_CASE(2, PER, W, 32) MTB_CASE(1, PER, W, 32)
+#define MTB_NARROW(V) MTB_CASE(V, 4 / V, 1, 8) MTB_CASE(V, 4 / V, 1, 16) MTB_CASE(V, 4 / V, 1, 32) MTB_CASE(V, 8 / V, 1, 32)
+#define MTB_WIDE(PER, W) MTB_CASE(2, PER, W, 32) MTB_CASE(1, PER, W, 32)
+  MTB_NARROW(4) MTB_NARROW(2) MTB_NARROW(1) MTB_ALL(1, 8) MTB_ALL(2, 8) MTB_ALL(4, 8)
+  MTB_CASE(4, 4, 1, 32) MTB_CASE(4, 8, 2, 32) MTB_CASE(4, 2, 16, 32) MTB_CASE(4, 4, 16, 32) MTB_CASE(4, 4, 32, 32)
+  MTB_CASE(2, 4, 2, 32) MTB_CASE(2, 4, 4, 32) MTB_CASE(1, 8, 2, 32) MTB_WIDE(8, 4) MTB_WIDE(8, 8) MTB_WIDE(8, 16) MTB_WIDE(8, 32) {
     MTB_LAUNCH(add_rms_norm_long_kernel, (unsigned)rows, kLongThreads, 0, st, a, out, y, rstd, block_rstd);
   }
-#undef MTB_BOTH
+#undef MTB_WIDE
+#undef MTB_NARROW
+#undef MTB_ALL
 #undef MTB_CASE
   MTB_LAUNCH_CHECK("add_rms_norm_kernel");
   return MTB_OK;
@@ -469,13 +583,19 @@ MTB_API int mtb_add_rms_norm_forward_f32(long long rows, int c, const float* res
 MTB_API long long mtb_add_rms_norm_workspace_bytes(long long rows, int c) {
   // whichever kernel it will be: a row of three sums for each CTA, and one for each stretch that does not fill a row of the gate
   long long most = 0;
-  for (const bool vectors : {false, true}) {
-    const Plan p = backward_plan(rows, c, vectors);
-    const long long floats = (long long)p.ctas * (3 + p.groups) * c;
+  for (const int align : {1, 2, 4}) {
+    const Plan p = backward_plan(c, align);
+    const long long floats = (long long)p.ctas * (3 + 4 * p.groups) * c;
     if (floats > most) most = floats;
   }
   return 4 * most;
 }
+
+// The kernels that backward_plan names, each as a case of whatever MTB_CASE is.
+#define MTB_OF(V, AHEAD) \
+  MTB_CASE(V, 4 / V, 1, 8, false) MTB_CASE(V, 4 / V, 1, 16, false) MTB_CASE(V, 4 / V, 1, 32, false) MTB_CASE(V, 8 / V, 1, 32, false) MTB_CASE(V, 8 / V, 2, 32, false) \
+  MTB_CASE(V, 8 / V, 4, 32, false) MTB_CASE(V, 8 / V, 8, 32, AHEAD) MTB_CASE(V, 8 / V, 16, 32, AHEAD) MTB_CASE(V, 8 / V, 32, 32, AHEAD)
+#define MTB_KERNELS MTB_OF(4, true) MTB_OF(2, false) MTB_OF(1, false)
 
 MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dnew, const float* dy, const float* x, const float* rstd, const float* block,
                                           const float* block_rstd, const float* weight, const float* post_weight, const float* gate, long long rows_per_gate, double scale,
@@ -490,33 +610,44 @@ MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dn
   if (!post_weight) dpost_weight = nullptr;
   if (!gate) dgate = nullptr;
   const Operands a{x, block, weight, post_weight, gate, rows, c, gate ? rows_per_gate : 1, block ? (float)scale : 1.f, 0.f};
-  const Plan p = backward_plan(rows, c, aligned(dnew, dy, x, block, weight, post_weight, gate, dresidual, dblock, dgate));
+  const Plan p = backward_plan(c, alignment(dnew, dy, x, block, weight, post_weight, gate, dresidual, dblock, dgate));
   const bool each = dgate && rows_per_gate == 1 && rows > 0, of_gate = dgate && !each && rows_per_gate < rows;
   Stretches s{0, 1, 1, 1, 0};
   float *partial = (float*)workspace, *gate_rows = nullptr;
   const bool summed = dweight || dpost_weight || (dgate && !each && !of_gate);
   if (rows > 0) {
-    s = stretches_of(p, rows, of_gate ? rows_per_gate : rows);
+    int ctas = p.ctas;
+#define MTB_CASE(V, PER, W, LANES, AHEAD) \
+  if (p.v == V && p.per == PER && p.warps == W && p.lanes == LANES && p.ahead == AHEAD) { \
+    static unsigned long long opted; \
+    static int known; \
+    constexpr int kAhead = 16 * V * PER * GroupSum<W>::kThreads; \
+    if (AHEAD) \
+      if (int rc = mtb_opt_in_smem((const void*)add_rms_norm_backward_kernel<V, PER, W, LANES, AHEAD>, kAhead, &opted)) return rc; \
+    const int most = mtb_sm_count() * resident(add_rms_norm_backward_kernel<V, PER, W, LANES, AHEAD>, GroupSum<W>::kThreads, AHEAD ? kAhead : W == 1 ? 12 * 256 : 0, &known); \
+    ctas = most < ctas ? most : ctas; \
+  } else
+    MTB_KERNELS {}
+#undef MTB_CASE
+    s = stretches_of(p, ctas, rows, of_gate ? rows_per_gate : rows);
     gate_rows = each || (of_gate && s.parts == 1) ? dgate : of_gate ? partial + (long long)p.ctas * 3 * c : nullptr;
     const Gradients d{dnew, dy, rstd, block_rstd, dresidual, dblock, summed ? partial : nullptr, gate_rows, each ? 1 : 0, s.stretches, s.parts, s.stretch, s.rows_of_gate};
-#define MTB_CASE(V, PER, W) \
-  if (p.v == V && p.per == PER && p.warps == W) { \
-    MTB_LAUNCH((add_rms_norm_backward_kernel<V, PER, W>), (unsigned)s.ctas, GroupSum<W>::kThreads, W == 1 ? 12 * c : 0, st, a, d); \
+#define MTB_CASE(V, PER, W, LANES, AHEAD) \
+  if (p.v == V && p.per == PER && p.warps == W && p.lanes == LANES && p.ahead == AHEAD) { \
+    MTB_LAUNCH((add_rms_norm_backward_kernel<V, PER, W, LANES, AHEAD>), (unsigned)s.ctas, GroupSum<W>::kThreads, AHEAD ? 16 * V * PER * GroupSum<W>::kThreads : W == 1 ? 12 * c : 0, st, a, d); \
   } else
-    MTB_CASE(4, 1, 1) MTB_CASE(4, 2, 1) MTB_CASE(4, 1, 4) MTB_CASE(4, 2, 4) MTB_CASE(4, 2, 8) MTB_CASE(4, 2, 16) MTB_CASE(4, 4, 16)
-    MTB_CASE(1, 1, 1) MTB_CASE(1, 2, 1) MTB_CASE(1, 4, 1) MTB_CASE(1, 8, 1) MTB_CASE(1, 4, 4) MTB_CASE(1, 8, 4) MTB_CASE(1, 8, 8) MTB_CASE(1, 8, 16) {
+    MTB_KERNELS {
       MTB_LAUNCH(add_rms_norm_backward_long_kernel, (unsigned)s.ctas, kLongThreads, 0, st, a, d);
     }
 #undef MTB_CASE
     MTB_LAUNCH_CHECK("add_rms_norm_backward_kernel");
   }
   // a gate of every row is written; one of several rows is unless its stretches are shorter
-  const bool parts = of_gate && s.parts > 1, shared_gate = dgate && !each && !of_gate;
-  const long long tasks = 2 + (shared_gate ? 1 : parts ? rows / rows_per_gate : 0);
-  if (!dweight && !dpost_weight && tasks == 2) return MTB_OK;
-  for (long long first = 0; first < tasks; first += 65535) {
-    const Columns t{partial, gate_rows, dweight, dpost_weight, dgate, c, s.ctas, shared_gate ? 1 : 0, (int)first, s.parts};
-    MTB_LAUNCH(add_rms_norm_columns_kernel, dim3(mtb_div_up(c, 32), (unsigned)(tasks - first < 65535 ? tasks - first : 65535)), 256, 0, st, t);
+  const bool shared_gate = dgate && !each && !of_gate, by_parts = of_gate && s.parts > 1;
+  if (dweight || dpost_weight || shared_gate || by_parts) {
+    const long long gates = by_parts ? rows / rows_per_gate : 0;
+    const Columns t{partial, gate_rows, dweight, dpost_weight, shared_gate || by_parts ? dgate : nullptr, s.ctas, c, mtb_div_up(c, 32), (int)s.parts, (int)gates};
+    MTB_LAUNCH(add_rms_norm_columns_kernel, 3 * t.blocks + (by_parts ? mtb_stream_grid(gates * c, 256) : 0), 256, 0, st, t);
     MTB_LAUNCH_CHECK("add_rms_norm_columns_kernel");
   }
   return MTB_OK;
