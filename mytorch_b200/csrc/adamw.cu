@@ -50,6 +50,33 @@ __global__ void __launch_bounds__(256) adamw_begin_kernel(const __grid_constant_
   out[threadIdx.x] = Corrections{(float)(lr / (1.0 - pow(b1, (double)step))), (float)(1.0 / sqrt(1.0 - pow(b2, (double)step))), (unsigned)step, grad_scale};
 }
 
+// Which tensor a CTA's chunk of elements is of: chunk b is one of tensor k with start[k] <= b < start[k + 1].  `near` says where to look from: bisection took a
+// tenth of the instructions of the update in 8 bits.
+template <int N>
+struct Chunks {
+  static constexpr int kNear = 128;
+  int start[N + 1], count, shift;
+  unsigned char near[kNear];  // of chunk j << shift
+
+  int fill(int tensors, const long long* sizes, long long stride) {  // the number of chunks
+    count = tensors;
+    start[0] = 0;
+    for (int k = 0; k < count; ++k) start[k + 1] = start[k] + (int)((sizes[stride * k] + kChunk - 1) / kChunk);
+    shift = 0;
+    while (start[count] >> shift >= kNear) ++shift;
+    for (int j = 0, k = 0; j < kNear; ++j) {
+      while (k + 1 < count && start[k + 1] <= (long long)j << shift) ++k;
+      near[j] = (unsigned char)k;
+    }
+    return start[count];
+  }
+  __device__ __forceinline__ int tensor(int chunk) const {
+    int k = near[chunk >> shift];
+    while (start[k + 1] <= chunk) ++k;
+    return k;
+  }
+};
+
 // N tensors: a table of a few costs its launch less.
 template <class M, int N>
 struct Table {
@@ -58,21 +85,10 @@ struct Table {
   M* m[N];  // 32 bits: the first moments; 8 bits: [block][first 256 | second 256]
   M* v[N];  // 32 bits: the second moments; 8 bits: [block][scale of the first, of the second]
   long long n[N];
-  int chunk_start[N + 1];  // CTA b works on tensor k with chunk_start[k] <= b < chunk_start[k + 1]
   unsigned short slot[N];  // which corrections
   unsigned key[N];
-  int count;
+  Chunks<N> chunks;
 };
-
-template <class T>
-__device__ __forceinline__ int tensor_of(const T& t, int chunk) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {  // last k with chunk_start[k] <= chunk
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.chunk_start[mid] <= chunk) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
 
 // Root and quotient to 2^-22 of themselves, the step's share of which is far under a parameter's last place.
 __device__ __forceinline__ void update(float& p, float m, float v, const Hyper& h, const Corrections& c) {
@@ -90,8 +106,8 @@ template <int N>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<float, N> t, Hyper h, const Corrections* __restrict__ corrections) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const int chunk = t.chunk_start[t.count] - 1 - (int)blockIdx.x, k = tensor_of(t, chunk);
-  const long long e = (long long)(chunk - t.chunk_start[k]) * kChunk, left = t.n[k] - e;
+  const int chunk = (int)(gridDim.x - 1 - blockIdx.x), k = t.chunks.tensor(chunk);
+  const long long e = (long long)(chunk - t.chunks.start[k]) * kChunk, left = t.n[k] - e;
   const int n = left < kChunk ? (int)left : kChunk;
   float *p = t.p[k] + e, *m = t.m[k] + e, *v = t.v[k] + e;
   const float* g = t.g[k] + e;
@@ -158,24 +174,40 @@ __host__ __device__ __forceinline__ unsigned mix(unsigned x) {
 }
 constexpr unsigned kGolden = 0x9E3779B1u;
 
-// What a block's scale stands for, and its reciprocal.
+// What a block's scale stands for.
 __device__ __forceinline__ float unit_of(unsigned scale) { return scale == 255 ? __uint_as_float(0x7FC00000u) : __uint_as_float(scale << 23); }
-__device__ __forceinline__ float per_unit(unsigned scale) { return __uint_as_float(scale >= 254 ? 0x00400000u : (254u - scale) << 23); }
-// The scale for values of which the largest has these bits.
-__device__ __forceinline__ unsigned scale_of(unsigned bits) { return bits == 0 ? 0u : bits < 0x00800000u ? 1u : bits >> 23; }
+__device__ __forceinline__ float per_unit(unsigned scale) { return __uint_as_float(scale >= 254 ? 0x00400000u : (254u - scale) << 23); }  // its reciprocal
+// The scale for values of which the largest is this; NaN where one is.
+__device__ __forceinline__ unsigned scale_of(float most) {
+  const unsigned bits = __float_as_uint(most) & 0x7FFFFFFFu;
+  return bits == 0 ? 0u : bits < 0x00800000u ? 1u : bits >> 23;
+}
 
-__device__ __forceinline__ float decode_first(unsigned code, float unit) {
-  return __uint_as_float((code & 0x7Fu) << 20 | (code & 0x80u) << 24) * 0x1p113f * unit;
-}
-__device__ __forceinline__ float decode_second(unsigned code, float unit) { return __uint_as_float(code << 20) * 0x1p97f * unit; }
-// random: 16 bits.  The reciprocal's product with a value is exact where it is not far under the lowest code.
-__device__ __forceinline__ unsigned encode_first(float m, float per, unsigned random) {
-  return (__float_as_uint(fabsf(m) * per * 0x1p-113f) + (random << 4) + 8u) >> 20 | (__float_as_uint(m) >> 31) << 7;
-}
-__device__ __forceinline__ unsigned encode_second(float v, float per, unsigned random) {
-  const unsigned code = (__float_as_uint(v * per * 0x1p-97f) + (random << 4) + 8u) >> 20;
-  return v > 0.f && code == 0 ? 1u : code;
-}
+// The float32 whose upper bits the code in byte B of a word is.
+template <int B>
+__device__ __forceinline__ float first_bits(unsigned w) { return __uint_as_float((unsigned)((int)(w << (24 - 8 * B)) >> 4) & 0x87F00000u); }
+template <int B>
+__device__ __forceinline__ float second_bits(unsigned w) { return __uint_as_float((B == 3 ? w >> 4 : w << (20 - 8 * B)) & 0x0FF00000u); }
+
+// Powers of two by which such a float is multiplied to be what the code stands for, or the other way, in two products where one power does not fit a float32.
+struct Powers {
+  float one, other;
+  bool two;
+
+  static __device__ __forceinline__ Powers decode(unsigned scale, int up) {  // 2^up unit
+    const bool two = scale + up > 253;
+    const float unit = unit_of(scale), power = __uint_as_float((unsigned)(127 + up) << 23);
+    return Powers{two ? power : power * unit, unit, two};
+  }
+  static __device__ __forceinline__ Powers encode(unsigned scale, int down) {  // 2^-down / unit
+    const bool two = scale + down > 253;
+    const float per = per_unit(scale), power = __uint_as_float((unsigned)(127 - down) << 23);
+    return Powers{two ? per : per * power, power, two};
+  }
+  __device__ __forceinline__ float operator()(float x) const { return x * one; }
+  __device__ __forceinline__ float again(float x) const { return x * other; }
+};
+constexpr int kFirst = 113, kSecond = 97;  // the highest exponents, 15 and 31 in a float32, are that of twice the unit
 
 // A lane's eight values of a block, and their codes, a byte each in four words.  VECTORS: four at 4 lane and four at 128 + 4 lane, where parameters and gradients
 // begin at 16 bytes; else at lane + 32 j, a value or a byte a load, which is as many bytes of memory.
@@ -205,67 +237,141 @@ struct Lane {
         if (at(j) < n) __stcs(to + at(j), x[j]);
     }
   }
-  __device__ __forceinline__ void codes(const unsigned char* from, unsigned (&c)[8]) const {
+  // Of VECTORS two words of four codes, else eight words of one.
+  static constexpr int kWords = VECTORS ? 2 : 8;
+  __device__ __forceinline__ void codes(const unsigned char* from, unsigned (&w)[8]) const {
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) w[u] = VECTORS ? __ldcs((const unsigned*)(from + 128 * u) + lane) : (unsigned)__ldcs(from + at(u));
+  }
+  __device__ __forceinline__ void decode(const unsigned (&w)[8], unsigned scale, float (&x)[8], bool second) const {
     if (VECTORS) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const unsigned w = __ldcs((const unsigned*)(from + 128 * u) + lane);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c[4 * u + j] = w >> 8 * j & 0xFFu;
+        x[4 * u] = second ? second_bits<0>(w[u]) : first_bits<0>(w[u]);
+        x[4 * u + 1] = second ? second_bits<1>(w[u]) : first_bits<1>(w[u]);
+        x[4 * u + 2] = second ? second_bits<2>(w[u]) : first_bits<2>(w[u]);
+        x[4 * u + 3] = second ? second_bits<3>(w[u]) : first_bits<3>(w[u]);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) c[j] = __ldcs(from + at(j));
+      for (int j = 0; j < 8; ++j) x[j] = second ? second_bits<0>(w[j]) : first_bits<0>(w[j]);
+    }
+    const Powers power = Powers::decode(scale, second ? kSecond : kFirst);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = power(x[j]);
+    if (power.two) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = power.again(x[j]);
     }
   }
-  __device__ __forceinline__ void put_codes(unsigned char* to, const unsigned (&c)[8]) const {
+  // t: codes above 20 bits of fraction; signs: values with the codes' signs, or NULL.
+  __device__ __forceinline__ void put_codes(unsigned char* to, const unsigned (&t)[8], const float* signs, bool none) const {
     if (VECTORS) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) __stcs((unsigned*)(to + 128 * u) + lane, c[4 * u] | c[4 * u + 1] << 8 | c[4 * u + 2] << 16 | c[4 * u + 3] << 24);
+      for (int u = 0; u < 2; ++u) {
+        unsigned w = t[4 * u] >> 20 | t[4 * u + 1] >> 20 << 8 | t[4 * u + 2] >> 20 << 16 | t[4 * u + 3] >> 20 << 24;
+        if (signs) {
+          const unsigned a = __byte_perm(__float_as_uint(signs[4 * u]), __float_as_uint(signs[4 * u + 1]), 0x0073);
+          const unsigned b = __byte_perm(__float_as_uint(signs[4 * u + 2]), __float_as_uint(signs[4 * u + 3]), 0x0073);
+          w |= __byte_perm(a, b, 0x5410) & 0x80808080u;
+        }
+        __stcs((unsigned*)(to + 128 * u) + lane, none ? 0u : w);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) __stcs(to + at(j), (unsigned char)c[j]);
+      for (int j = 0; j < 8; ++j) __stcs(to + at(j), (unsigned char)(none ? 0u : t[j] >> 20 | (signs ? __float_as_uint(signs[j]) >> 31 << 7 : 0u)));
     }
   }
 };
 
-// A block by a warp.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// The same as update() where eps hides what becomes of a root of a value under the smallest normal number: in 1e-10 it is under 2^-24.
+__device__ __forceinline__ void update_quickly(float& p, float m, float v, const Hyper& h, const Corrections& c) {
+  float root, per;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(per) : "f"(fmaf(root, c.root, h.eps)));
+  p = fmaf(p, h.keep, -(c.step_size * m * per));
+}
+
+// A block by a warp.  What bounds it is the number of instructions, 45 a value where a scale's power fits a float32: words of codes taken apart and put together whole,
+// and everything that a scale decides decided once a block.
 template <bool VECTORS>
 __device__ __forceinline__ void update_block(const Lane<VECTORS> l, float* p, const float* g, int n, unsigned char* codes, unsigned char* scales, unsigned first, unsigned key,
                                              const Hyper& h, const Corrections* corrections) {
-  float pp[8], gg[8];
+  float pp[8], gg[8], m[8], v[8];
   unsigned cm[8], cv[8];
   l.values(g, n, gg);
-  l.values(p, n, pp);
   l.codes(codes, cm);
   l.codes(codes + kBlock, cv);
+  l.values(p, n, pp);
   const unsigned scale = *(const unsigned short*)scales;
   const Corrections c = *corrections;
-  key = mix(key + c.t);
-  const float unit_m = unit_of(scale & 0xFFu), unit_v = unit_of(scale >> 8);
-  float m[8], v[8];
-  unsigned most_m = 0, most_v = 0;
+  l.decode(cm, scale & 0xFFu, m, false);
+  l.decode(cv, scale >> 8, v, true);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float x = gg[j] * c.grad_scale, root = h.c2 * x;
-    m[j] = __fmaf_rn(h.c1, x, __fmul_rn(h.b1, decode_first(cm[j], unit_m)));
-    v[j] = __fmaf_rn(root, root, __fmul_rn(h.b2, decode_second(cv[j], unit_v)));
-    if (n < kBlock && l.at(j) >= n) m[j] = v[j] = 0.f;
-    update(pp[j], m[j], v[j], h, c);
-    most_m = max(most_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-    most_v = max(most_v, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    m[j] = __fmaf_rn(h.c1, x, __fmul_rn(h.b1, m[j]));
+    v[j] = __fmaf_rn(root, root, __fmul_rn(h.b2, v[j]));
   }
-  l.put(p, n, pp);
-  const unsigned scale_m = scale_of(__reduce_max_sync(0xFFFFFFFFu, most_m)), scale_v = scale_of(__reduce_max_sync(0xFFFFFFFFu, most_v));
-  const float per_m = per_unit(scale_m), per_v = per_unit(scale_v);
+  if (n < kBlock) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (l.at(j) >= n) m[j] = v[j] = 0.f;
+  }
+  float most_m = 0, most_v = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const unsigned r = mix(key + (first + l.at(j)) * kGolden);
-    cm[j] = scale_m == 255 ? 0u : encode_first(m[j], per_m, r >> 16);
-    cv[j] = scale_v == 255 ? 0u : encode_second(v[j], per_v, r & 0xFFFFu);
+    most_m = max_nan(most_m, fabsf(m[j]));
+    most_v = max_nan(most_v, v[j]);
   }
-  l.put_codes(codes, cm);
-  l.put_codes(codes + kBlock, cv);
+  if (h.eps >= 1e-10f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) update_quickly(pp[j], m[j], v[j], h, c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) update(pp[j], m[j], v[j], h, c);
+  }
+  l.put(p, n, pp);
+  // a NaN's bits are above infinity's, and scale_of takes both for 255
+  const unsigned scale_m = scale_of(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_m))));
+  const unsigned scale_v = scale_of(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_v))));
+  // To codes with 20 bits of fraction, of which 16 are compared with a random number: it and a half are added.
+  const Powers to_m = Powers::encode(scale_m, kFirst), to_v = Powers::encode(scale_v, kSecond);
+  float x[8], y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] = to_m(fabsf(m[j]));
+    y[j] = to_v(v[j]);
+  }
+  if (to_m.two) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = to_m.again(x[j]);
+  }
+  if (to_v.two) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = to_v.again(y[j]);
+  }
+  key = mix(key + c.t) + (first + l.at(0)) * kGolden;
+  bool zero = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned r = mix(key + (unsigned)(l.at(j) - l.at(0)) * kGolden);
+    cm[j] = __float_as_uint(x[j]) + ((r >> 12 & 0xFFFF0u) | 8u);
+    cv[j] = max(__float_as_uint(y[j]) + ((r << 4 & 0xFFFF0u) | 8u), 1u << 20);  // not to zero
+    zero |= v[j] == 0.f;
+  }
+  if (__any_sync(0xFFFFFFFFu, zero)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (v[j] == 0.f) cv[j] = 0;
+  }
+  l.put_codes(codes, cm, m, scale_m == 255);
+  l.put_codes(codes + kBlock, cv, nullptr, scale_v == 255);
   if (l.lane == 0) *(unsigned short*)scales = (unsigned short)(scale_m | scale_v << 8);
 }
 
@@ -273,8 +379,8 @@ template <int N>
 __global__ void __launch_bounds__(kThreads) adamw8_kernel(const __grid_constant__ Table<unsigned char, N> t, Hyper h, const Corrections* __restrict__ corrections) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const int chunk = t.chunk_start[t.count] - 1 - (int)blockIdx.x, k = tensor_of(t, chunk), lane = threadIdx.x & 31;
-  const long long block = (long long)(chunk - t.chunk_start[k]) * (kChunk / kBlock) + (threadIdx.x >> 5), e = block * kBlock, left = t.n[k] - e;
+  const int chunk = (int)(gridDim.x - 1 - blockIdx.x), k = t.chunks.tensor(chunk), lane = threadIdx.x & 31;
+  const long long block = (long long)(chunk - t.chunks.start[k]) * (kChunk / kBlock) + (threadIdx.x >> 5), e = block * kBlock, left = t.n[k] - e;
   if (left <= 0) return;
   const int n = left < kBlock ? (int)left : kBlock;
   float* p = t.p[k] + e;
@@ -291,22 +397,17 @@ struct MomentsTable {
   const unsigned char *codes[N], *scales[N];
   float *m[N], *v[N];
   long long n[N];
-  int chunk_start[N + 1];
-  int count;
+  Chunks<N> chunks;
 };
 template <bool VECTORS>
 __device__ __forceinline__ void write_block(const Lane<VECTORS> l, const unsigned char* codes, const unsigned char* scales, float* m, float* v, int n) {
   unsigned cm[8], cv[8];
+  float x[8], y[8];
   l.codes(codes, cm);
   l.codes(codes + kBlock, cv);
   const unsigned scale = *(const unsigned short*)scales;
-  const float unit_m = unit_of(scale & 0xFFu), unit_v = unit_of(scale >> 8);
-  float x[8], y[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] = decode_first(cm[j], unit_m);
-    y[j] = decode_second(cv[j], unit_v);
-  }
+  l.decode(cm, scale & 0xFFu, x, false);
+  l.decode(cv, scale >> 8, y, true);
   l.put(m, n, x);
   l.put(v, n, y);
 }
@@ -314,8 +415,8 @@ template <int N>
 __global__ void __launch_bounds__(kThreads) adamw8_moments_kernel(const __grid_constant__ MomentsTable<N> t) {
   mtb_launch_dependents();
   mtb_wait_prior();
-  const int k = tensor_of(t, blockIdx.x), lane = threadIdx.x & 31;
-  const long long block = (long long)((int)blockIdx.x - t.chunk_start[k]) * (kChunk / kBlock) + (threadIdx.x >> 5), e = block * kBlock, left = t.n[k] - e;
+  const int k = t.chunks.tensor(blockIdx.x), lane = threadIdx.x & 31;
+  const long long block = (long long)((int)blockIdx.x - t.chunks.start[k]) * (kChunk / kBlock) + (threadIdx.x >> 5), e = block * kBlock, left = t.n[k] - e;
   if (left <= 0) return;
   const int n = left < kBlock ? (int)left : kBlock;
   float *m = t.m[k] + e, *v = t.v[k] + e;
@@ -373,9 +474,8 @@ int run(const char* name, K kernel, int count, void* const* params, const long l
         const Corrections* corrections, cudaStream_t st) {
   for (int base = (count - 1) / N * N; count > 0 && base >= 0; base -= N) {
     Table<M, N> t;
-    t.count = count - base < N ? count - base : N;
-    long long chunks = 0;
-    for (int k = 0; k < t.count; ++k) {
+    const int tensors = count - base < N ? count - base : N, chunks = t.chunks.fill(tensors, sizes + (long long)stride * base, stride);
+    for (int k = 0; k < tensors; ++k) {
       const Tensor a = tensor_at(params, base + k);
       const long long* size = sizes + (long long)stride * (base + k);
       t.p[k] = a.p;
@@ -385,10 +485,7 @@ int run(const char* name, K kernel, int count, void* const* params, const long l
       t.n[k] = size[0];
       t.slot[k] = slots[base + k];
       t.key[k] = stride > 1 ? mix((unsigned)size[1]) : 0;
-      t.chunk_start[k] = (int)chunks;
-      chunks += (t.n[k] + kChunk - 1) / kChunk;
     }
-    t.chunk_start[t.count] = (int)chunks;
     if (chunks == 0) continue;
     MTB_LAUNCH(kernel, dim3((unsigned)chunks), kThreads, 0, st, t, h, corrections);
     MTB_LAUNCH_CHECK(name);
@@ -451,19 +548,15 @@ template <int N>
 static int moments_of(int count, void* const* params, const long long* sizes, cudaStream_t st) {
   for (int base = 0; base < count; base += N) {
     MomentsTable<N> t;
-    t.count = count - base < N ? count - base : N;
-    long long chunks = 0;
-    for (int k = 0; k < t.count; ++k) {
+    const int tensors = count - base < N ? count - base : N, chunks = t.chunks.fill(tensors, sizes + base, 1);
+    for (int k = 0; k < tensors; ++k) {
       void* const* a = params + 4 * (long long)(base + k);
       t.codes[k] = (const unsigned char*)a[0];
       t.scales[k] = (const unsigned char*)a[1];
       t.m[k] = (float*)a[2];
       t.v[k] = (float*)a[3];
       t.n[k] = sizes[base + k];
-      t.chunk_start[k] = (int)chunks;
-      chunks += (t.n[k] + kChunk - 1) / kChunk;
     }
-    t.chunk_start[t.count] = (int)chunks;
     if (chunks == 0) continue;
     MTB_LAUNCH(adamw8_moments_kernel<N>, dim3((unsigned)chunks), kThreads, 0, st, t);
     MTB_LAUNCH_CHECK("adamw8_moments_kernel");
