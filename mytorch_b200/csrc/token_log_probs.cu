@@ -4,16 +4,18 @@
 // A logit of -inf has probability 0 and adds nothing to the entropy or its gradient; a row of nothing else, or with a NaN or +inf, is NaN.
 // Alternatives are in the order of their logits, NaN before everything, equal ones by place, which one whole number holds (`key_of`).
 //
-// Bound by memory: forward reads a row once, backward reads and writes it once.  4096 rows of 50000: forward 132 us without alternatives, 6.2 TB/s, 152 with 8, 5.4;
-// backward 246 us, 6.7 TB/s.  Each thread keeps a running maximum and both sums of its share of the row, four loads of 16 bytes on their way at a time (44 registers: 40 warps an
-// SM; a second set on its way ahead of use costs a quarter of the warps: 146 instead of 129 without alternatives).
+// Bound by memory: forward reads a row once, backward reads and writes it once.  4096 rows of 50000, logits out of HBM: forward 132 us without alternatives, 6.2 TB/s, 155 with 8,
+// 5.3; backward 265 us, 6.2 TB/s.  Each thread keeps a running maximum and both sums of its share of the row, four loads of 16 bytes on their way at a time.  What counts is
+// how many warps are under way (40 an SM): a second set of loads ahead of use costs a quarter of them, 146 us, reloading each register as soon as it is used 162, copies
+// through shared memory two batches ahead and across rows 149.
 //
-// Alternatives.  A thread also keeps the maxima of the four groups that its quads fall into, nothing else.  When the row is through, the r-th largest of the
-// groups' maxima in each of enough warps is a bound that `top` values reach, and only groups whose maximum reaches it can hold an alternative: mostly little more than
-// `top` of the row's 1024 (512, 128) groups, whose values are read again, and what reaches the bound is put in order by counting.  An exact bound by sorting all maxima: 180 us with 8
-// of 50000; one group a thread, which reads four times as much again out of HBM, as the rows under way are more than the L2 holds: 170; candidates picked
-// while the row comes by would cost every batch of values an insertion at first.  Where very many values equal the bound, as where a mask leaves fewer than `top`, those above it are taken
-// and then the first of the row that equal it; rows with a NaN, and more candidates than there is room for, take `top` passes that find one each.
+// Alternatives.  A thread also keeps the maxima of the four groups that its quads fall into, nothing else.  When the row is through, the top-th largest of the maxima of 64 parts
+// of it is a bound that `top` values reach, and only groups whose maximum reaches it can hold an alternative: little more than `top` of the row's 1024 (512, 128) groups, whose values
+// are read again, and what reaches the bound is put in order by counting.  The bound takes a third of the 23 us that 8 alternatives cost, the second reading the rest.  An
+// exact bound by sorting all groups' maxima: 180 us; the r-th largest of each warp's: 163; one group a thread, which reads four times as much again out of HBM, as the
+// rows under way are more than the L2 holds: 170; candidates picked while the row comes by would cost every batch of values an insertion at first.  Where very many
+// values equal the bound, as where a mask leaves fewer than `top`, those above it are taken and then the first of the row that equal it; rows with a NaN, and more candidates
+// than there is room for, take `top` passes that find one each.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -74,11 +76,15 @@ struct Sums {
     s_low *= f;
     ref = r;
   }
-  // Over the warp, in all its lanes.
-  __device__ __forceinline__ void reduce() {
+  // Over the warp, in all its lanes.  RUN: to `runs` the largest value of each run of so many lanes.
+  template <int RUN = 32>
+  __device__ __forceinline__ void reduce(float* runs = nullptr) {
     float to = most;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) to = max_nan(to, __shfl_xor_sync(0xFFFFFFFFu, to, o));
+    for (int o = 1; o < 32; o *= 2) {
+      if (RUN < 32 && o == RUN && (threadIdx.x & (RUN - 1)) == 0) runs[(threadIdx.x & 31) / RUN] = to;
+      to = max_nan(to, __shfl_xor_sync(0xFFFFFFFFu, to, o));
+    }
     raise(to);
     s += s_low;
     t += t_low;
@@ -147,6 +153,7 @@ template <int W>
 struct Shared {
   static constexpr int kCandidates = W == 1 ? 256 : 512, kGroups = W == 1 ? 128 : 256;
   alignas(16) float part[W][4];
+  float runs[64];
   Key candidate[kCandidates], list[W];
   int group[kGroups], groups, candidates;
 };
@@ -181,19 +188,14 @@ __device__ __forceinline__ void take(const Row& row, int begin, int end, Shared<
     if (k >= each) { k -= each; ++g; }
   }
 }
-// The r-th largest of the values that the lanes of a warp hold, `more` of them each in descending order, in all lanes.
-template <int MORE>
-__device__ __forceinline__ float largest_but(int r, float (&m)[MORE], int lane) {
-  unsigned o[MORE];
-#pragma unroll
-  for (int i = 0; i < MORE; ++i) o[i] = ordered(m[i]);
-  unsigned most = 0;
+// The r-th largest of the values that the lanes of a warp hold, two each, the larger first, in all lanes.
+__device__ __forceinline__ float largest_but(int r, const float (&m)[2]) {
+  unsigned o[2] = {ordered(m[0]), ordered(m[1])}, most = 0;
   for (int k = 0; k < r; ++k) {
     most = __reduce_max_sync(0xFFFFFFFFu, o[0]);
-    if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, o[0] == most)) - 1) {
-#pragma unroll
-      for (int i = 0; i + 1 < MORE; ++i) o[i] = o[i + 1];
-      o[MORE - 1] = 0;
+    if ((threadIdx.x & 31) == __ffs(__ballot_sync(0xFFFFFFFFu, o[0] == most)) - 1) {
+      o[0] = o[1];
+      o[1] = 0;
     }
   }
   return value_of((Key)most << 32);
@@ -242,7 +244,6 @@ __device__ __forceinline__ Sums look(const Row& row, int begin, int end, int top
   const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5, id = W == 1 ? lane : threadIdx.x;
   Sums sums;
   constexpr int G = kSplit;
-  const int each = (top + W - 1) / W;
   float most[G];  // of the thread's groups
 #pragma unroll
   for (int u = 0; u < G; ++u) most[u] = -INFINITY;
@@ -271,31 +272,30 @@ __device__ __forceinline__ Sums look(const Row& row, int begin, int end, int top
     Sums::add(sums.s, sums.s_low, (s[0] + s[1]) + (s[2] + s[3]));
     Sums::add(sums.t, sums.t_low, (t[0] + t[1]) + (t[2] + t[3]));
   }
-  sums.reduce();
-  // a bound that `top` values reach: `each` of each warp's groups reach that warp's
-  float bound = INFINITY;
-  if (top) {
-    float m[G];
-#pragma unroll
-    for (int u = 0; u < G; ++u) m[u] = most[u];
-    exchange(m[0], m[1]); exchange(m[2], m[3]); exchange(m[0], m[2]); exchange(m[1], m[3]); exchange(m[1], m[2]);
-    bound = largest_but(each, m, lane);
-  }
-  if (W > 1 && lane == 0) { shared.part[warp][0] = sums.most; shared.part[warp][1] = sums.s; shared.part[warp][2] = sums.t; shared.part[warp][3] = bound; }
+  // a bound that `top` values reach: of 64 parts of the row, the top-th largest of their maxima
+  constexpr int kRun = W == 1 ? 32 : W / 2;  // threads of a part
+  float m[2] = {fmaxf(most[0], most[1]), fmaxf(most[2], most[3])};
+  sums.reduce<kRun>(&shared.runs[warp * (32 / kRun)]);
+  if (W > 1 && lane == 0) { shared.part[warp][0] = sums.most; shared.part[warp][1] = sums.s; shared.part[warp][2] = sums.t; }
   if (id == 0) shared.groups = shared.candidates = 0;
   meet<W>();
   if (W > 1) {
     const float4 p = *(const float4*)shared.part[lane < W ? lane : 0];
+    if (top) {
+      m[0] = shared.runs[lane];
+      m[1] = shared.runs[32 + lane];
+    }
     sums = Sums();
     sums.most = p.x;
     sums.ref = fmaxf(p.x, kLowest);
     sums.s = lane < W ? p.y : 0.f;
     sums.t = lane < W ? p.z : 0.f;
     sums.reduce();
-    if (top) {
-      float m[1] = {lane < W ? p.w : -INFINITY};
-      bound = largest_but((top + each - 1) / each, m, lane);  // so many warps are enough
-    }
+  }
+  float bound = sums.most;
+  if (top > 1) {
+    exchange(m[0], m[1]);
+    bound = largest_but(top, m);
   }
   if (!top) return sums;
   bool slow = sums.most != sums.most;
@@ -598,8 +598,8 @@ MTB_API int mtb_token_log_probs_forward_f32(long long n, int v, const float* log
   int ctas = 1;
   const bool many = n > 8LL * mtb_sm_count();
   while (ctas < kMostCtas && n * ctas * 2 <= 6 * mtb_sm_count() && v / (2 * ctas) >= 4096) ctas *= 2;
-  // Otherwise a row by so many warps that there are enough of them under way.  With 8 alternatives by 1, 4 and 8 warps: 16384 x 1000 21, 47, 87 us (an earlier bound); 1184 x 4000
-  // 8.7, 9.4, 11.9; 2368 x 8000 32, 20, 25; 4096 x 30000 125, 94, 101; 1600 x 128000 398, 189, 161; of few rows 592 x 4000 8.6, 8.6, 7.7.
+  // Otherwise a row by so many warps that there are enough of them under way.  With 8 alternatives by 1, 4 and 8 warps (measured with a looser bound): 16384 x 1000 21, 47, 87 us;
+  // 1184 x 4000 8.7, 9.4, 11.9; 2368 x 8000 32, 20, 25; 4096 x 30000 125, 94, 101; 1600 x 128000 398, 189, 161; of few rows 592 x 4000 8.6, 8.6, 7.7.
   if (ctas > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n * ctas));
