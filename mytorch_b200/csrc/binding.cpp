@@ -771,6 +771,11 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (int i = 0; i < 5; ++i)
       if (!from_py(PyTuple_GET_ITEM(group, 1 + i), t.h[i])) return nullptr;
     if ((t.maximize = PyObject_IsTrue(PyTuple_GET_ITEM(group, 6))) < 0) return nullptr;
+    const double most = bits == 8 ? 1 - 0.5 / (1 << 20) : 1;  // betas count with 20 bits there
+    if (!(t.h[0] >= 0 && t.h[1] >= 0 && t.h[1] < most && t.h[2] >= 0 && t.h[2] < most && t.h[3] >= 0 && t.h[4] >= 0)) {  // before any group is updated
+      PyErr_SetString(PyExc_RuntimeError, "AdamW: lr, eps and weight_decay are numbers from 0 up, betas from 0 to below 1, in 8 bits to below 1 - 2^-21");
+      return nullptr;
+    }
     PyObject* params = PyTuple_GET_ITEM(group, 0);
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
       PyObject *param = PyList_GET_ITEM(params, i), *grad = on.look(param, N_grad), *shape;

@@ -359,3 +359,16 @@ def test_what_is_wrong_is_said_before_anything_changes():
         two.state[b]["step"] = two.state[a]["step"]
         with pytest.raises(RuntimeError, match="share a step"):
             two.step()
+        two.state[b]["step"] = mt.tensor(np.ones(1, np.int64), device="cuda:0")
+        before = [g.host(t) for t in (a, b)]
+        for wrong in ({"lr": -1.0}, {"betas": (0.9, 1.0)}, {"eps": float("nan")}, {"betas": (0.9, 1 - 1e-7)}):
+            group = two.param_groups[1]  # the second: the first is not updated either
+            held = dict(group)
+            group.update(wrong)
+            if bits == 32 and wrong == {"betas": (0.9, 1 - 1e-7)}:
+                two.step()
+            else:
+                with pytest.raises(RuntimeError, match="betas from 0 to below 1"):
+                    two.step()
+                assert all(np.array_equal(g.host(t), x) for t, x in zip((a, b), before))
+            group.update(held)
