@@ -762,7 +762,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   std::vector<const float*> grads;
   std::vector<long long> sizes;
   OnDevice on;
-  PyObject* like = nullptr;
+  PyObject *like = nullptr, *last_step = nullptr;  // parameters mostly share their counter: looked at once
+  long long* step = nullptr;
   unsigned ordinal = 0;
   for (Py_ssize_t g = 0; g < groups; ++g) {
     PyObject* group = PyList_GET_ITEM(args[0], g);
@@ -780,13 +781,17 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
       PyObject *param = PyList_GET_ITEM(params, i), *grad = on.look(param, N_grad), *shape;
       float *p, *d;
-      long long size, *step;
+      long long size;
       if (!grad || grad == Py_None || !on.take(param, p, shape) || !on.take_like(grad, d, shape)) Py_RETURN_NONE;
       if (!count_elements(shape, size)) return nullptr;
       PyObject* state = PyDict_GetItemWithError(args[1], param);
       if (PyErr_Occurred()) return nullptr;
       if (!state || !PyDict_Check(state)) Py_RETURN_NONE;
-      if (!take_state(on, state, N_step, g_int64, 1, 0, step)) { if (PyErr_Occurred()) return nullptr; Py_RETURN_NONE; }
+      PyObject* of_step = PyDict_GetItemWithError(state, N_step);
+      if (!of_step || of_step != last_step) {
+        if (!take_state(on, state, N_step, g_int64, 1, 0, step)) { if (PyErr_Occurred()) return nullptr; Py_RETURN_NONE; }
+        last_step = of_step;
+      }
       if (bits == 8) {
         const long long blocks = (size + kMomentBlock - 1) / kMomentBlock;
         unsigned char *codes, *scales;
