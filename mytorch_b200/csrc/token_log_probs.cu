@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __gr
   r.h = a.stats[3 * index + 2];
   r.per_s = 1.f / s;
   r.log_s = logf(s);
-  r.g = !a.dlog_probs || (a.ignores && token == a.ignore_index) ? 0.f : a.dlog_probs[index];
+  r.g = !a.dlog_probs || (a.ignores && token == a.ignore_index) || token < 0 || token >= a.v ? 0.f : a.dlog_probs[index];
   r.gh = a.dentropy ? a.dentropy[index] : 0.f;
   const bool mine = a.dtop && lane < a.top;
   const float extra = mine ? a.dtop[index * a.top + lane] : 0.f;

@@ -21,7 +21,7 @@ def token_log_probs(logits: Tensor, tokens: Tensor, top=0, ignore_index=None) ->
     ones by index, of shape tokens.shape + (top,).  The first three have gradients.
 
     ``ignore_index``: a row with this token has log probability 0 and no gradient from it; entropy and alternatives are those of its logits.  Another token outside [0, V)
-    has log probability NaN.  A logit of -inf is a token that cannot be; a row of nothing else, or with NaN or +inf in it, is NaN, its alternatives in the order of
+    has log probability NaN and no gradient from it either.  A logit of -inf is a token that cannot be; a row of nothing else, or with NaN or +inf in it, is NaN, its alternatives in the order of
     its logits (NaN first)."""
     if len(logits.shape) not in (2, 3) or logits.shape[-1] < 1:
         raise InvalidShapeError(logits.shape)

@@ -156,7 +156,7 @@ def _states(opt, p):
 
 @pytest.mark.parametrize("limit", [None, 0.5], ids=["", "clipped"])
 @pytest.mark.parametrize("offset,size", [(0, 1.0), (1, 1e-6), (0, 1e-17), (3, 1e12)])
-@pytest.mark.parametrize("sizes", [[1], [5, 0, 3], [255], [256], [257, 1, 4099], [1000] * 3, [9000, 7]], ids=lambda s: f"{len(s)}x{s[0]}")
+@pytest.mark.parametrize("sizes", [[1], [5, 0, 3], [255], [256], [257, 1, 4099], [1000] * 3, [9000, 7], [257, 600], [255, 700]], ids=lambda s: f"{len(s)}x{s[0]}")
 def test_8_bits(sizes, offset, size, limit):
     import gpu_util as g
     from mytorch_b200.optim import AdamW
@@ -372,3 +372,39 @@ def test_what_is_wrong_is_said_before_anything_changes():
                     two.step()
                 assert all(np.array_equal(g.host(t), x) for t, x in zip((a, b), before))
             group.update(held)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_tensor_past_32_bits(bits):
+    """The last values of a tensor of more than 2^31, whose other gradients are zero: those of a short one (the roundings of 8 bits know the place modulo 2^32)."""
+    import gpu_util as g
+    import mytorch_b200 as mt
+    from mytorch_b200.backends.cuda.env import CudaEnv, CudaMemoryView
+    from mytorch_b200.optim import AdamW
+
+    n, last = (1 << 31) + 300, 700
+    rng = np.random.default_rng(9)
+    p, grad = (mt.Tensor(shape=(n,), dtype=mt.float32, device="cuda:0", requires_grad=k == 0) for k in range(2))
+    values = [rng.standard_normal(last).astype(np.float32) for _ in range(2)]
+    for t, a in zip((p, grad), values):
+        t.fill_(0)
+        CudaMemoryView(t._native_array, 4 * (n - last), 4 * last, 0).write(a)
+    p.grad = grad
+    opt = AdamW([p], lr=0.01, weight_decay=0.1, state_bits=bits)
+    opt.step()
+    b = (0.9, 0.999) if bits == 32 else tuple(round(x * 2 ** 20) / 2 ** 20 for x in (0.9, 0.999))
+    x = values[1].astype(np.float64)
+    step = 0.01 * x / (np.abs(x) + 1e-8)  # the first step: m / (1 - b1) and v / (1 - b2) are x and x^2
+    want = values[0] * (1 - 0.001) - step
+    got = CudaMemoryView(p._native_array, 4 * (n - last), 4 * last, 0).read((last,), np.float32)
+    assert (np.abs(got - want) <= U * (4 * np.abs(values[0]) + 24 * np.abs(step))).all()
+    if bits == 8:
+        blocks = -(-n // BLOCK)
+        codes = CudaMemoryView(opt.state[p]["moments"]._native_array, (blocks - 4) * 512, 4 * 512, 0).read((4, 512), np.uint8)
+        scales = CudaMemoryView(opt.state[p]["scales"]._native_array, (blocks - 4) * 2, 8, 0).read((4, 2), np.uint8)
+        part = 4 * BLOCK - (blocks * BLOCK - n)  # values of the last four blocks
+        m = _decode(codes, scales, 0, part)[-last:]
+        big = np.abs(m) > 2.0 ** -8 * np.abs(m).max()
+        assert (np.abs(m - (1 - b[0]) * x)[big] <= np.abs((1 - b[0]) * x)[big] / 8).all()
+    del opt, p, grad
+    CudaEnv.instance().lib.pool_trim()

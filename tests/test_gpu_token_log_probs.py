@@ -164,7 +164,6 @@ def _only_ignored(got, tokens, used):
 def test_gradient_against_differences():
     """(f(z + e) - f(z - e)) / 2e in 64 bits of f = sum of w log_probs + q entropy + r top: the formula's error is e^2 / 6 times a third derivative, under 1e-7 here."""
     import gpu_util as g
-    import mytorch_b200 as mt
     import mytorch_b200.nn.functional as F
 
     rng = np.random.default_rng(3)
@@ -188,7 +187,25 @@ def test_gradient_against_differences():
             up[i, j] += e
             down[i, j] -= e
             assert abs((f(up) - f(down)) / (2 * e) - got[i, j]) <= 1e-5
-    assert mt.DAGTracker is not None if hasattr(mt, "DAGTracker") else True
+
+
+def test_rows_without_a_token():
+    """Tokens outside the row have log probability NaN, ignored ones 0; neither has a gradient from it, nor does a token that cannot be have one elsewhere than by p."""
+    import gpu_util as g
+    import mytorch_b200.nn.functional as F
+
+    for v in (9, 2000, 40000):
+        z = np.zeros((6, v), np.float32)
+        z[5, 0] = -np.inf
+        tokens = np.array([0, -1, v, -100, 2 ** 40, 0])
+        x = g.dev(z, True)
+        out = F.token_log_probs(x, g.dev(tokens), ignore_index=-100)
+        got = g.host(out.log_probs)
+        assert np.isfinite(got[0]) and np.isnan(got[[1, 2, 4]]).all() and got[3] == 0 and got[5] == -np.inf
+        ones = g.dev(np.ones(6, np.float32))
+        node = out.log_probs._grad_node
+        dz = g.host(g.op("token_log_probs_backward")(ones, None, None, *node.helpers, x, g.dev(tokens), -100)[0])
+        assert not dz[1:5].any() and abs(dz[0, 0] - (1 - 1 / v)) <= 1e-6 and abs(dz[5, 0] - 1) <= 1e-6 and abs(dz[5, 1] + 1 / (v - 1)) <= 1e-6
 
 
 def test_shapes_strides_and_windows():
