@@ -220,7 +220,10 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads) add_rms_norm_bac
         }
       }
       const long long then = !AHEAD ? -1 : row + 1 < last ? row + 1 : begin + groups < d.stretches ? first_of(begin + groups) : -1;
-      if (!d.dy && then >= 0) fetch_row(then);
+      if (!d.dy && then >= 0) {
+        __syncthreads();  // all values have been read, as below
+        fetch_row(then);
+      }
       if (d.dy) {
         float s = 0;
 #pragma unroll
@@ -236,7 +239,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads) add_rms_norm_bac
           }
         }
         const float mean = sum(s) * per_c;
-        if (then >= 0) fetch_row(then);  // all values have been read
+        if (then >= 0) fetch_row(then);  // all values have been read: the sum has a barrier
 #pragma unroll
         for (int k = 0; k < PER; ++k)
 #pragma unroll

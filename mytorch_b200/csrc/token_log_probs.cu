@@ -167,6 +167,7 @@ __device__ __forceinline__ void meet() {
 template <int W>
 __device__ __forceinline__ void take(const Row& row, int begin, int end, Shared<W>& shared, int groups, int id, float bound, bool above = false) {
   constexpr int T = 32 * W, kStride = kSplit * T;
+  if (groups <= 0) return;
   const int each = (end - begin + kStride - 1) / kStride;  // quads of a group, rounded up
   int g = id / each, k = id - g * each;
   const int step_g = T / each, step_k = T - step_g * each;
