@@ -599,8 +599,9 @@ MTB_API int mtb_token_log_probs_forward_f32(long long n, int v, const float* log
   int ctas = 1;
   const bool many = n > 8LL * mtb_sm_count();
   while (ctas < kMostCtas && n * ctas * 2 <= 6 * mtb_sm_count() && v / (2 * ctas) >= 4096) ctas *= 2;
-  // Otherwise a row by so many warps that there are enough of them under way.  With 8 alternatives by 1, 4 and 8 warps (measured with a looser bound): 16384 x 1000 21, 47, 87 us;
-  // 1184 x 4000 8.7, 9.4, 11.9; 2368 x 8000 32, 20, 25; 4096 x 30000 125, 94, 101; 1600 x 128000 398, 189, 161; of few rows 592 x 4000 8.6, 8.6, 7.7.
+  // Otherwise a row by so many warps that there are enough of them under way, and few as long as the CTAs that an SM holds take turns anyway: then one's search for
+  // alternatives is the others' time for loads.  With 8 alternatives by 1, 4 and 8 warps (measured with a looser bound): 16384 x 1000 21, 47, 87 us; 1184 x 4000 8.7, 9.4, 11.9; of few
+  // rows 592 x 4000 8.6, 8.6, 7.7; by 4 and 8: 4096 x 20000 64, 72; 4096 x 33000 105, 112; 4096 x 50000 152, 162, with 32 alternatives 196, 184; 1600 x 128000 177, 160.
   if (ctas > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n * ctas));
@@ -617,7 +618,7 @@ MTB_API int mtb_token_log_probs_forward_f32(long long n, int v, const float* log
     MTB_CUDA(cudaLaunchKernelEx(&cfg, log_probs_cluster_kernel, a));
   } else if (v <= 1024 || (v <= 4096 && many)) {
     MTB_LAUNCH(log_probs_kernel<1>, (unsigned)mtb_div_up(n, kWarps), kThreads, 0, st, a);
-  } else if (v <= 32768 && many) {
+  } else if ((v <= 32768 && many) || (v <= 65536 && top <= 16 && n >= 25LL * mtb_sm_count())) {
     MTB_LAUNCH(log_probs_kernel<4>, (unsigned)n, 128, 0, st, a);
   } else {
     MTB_LAUNCH(log_probs_kernel<kWarps>, (unsigned)n, kThreads, 0, st, a);
