@@ -504,12 +504,14 @@ Plan forward_plan(long long rows, int c, int align) {
   return n <= 512 ? plan(8, 2) : n <= 1024 ? plan(8, 4) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(8, 32) : plan(0, 0);
 }
 
-// Eight values a thread and tensor.  With post norm and gate, us: 65536 x 300 by 2 warps 101, by 4 107, by 1 (16 values) 121; 32768 x 1024 by 4 135, by 8 136, by 2 138; 32768 x 750 in
-// vectors of two by 4 122, single values 132; 32768 x 1023 by 4 158, by 8 171.
+// Eight values a thread and tensor, four where rows are narrow or would leave many threads idle.  With post norm and gate, us: 65536 x 300 by 3 warps (four values) 106, by 2 112, by 1
+// (16 values) 121; 65536 x 301 by 3 warps 114, by 2 134; 32768 x 1024 by 4 135, by 8 136, by 2 138; 32768 x 750 in vectors of two by 4 122, single values 132; 32768 x 1023 by 4 158, by 8
+// 171.
 Plan backward_plan(int c, int align) {
   const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, n = c / v, sms = mtb_sm_count();
   const auto plan = [&](int per, int warps, int per_sm, bool ahead = false, int lanes = 32) { return Plan{v, per, warps, lanes, warps == 1 ? 256 / lanes : 1, sms * per_sm, ahead}; };
   if (c <= 128) return plan(4 / v, 1, 5, false, c <= 32 ? 8 : c <= 64 ? 16 : 32);
+  if (c > 256 && c <= 384) return plan(4 / v, 3, 14);
   const int per = 8 / v;
   for (const auto [warps, most] : {std::pair{1, 3}, {2, 12}, {4, 6}, {8, 3}, {16, 2}, {32, 1}})
     if (n <= 32 * warps * per) return plan(per, warps, most, v == 4 && warps >= 8);
@@ -596,7 +598,7 @@ MTB_API long long mtb_add_rms_norm_workspace_bytes(long long rows, int c) {
 
 // The kernels that backward_plan names, each as a case of whatever MTB_CASE is.
 #define MTB_OF(V, AHEAD) \
-  MTB_CASE(V, 4 / V, 1, 8, false) MTB_CASE(V, 4 / V, 1, 16, false) MTB_CASE(V, 4 / V, 1, 32, false) MTB_CASE(V, 8 / V, 1, 32, false) MTB_CASE(V, 8 / V, 2, 32, false) \
+  MTB_CASE(V, 4 / V, 1, 8, false) MTB_CASE(V, 4 / V, 1, 16, false) MTB_CASE(V, 4 / V, 1, 32, false) MTB_CASE(V, 8 / V, 1, 32, false) MTB_CASE(V, 4 / V, 3, 32, false) MTB_CASE(V, 8 / V, 2, 32, false) \
   MTB_CASE(V, 8 / V, 4, 32, false) MTB_CASE(V, 8 / V, 8, 32, AHEAD) MTB_CASE(V, 8 / V, 16, 32, AHEAD) MTB_CASE(V, 8 / V, 32, 32, AHEAD)
 #define MTB_KERNELS MTB_OF(4, true) MTB_OF(2, false) MTB_OF(1, false)
 
