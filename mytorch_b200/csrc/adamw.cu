@@ -189,23 +189,17 @@ __device__ __forceinline__ float first_bits(unsigned w) { return __uint_as_float
 template <int B>
 __device__ __forceinline__ float second_bits(unsigned w) { return __uint_as_float((B == 3 ? w >> 4 : w << (20 - 8 * B)) & 0x0FF00000u); }
 
-// Powers of two by which such a float is multiplied to be what the code stands for, or the other way, in two products where one power does not fit a float32.
+// Power of two by which such a float is multiplied to be what the code stands for, or the other way; two products where one power does not fit a float32, which is
+// the same for all of a block.  A scale of 0 stands for zeros, whatever they are multiplied by.
 struct Powers {
-  float one, other;
-  bool two;
+  unsigned scale;
+  int by;  // in one product: 2^(scale - 127 + by), or 2^(127 - scale - by)
 
-  static __device__ __forceinline__ Powers decode(unsigned scale, int up) {  // 2^up unit
-    const bool two = scale + up > 253;
-    const float unit = unit_of(scale), power = __uint_as_float((unsigned)(127 + up) << 23);
-    return Powers{two ? power : power * unit, unit, two};
-  }
-  static __device__ __forceinline__ Powers encode(unsigned scale, int down) {  // 2^-down / unit
-    const bool two = scale + down > 253;
-    const float per = per_unit(scale), power = __uint_as_float((unsigned)(127 - down) << 23);
-    return Powers{two ? per : per * power, power, two};
-  }
-  __device__ __forceinline__ float operator()(float x) const { return x * one; }
-  __device__ __forceinline__ float again(float x) const { return x * other; }
+  __device__ __forceinline__ bool two() const { return scale + by > 253; }
+  __device__ __forceinline__ float up() const { return __uint_as_float((scale + by) << 23); }
+  __device__ __forceinline__ float down() const { return __uint_as_float((254u - scale - by) << 23); }
+  __device__ __forceinline__ float up_twice(float x) const { return x * __uint_as_float((unsigned)(127 + by) << 23) * unit_of(scale); }
+  __device__ __forceinline__ float down_twice(float x) const { return x * per_unit(scale) * __uint_as_float((unsigned)(127 - by) << 23); }
 };
 constexpr int kFirst = 113, kSecond = 97;  // the highest exponents, 15 and 31 in a float32, are that of twice the unit
 
@@ -256,12 +250,14 @@ struct Lane {
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = second ? second_bits<0>(w[j]) : first_bits<0>(w[j]);
     }
-    const Powers power = Powers::decode(scale, second ? kSecond : kFirst);
+    const Powers power{scale, second ? kSecond : kFirst};
+    if (power.two()) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = power(x[j]);
-    if (power.two) {
+      for (int j = 0; j < 8; ++j) x[j] = power.up_twice(x[j]);
+    } else {
+      const float up = power.up();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = power.again(x[j]);
+      for (int j = 0; j < 8; ++j) x[j] *= up;
     }
   }
   // t: codes above 20 bits of fraction; signs: values with the codes' signs, or NULL.
@@ -341,20 +337,23 @@ __device__ __forceinline__ void update_block(const Lane<VECTORS> l, float* p, co
   const unsigned scale_m = scale_of(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_m))));
   const unsigned scale_v = scale_of(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most_v))));
   // To codes with 20 bits of fraction, of which 16 are compared with a random number: it and a half are added.
-  const Powers to_m = Powers::encode(scale_m, kFirst), to_v = Powers::encode(scale_v, kSecond);
+  const Powers to_m{scale_m, kFirst}, to_v{scale_v, kSecond};
   float x[8], y[8];
+  if (to_m.two()) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] = to_m(fabsf(m[j]));
-    y[j] = to_v(v[j]);
+    for (int j = 0; j < 8; ++j) x[j] = to_m.down_twice(fabsf(m[j]));
+  } else {
+    const float down = to_m.down();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = fabsf(m[j]) * down;
   }
-  if (to_m.two) {
+  if (to_v.two()) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = to_m.again(x[j]);
-  }
-  if (to_v.two) {
+    for (int j = 0; j < 8; ++j) y[j] = to_v.down_twice(v[j]);
+  } else {
+    const float down = to_v.down();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = to_v.again(y[j]);
+    for (int j = 0; j < 8; ++j) y[j] = v[j] * down;
   }
   key = mix(key + c.t) + (first + l.at(0)) * kGolden;
   bool zero = false;

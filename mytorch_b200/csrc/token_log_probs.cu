@@ -77,11 +77,12 @@ struct Sums {
     ref = r;
   }
   // Over the warp, in all its lanes.  RUN: to `runs` the largest value of each run of so many lanes.
-  template <int RUN = 32>
+  // LANES: over each of so many, which hold the same as the others.
+  template <int RUN = 32, int LANES = 32>
   __device__ __forceinline__ void reduce(float* runs = nullptr) {
     float to = most;
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
+    for (int o = 1; o < LANES; o *= 2) {
       if (RUN < 32 && o == RUN && (threadIdx.x & (RUN - 1)) == 0) runs[(threadIdx.x & 31) / RUN] = to;
       to = max_nan(to, __shfl_xor_sync(0xFFFFFFFFu, to, o));
     }
@@ -90,7 +91,7 @@ struct Sums {
     t += t_low;
     s_low = t_low = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = LANES / 2; o > 0; o >>= 1) {
       s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
       t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
     }
@@ -281,7 +282,7 @@ __device__ __forceinline__ Sums look(const Row& row, int begin, int end, int top
   if (id == 0) shared.groups = shared.candidates = 0;
   meet<W>();
   if (W > 1) {
-    const float4 p = *(const float4*)shared.part[lane < W ? lane : 0];
+    const float4 p = *(const float4*)shared.part[lane % W];
     if (top) {
       m[0] = shared.runs[lane];
       m[1] = shared.runs[32 + lane];
@@ -289,9 +290,9 @@ __device__ __forceinline__ Sums look(const Row& row, int begin, int end, int top
     sums = Sums();
     sums.most = p.x;
     sums.ref = fmaxf(p.x, kLowest);
-    sums.s = lane < W ? p.y : 0.f;
-    sums.t = lane < W ? p.z : 0.f;
-    sums.reduce();
+    sums.s = p.y;
+    sums.t = p.z;
+    sums.reduce<32, W>();
   }
   float bound = sums.most;
   if (top > 1) {
