@@ -333,21 +333,22 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads) add_rms_norm_bac
   }
 }
 
-// Sums over rows of scratch.  The first CTAs add up three rows of c columns, 32 columns a CTA by eight lanes each: dweight, dpost_weight, the gate that all rows share; the others
-// the gate's rows from their stretches', a column a thread.
+// Sums over rows of scratch.  The first CTAs add up three rows of c columns, 32 columns a CTA by 32 warps: dweight, dpost_weight, the gate that all rows share; the others
+// the gate's rows from their stretches', a column a thread.  Latency bounds it: by eight warps a CTA the gradient of 32768 x 1024 takes 140 us instead of 135, of 65536 x 300 106 instead of 97.
 struct Columns {
   const float *partial, *gate_rows;
   float *dweight, *dpost_weight, *dgate;
   int rows, c, blocks;  // CTAs of one of the three
   int parts, gates;     // gates 0: one that all rows share
 };
-__global__ void __launch_bounds__(256) add_rms_norm_columns_kernel(const __grid_constant__ Columns t) {
-  __shared__ float part[8][33];
+constexpr int kColumnThreads = 1024, kColumnWarps = kColumnThreads / 32;
+__global__ void __launch_bounds__(kColumnThreads) add_rms_norm_columns_kernel(const __grid_constant__ Columns t) {
+  __shared__ float part[kColumnWarps][33];
   mtb_wait_prior();
   const int c = t.c;
   if ((int)blockIdx.x >= 3 * t.blocks) {
-    const long long count = (long long)t.gates * c, step = (gridDim.x - 3LL * t.blocks) * 256;
-    for (long long n = (blockIdx.x - 3LL * t.blocks) * 256 + threadIdx.x; n < count; n += step) {
+    const long long count = (long long)t.gates * c, step = (gridDim.x - 3LL * t.blocks) * kColumnThreads;
+    for (long long n = (blockIdx.x - 3LL * t.blocks) * kColumnThreads + threadIdx.x; n < count; n += step) {
       const float* from = t.gate_rows + n / c * (t.parts - 1) * c + n;
       float s = 0;
 #pragma unroll 8
@@ -364,20 +365,20 @@ __global__ void __launch_bounds__(256) add_rms_norm_columns_kernel(const __grid_
   float s[4] = {0, 0, 0, 0};
   if (i < c) {
     int r = row;
-    for (; r + 24 < t.rows; r += 32) {
+    for (; r + 3 * kColumnWarps < t.rows; r += 4 * kColumnWarps) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s[u] += from[(r + 8 * u) * stride];
+      for (int u = 0; u < 4; ++u) s[u] += from[(r + kColumnWarps * u) * stride];
     }
-    for (; r < t.rows; r += 8) s[0] += from[r * stride];
+    for (; r < t.rows; r += kColumnWarps) s[0] += from[r * stride];
   }
   part[row][lane] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
-  if (row == 0 && i < c) {
-    float x = 0;
+  // a warp a column: 32 of them, one value a lane
+  float x = part[lane][row];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x += part[k][lane];
-    out[i] = x;
-  }
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  const int column = i - lane + row;
+  if (lane == 0 && column < c) out[column] = x;
 }
 
 // ------------------------------------------------------------------ rows that no group holds: through memory, a CTA a row
@@ -504,7 +505,7 @@ Plan forward_plan(long long rows, int c, int align) {
   return n <= 512 ? plan(8, 2) : n <= 1024 ? plan(8, 4) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(8, 32) : plan(0, 0);
 }
 
-// Eight values a thread and tensor, four where rows are narrow or would leave many threads idle.  With post norm and gate, us: 65536 x 300 by 3 warps (four values) 106, by 2 112, by 1
+// Eight values a thread and tensor, four where rows are narrow or would leave many threads idle.  With post norm and gate, us (with slower sums over CTAs than now): 65536 x 300 by 3 warps (four values) 106, by 2 112, by 1
 // (16 values) 121; 65536 x 301 by 3 warps 114, by 2 134; 32768 x 1024 by 4 135, by 8 136, by 2 138; 32768 x 750 in vectors of two by 4 122, single values 132; 32768 x 1023 by 4 158, by 8
 // 171.
 Plan backward_plan(int c, int align) {
@@ -652,7 +653,7 @@ MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dn
   if (dweight || dpost_weight || shared_gate || by_parts) {
     const long long gates = by_parts ? rows / rows_per_gate : 0;
     const Columns t{partial, gate_rows, dweight, dpost_weight, shared_gate || by_parts ? dgate : nullptr, s.ctas, c, mtb_div_up(c, 32), (int)s.parts, (int)gates};
-    MTB_LAUNCH(add_rms_norm_columns_kernel, 3 * t.blocks + (by_parts ? mtb_stream_grid(gates * c, 256) : 0), 256, 0, st, t);
+    MTB_LAUNCH(add_rms_norm_columns_kernel, 3 * t.blocks + (by_parts ? mtb_stream_grid(gates * c, kColumnThreads, 2) : 0), kColumnThreads, 0, st, t);
     MTB_LAUNCH_CHECK("add_rms_norm_columns_kernel");
   }
   return MTB_OK;
