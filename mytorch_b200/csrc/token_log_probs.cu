@@ -456,14 +456,18 @@ __global__ void __launch_bounds__(W == 1 ? kThreads : 32 * W) log_probs_kernel(c
   leave(a, index, id, given, sums, found[part]);
 }
 
-// A row by a cluster of CTAs, each of which finds the alternatives of its part; the first puts them together.
+// A row by a cluster of CTAs, each of which finds the alternatives of its part; the first puts them together.  Its shared memory is there for the others once it has started: each
+// arrives first of all and waits for the others before it writes to it.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 __global__ void __launch_bounds__(kThreads) log_probs_cluster_kernel(const __grid_constant__ Forward a) {
   __shared__ Shared<kWarps> shared;
   __shared__ Key found[kMostTop], all[kMostCtas][kMostTop];
   __shared__ float parts[kMostCtas][3];
   mtb_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // the first CTA's shared memory is there once it has started
+  cluster_arrive();
   mtb_wait_prior();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const long long index = blockIdx.x / ctas;
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(kThreads) log_probs_cluster_kernel(const __gri
   const int each = (row.quads + ctas - 1) / ctas, begin = rank * each < row.quads ? rank * each : row.quads, end = begin + each < row.quads ? begin + each : row.quads;
   Given given(a, index, rank == 0 ? threadIdx.x : 1);
   const Sums mine = look<kWarps>(row, begin, end, a.top, shared, found, [&] { given(); });
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  cluster_wait();
   if (a.top && threadIdx.x < kMostTop) cluster.map_shared_rank(&all[0][0], 0)[rank * kMostTop + threadIdx.x] = threadIdx.x < a.top ? found[threadIdx.x] : 0;
   if (threadIdx.x == 0) {
     float* to = cluster.map_shared_rank(&parts[0][0], 0) + 3 * rank;
