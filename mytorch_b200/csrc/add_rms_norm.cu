@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads) add_rms_norm_bac
         if (i < c) {
           VecF<V> r;
 #pragma unroll
-          for (int j = 0; j < V; ++j) r.v[j] = rb * (D[k].v[j] - b[k].v[j] * mean);
+          for (int j = 0; j < V; ++j) r.v[j] = a.post_weight ? rb * (D[k].v[j] - b[k].v[j] * mean) : D[k].v[j];  // of an infinite block too
           store<V>(d.dblock + at + i, r);
         }
       }
@@ -444,8 +444,8 @@ __global__ void __launch_bounds__(kLongThreads) add_rms_norm_backward_long_kerne
       for (int i = threadIdx.x; d.dy && i < c; i += kLongThreads) s += d.dy[at + i] * (a.weight ? a.weight[i] : 1.f) * a.x[at + i] * rho;
       const float c1 = over_cta(s, shared) / c;
       const auto total = [&](int i) {
-        const float u = d.dy ? d.dy[at + i] * (a.weight ? a.weight[i] : 1.f) : 0.f;
-        return (d.dnew ? d.dnew[at + i] : 0.f) + rho * (u - a.x[at + i] * rho * c1);
+        const float D = d.dnew ? d.dnew[at + i] : 0.f;
+        return d.dy ? D + rho * (d.dy[at + i] * (a.weight ? a.weight[i] : 1.f) - a.x[at + i] * rho * c1) : D;
       };
       float c2 = 0;
       if (a.block && a.post_weight) {
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kLongThreads) add_rms_norm_backward_long_kerne
           float* to = d.gate_rows + (d.gate_each ? at : stretch * c) + i;
           *to = d.gate_each || row == first ? each : *to + each;
         }
-        if (d.dblock) d.dblock[at + i] = rb * (dinner * w - hat * c2);
+        if (d.dblock) d.dblock[at + i] = a.post_weight ? rb * (dinner * w - hat * c2) : dinner;
       }
     }
   }

@@ -248,6 +248,24 @@ def test_rows_of_zeros_and_of_no_numbers():
         assert np.isfinite(np.delete(new[1], c // 2)).all()
 
 
+@pytest.mark.parametrize("gate", [None, "channel", "sample", "full"])
+@pytest.mark.parametrize("c", [5, 64, 130, 1000, 4096, 20000])
+def test_gradient_of_the_sum_alone_beside_infinite_values(c, gate):
+    """Without a norm the sum's gradient does not know the block's values but in the gate's: those of the operands are finite, and products of at most two numbers."""
+    import gpu_util as g
+    import mytorch_b200.nn.functional as F
+
+    a = _inputs((3, c), False, gate)
+    a["block"][:, c // 2], a["residual"][1, c // 3] = np.inf, -np.inf
+    t = {k: g.dev(v, k in ("residual", "block")) for k, v in a.items()}
+    new, _ = F.add_rms_norm(t["residual"], t["block"], t["weight"], None, t.get("gate"), 0.5, EPS)
+    (new * g.dev(a["dnew"])).reshape((3 * c,)).sum().backward()
+    gr = _gate_rows(a, (3, c), c, gate)
+    for name, factor in (("residual", 0.5), ("block", gr)):
+        want = a["dnew"].astype(np.float64) * factor
+        assert (np.abs(g.host(t[name].grad) - want) <= U * np.abs(want)).all()
+
+
 def test_no_rows():
     import gpu_util as g
     import mytorch_b200.nn.functional as F
