@@ -491,7 +491,8 @@ int resident(K kernel, int threads, int smem, int* known) {
 
 // Vectors of four, of two where rows or operands begin at 8 bytes, else single values; as few warps a row as hold it.  Of few rows eight warps a row.
 // Measured with post norm and gate, us: 65536 x 256 by 1 warp 46, by 2 45, by 4 72; 32768 x 1024 by 1 98, by 2 93, by 4 93, by 8 102; 8192 x 4096 by 8 98, by 16 95, by
-// 32 164; in vectors of two 32768 x 750 by 2 warps 74, by 4 70, by 8 92, in single values 78; 32768 x 1023 by 4 107, by 8 111, by 16 198.
+// 32 164; in vectors of two 32768 x 750 by 2 warps 74, by 4 70, by 8 92, in single values 78; 32768 x 1023 by 4 107, by 8 111, by 16 198; 16384 x 1535 by 8 with eight a
+// thread 87, with six 77; 4096 x 8185 by 32 180, by 16 with sixteen a thread 147.
 Plan forward_plan(long long rows, int c, int align) {
   const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, n = c / v;
   const auto plan = [&](int per, int warps, int lanes = 32) { return Plan{v, per, warps, lanes, warps == 1 ? 256 / lanes : 1, 0, false}; };
@@ -502,18 +503,21 @@ Plan forward_plan(long long rows, int c, int align) {
   if (c <= 256) return plan(8 / v, 1);
   if (v == 4) return n <= 128 ? plan(4, 1) : n <= 256 ? plan(8, 2) : n <= 512 ? plan(2, 8) : n <= 1024 ? plan(2, 16) : n <= 2048 ? plan(4, 16) : n <= 4096 ? plan(4, 32) : plan(0, 0);
   if (v == 2) return n <= 256 ? plan(4, 2) : n <= 512 ? plan(4, 4) : n <= 1024 ? plan(8, 4) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(8, 32) : plan(0, 0);
-  return n <= 512 ? plan(8, 2) : n <= 1024 ? plan(8, 4) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(8, 32) : plan(0, 0);
+  return n <= 512 ? plan(8, 2) : n <= 1024 ? plan(8, 4) : n <= 1536 ? plan(6, 8) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(16, 16) : plan(0, 0);
 }
 
-// Eight values a thread and tensor, four where rows are narrow or would leave many threads idle.  With post norm and gate, us (with slower sums over CTAs than now): 65536 x 300 by 3 warps (four values) 106, by 2 112, by 1
+// Eight values a thread and tensor, four where rows are narrow, and four or six where eight would leave many threads idle.  With post norm and gate, us (with slower sums over CTAs than now): 65536 x 300 by 3 warps (four values) 106, by 2 112, by 1
 // (16 values) 121; 65536 x 301 by 3 warps 114, by 2 134; 32768 x 1024 by 4 135, by 8 136, by 2 138; 32768 x 750 in vectors of two by 4 122, single values 132; 32768 x 1023 by 4 158, by 8
-// 171.
+// 171; 8192 x 3001 by 16 with eight a thread 173, with six 157.
 Plan backward_plan(int c, int align) {
   const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, n = c / v, sms = mtb_sm_count();
   const auto plan = [&](int per, int warps, int per_sm, bool ahead = false, int lanes = 32) { return Plan{v, per, warps, lanes, warps == 1 ? 256 / lanes : 1, sms * per_sm, ahead}; };
   if (c <= 128) return plan(4 / v, 1, 5, false, c <= 32 ? 8 : c <= 64 ? 16 : 32);
   if (c > 256 && c <= 384) return plan(4 / v, 3, 14);
   const int per = 8 / v;
+  if (v != 4)
+    for (const int warps : {8, 16})
+      if (n > 32 * warps / 2 * per && n <= 32 * warps * (6 / v)) return plan(6 / v, warps, warps == 8 ? 3 : 2);
   for (const auto [warps, most] : {std::pair{1, 3}, {2, 12}, {4, 6}, {8, 3}, {16, 2}, {32, 1}})
     if (n <= 32 * warps * per) return plan(per, warps, most, v == 4 && warps >= 8);
   return plan(0, 0, 1);
@@ -575,7 +579,7 @@ MTB_API int mtb_add_rms_norm_forward_f32(long long rows, int c, const float* res
 #define MTB_WIDE(PER, W) MTB_CASE(2, PER, W, 32) MTB_CASE(1, PER, W, 32)
   MTB_NARROW(4) MTB_NARROW(2) MTB_NARROW(1) MTB_ALL(1, 8) MTB_ALL(2, 8) MTB_ALL(4, 8)
   MTB_CASE(4, 4, 1, 32) MTB_CASE(4, 8, 2, 32) MTB_CASE(4, 2, 16, 32) MTB_CASE(4, 4, 16, 32) MTB_CASE(4, 4, 32, 32)
-  MTB_CASE(2, 4, 2, 32) MTB_CASE(2, 4, 4, 32) MTB_CASE(1, 8, 2, 32) MTB_WIDE(8, 4) MTB_WIDE(8, 8) MTB_WIDE(8, 16) MTB_WIDE(8, 32) {
+  MTB_CASE(2, 4, 2, 32) MTB_CASE(2, 4, 4, 32) MTB_CASE(1, 8, 2, 32) MTB_WIDE(8, 4) MTB_WIDE(8, 8) MTB_WIDE(8, 16) MTB_CASE(2, 8, 32, 32) MTB_CASE(1, 6, 8, 32) MTB_CASE(1, 16, 16, 32) {
     MTB_LAUNCH(add_rms_norm_long_kernel, (unsigned)rows, kLongThreads, 0, st, a, out, y, rstd, block_rstd);
   }
 #undef MTB_WIDE
@@ -601,7 +605,8 @@ MTB_API long long mtb_add_rms_norm_workspace_bytes(long long rows, int c) {
 #define MTB_OF(V, AHEAD) \
   MTB_CASE(V, 4 / V, 1, 8, false) MTB_CASE(V, 4 / V, 1, 16, false) MTB_CASE(V, 4 / V, 1, 32, false) MTB_CASE(V, 8 / V, 1, 32, false) MTB_CASE(V, 4 / V, 3, 32, false) MTB_CASE(V, 8 / V, 2, 32, false) \
   MTB_CASE(V, 8 / V, 4, 32, false) MTB_CASE(V, 8 / V, 8, 32, AHEAD) MTB_CASE(V, 8 / V, 16, 32, AHEAD) MTB_CASE(V, 8 / V, 32, 32, AHEAD)
-#define MTB_KERNELS MTB_OF(4, true) MTB_OF(2, false) MTB_OF(1, false)
+#define MTB_SIX(V) MTB_CASE(V, 6 / V, 8, 32, false) MTB_CASE(V, 6 / V, 16, 32, false)
+#define MTB_KERNELS MTB_OF(4, true) MTB_OF(2, false) MTB_OF(1, false) MTB_SIX(2) MTB_SIX(1)
 
 MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dnew, const float* dy, const float* x, const float* rstd, const float* block,
                                           const float* block_rstd, const float* weight, const float* post_weight, const float* gate, long long rows_per_gate, double scale,
