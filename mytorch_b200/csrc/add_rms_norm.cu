@@ -8,8 +8,6 @@
 // Bound by memory: 16 bytes a value forward, 24 backward, each once, if a row stays in registers between its sums and what is made of them.  So a group of W warps holds
 // a row, PER vectors a thread and tensor, and goes on to its next one; W is 1 where a row fits a warp, which then waits for no other, and narrow rows lie side by side in
 // a warp, LANES lanes each.
-#include <utility>
-
 #include "colreduce.cuh"
 
 namespace {
@@ -160,8 +158,13 @@ struct Gradients {
 
 // AHEAD: the next row's values come to shared memory meanwhile.  That pays where many warps wait for one another at a row's sums (16384 x 2048 with post norm and gate 153 -> 136 us,
 // 8192 x 4096 167 -> 142), not where rows of other groups are under way on the SM (32768 x 1024 135 -> 146), nor by copies of 4 bytes (32768 x 1023 158 -> 215).
+// Where it is not 0: registers for so many on an SM; what else the compiler takes leaves a third of the warps (32768 x 750 by six values a thread and 4 warps 125 -> 111 us,
+// 12672 x 2601 by eight and 12 warps 302 -> 207), but for kernels that would then spill (16384 x 2047 by eight and 8 warps 171 -> 190).
+template <int V, int PER, int W, int LANES>
+constexpr int kBackwardCtas = V * PER == 6 ? (W == 1 ? 3 : 24 / W) : W == 24 ? 1 : V != 4 && W == 12 ? 2 : V != 4 && V * PER == 4 && W == 1 && LANES == 32 ? 4 : 0;
+
 template <int V, int PER, int W, int LANES, bool AHEAD>
-__global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads) add_rms_norm_backward_kernel(const __grid_constant__ Operands a, const __grid_constant__ Gradients d) {
+__global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V, PER, W, LANES>) add_rms_norm_backward_kernel(const __grid_constant__ Operands a, const __grid_constant__ Gradients d) {
   constexpr int kGroups = GroupSum<W, LANES>::kGroups, kShare = GroupSum<W, LANES>::kShare;
   extern __shared__ __align__(16) float shared[];  // AHEAD: [x, dy, dnew, block][PER][thread][V]; W 1: [3][c]
   __shared__ float part[2][W];
@@ -489,38 +492,46 @@ int resident(K kernel, int threads, int smem, int* known) {
   return *known > 0 ? *known : 1;
 }
 
-// Vectors of four, of two where rows or operands begin at 8 bytes, else single values; as few warps a row as hold it.  Of few rows eight warps a row.
-// Measured with post norm and gate, us: 65536 x 256 by 1 warp 46, by 2 45, by 4 72; 32768 x 1024 by 1 98, by 2 93, by 4 93, by 8 102; 8192 x 4096 by 8 98, by 16 95, by
-// 32 164; in vectors of two 32768 x 750 by 2 warps 74, by 4 70, by 8 92, in single values 78; 32768 x 1023 by 4 107, by 8 111, by 16 198; 16384 x 1535 by 8 with eight a
-// thread 87, with six 77; 4096 x 8185 by 32 180, by 16 with sixteen a thread 147.
+// What holds a row: values a thread and tensor, warps.  Taken is the first of a table that is large enough.
+struct Share {
+  int values, warps;
+};
+template <int N>
+Share share_of(const Share (&table)[N], int c) {
+  for (const Share s : table)
+    if (c <= 32 * s.warps * s.values) return s;
+  return Share{0, 0};
+}
+
+// Vectors of four, of two where rows or operands begin at 8 bytes, else single values; the smallest group that holds a row, of few values a thread, so that other rows are under
+// way meanwhile.  Of few rows eight warps a row.  Measured with post norm and gate, us: 33 million values in rows of 256 by 1 warp 93, by 2 with four values 86, but of 192 90 and 106;
+// of 520 by 3 92, by 2 with 32 values 131; of 1200 by 5 85, by 8 110; of 2400 by 10 85, by 16 124; of 4096 by 8 98, by 16 95, by 32 164; in vectors of two, of 750 by 3 86, by 4 93; in
+// single values, of 575 by 3 with six 96, by 4 with eight 118; of 2301 by 10 112, by 16 143; of 8185 by 16 with sixteen values 147, by 32 with eight 180.
+constexpr Share kForwardSharesOfFour[] = {{8, 1}, {16, 1}, {8, 3}, {8, 4}, {8, 5}, {8, 6}, {8, 8}, {8, 10}, {8, 12}, {8, 16}, {16, 16}, {16, 32}};
+constexpr Share kForwardShares[] = {{8, 1}, {6, 2}, {8, 2}, {6, 3}, {8, 3}, {8, 4}, {8, 5}, {8, 6}, {8, 8}, {8, 10}, {8, 12}, {8, 16}, {16, 16}, {16, 32}};
 Plan forward_plan(long long rows, int c, int align) {
-  const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, n = c / v;
+  const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1;
   const auto plan = [&](int per, int warps, int lanes = 32) { return Plan{v, per, warps, lanes, warps == 1 ? 256 / lanes : 1, 0, false}; };
   if (rows <= 8LL * mtb_sm_count() && c > 256)
     for (const int per : {1, 2, 4})
-      if (n <= 256 * per) return plan(per, 8);
+      if (c <= 256 * per * v) return plan(per, 8);
   if (c <= 128) return plan(4 / v, 1, c <= 32 ? 8 : c <= 64 ? 16 : 32);
-  if (c <= 256) return plan(8 / v, 1);
-  if (v == 4) return n <= 128 ? plan(4, 1) : n <= 256 ? plan(8, 2) : n <= 512 ? plan(2, 8) : n <= 1024 ? plan(2, 16) : n <= 2048 ? plan(4, 16) : n <= 4096 ? plan(4, 32) : plan(0, 0);
-  if (v == 2) return n <= 256 ? plan(4, 2) : n <= 512 ? plan(4, 4) : n <= 1024 ? plan(8, 4) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(8, 32) : plan(0, 0);
-  return n <= 512 ? plan(8, 2) : n <= 1024 ? plan(8, 4) : n <= 1536 ? plan(6, 8) : n <= 2048 ? plan(8, 8) : n <= 4096 ? plan(8, 16) : n <= 8192 ? plan(16, 16) : plan(0, 0);
+  const Share s = v == 4 ? share_of(kForwardSharesOfFour, c) : share_of(kForwardShares, c);
+  return plan(s.values / v, s.warps);
 }
 
-// Eight values a thread and tensor, four where rows are narrow, and four or six where eight would leave many threads idle.  With post norm and gate, us (with slower sums over CTAs than now): 65536 x 300 by 3 warps (four values) 106, by 2 112, by 1
-// (16 values) 121; 65536 x 301 by 3 warps 114, by 2 134; 32768 x 1024 by 4 135, by 8 136, by 2 138; 32768 x 750 in vectors of two by 4 122, single values 132; 32768 x 1023 by 4 158, by 8
-// 171; 8192 x 3001 by 16 with eight a thread 173, with six 157.
+// The smallest group that holds a row: what idles costs as what works does.  With post norm and gate, us: 65536 x 300 by 3 warps with four values a thread 98, by 2 with
+// eight 104; 43840 x 752 by 3 with eight 141, by 4 155; 13696 x 2400 by 12 151, by 16 176; 5440 x 6000 by 24 162, by 32 216; in single values 65536 x 575 by 3 with six 179, by 4
+// with eight 220; 27456 x 1201 by 5 158, by 8 with six 183, with eight 217; 8192 x 4601 by 24 with six 271, by 32 with eight 383.  Not in between: 22720 x 1450 in vectors of two by 12
+// with six 194, by 8 with six 156.
+constexpr Share kSharesOfFour[] = {{4, 2}, {4, 3}, {8, 2}, {8, 3}, {8, 4}, {8, 5}, {8, 8}, {8, 12}, {8, 16}, {8, 24}, {8, 32}};
+constexpr Share kShares[] = {{6, 1}, {4, 2}, {4, 3}, {8, 2}, {6, 3}, {6, 4}, {8, 4}, {8, 5}, {6, 8}, {8, 8}, {6, 12}, {8, 10}, {8, 12}, {8, 16}, {6, 24}, {8, 24}, {8, 32}};
 Plan backward_plan(int c, int align) {
-  const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, n = c / v, sms = mtb_sm_count();
+  const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, sms = mtb_sm_count();
   const auto plan = [&](int per, int warps, int per_sm, bool ahead = false, int lanes = 32) { return Plan{v, per, warps, lanes, warps == 1 ? 256 / lanes : 1, sms * per_sm, ahead}; };
   if (c <= 128) return plan(4 / v, 1, 5, false, c <= 32 ? 8 : c <= 64 ? 16 : 32);
-  if (c > 256 && c <= 384) return plan(4 / v, 3, 14);
-  const int per = 8 / v;
-  if (v != 4)
-    for (const int warps : {8, 16})
-      if (n > 32 * warps / 2 * per && n <= 32 * warps * (6 / v)) return plan(6 / v, warps, warps == 8 ? 3 : 2);
-  for (const auto [warps, most] : {std::pair{1, 3}, {2, 12}, {4, 6}, {8, 3}, {16, 2}, {32, 1}})
-    if (n <= 32 * warps * per) return plan(per, warps, most, v == 4 && warps >= 8);
-  return plan(0, 0, 1);
+  const Share s = v == 4 ? share_of(kSharesOfFour, c) : share_of(kShares, c);
+  return s.warps ? plan(s.values / v, s.warps, s.warps == 1 ? 3 : 32 / s.warps, v == 4 && s.warps >= 8) : plan(0, 0, 1);
 }
 
 // How rows come in stretches (see Gradients): as many as there are groups, or more where the gate has more rows.
@@ -574,17 +585,17 @@ MTB_API int mtb_add_rms_norm_forward_f32(long long rows, int c, const float* res
     const long long most = (long long)mtb_sm_count() * resident(add_rms_norm_kernel<V, PER, W, LANES>, GroupSum<W>::kThreads, 0, &known); \
     MTB_LAUNCH((add_rms_norm_kernel<V, PER, W, LANES>), (unsigned)(needed < most ? needed : most), GroupSum<W>::kThreads, 0, st, a, out, y, rstd, block_rstd); \
   } else
-#define MTB_ALL(PER, W) MTB_CASE(4, PER, W, 32) MTB_CASE(2, PER, W, 32) MTB_CASE(1, PER, W, 32)
-#define MTB_NARROW(V) MTB_CASE(V, 4 / V, 1, 8) MTB_CASE(V, 4 / V, 1, 16) MTB_CASE(V, 4 / V, 1, 32) MTB_CASE(V, 8 / V, 1, 32)
-#define MTB_WIDE(PER, W) MTB_CASE(2, PER, W, 32) MTB_CASE(1, PER, W, 32)
-  MTB_NARROW(4) MTB_NARROW(2) MTB_NARROW(1) MTB_ALL(1, 8) MTB_ALL(2, 8) MTB_ALL(4, 8)
-  MTB_CASE(4, 4, 1, 32) MTB_CASE(4, 8, 2, 32) MTB_CASE(4, 2, 16, 32) MTB_CASE(4, 4, 16, 32) MTB_CASE(4, 4, 32, 32)
-  MTB_CASE(2, 4, 2, 32) MTB_CASE(2, 4, 4, 32) MTB_CASE(1, 8, 2, 32) MTB_WIDE(8, 4) MTB_WIDE(8, 8) MTB_WIDE(8, 16) MTB_CASE(2, 8, 32, 32) MTB_CASE(1, 6, 8, 32) MTB_CASE(1, 16, 16, 32) {
+#define MTB_EIGHT(V, W) MTB_CASE(V, 8 / V, W, 32)
+#define MTB_OF(V) \
+  MTB_CASE(V, 4 / V, 1, 8) MTB_CASE(V, 4 / V, 1, 16) MTB_CASE(V, 4 / V, 1, 32) MTB_EIGHT(V, 1) MTB_EIGHT(V, 3) MTB_EIGHT(V, 4) MTB_EIGHT(V, 5) MTB_EIGHT(V, 6) MTB_EIGHT(V, 8) MTB_EIGHT(V, 10) \
+  MTB_EIGHT(V, 12) MTB_EIGHT(V, 16) MTB_CASE(V, 16 / V, 16, 32) MTB_CASE(V, 16 / V, 32, 32) MTB_CASE(V, 1, 8, 32) MTB_CASE(V, 2, 8, 32) MTB_CASE(V, 4, 8, 32)
+#define MTB_BESIDE(V) MTB_OF(V) MTB_EIGHT(V, 2) MTB_CASE(V, 6 / V, 2, 32) MTB_CASE(V, 6 / V, 3, 32)
+  MTB_OF(4) MTB_CASE(4, 4, 1, 32) MTB_BESIDE(2) MTB_BESIDE(1) {
     MTB_LAUNCH(add_rms_norm_long_kernel, (unsigned)rows, kLongThreads, 0, st, a, out, y, rstd, block_rstd);
   }
-#undef MTB_WIDE
-#undef MTB_NARROW
-#undef MTB_ALL
+#undef MTB_BESIDE
+#undef MTB_OF
+#undef MTB_EIGHT
 #undef MTB_CASE
   MTB_LAUNCH_CHECK("add_rms_norm_kernel");
   return MTB_OK;
@@ -602,11 +613,13 @@ MTB_API long long mtb_add_rms_norm_workspace_bytes(long long rows, int c) {
 }
 
 // The kernels that backward_plan names, each as a case of whatever MTB_CASE is.
+#define MTB_EIGHT(V, W, AHEAD) MTB_CASE(V, 8 / V, W, 32, AHEAD)
+#define MTB_SIX(V, W) MTB_CASE(V, 6 / V, W, 32, false)
 #define MTB_OF(V, AHEAD) \
-  MTB_CASE(V, 4 / V, 1, 8, false) MTB_CASE(V, 4 / V, 1, 16, false) MTB_CASE(V, 4 / V, 1, 32, false) MTB_CASE(V, 8 / V, 1, 32, false) MTB_CASE(V, 4 / V, 3, 32, false) MTB_CASE(V, 8 / V, 2, 32, false) \
-  MTB_CASE(V, 8 / V, 4, 32, false) MTB_CASE(V, 8 / V, 8, 32, AHEAD) MTB_CASE(V, 8 / V, 16, 32, AHEAD) MTB_CASE(V, 8 / V, 32, 32, AHEAD)
-#define MTB_SIX(V) MTB_CASE(V, 6 / V, 8, 32, false) MTB_CASE(V, 6 / V, 16, 32, false)
-#define MTB_KERNELS MTB_OF(4, true) MTB_OF(2, false) MTB_OF(1, false) MTB_SIX(2) MTB_SIX(1)
+  MTB_CASE(V, 4 / V, 1, 8, false) MTB_CASE(V, 4 / V, 1, 16, false) MTB_CASE(V, 4 / V, 1, 32, false) MTB_CASE(V, 4 / V, 2, 32, false) MTB_CASE(V, 4 / V, 3, 32, false) MTB_EIGHT(V, 2, false) \
+  MTB_EIGHT(V, 4, false) MTB_EIGHT(V, 5, false) MTB_EIGHT(V, 8, AHEAD) MTB_EIGHT(V, 12, AHEAD) MTB_EIGHT(V, 16, AHEAD) MTB_EIGHT(V, 24, AHEAD) MTB_EIGHT(V, 32, AHEAD)
+#define MTB_BESIDE(V) MTB_OF(V, false) MTB_EIGHT(V, 10, false) MTB_SIX(V, 1) MTB_SIX(V, 3) MTB_SIX(V, 4) MTB_SIX(V, 8) MTB_SIX(V, 12) MTB_SIX(V, 24)
+#define MTB_KERNELS MTB_OF(4, true) MTB_EIGHT(4, 3, false) MTB_BESIDE(2) MTB_BESIDE(1)
 
 MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dnew, const float* dy, const float* x, const float* rstd, const float* block,
                                           const float* block_rstd, const float* weight, const float* post_weight, const float* gate, long long rows_per_gate, double scale,

@@ -153,6 +153,19 @@ def test_backward(shape, gate, post):
             assert off.max() <= 1, (name, off.max())
 
 
+@pytest.mark.parametrize("c", [129, 191, 194, 255, 260, 383, 386, 511, 513, 575, 578, 580, 767, 770, 772, 1023, 1025, 1028, 1279, 1282, 1284, 1535, 1538, 2047, 2050, 2052, 2303, 2306, 2559, 2562,
+                               3001, 3071, 3080, 4095, 4098, 4100, 4607, 4610, 6143, 6145, 6148, 8191, 8194, 16383, 16386])
+def test_widths_about_the_ends_of_each_group(c):
+    """The widest and the narrowest rows that a number of warps and values a thread holds."""
+    test_backward((2, 5, c), "sample", True)
+
+
+@pytest.mark.parametrize("c", [129, 255, 260, 383, 386, 511, 516, 575, 578, 767, 772, 1023, 1025, 1028, 1279, 1282, 1535, 1540, 2047, 2052, 2306, 2559, 2564, 3071, 3080])
+def test_widths_of_many_rows(c):
+    """As above, for a forward pass of more rows than would be spread over eight warps each."""
+    test_forward((4, 300, c), "channel", True)
+
+
 @pytest.mark.parametrize("shape", [(1, 1), (3, 5), (2, 64), (9, 1000), (2, 3, 4096), (2, 66, 3, 5)])
 def test_the_norm_by_itself(shape):
     import gpu_util as g
