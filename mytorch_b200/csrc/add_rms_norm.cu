@@ -8,7 +8,13 @@
 // Bound by memory: 16 bytes a value forward, 24 backward, each once, if a row stays in registers between its sums and what is made of them.  So a group of W warps holds
 // a row, PER vectors a thread and tensor, and goes on to its next one; W is 1 where a row fits a warp, which then waits for no other, and narrow rows lie side by side in
 // a warp, LANES lanes each.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "colreduce.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -20,13 +26,17 @@ struct Operands {
   float scale, eps;
 };
 
+constexpr int kMostCtas = 8;  // of a row
+
 // Sums over the threads that share a row, W warps or LANES lanes of one, in all of them.  Two buffers taken in turn: a third sum writes where the first was read before
-// the second.
-template <int W, int LANES = 32>
+// the second.  JOINED: those of a cluster's CTAs, each of which gives its own to all of them.
+template <int W, int LANES = 32, bool JOINED = false>
 struct GroupSum {
   static constexpr int kThreads = W == 1 ? 256 : 32 * W;
   static constexpr int kGroups = W == 1 ? 256 / LANES : 1, kShare = W == 1 ? LANES : 32 * W;
   float (*part)[W];
+  float (*given)[kMostCtas] = nullptr;
+  int ctas = 1, rank = 0;
   int turn = 0;
 
   __device__ __forceinline__ float operator()(float x) {
@@ -38,6 +48,13 @@ struct GroupSum {
     x = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) x += part[turn][w];
+    if (JOINED) {
+      cg::cluster_group cluster = cg::this_cluster();
+      if ((int)threadIdx.x < ctas) cluster.map_shared_rank(&given[turn][0], threadIdx.x)[rank] = x;
+      cluster.sync();
+      x = 0;
+      for (int r = 0; r < ctas; ++r) x += given[turn][r];
+    }
     turn ^= 1;
     return x;
   }
@@ -149,7 +166,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads) add_rms_norm_ker
 struct Gradients {
   const float *dnew, *dy, *rstd, *block_rstd;
   float *dresidual, *dblock;
-  float* partial;     // [CTA][3][c]: dweight, dpost_weight, dgate of a gate that all rows share; NULL: nobody asks
+  float* partial;     // [CTA or cluster][3][c]: dweight, dpost_weight, dgate of a gate that all rows share; NULL: nobody asks
   float* gate_rows;   // a row for every row (a gate like the block), or for every stretch; NULL: neither
   int gate_each;      // 1: of every row
   // Rows come in stretches, none of which goes past a row of the gate: `parts` for each of its rows, `stretch` rows each but for the last.
@@ -160,30 +177,39 @@ struct Gradients {
 // 8192 x 4096 167 -> 142), not where rows of other groups are under way on the SM (32768 x 1024 135 -> 146), nor by copies of 4 bytes (32768 x 1023 158 -> 215).
 // Where it is not 0: registers for so many on an SM; what else the compiler takes leaves a third of the warps (32768 x 750 by six values a thread and 4 warps 125 -> 111 us,
 // 12672 x 2601 by eight and 12 warps 302 -> 207), but for kernels that would then spill (16384 x 2047 by eight and 8 warps 171 -> 190).
-template <int V, int PER, int W, int LANES>
-constexpr int kBackwardCtas = V * PER == 6 ? (W == 1 ? 3 : 24 / W) : W == 24 ? 1 : V != 4 && W == 12 ? 2 : V != 4 && V * PER == 4 && W == 1 && LANES == 32 ? 4 : 0;
+template <int V, int PER, int W, int LANES, bool JOINED>
+constexpr int kBackwardCtas = JOINED ? (W == 8 && V != 4 ? 2 : 24 / W) : V * PER == 6 ? (W == 1 ? 3 : 24 / W) : W == 24 ? 1 : V != 4 && W == 12 ? 2 : V != 4 && V * PER == 4 && W == 1 && LANES == 32 ? 4 : 0;
 
-template <int V, int PER, int W, int LANES, bool AHEAD>
-__global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V, PER, W, LANES>) add_rms_norm_backward_kernel(const __grid_constant__ Operands a, const __grid_constant__ Gradients d) {
-  constexpr int kGroups = GroupSum<W, LANES>::kGroups, kShare = GroupSum<W, LANES>::kShare;
+template <int V, int PER, int W, int LANES, bool AHEAD, bool JOINED = false>
+__global__ void __launch_bounds__(GroupSum<W, LANES, JOINED>::kThreads, kBackwardCtas<V, PER, W, LANES, JOINED>) add_rms_norm_backward_kernel(const __grid_constant__ Operands a, const __grid_constant__ Gradients d) {
+  constexpr int kGroups = GroupSum<W, LANES, JOINED>::kGroups, kShare = GroupSum<W, LANES, JOINED>::kShare;
   extern __shared__ __align__(16) float shared[];  // AHEAD: [x, dy, dnew, block][PER][thread][V]; W 1: [3][c]
-  __shared__ float part[2][W];
-  GroupSum<W, LANES> sum{part};
+  __shared__ float part[2][W], given[JOINED ? 2 : 1][JOINED ? kMostCtas : 1];
+  GroupSum<W, LANES, JOINED> sum{part};
   mtb_launch_dependents();
   mtb_wait_prior();
-  const int id = threadIdx.x % kShare, beside = W == 1 ? (threadIdx.x & 31) / LANES : 0;
-  const long long groups = (long long)gridDim.x * kGroups;
+  if constexpr (JOINED) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();  // all of them have started: their shared memory is there
+    sum.given = given;
+    sum.ctas = (int)cluster.num_blocks();
+    sum.rank = (int)cluster.block_rank();
+  }
+  const int share = JOINED ? sum.ctas * kShare : kShare;
+  const long long unit = JOINED ? blockIdx.x / sum.ctas : blockIdx.x;  // the CTA, or the cluster
+  const int id = (JOINED ? sum.rank * kShare : 0) + threadIdx.x % kShare, beside = W == 1 ? (threadIdx.x & 31) / LANES : 0;
+  const long long groups = (long long)(JOINED ? gridDim.x / sum.ctas : gridDim.x) * kGroups;
   const float per_c = 1.f / a.c;
   VecF<V> dw[PER], dpw[PER], dg[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) dw[k] = dpw[k] = dg[k] = filled<V>(0);
   // where a row's values of this thread lie
-  const auto slot = [&](int tensor, int j) { return shared + ((tensor * PER + j) * GroupSum<W>::kThreads + (int)threadIdx.x) * V; };
+  const auto slot = [&](int tensor, int j) { return shared + ((tensor * PER + j) * GroupSum<W, LANES, JOINED>::kThreads + (int)threadIdx.x) * V; };
   const auto fetch_row = [&](long long row) {
     const long long at = row * a.c;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int i = (id + j * kShare) * V;
+      const int i = (id + j * share) * V;
       if (i < a.c) {
         fetch<V>(slot(0, j), a.x + at + i);
         if (d.dy) fetch<V>(slot(1, j), d.dy + at + i);
@@ -193,7 +219,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
     }
   };
   const auto first_of = [&](long long stretch) { const long long g = stretch / d.parts; return g * d.rows_of_gate + (stretch - g * d.parts) * d.stretch; };
-  long long begin = blockIdx.x * (long long)kGroups + (W == 1 ? threadIdx.x / 32 * (32 / LANES) : 0);
+  long long begin = unit * kGroups + (W == 1 ? threadIdx.x / 32 * (32 / LANES) : 0);
   if (AHEAD && begin < d.stretches) fetch_row(first_of(begin));
   for (; begin < d.stretches; begin += groups) {
     const long long stretch = LANES == 32 || begin + beside < d.stretches ? begin + beside : begin;
@@ -210,7 +236,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
       if (AHEAD) fetched();
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * kShare) * V;
+        const int i = (id + k * share) * V;
         x[k] = dy[k] = D[k] = b[k] = filled<V>(0);
         g[k] = filled<V>(1);
         if (i < c) {
@@ -231,7 +257,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
         float s = 0;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const int i = (id + k * kShare) * V;
+          const int i = (id + k * share) * V;
           const VecF<V> w = a.weight && i < c ? load<V>(a.weight + i) : filled<V>(1);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
@@ -251,7 +277,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
       if (d.dresidual) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const int i = (id + k * kShare) * V;
+          const int i = (id + k * share) * V;
           if (i < c) {
             VecF<V> r;
 #pragma unroll
@@ -264,7 +290,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
       float s = 0;
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * kShare) * V;
+        const int i = (id + k * share) * V;
         const VecF<V> w = a.post_weight && i < c ? load<V>(a.post_weight + i) : filled<V>(1);
         VecF<V> each;
 #pragma unroll
@@ -283,7 +309,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
       const float mean = a.post_weight ? sum(s) * per_c : 0.f;
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * kShare) * V;
+        const int i = (id + k * share) * V;
         if (i < c) {
           VecF<V> r;
 #pragma unroll
@@ -295,7 +321,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
     if (d.gate_rows && !d.gate_each) {
 #pragma unroll
       for (int k = 0; k < PER; ++k) {
-        const int i = (id + k * kShare) * V;
+        const int i = (id + k * share) * V;
         if (i < a.c && there) store<V>(d.gate_rows + stretch * a.c + i, dg[k]);
         dg[k] = filled<V>(0);
       }
@@ -303,7 +329,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
   }
   if (!d.partial) return;
   const int c = a.c;
-  float* mine = d.partial + (long long)blockIdx.x * 3 * c;
+  float* mine = d.partial + unit * 3 * c;
   if (W == 1) {  // the CTA's groups one after the other: the same order every time
     float* joined = shared;
     for (int w = 0; w < kGroups; ++w) {
@@ -312,7 +338,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
         for (int k = 0; k < PER; ++k)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const int i = (id + k * kShare) * V + j;
+            const int i = (id + k * share) * V + j;
             if (i < c) {
               joined[i] = w ? joined[i] + dw[k].v[j] : dw[k].v[j];
               joined[c + i] = w ? joined[c + i] + dpw[k].v[j] : dpw[k].v[j];
@@ -326,7 +352,7 @@ __global__ void __launch_bounds__(GroupSum<W, LANES>::kThreads, kBackwardCtas<V,
   } else {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = (id + k * kShare) * V;
+      const int i = (id + k * share) * V;
       if (i < c) {
         store<V>(mine + i, dw[k]);
         store<V>(mine + c + i, dpw[k]);
@@ -481,8 +507,9 @@ __global__ void __launch_bounds__(kLongThreads) add_rms_norm_backward_long_kerne
 struct Plan {
   int v, per, warps, lanes;  // warps 0: through memory
   int groups;         // of a CTA
-  int ctas;           // the most that the grid has
+  int ctas;           // the most that the grid has, or clusters
   bool ahead;
+  int joined = 1;     // CTAs of a row: a cluster
 };
 
 // How many CTAs of a kernel an SM holds: the grid is no larger, so that none waits for another to end.
@@ -490,6 +517,42 @@ template <class K>
 int resident(K kernel, int threads, int smem, int* known) {
   if (!*known && cudaOccupancyMaxActiveBlocksPerMultiprocessor(known, kernel, threads, smem) != cudaSuccess) *known = 0;
   return *known > 0 ? *known : 1;
+}
+
+// The same of clusters.
+template <class... P>
+int resident_clusters(void (*kernel)(P...), int ctas, int threads, int smem, int* known) {
+  if (!*known) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(known, kernel, &cfg) != cudaSuccess) *known = 0;
+  }
+  return *known > 0 ? *known : 1;
+}
+template <class... P, class... A>
+cudaError_t launch_clusters(void (*kernel)(P...), int clusters, int ctas, int threads, int smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * ctas));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
 // What holds a row: values a thread and tensor, warps.  Taken is the first of a table that is large enough.
@@ -526,12 +589,25 @@ Plan forward_plan(long long rows, int c, int align) {
 // with six 194, by 8 with six 156.
 constexpr Share kSharesOfFour[] = {{4, 2}, {4, 3}, {8, 2}, {8, 3}, {8, 4}, {8, 5}, {8, 8}, {8, 12}, {8, 16}, {8, 24}, {8, 32}};
 constexpr Share kShares[] = {{6, 1}, {4, 2}, {4, 3}, {8, 2}, {6, 3}, {6, 4}, {8, 4}, {8, 5}, {6, 8}, {8, 8}, {6, 12}, {8, 10}, {8, 12}, {8, 16}, {6, 24}, {8, 24}, {8, 32}};
+// A longer row by as many CTAs of eight values a thread as hold it, by 8 warps each as long as that is no more than eight: others of the SM's go on while a cluster waits for one of its
+// own.  1984 x 16384 by eight CTAs of 8 warps 237, by six of 12 288, by four of 16 317, through memory 765.
+constexpr int kJoinedWarps[] = {8, 12, 16};
 Plan backward_plan(int c, int align) {
   const int v = align >= 4 && c % 4 == 0 ? 4 : align >= 2 && c % 2 == 0 ? 2 : 1, sms = mtb_sm_count();
   const auto plan = [&](int per, int warps, int per_sm, bool ahead = false, int lanes = 32) { return Plan{v, per, warps, lanes, warps == 1 ? 256 / lanes : 1, sms * per_sm, ahead}; };
   if (c <= 128) return plan(4 / v, 1, 5, false, c <= 32 ? 8 : c <= 64 ? 16 : 32);
   const Share s = v == 4 ? share_of(kSharesOfFour, c) : share_of(kShares, c);
-  return s.warps ? plan(s.values / v, s.warps, s.warps == 1 ? 3 : 32 / s.warps, v == 4 && s.warps >= 8) : plan(0, 0, 1);
+  if (s.warps) return plan(s.values / v, s.warps, s.warps == 1 ? 3 : 32 / s.warps, v == 4 && s.warps >= 8);
+  for (const int warps : kJoinedWarps) {
+    const int ctas = (c + 256 * warps - 1) / (256 * warps);
+    if (ctas <= kMostCtas) {
+      Plan p = plan(8 / v, warps, 24 / warps, v == 4);
+      p.ctas /= ctas;  // clusters
+      p.joined = ctas;
+      return p;
+    }
+  }
+  return plan(0, 0, 1);
 }
 
 // How rows come in stretches (see Gradients): as many as there are groups, or more where the gate has more rows.
@@ -620,6 +696,7 @@ MTB_API long long mtb_add_rms_norm_workspace_bytes(long long rows, int c) {
   MTB_EIGHT(V, 4, false) MTB_EIGHT(V, 5, false) MTB_EIGHT(V, 8, AHEAD) MTB_EIGHT(V, 12, AHEAD) MTB_EIGHT(V, 16, AHEAD) MTB_EIGHT(V, 24, AHEAD) MTB_EIGHT(V, 32, AHEAD)
 #define MTB_BESIDE(V) MTB_OF(V, false) MTB_EIGHT(V, 10, false) MTB_SIX(V, 1) MTB_SIX(V, 3) MTB_SIX(V, 4) MTB_SIX(V, 8) MTB_SIX(V, 12) MTB_SIX(V, 24)
 #define MTB_KERNELS MTB_OF(4, true) MTB_EIGHT(4, 3, false) MTB_BESIDE(2) MTB_BESIDE(1)
+#define MTB_CLUSTERS MTB_JOINED(4, 8) MTB_JOINED(4, 12) MTB_JOINED(4, 16) MTB_JOINED(2, 8) MTB_JOINED(2, 12) MTB_JOINED(2, 16) MTB_JOINED(1, 8) MTB_JOINED(1, 12) MTB_JOINED(1, 16)
 
 MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dnew, const float* dy, const float* x, const float* rstd, const float* block,
                                           const float* block_rstd, const float* weight, const float* post_weight, const float* gate, long long rows_per_gate, double scale,
@@ -642,7 +719,7 @@ MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dn
   if (rows > 0) {
     int ctas = p.ctas;
 #define MTB_CASE(V, PER, W, LANES, AHEAD) \
-  if (p.v == V && p.per == PER && p.warps == W && p.lanes == LANES && p.ahead == AHEAD) { \
+  if (p.v == V && p.per == PER && p.warps == W && p.lanes == LANES && p.ahead == AHEAD && p.joined == 1) { \
     static unsigned long long opted; \
     static int known; \
     constexpr int kAhead = 16 * V * PER * GroupSum<W>::kThreads; \
@@ -653,16 +730,32 @@ MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dn
   } else
     MTB_KERNELS {}
 #undef MTB_CASE
+#define MTB_JOINED(V, W) \
+  if (p.v == V && p.warps == W && p.joined > 1) { \
+    static unsigned long long opted; \
+    static int known[kMostCtas + 1]; \
+    const auto kernel = add_rms_norm_backward_kernel<V, 8 / V, W, 32, V == 4, true>; \
+    if (V == 4) \
+      if (int rc = mtb_opt_in_smem((const void*)kernel, 16 * 8 * 32 * W, &opted)) return rc; \
+    ctas = std::min(ctas, resident_clusters(kernel, p.joined, 32 * W, V == 4 ? 16 * 8 * 32 * W : 0, &known[p.joined])); \
+  }
+    MTB_CLUSTERS
+#undef MTB_JOINED
     s = stretches_of(p, ctas, rows, of_gate ? rows_per_gate : rows);
     gate_rows = each || (of_gate && s.parts == 1) ? dgate : of_gate ? partial + (long long)p.ctas * 3 * c : nullptr;
     const Gradients d{dnew, dy, rstd, block_rstd, dresidual, dblock, summed ? partial : nullptr, gate_rows, each ? 1 : 0, s.stretches, s.parts, s.stretch, s.rows_of_gate};
 #define MTB_CASE(V, PER, W, LANES, AHEAD) \
-  if (p.v == V && p.per == PER && p.warps == W && p.lanes == LANES && p.ahead == AHEAD) { \
+  if (p.v == V && p.per == PER && p.warps == W && p.lanes == LANES && p.ahead == AHEAD && p.joined == 1) { \
     MTB_LAUNCH((add_rms_norm_backward_kernel<V, PER, W, LANES, AHEAD>), (unsigned)s.ctas, GroupSum<W>::kThreads, AHEAD ? 16 * V * PER * GroupSum<W>::kThreads : W == 1 ? 12 * c : 0, st, a, d); \
   } else
-    MTB_KERNELS {
+#define MTB_JOINED(V, W) \
+  if (p.v == V && p.warps == W && p.joined > 1) { \
+    MTB_CUDA(launch_clusters(add_rms_norm_backward_kernel<V, 8 / V, W, 32, V == 4, true>, s.ctas, p.joined, 32 * W, V == 4 ? 16 * 8 * 32 * W : 0, st, a, d)); \
+  } else
+    MTB_KERNELS MTB_CLUSTERS {
       MTB_LAUNCH(add_rms_norm_backward_long_kernel, (unsigned)s.ctas, kLongThreads, 0, st, a, d);
     }
+#undef MTB_JOINED
 #undef MTB_CASE
     MTB_LAUNCH_CHECK("add_rms_norm_backward_kernel");
   }

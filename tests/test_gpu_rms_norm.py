@@ -154,7 +154,7 @@ def test_backward(shape, gate, post):
 
 
 @pytest.mark.parametrize("c", [129, 191, 194, 255, 260, 383, 386, 511, 513, 575, 578, 580, 767, 770, 772, 1023, 1025, 1028, 1279, 1282, 1284, 1535, 1538, 2047, 2050, 2052, 2303, 2306, 2559, 2562,
-                               3001, 3071, 3080, 4095, 4098, 4100, 4607, 4610, 6143, 6145, 6148, 8191, 8194, 16383, 16386])
+                               3001, 3071, 3080, 4095, 4098, 4100, 4607, 4610, 6143, 6145, 6148, 8191, 8194, 10241, 16380, 16383, 16386, 24572, 24575, 24578, 32767, 32768, 32770])
 def test_widths_about_the_ends_of_each_group(c):
     """The widest and the narrowest rows that a number of warps and values a thread holds."""
     test_backward((2, 5, c), "sample", True)
