@@ -156,7 +156,7 @@ struct Shared {
   alignas(16) float part[W][4];
   float runs[64];
   Key candidate[kCandidates], list[W];
-  int group[kGroups], groups, candidates;
+  int group[kGroups], groups, candidates, taken;  // taken: a word of its own, `candidates` may still be read by a warp that comes late
 };
 constexpr int kSplit = 4;  // a thread's quads fall into groups by their number modulo this
 template <int W>
@@ -337,9 +337,9 @@ __device__ __forceinline__ Sums look(const Row& row, int begin, int end, int top
       if (count < top) {
         if (warp == 0) count = take_equal(row, begin, end, shared, lane, bound, count, top);
         if (W > 1) {
-          if (id == 0) shared.candidates = count;
+          if (id == 0) shared.taken = count;
           __syncthreads();
-          count = shared.candidates;
+          count = shared.taken;
         }
       }
     }
