@@ -41,13 +41,14 @@ def _numel(shape):
     return n
 
 
-def _grad_buffer(param):
+def _grad_buffer(param, *others):
     """Output tensor for a parameter's gradient.  Under the data-parallel wrapper every parameter
     owns a window of the flat all-reduce buffer (``param._grad_slot``) and its first gradient of a
     backward pass is written straight into it; otherwise (no wrapper, or a second contribution that
-    the tape will add to the first) a fresh tensor."""
+    the tape will add to the first) a fresh tensor.  ``others``: what the call has asked a buffer for already; a parameter
+    in two roles has two gradients, of which one goes to the window."""
     slot = getattr(param, "_grad_slot", None)
-    if slot is None or param.grad is not None:
+    if slot is None or param.grad is not None or any(param is t for t in others):
         return _new(param.shape, param)
     return _on_device(param.shape, param.dtype, param.device, slot)
 
@@ -540,7 +541,7 @@ def cuda_batch_norm2d_add_relu_backward(output_grad, mean, var, x, residual, wei
     dx, dres = _new(x.shape, x), _new(x.shape, x)
     affine = weight is not None and bias is not None
     dg = _grad_buffer(weight) if affine else None
-    db = _grad_buffer(bias) if affine else None
+    db = _grad_buffer(bias, weight) if affine else None
     ws, ws_bytes = env.workspace(env.lib.batch_norm2d_workspace_bytes(n, c, h, w))
     tail = (weight, bias, float(eps), dx, dres, dg, db, ws, ws_bytes, env.stream())
     mask = getattr(mean, "_relu_mask", None)
@@ -595,7 +596,7 @@ def cuda_batch_norm2d_relu_halved_backward(output_grad, mean, var, x, weight, bi
         env.lib.copy_f32(dy, output_grad, _numel(dy.shape), env.stream())
     affine = weight is not None and bias is not None
     dg = _grad_buffer(weight) if affine else None
-    db = _grad_buffer(bias) if affine else None
+    db = _grad_buffer(bias, weight) if affine else None
     ws, ws_bytes = env.workspace(env.lib.batch_norm2d_workspace_bytes(n, c, h, w))
     env.lib.batch_norm2d_relu_pool_backward_f32(n, c, h, w, dy, mean, var, x, mean._pool_tiemask, weight, bias, float(eps), dx, dg, db, ws, ws_bytes, env.stream())
     return [dx, dg, db]
@@ -608,7 +609,7 @@ def cuda_batch_norm2d_backward(output_grad, mean, var, x, weight, bias, eps, rel
     dx = _new(x.shape, x)
     affine = weight is not None and bias is not None
     dg = _grad_buffer(weight) if affine else None
-    db = _grad_buffer(bias) if affine else None
+    db = _grad_buffer(bias, weight) if affine else None
     ws, ws_bytes = env.workspace(env.lib.batch_norm2d_workspace_bytes(n, c, h, w))
     env.lib.batch_norm2d_backward_f32(n, c, h, w, output_grad, mean, var, x, weight, bias, float(eps),
                                       int(bool(relu)), dx, dg, db, ws, ws_bytes, env.stream())
@@ -646,7 +647,7 @@ def cuda_group_norm_backward(output_grad, mean, rstd, x, weight, bias, num_group
     n, c, hw = _image_extents(x)
     dx = _new(x.shape, x) if needed[0] else None
     dg = _grad_buffer(weight) if weight is not None and needed[1] else None
-    db = _grad_buffer(bias) if bias is not None and needed[2] else None
+    db = _grad_buffer(bias, weight) if bias is not None and needed[2] else None
     ws, ws_bytes = env.workspace(env.lib.group_norm_workspace_bytes(n, c, hw, num_groups))
     env.lib.group_norm_backward_f32(n, c, hw, num_groups, output_grad, mean, rstd, x, weight, bias, _ACTIVATIONS[activation], dx, dg, db, ws, ws_bytes,
                                     env.stream())
@@ -727,7 +728,8 @@ def cuda_add_rms_norm_backward(dnew, dy, new, rstd, block_rstd, residual, block,
     env = _env(new)
     rows, c = _channel_rows(new)
     out = [_new(new.shape, new) if needed[0] else None, _new(new.shape, new) if needed[1] and block is not None else None]
-    out += [_grad_buffer(t) if n and t is not None else None for n, t in zip(needed[2:], (weight, post_weight, gate))]
+    summed = (weight, post_weight, gate)
+    out += [_grad_buffer(t, *summed[:k]) if needed[2 + k] and t is not None else None for k, t in enumerate(summed)]
     ws, ws_bytes = env.workspace(env.lib.add_rms_norm_workspace_bytes(rows, c))
     dgate = out[4] if rows or gate is None or len(gate.shape) == 1 else None  # a gate of no rows
     env.lib.add_rms_norm_backward_f32(rows, c, dnew, dy, new, rstd, block, block_rstd, weight, post_weight, gate, _rows_per_gate(new, gate), float(scale), *out[:4], dgate,
