@@ -731,7 +731,10 @@ def cuda_add_rms_norm_backward(dnew, dy, new, rstd, block_rstd, residual, block,
     summed = (weight, post_weight, gate)
     out += [_grad_buffer(t, *summed[:k]) if needed[2 + k] and t is not None else None for k, t in enumerate(summed)]
     ws, ws_bytes = env.workspace(env.lib.add_rms_norm_workspace_bytes(rows, c))
-    dgate = out[4] if rows or gate is None or len(gate.shape) == 1 else None  # a gate of no rows
+    dgate = out[4]
+    if dgate is not None and rows == 0 and len(gate.shape) > 1:  # samples without a position: their gates' rows are no row's
+        env.lib.memset_async(dgate, 0, 4 * _numel(gate.shape), env.stream())
+        dgate = None
     env.lib.add_rms_norm_backward_f32(rows, c, dnew, dy, new, rstd, block, block_rstd, weight, post_weight, gate, _rows_per_gate(new, gate), float(scale), *out[:4], dgate,
                                       ws, ws_bytes, env.stream())
     return out

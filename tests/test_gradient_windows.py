@@ -69,3 +69,16 @@ def test_a_window_once_a_call(monkeypatch, call):
     assert len(set(written)) == len(got)  # each is written to, in a place of its own
     w.grad = _t(6)  # there is a gradient already: none goes to the window
     assert all(t._native_array is not w._grad_slot for t in call(w))
+
+
+@pytest.mark.parametrize("shape", [(4, 0, 6), (4, 6, 0, 3)])
+def test_a_gate_of_no_rows_is_cleared(monkeypatch, shape):
+    """A row of the gate a sample, and samples without a position: no kernel writes its gradient."""
+    env = _Env()
+    monkeypatch.setattr(ops, "_env", lambda t: env)
+    monkeypatch.setattr(ops, "_new", lambda shape, like, dtype=None: mt.tensor(np.full(shape, 7, np.float32)))
+    x, row, gate = _t(*shape), _t(0), _t(4, 6)
+    dgate = ops.cuda_add_rms_norm_backward(x, x, x, row, row, x, x, None, None, gate)[4]
+    assert dgate.shape == (4, 6)
+    cleared = env.lib.given.get("memset_async")
+    assert cleared is not None and cleared[0] is dgate and cleared[1:3] == (0, 4 * 24)
