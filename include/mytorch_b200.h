@@ -310,7 +310,8 @@ int mtb_cross_entropy_backward_f32(int batch, int classes, const float* logits, 
  * tokens: one a row, int32 (token_kind 0) or int64 (1); with `ignores` a row whose token is ignore_index has log probability 0 and no gradient from it, another
  * token outside [0, v) has NaN and no gradient from it.  top: how many alternatives, at most 32 and at most v, in descending order of their logits, equal ones by place.  top_log_probs,
  * top_tokens: [n][top].  stats: [n][3], the largest logit, the sum of exp(z - largest) and the entropy, for the backward; may be NULL.
- * Backward: dlog_probs, dentropy [n] and dtop [n][top] may be NULL each; the top_tokens of a row are distinct. */
+ * Backward: dlog_probs, dentropy [n] and dtop [n][top] may be NULL each; the top_tokens of a row are distinct.  A row that only zeros reach
+ * has gradient zero, whatever its logits. */
 int mtb_token_log_probs_forward_f32(long long n, int v, const float* logits, int token_kind, const void* tokens, int ignores, long long ignore_index, int top,
                                     float* log_probs, float* entropy, float* stats, float* top_log_probs, long long* top_tokens, void* stream);
 int mtb_token_log_probs_backward_f32(long long n, int v, const float* logits, int token_kind, const void* tokens, int ignores, long long ignore_index, int top,

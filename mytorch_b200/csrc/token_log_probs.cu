@@ -517,6 +517,8 @@ struct Backward {
 struct RowGradient {
   float m, per_s, log_s, h, g, gh, all;
 
+  // Where no gradient reaches the row: zero for a value of 0, which stands for each of the row's, as these may make everything NaN.
+  __device__ __forceinline__ void clear() { m = per_s = log_s = h = 0; }
   // exp here by the function, whose error does not grow with its argument: an element moves 8 bytes, there is time.
   __device__ __forceinline__ float at(float z) const {
     const float d = z - m, p = expf(d) * per_s;
@@ -556,10 +558,16 @@ __global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __gr
   r.all = extra;
   for (int o = 16; o > 0; o >>= 1) r.all += __shfl_xor_sync(0xFFFFFFFFu, r.all, o);
   r.all += r.g;
+  const bool none = !__any_sync(0xFFFFFFFFu, extra != 0.f) && r.g == 0.f && r.gh == 0.f;
+  if (none) r.clear();
   for (int q = begin; q < end; q += U * T) {
     if (W == 1 && q > begin) {
 #pragma unroll
       for (int u = 0; u < U; ++u) f[u] = row.quad(q + id + u * T, end);
+    }
+    if (none) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) f[u] = make_float4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -581,9 +589,9 @@ __global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __gr
   meet<W>();
   if (W > 1 && threadIdx.x >= 32) return;
   const long long first = row.place(begin), last = row.place(end);  // the places of this part
-  if (mine && other >= first && other < last && other >= 0 && other < a.v) to[row.lead + other] = r.at(row.z[row.lead + other]) + (other == token ? extra + r.g : extra);
+  if (mine && other >= first && other < last && other >= 0 && other < a.v) to[row.lead + other] = r.at(none ? 0.f : row.z[row.lead + other]) + (other == token ? extra + r.g : extra);
   if (!__any_sync(0xFFFFFFFFu, mine && other == token) && lane == 0 && token >= first && token < last && token >= 0 && token < a.v)
-    to[row.lead + token] = r.at(row.z[row.lead + token]) + r.g;
+    to[row.lead + token] = r.at(none ? 0.f : row.z[row.lead + token]) + r.g;
 }
 
 bool sizes_fine(long long n, int v, int token_kind, int top) {

@@ -22,7 +22,8 @@ def token_log_probs(logits: Tensor, tokens: Tensor, top=0, ignore_index=None) ->
 
     ``ignore_index``: a row with this token has log probability 0 and no gradient from it; entropy and alternatives are those of its logits.  Another token outside [0, V)
     has log probability NaN and no gradient from it either.  A logit of -inf is a token that cannot be; a row of nothing else, or with NaN or +inf in it, is NaN, its alternatives in the order of
-    its logits (NaN first)."""
+    its logits (NaN first), and so is its gradient.  A row that no gradient reaches, as one of an ignored token where nothing is made of its entropy and alternatives, has
+    gradient zero, whatever its logits."""
     if len(logits.shape) not in (2, 3) or logits.shape[-1] < 1:
         raise InvalidShapeError(logits.shape)
     if tokens.dtype is not int32 and tokens.dtype is not int64:
