@@ -24,7 +24,7 @@ constexpr int kChunk = 2048;  // elements of a CTA: eight a thread, all of whose
 constexpr int kSteps = 256;
 
 struct Hyper {
-  float b1, b2, c1, c2, eps, keep;  // c1 = 1 - b1, c2 = 1 - b2 (8 bits: its root), keep = 1 - lr wd
+  float b1, b2, c1, c2, eps, decay;  // c1 = 1 - b1, c2 = 1 - b2 (8 bits: its root), decay = lr wd: as 1 - lr wd it would lose all but a bit or two where it is a millionth
 };
 
 // What a step makes of t, for every counter of a call, and what multiplies the gradients.
@@ -90,11 +90,12 @@ struct Table {
   Chunks<N> chunks;
 };
 
-// Root and quotient to 2^-22 of themselves, the step's share of which is far under a parameter's last place.
+// Root and quotient to 2^-22 of themselves, the step's share of which is far under a parameter's last place.  Decay and step are added up first, so that only their sum is
+// rounded against the parameter.
 __device__ __forceinline__ void update(float& p, float m, float v, const Hyper& h, const Corrections& c) {
   float root;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
-  p = fmaf(p, h.keep, -__fdividef(c.step_size * m, fmaf(root, c.root, h.eps)));
+  p -= fmaf(h.decay, p, __fdividef(c.step_size * m, fmaf(root, c.root, h.eps)));
 }
 __device__ __forceinline__ void moments(float g, float& m, float& v, const Hyper& h) {
   m = fmaf(h.b1, m, h.c1 * g);
@@ -290,7 +291,7 @@ __device__ __forceinline__ void update_quickly(float& p, float m, float v, const
   float root, per;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(per) : "f"(fmaf(root, c.root, h.eps)));
-  p = fmaf(p, h.keep, -(c.step_size * m * per));
+  p -= fmaf(h.decay, p, c.step_size * m * per);
 }
 
 // A block by a warp.  What bounds it is the number of instructions, 517 a warp with its eight values a lane (41 us of the integer pipe, 46 of issue slots and 54 of HBM in 73 us for 25.6 M
@@ -555,7 +556,7 @@ MTB_API int mtb_adamw_f32(int count, void* const* params, const long long* sizes
   cudaStream_t st = (cudaStream_t)stream;
   Corrections* corrections = (Corrections*)scratch;
   if (int rc = begin(count, params, lr, beta1, beta2, grad_scale, MtbClip{sums, nsums, grad_scale, max_norm, norm}, corrections, slots, st)) return rc;
-  const Hyper h{(float)beta1, (float)beta2, (float)(1 - beta1), (float)(1 - beta2), (float)eps, (float)(1 - lr * weight_decay)};
+  const Hyper h{(float)beta1, (float)beta2, (float)(1 - beta1), (float)(1 - beta2), (float)eps, (float)(lr * weight_decay)};
   return count <= kFew ? run<float, kFew>("adamw_kernel", adamw_kernel<kFew>, count, params, sizes, 1, slots, h, corrections, st)
                        : run<float, kMany>("adamw_kernel", adamw_kernel<kMany>, count, params, sizes, 1, slots, h, corrections, st);
 }
@@ -576,7 +577,7 @@ MTB_API int mtb_adamw8_f32(int count, void* const* params, const long long* size
   cudaStream_t st = (cudaStream_t)stream;
   Corrections* corrections = (Corrections*)scratch;
   if (int rc = begin(count, params, lr, b1, b2, grad_scale, MtbClip{sums, nsums, grad_scale, max_norm, norm}, corrections, slots, st)) return rc;
-  const Hyper h{(float)b1, (float)b2, (float)(1 - b1), (float)std::sqrt(1 - b2), (float)eps, (float)(1 - lr * weight_decay)};
+  const Hyper h{(float)b1, (float)b2, (float)(1 - b1), (float)std::sqrt(1 - b2), (float)eps, (float)(lr * weight_decay)};
   return count <= kFew ? run<unsigned char, kFew>("adamw8_kernel", adamw8_kernel<kFew>, count, params, sizes, 2, slots, h, corrections, st)
                        : run<unsigned char, kMany>("adamw8_kernel", adamw8_kernel<kMany>, count, params, sizes, 2, slots, h, corrections, st);
 }

@@ -1,0 +1,30 @@
+"""AdamW's weight decay of a millionth and less a step: what a parameter loses is right on average over many of them, though each is rounded to float32.
+
+The mean of (p' - exact p') sign(p) over n values, relative to that of |p|.  Each rounding of the result is off by at most 2^-24 |p| and, as the steps' sizes are spread over many of its
+last places, evenly: 8 standard deviations of a mean are 8 * 2^-24 / sqrt(3 n).  The steps' own roundings have the sign of the step, as often that of p as not: under 2^-20 of a step each,
+the mean's share of them 8 * 2^-20 lr / sqrt(n).  The decay as a float32 and its product: 2^-23 of it."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("lr", [1e-4, 1e-5, 2e-6])
+def test_small_decays_are_not_rounded_away(bits, offset, lr):
+    import gpu_util as g
+    from mytorch_b200.optim import AdamW
+    from test_gpu_adamw import _window
+
+    n, wd, eps, b1, b2 = 1 << 22, 0.01, 1.0, 0.5, 0.75
+    rng = np.random.default_rng(7)
+    p0 = (rng.uniform(1, 2, n) * rng.choice([-1, 1], n)).astype(np.float32)
+    grad = rng.standard_normal(n).astype(np.float32)
+    p = _window(p0, offset)
+    p.requires_grad, p.grad = True, _window(grad, offset)
+    AdamW([p], lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd, state_bits=bits).step()
+    g64, p64 = grad.astype(np.float64), p0.astype(np.float64)
+    exact = p64 * (1 - lr * wd) - lr * g64 / (np.abs(g64) + eps)  # the first step: both corrections undo the moments' weights
+    mean = ((g.host(p) - exact) * np.sign(p64)).mean() / np.abs(p64).mean()
+    assert abs(mean) <= 8 * (2.0 ** -24 / np.sqrt(3 * n) + 2.0 ** -20 * lr / np.sqrt(n)) + 2.0 ** -23 * lr * wd
