@@ -594,6 +594,34 @@ __global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __gr
     to[row.lead + token] = r.at(none ? 0.f : row.z[row.lead + token]) + r.g;
 }
 
+void describe(cudaLaunchConfig_t& cfg, cudaLaunchAttribute (&attr)[2], long long rows, int ctas) {
+  cfg.gridDim = dim3((unsigned)(rows * ctas));
+  cfg.blockDim = dim3(kThreads);
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+}
+// How many clusters of so many CTAs are resident at a time.
+int resident_clusters(int ctas) {
+  static int known[kMostCtas + 1];
+  if (!known[ctas]) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    describe(cfg, attr, 1, ctas);
+    cfg.numAttrs = 1;
+    int most = 0;
+    if (cudaOccupancyMaxActiveClusters(&most, log_probs_cluster_kernel, &cfg) != cudaSuccess || most < 1) {
+      cudaGetLastError();  // not of the launch that follows
+      most = 1;
+    }
+    known[ctas] = most;
+  }
+  return known[ctas];
+}
+
 bool sizes_fine(long long n, int v, int token_kind, int top) {
   return n >= 0 && n < 1LL << 31 && v > 0 && v <= 1 << 30 && top >= 0 && top <= kMostTop && top <= v && (token_kind == 0 || token_kind == 1);
 }
@@ -607,26 +635,22 @@ MTB_API int mtb_token_log_probs_forward_f32(long long n, int v, const float* log
   MTB_REQUIRE(logits && tokens && log_probs && entropy && (top == 0 || (top_log_probs && top_tokens)), "token_log_probs_forward: bad arguments");
   cudaStream_t st = (cudaStream_t)stream;
   const Forward a{n, v, token_kind, ignores, top, ignore_index, logits, tokens, log_probs, entropy, stats, top_log_probs, top_tokens};
-  // Few rows: CTAs side by side on each, as long as all fit (six an SM) and each has enough of it.  One row of 50000 with 8 alternatives 11.8 -> 6.3 us, 300 rows 26 -> 20.6;
-  // 64 rows of 10007 would take 7.6 instead of 5.6.
+  // Few rows: CTAs side by side on each, as long as each has enough of it and all clusters are resident: where some wait, rows by one CTA each take less, but for long ones, where
+  // up to six CTAs an SM, some of which wait, still take less than whole rows.  With 8 alternatives, by clusters of 2 and by one CTA each, 370 rows (all resident) of 33000 17.0 and 16.0
+  // us, of 50000 20.5 and 21.0, of 131072 38 and 45; 400 rows of 16384 15.2 and 12.2, of 33000 23.0 and 21.0, of 50000 28.1 and 27.9, of 65536 32.2 and 33.3, of 131072 53.7 and 60.9.  By
+  // clusters of 8 and of 4, 100 rows of 33000 15.3 and 12.8, of 65536 16.0 and 14.5, of 131072 21.8 and 21.7, of 262144 33.1 and 36.5; one row of 50000 6.7 and 7.2, by one CTA 10.5.
   int ctas = 1;
-  const bool many = n > 8LL * mtb_sm_count();
-  while (ctas < kMostCtas && n * ctas * 2 <= 6 * mtb_sm_count() && v / (2 * ctas) >= 4096) ctas *= 2;
+  const int sms = mtb_sm_count();
+  const bool many = n > 8LL * sms;
+  while (ctas < kMostCtas && v / (2 * ctas) >= 4096 && n <= (v < 1 << 16 ? resident_clusters(2 * ctas) : 6 * sms / (2 * ctas))) ctas *= 2;
   // Otherwise a row by so many warps that there are enough of them under way, and few as long as the CTAs that an SM holds take turns anyway: then one's search for
   // alternatives is the others' time for loads.  With 8 alternatives by 1, 4 and 8 warps (measured with a looser bound): 16384 x 1000 21, 47, 87 us; 1184 x 4000 8.7, 9.4, 11.9; of few
   // rows 592 x 4000 8.6, 8.6, 7.7; by 4 and 8: 4096 x 20000 64, 72; 4096 x 33000 105, 112; 4096 x 50000 152, 162, with 32 alternatives 196, 184; 1600 x 128000 177, 160.
   if (ctas > 1) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(n * ctas));
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = st;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ctas;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
+    describe(cfg, attr, n, ctas);
+    cfg.stream = st;
     cfg.numAttrs = 2;
     MTB_CUDA(cudaLaunchKernelEx(&cfg, log_probs_cluster_kernel, a));
   } else if (v <= 1024 || (v <= 4096 && many)) {
