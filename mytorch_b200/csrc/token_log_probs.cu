@@ -644,8 +644,11 @@ MTB_API int mtb_token_log_probs_forward_f32(long long n, int v, const float* log
   const bool many = n > 8LL * sms;
   while (ctas < kMostCtas && v / (2 * ctas) >= 4096 && n <= (v < 1 << 16 ? resident_clusters(2 * ctas) : 6 * sms / (2 * ctas))) ctas *= 2;
   // Otherwise a row by so many warps that there are enough of them under way, and few as long as the CTAs that an SM holds take turns anyway: then one's search for
-  // alternatives is the others' time for loads.  With 8 alternatives by 1, 4 and 8 warps (measured with a looser bound): 16384 x 1000 21, 47, 87 us; 1184 x 4000 8.7, 9.4, 11.9; of few
-  // rows 592 x 4000 8.6, 8.6, 7.7; by 4 and 8: 4096 x 20000 64, 72; 4096 x 33000 105, 112; 4096 x 50000 152, 162, with 32 alternatives 196, 184; 1600 x 128000 177, 160.
+  // alternatives is the others' time for loads.  On both sides of each limit, with 8 alternatives, us, by 1 and 4 warps: 16384 x 1024 22.7, 54.6; 800 x 1025 5.5, 6.6, but 300 x 1025
+  // 5.0, 4.2; 3000 x 2048 12.7, 13.7; 3000 x 4096 20.1, 18.0; 4000 x 4096 20.7, 21.6; 4000 x 6000 29.3, 26.7.  By 4 and 8: 800 x 2048 6.6, 8.1; 592 x 4096 8.0, 6.9; 1000 x 16384
+  // 19.8, 19.8; 1184 x 16384 20.6, 22.0; of all counts from 1185 to 3000, in whose last turns the SMs have more or less to do, x 28000 0.94 to 1.06 of the time, x 32768 0.98 to 1.09; 3400 x 50000
+  // 130.8, 129.8; 4096 x 50000 151.0, 159.1; 4096 x 56000 170.1, 171.0; 4096 x 65536 195, 194; with 12 alternatives 4096 x 50000 158, 162, x 56000 177, 175, with 16 165, 166 and 184, 179.
+  const bool most = n >= 25LL * sms;
   if (ctas > 1) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -653,9 +656,9 @@ MTB_API int mtb_token_log_probs_forward_f32(long long n, int v, const float* log
     cfg.stream = st;
     cfg.numAttrs = 2;
     MTB_CUDA(cudaLaunchKernelEx(&cfg, log_probs_cluster_kernel, a));
-  } else if (v <= 1024 || (v <= 4096 && many)) {
+  } else if (v <= 1024 || (v <= 2048 && many) || (v <= 4096 && most)) {
     MTB_LAUNCH(log_probs_kernel<1>, (unsigned)mtb_div_up(n, kWarps), kThreads, 0, st, a);
-  } else if ((v <= 32768 && many) || (v <= 65536 && top <= 16 && n >= 25LL * mtb_sm_count())) {
+  } else if (v <= 2048 || (v <= 28000 && many) || (v <= 56000 && top <= 12 && most)) {
     MTB_LAUNCH(log_probs_kernel<4>, (unsigned)n, 128, 0, st, a);
   } else {
     MTB_LAUNCH(log_probs_kernel<kWarps>, (unsigned)n, kThreads, 0, st, a);
