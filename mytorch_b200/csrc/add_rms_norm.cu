@@ -678,12 +678,12 @@ MTB_API int mtb_add_rms_norm_forward_f32(long long rows, int c, const float* res
 }
 
 MTB_API long long mtb_add_rms_norm_workspace_bytes(long long rows, int c) {
-  // whichever kernel it will be: a row of three sums for each CTA, and one for each stretch that does not fill a row of the gate
-  long long most = 0;
+  // whichever kernel it will be: a row of three sums for each CTA that has rows, and one for each stretch that does not fill a row of the gate (four a group at most)
+  long long most = 4;  // what begins at 16 bytes
   for (const int align : {1, 2, 4}) {
     const Plan p = backward_plan(c, align);
-    const long long floats = (long long)p.ctas * (3 + 4 * p.groups) * c;
-    if (floats > most) most = floats;
+    const long long ctas = std::min<long long>(p.ctas, (rows + p.groups - 1) / p.groups), stretches = std::min(rows, 4LL * p.ctas * p.groups);
+    most = std::max(most, (3 * ctas + stretches) * c);
   }
   return 4 * most;
 }
@@ -742,7 +742,7 @@ MTB_API int mtb_add_rms_norm_backward_f32(long long rows, int c, const float* dn
     MTB_CLUSTERS
 #undef MTB_JOINED
     s = stretches_of(p, ctas, rows, of_gate ? rows_per_gate : rows);
-    gate_rows = each || (of_gate && s.parts == 1) ? dgate : of_gate ? partial + (long long)p.ctas * 3 * c : nullptr;
+    gate_rows = each || (of_gate && s.parts == 1) ? dgate : of_gate ? partial + (long long)s.ctas * 3 * c : nullptr;
     const Gradients d{dnew, dy, rstd, block_rstd, dresidual, dblock, summed ? partial : nullptr, gate_rows, each ? 1 : 0, s.stretches, s.parts, s.stretch, s.rows_of_gate};
 #define MTB_CASE(V, PER, W, LANES, AHEAD) \
   if (p.v == V && p.per == PER && p.warps == W && p.lanes == LANES && p.ahead == AHEAD && p.joined == 1) { \
