@@ -26,6 +26,8 @@ class AdamW(Optimizer):
         if max_grad_norm is not None and not max_grad_norm >= 0:
             raise RuntimeError(f"max_grad_norm is a number from 0 up: {max_grad_norm}")
         for g in self.param_groups:
+            if len({id(p) for p in g["params"]}) != len(g["params"]):  # the updates of a group run side by side
+                raise RuntimeError("AdamW: a parameter occurs twice in a group")
             if len(g["betas"]) != 2 or not all(0 <= b < 1 for b in g["betas"]) or not all(g[k] >= 0 for k in ("lr", "eps", "weight_decay")):
                 raise RuntimeError(f"AdamW: betas are two numbers from 0 to below 1, lr, eps and weight_decay numbers from 0 up: {[g[k] for k in self.defaults]}")
         self.grad_scale = 1.0  # set to 1/world_size by the data-parallel wrapper
