@@ -294,9 +294,9 @@ __device__ __forceinline__ void update_quickly(float& p, float m, float v, const
   p -= fmaf(h.decay, p, c.step_size * m * per);
 }
 
-// A block by a warp.  What bounds it is the number of instructions, 517 a warp with its eight values a lane (41 us of the integer pipe, 46 of issue slots and 54 of HBM in 73 us for 25.6 M
+// A block by a warp.  What bounds it is the number of instructions, 524 a warp with its eight values a lane (41 us of the integer pipe, 46 of issue slots and 54 of HBM in 73 us for 25.6 M
 // values): words of codes are taken apart and put together whole, and everything that a scale decides is decided once a block.  Two to eight blocks a warp: 5 to 60 us more; 48
-// registers instead of 63, five CTAs an SM: no difference.
+// registers instead of 64, five CTAs an SM: no difference.
 template <bool VECTORS>
 __device__ __forceinline__ void update_block(const Lane<VECTORS> l, float* p, const float* g, int n, unsigned char* codes, unsigned char* scales, unsigned first, unsigned key,
                                              const Hyper& h, const Corrections* corrections) {

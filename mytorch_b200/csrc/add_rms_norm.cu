@@ -176,7 +176,9 @@ struct Gradients {
 // AHEAD: the next row's values come to shared memory meanwhile.  That pays where many warps wait for one another at a row's sums (16384 x 2048 with post norm and gate 153 -> 136 us,
 // 8192 x 4096 167 -> 142), not where rows of other groups are under way on the SM (32768 x 1024 135 -> 146), nor by copies of 4 bytes (32768 x 1023 158 -> 215).
 // Where it is not 0: registers for so many on an SM; what else the compiler takes leaves a third of the warps (32768 x 750 by six values a thread and 4 warps 125 -> 111 us,
-// 12672 x 2601 by eight and 12 warps 302 -> 207), but for kernels that would then spill (16384 x 2047 by eight and 8 warps 171 -> 190).
+// 12672 x 2601 by eight and 12 warps 302 -> 207).  Kernels that lose more by spilling have none (16384 x 2047 by eight and 8 warps 171 -> 190).  With it spill: groups of 12 and 24 warps of
+// pairs or single values 8 to 24 bytes a thread, six values of a warp 16, clusters by 8 and 12 warps of fours 20, by 12 of pairs 52 and of single values 136.  Without it: pairs by 2 and 5 warps
+// 4, and, as 32 warps a CTA have 64 registers each at most, these 108 of fours, 140 of pairs, 152 of single values.
 template <int V, int PER, int W, int LANES, bool JOINED>
 constexpr int kBackwardCtas = JOINED ? (W == 8 && V != 4 ? 2 : 24 / W) : V * PER == 6 ? (W == 1 ? 3 : 24 / W) : W == 24 ? 1 : V != 4 && W == 12 ? 2 : V != 4 && V * PER == 4 && W == 1 && LANES == 32 ? 4 : 0;
 

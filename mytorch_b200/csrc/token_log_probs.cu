@@ -4,14 +4,14 @@
 // A logit of -inf has probability 0 and adds nothing to the entropy or its gradient; a row of nothing else, or with a NaN or +inf, is NaN.
 // Alternatives are in the order of their logits, NaN before everything, equal ones by place, which one whole number holds (`key_of`).
 //
-// Bound by memory: forward reads a row once, backward reads and writes it once.  4096 rows of 50000, logits out of HBM: forward 130 us without alternatives, 6.3 TB/s, 151 with 8,
-// 5.4; backward 265 us, 6.2 TB/s.  Each thread keeps a running maximum and both sums of its share of the row, four loads of 16 bytes on their way at a time.  What counts is
+// Bound by memory: forward reads a row once, backward reads and writes it once.  4096 rows of 50000, logits out of HBM: forward 130 us without alternatives, 6.3 TB/s, 150 with 8,
+// 5.5; backward 255 us, 6.4 TB/s.  Each thread keeps a running maximum and both sums of its share of the row, four loads of 16 bytes on their way at a time.  What counts is
 // how many warps are under way (40 an SM): a second set of loads ahead of use costs a quarter of them, 146 us, reloading each register as soon as it is used 162, copies
 // through shared memory two batches ahead and across rows 149, CTAs whose warps go on to the next row while one of them looks for the last one's alternatives 146, with 8 of them 174.
 //
 // Alternatives.  A thread also keeps the maxima of the four groups that its quads fall into, nothing else.  When the row is through, the top-th largest of the maxima of 64 parts
 // of it is a bound that `top` values reach, and only groups whose maximum reaches it can hold an alternative: little more than `top` of the row's 1024 (512, 128) groups, whose values
-// are read again, and what reaches the bound is put in order by counting.  The bound takes a third of the 23 us that 8 alternatives cost, the second reading the rest.  An
+// are read again, and what reaches the bound is put in order by counting.  The bound takes a third of the 20 us that 8 alternatives cost, the second reading the rest.  An
 // exact bound by sorting all groups' maxima: 180 us; the r-th largest of each warp's: 163; one group a thread, which reads four times as much again out of HBM, as the
 // rows under way are more than the L2 holds: 170; candidates picked while the row comes by would cost every batch of values an insertion at first.  Where very many
 // values equal the bound, as where a mask leaves fewer than `top`, those above it are taken and then the first of the row that equal it; rows with a NaN, and more candidates

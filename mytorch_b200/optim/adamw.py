@@ -17,7 +17,8 @@ class AdamW(Optimizer):
     share), and ``exp_avg`` and ``exp_avg_sq`` like the parameter.  With ``state_bits=8`` these are ``moments`` and ``scales``: blocks of 256 values in the order of the
     parameter's memory share a scale, a first moment keeps 3 bits behind its leading one and a second one as many over a wider range, rounded at random (by ``seed``, the
     parameter's place, the step and the value's place: the same every time) so that small steps add up; ``moments()`` says what they stand for.  The betas then count
-    with 20 bits.  Where a gradient is not finite, its whole block of moments reads NaN."""
+    with 20 bits.  Where a gradient is not finite, its whole block of moments reads NaN from then on, and the block's parameters do after the
+    next step.  Like ``lr`` and the betas, ``seed`` is not part of a checkpoint: a resumed run rounds as the first one would have if it is given again."""
 
     def __init__(self, params, lr=0.001, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, maximize=False, max_grad_norm=None, state_bits=32, seed=0):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize))
