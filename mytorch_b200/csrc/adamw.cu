@@ -90,12 +90,18 @@ struct Table {
   Chunks<N> chunks;
 };
 
+// What a parameter loses: decay and step, added up.  An infinite parameter counts as the largest, whose product with a decay of 0 is no NaN, and from which the difference stays infinite.
+__device__ __forceinline__ float loss_of(float p, float decay, float step) {
+  float finite;
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(finite) : "f"(p), "f"(3.402823466e38f));
+  return fmaf(decay, finite, step);
+}
 // Root and quotient to 2^-22 of themselves, the step's share of which is far under a parameter's last place.  Decay and step are added up first, so that only their sum is
 // rounded against the parameter.
 __device__ __forceinline__ void update(float& p, float m, float v, const Hyper& h, const Corrections& c) {
   float root;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
-  p -= fmaf(h.decay, p, __fdividef(c.step_size * m, fmaf(root, c.root, h.eps)));
+  p -= loss_of(p, h.decay, __fdividef(c.step_size * m, fmaf(root, c.root, h.eps)));
 }
 __device__ __forceinline__ void moments(float g, float& m, float& v, const Hyper& h) {
   m = fmaf(h.b1, m, h.c1 * g);
@@ -291,7 +297,7 @@ __device__ __forceinline__ void update_quickly(float& p, float m, float v, const
   float root, per;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(per) : "f"(fmaf(root, c.root, h.eps)));
-  p -= fmaf(h.decay, p, c.step_size * m * per);
+  p -= loss_of(p, h.decay, c.step_size * m * per);
 }
 
 // A block by a warp.  What bounds it is the number of instructions, 524 a warp with its eight values a lane (41 us of the integer pipe, 46 of issue slots and 54 of HBM in 73 us for 25.6 M

@@ -1,5 +1,6 @@
 """AdamW (no counterpart in the reference): all parameters of a group in one launch, the step counted on the device, so that a captured update counts on
-when it is replayed.  ``state_bits=8`` holds both moments in a byte each.  Every parameter needs a gradient, as in ``SGD``."""
+when it is replayed.  ``state_bits=8`` holds both moments in a byte each.  Every parameter needs a gradient, as in ``SGD``, and occurs
+once in its group."""
 import ctypes
 
 from mytorch_b200.backends.backend_dispatcher import BackendDispatcher
