@@ -300,7 +300,7 @@ __device__ __forceinline__ void update_quickly(float& p, float m, float v, const
   p -= loss_of(p, h.decay, c.step_size * m * per);
 }
 
-// A block by a warp.  What bounds it is the number of instructions, 524 a warp with its eight values a lane (41 us of the integer pipe, 46 of issue slots and 54 of HBM in 73 us for 25.6 M
+// A block by a warp.  What bounds it is the number of instructions, 532 a warp with its eight values a lane (41 us of the integer pipe, 46 of issue slots and 54 of HBM in 73 us for 25.6 M
 // values): words of codes are taken apart and put together whole, and everything that a scale decides is decided once a block.  Two to eight blocks a warp: 5 to 60 us more; 48
 // registers instead of 64, five CTAs an SM: no difference.
 template <bool VECTORS>
